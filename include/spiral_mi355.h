@@ -38,6 +38,9 @@ typedef enum {
 } sp_status;
 
 typedef enum { SP_F32 = 0, SP_F16 = 1, SP_BF16 = 2 } sp_dtype;
+/* 8-bit floating point (sp_quantize_blocks, sp_gemm_abt_scaled only): four exponent bits and three of mantissa, largest number 448,
+ * no infinity; or five and two, largest number 57344. */
+typedef enum { SP_F8_E4M3 = 8, SP_F8_E5M2 = 9 } sp_f8;
 
 /* ------------------------------------------------------------------------------------------ */
 /* library                                                                                     */
@@ -140,6 +143,40 @@ int sp_gemm_config(int dtype_in, int64_t M, int64_t N, int64_t K,
  * added up from (4 on the split-K tiles, 1 on the workgroup tiles, 0 where one thread adds them up in order). */
 int sp_gemm_batched_config(int dtype_in, int64_t M, int64_t N, int64_t K, int64_t batch,
                            int32_t* tile_m, int32_t* tile_n, int32_t* tile_k, int32_t* threads, int32_t* k_parts);
+
+/* ------------------------------------------------------------------------------------------ */
+/* 8-bit blocks and their product                                                              */
+/* ------------------------------------------------------------------------------------------ */
+
+/*
+ * x (rows, cols) of dtype SP_F32, SP_F16 or SP_BF16 in 8-bit blocks with a scale each: over a block
+ *   scale = max(largest |x| / largest number of f8, 2^-126) in f32,   q = x / scale to the nearest number of f8, ties to even
+ * (where x / scale is within half an f32 rounding of a tie, to one of its two neighbours).  A block with an infinity or a NaN in it has that
+ * as its scale and NaNs as its numbers.  Blocks are 128 consecutive columns of one row (block_rows = 1) or 128 x 128 elements
+ * (block_rows = 128); the last ones along either side are smaller.
+ *   q        (rows, cols rounded up to a multiple of 16), the columns behind x's filled with zeros; scale (block rows, ceil(cols / 128))
+ *            f32, both NULL to leave this form out
+ *   q_t, scale_t   the same of the transpose of x, which is (cols, rows), or NULL
+ * At least one of the two forms.  Either is what sp_gemm_abt_scaled takes as an operand; x is read once.
+ * The reference has no 8-bit types; this stands beside its transposes and the TF32 rounding of its operands (ml/layers.spi:234-238).
+ */
+int sp_quantize_blocks(int dtype, int f8, int32_t block_rows, const void* x, void* q, float* scale, void* q_t, float* scale_t,
+                       int64_t rows, int64_t cols, void* stream);
+
+/*
+ * C = sum over the blocks b of 128 along K of  scale_a[m, b] * scale_b[n / block_n, b] * (sum over k in b of A[m, k] B[n, k])
+ *     + beta * C [+ bias[n]] [ReLU]
+ * A (M, K) of f8 type f8_a, B (N, K) of f8 type f8_b, row-major; K a multiple of 16.  scale_a (M, ceil(K / 128)) f32; scale_b
+ * (ceil(N / block_n), ceil(K / 128)) f32 with block_n = 1 or 128.  C (M, N) of dtype_out SP_F32, SP_F16 or SP_BF16; bias (N,) f32 or
+ * NULL; beta == 0: C is not read.  flags: SP_GEMM_RELU.  scale_a * scale_b has to be a finite f32.  A result depends on its row of A, its
+ * row of B, the shape and the type of C alone.
+ * C of f32: products are exact and sums f32.  C of 16 bits: the matrix pipe's 8-bit products, twice as fast, of which every eight that follow each
+ * other along K are cut off below 2^-13 of the power of two of the largest before they are added up in f32 (1.5e-5 of a sum of N(0, 1) products, in the 2-norm).
+ * Stands beside sp_gemm_abt (ml/matmul/run.spi:21-26), which multiplies 16- and 32-bit operands.
+ */
+int sp_gemm_abt_scaled(int f8_a, int f8_b, int dtype_out, const void* A, const float* scale_a, const void* B, const float* scale_b,
+                       int32_t block_n, void* C, const float* bias, int64_t M, int64_t N, int64_t K, float beta, uint32_t flags,
+                       void* stream);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Row primitives                                                                              */
@@ -291,6 +328,52 @@ typedef enum { SP_MAP_OUT_IDENTITY = 0, SP_MAP_OUT_SQRT = 1 } sp_map_out;
  * `local_length` is cols.  The order of a float sum depends on cols only.
  */
 int sp_row_reduce_f32(int op, int map_in, int map_out, const float* x, float* out, int64_t rows, int64_t cols, void* stream);
+
+/*
+ * y = (x - mean) * rstd * weight + bias row by row, with mean and var = the mean of (x - mean)^2 over the row in f32 and
+ * rstd = 1 / sqrt(var + eps).  x, y (rows, cols) of `dtype` (SP_F32, SP_F16, SP_BF16), any cols from 1 to 16384; weight, bias (cols,)
+ * of `weight_dtype` (SP_F32 or dtype), either may be NULL (1 and 0).  mean_out, rstd_out: (rows,) f32, or NULL.  y may be x.
+ * Stands beside SP_ROW_LN_L2 (ml/primitives.spi:701-703), which divides by the root of the sum of squares.
+ */
+int sp_layer_norm(int dtype, int weight_dtype, const void* x, const void* weight, const void* bias, void* y, float* mean_out,
+                  float* rstd_out, int64_t rows, int64_t cols, float eps, void* stream);
+
+/*
+ * The gradients of sp_layer_norm.  With h = (x - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - mean of g - h * mean of (g * h)),   dweight = sum over the rows of dy * h,   dbias = sum over the rows of dy.
+ * dy, dx like x; dx may be dy.  mean, rstd as sp_layer_norm wrote them.  dweight, dbias: (cols,) f32, or both NULL.  The sums
+ * over rows are f32, in an order that depends on the sizes alone.
+ * `workspace`: sp_layer_norm_backward_workspace_bytes(rows, cols) bytes of device memory that hold partial sums during the call
+ * (what they held before does not matter); may be NULL where dweight and dbias are.  Calls that may run at the same time need one each.
+ */
+int sp_layer_norm_backward(int dtype, int weight_dtype, const void* dy, const void* x, const float* mean, const float* rstd,
+                           const void* weight, void* dx, float* dweight, float* dbias, int64_t rows, int64_t cols, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+int64_t sp_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+
+/*
+ * Logits (rows, cols) of `dtype` (SP_F32, SP_F16, SP_BF16), any cols, before a token is chosen from them; in f32, for element j of a row:
+ *   x = seen ? (x > 0 ? x / repetition : x * repetition) : x          seen: j is among the row's tokens
+ *   x = x - frequency * count - presence * (count > 0)               count: how often, behind its first prompt_lengths tokens
+ *   x = x + bias of the row's entries whose id is j, in their order
+ *   x = temperature > 0 ? x / temperature : x
+ *   x = -inf where the mask's bit is 0
+ * out (rows, cols) f32 receives x (may be the logits, where those are f32); token (rows,) i32 or NULL: the lowest index of the row's largest x, -1 where no
+ * x is above -inf (a NaN is never chosen).
+ *   tokens (rows, history) i32, the first lengths[r] of row r count (all of them if lengths is NULL); prompt_lengths NULL: none
+ *   are the prompt's.  history < 2^20.  repetition, presence, frequency, temperature: (rows,) f32, each NULL to leave its step out.
+ *   bias_ids (rows, n_bias) i32, bias (rows, n_bias) f32, n_bias < 2048.  Tokens and bias_ids outside [0, cols) are passed over.
+ *   mask (mask_rows, ceil(cols / 32)) 32-bit words, bit j % 32 of word j / 32 set where j is allowed; mask_rows = rows, or 1 for all rows alike.
+ * `workspace`: sp_logits_penalize_workspace_bytes(rows, cols) bytes of device memory for the choice of a token (its former
+ * contents do not matter); may be NULL where token is.  Calls that may run at the same time need one each.
+ * Stands beside SP_ROW_MASKED_SOFTMAX and sp_row_ops (ml/primitives.spi:705-708,748-759), whose masks are a prefix of the row.
+ */
+int sp_logits_penalize(int dtype, const void* logits, float* out, int32_t* token, const int32_t* tokens, const int32_t* lengths,
+                       const int32_t* prompt_lengths, int64_t history, const float* repetition, const float* presence,
+                       const float* frequency, const float* temperature, const int32_t* bias_ids, const float* bias, int64_t n_bias,
+                       const int32_t* mask, int64_t mask_rows, int64_t rows, int64_t cols, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+int64_t sp_logits_penalize_workspace_bytes(int64_t rows, int64_t cols);
 
 typedef enum { SP_MAP_COPY = 0, SP_MAP_RELU = 1, SP_MAP_TANH = 2, SP_MAP_SIGMOID = 3 } sp_map_op;
 

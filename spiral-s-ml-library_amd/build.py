@@ -19,9 +19,9 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libspiral_mi355.so")
 HOST_LIB = os.path.join(HERE, "spiral_host.so")      # the Python modules' way into the library (csrc/host.cpp)
 HOST_STAMP = os.path.join(OBJ, "spiral_host.txt")
-SOURCES = ["api.hip", "row_ops.hip", "elementwise.hip", "gemm.hip", "gemm_wave.hip", "mlp.hip", "mlp_any.hip", "mlp_packed.hip", "mlp_resident.hip", "mlp_pipe.hip", "mlp_ensemble.hip", "mlp_stack.hip"]
+SOURCES = ["api.hip", "row_ops.hip", "elementwise.hip", "gemm.hip", "gemm_wave.hip", "mlp.hip", "mlp_any.hip", "mlp_packed.hip", "mlp_resident.hip", "mlp_pipe.hip", "mlp_ensemble.hip", "mlp_stack.hip", "norm.hip", "logits.hip", "quantize.hip", "gemm_scaled.hip"]
 # sources with MFMAs or wide stores in inline asm: their device assembly is kept and scanned (isa_check.py)
-ASM_MFMA_SOURCES = ["gemm.hip", "gemm_wave.hip", "mlp.hip", "mlp_any.hip", "mlp_packed.hip", "mlp_resident.hip", "mlp_pipe.hip", "mlp_ensemble.hip", "mlp_stack.hip", "row_ops.hip", "elementwise.hip"]
+ASM_MFMA_SOURCES = ["gemm.hip", "gemm_wave.hip", "mlp.hip", "mlp_any.hip", "mlp_packed.hip", "mlp_resident.hip", "mlp_pipe.hip", "mlp_ensemble.hip", "mlp_stack.hip", "row_ops.hip", "elementwise.hip", "quantize.hip", "gemm_scaled.hip", "norm.hip", "logits.hip"]
 # Kernel-argument preloading (gfx950): the first 14 dwords of a kernel's leading scalar parameters arrive in
 # registers with the wave instead of through a scalar load at kernel entry (a struct parameter is not preloaded;
 # the kernels that gain from it repeat the fields their first loads need as leading scalars).
@@ -105,7 +105,7 @@ def build(force=True, verbose=False):
     """Compile every HIP source and link the shared library.  Returns the library path."""
     os.makedirs(OBJ, exist_ok=True)
     cc = hipcc()
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_common.h"), os.path.join(CSRC, "gemm_dma.h"), os.path.join(CSRC, "parts.h"), os.path.join(CSRC, "mlp_common.h"), os.path.join(CSRC, "philox.h"), os.path.join(CSRC, "row_common.h"), os.path.join(ROOT, "include", "spiral_mi355.h")]
+    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "vec_io.h"), os.path.join(CSRC, "gemm_common.h"), os.path.join(CSRC, "gemm_dma.h"), os.path.join(CSRC, "parts.h"), os.path.join(CSRC, "mlp_common.h"), os.path.join(CSRC, "philox.h"), os.path.join(CSRC, "row_common.h"), os.path.join(ROOT, "include", "spiral_mi355.h")]
     newest_header = max(os.path.getmtime(h) for h in headers)
 
     def compile_one(src):

@@ -377,7 +377,7 @@ struct Entry<int(A...)> {
     X(sp_row_get_prob) X(sp_cem_resample) X(sp_cem_resample_philox) X(sp_row_reduce_f32) X(sp_cem_update_mask) X(sp_row_binarize)   \
     X(sp_map_f32) X(sp_reduce_sum) X(sp_reduce) X(sp_row_l1_normalize) X(sp_reduce_sum_static) X(sp_transpose_inner_b32)            \
     X(sp_mlp_forward) X(sp_mlp_pack_weights) X(sp_mlp_forward_packed) X(sp_mlp_forward_ensemble) X(sp_ensemble_binarize)            \
-    X(sp_stack_forward_f32)
+    X(sp_stack_forward_f32) X(sp_layer_norm) X(sp_layer_norm_backward) X(sp_logits_penalize) X(sp_quantize_blocks) X(sp_gemm_abt_scaled)
 
 bool bind_one(void* library, PyObject* stream, PyObject* functions, const char* name, PyCFunction call, PyMethodDef& def) {
     void* const fn = dlsym(library, name);

@@ -1,0 +1,269 @@
+// Logits of a whole vocabulary before a token is chosen: penalties for tokens that stand in the history, biases, temperature and a mask,
+// and the largest of what is left.  One pass: every logit is read once and written once, and that bounds it.
+//
+// A workgroup takes CHUNK columns of one row.  What the history and the biases say about them is gathered first in a 32-bit
+// word of LDS per column -- bits 0..19 the count behind the prompt, bit 20 "seen in the prompt", bits 21..31 the first bias entry that names
+// the column -- with integer atomics, whose order does not matter.  Columns whose word is zero, most of them, then cost one LDS read.
+// A column named by several bias entries (rare; a flag says whether there is one at all) goes through the entries again, in their order.
+// The arithmetic is that of the steps written out, each rounded to f32: nothing is contracted.
+#include "vec_io.h"
+
+#pragma clang fp contract(off)
+
+namespace sp {
+
+constexpr unsigned COUNT_MASK = (1u << 20) - 1u, SEEN_BIT = 1u << 20;
+constexpr int ENTRY_SHIFT = 21, MOST_ENTRIES = 2047;      // entry j is kept as 2047 - j: the first one is the largest, 0 is none
+constexpr int CHUNK = 8192, LOGITS_THREADS = 512;
+
+struct LogitsArgs {
+    float* out;
+    int32_t* token;
+    const int32_t *tokens, *lengths, *prompt_lengths;
+    const float *repetition, *presence, *frequency, *temperature;
+    const int32_t* bias_ids;
+    const float* bias;
+    const unsigned* mask;
+    long history, mask_step;      // mask_step: words from a row's mask to the next one's, 0 if all rows have the same
+    int n_bias;
+    float* best;                  // of every (row, chunk): the largest value, and behind them its column
+    int* best_at;
+};
+
+struct Best {
+    float v;
+    int at;
+    // the larger value, of equal ones the lower column; a NaN never wins, and -inf never does over "none"
+    __device__ __forceinline__ void take(float w, int j) {
+        if (w > v || (w == v && (unsigned)j < (unsigned)at)) { v = w; at = j; }
+    }
+};
+
+__device__ __forceinline__ Best best_of_wave(Best b) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) b.take(__shfl_xor(b.v, d, WAVE), __shfl_xor(b.at, d, WAVE));
+    return b;
+}
+
+// SPARSE: there is a history or there are biases.
+template <int DT, bool SPARSE>
+__global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const void* logits, long cols, unsigned chunks, const LogitsArgs a) {
+    constexpr int N = PER16<DT>;
+    __shared__ __attribute__((aligned(16))) unsigned words[SPARSE ? CHUNK : 4];
+    __shared__ int again;                                  // a column has more than one bias entry
+    __shared__ float wave_v[LOGITS_THREADS / 64];
+    __shared__ int wave_at[LOGITS_THREADS / 64];
+    const int tid = threadIdx.x;
+    const long row = blockIdx.x / chunks;
+    const unsigned chunk = blockIdx.x - (unsigned)row * chunks;
+    const long c0 = (long)chunk * CHUNK;
+    const int here = (int)(cols - c0 < CHUNK ? cols - c0 : CHUNK);     // columns of this workgroup
+    float rep = 1.f, pres = 0.f, freq = 0.f, temp = 0.f;
+    const bool has_rep = a.repetition != nullptr, has_pres = a.presence != nullptr, has_freq = a.frequency != nullptr;
+    if (has_rep) rep = a.repetition[row];
+    if (has_pres) pres = a.presence[row];
+    if (has_freq) freq = a.frequency[row];
+    if (a.temperature != nullptr) temp = a.temperature[row];
+    const int32_t* ids = a.bias_ids + row * a.n_bias;
+    const float* biases = a.bias + row * a.n_bias;
+    if constexpr (SPARSE) {
+        for (int i = tid * 4; i < CHUNK; i += LOGITS_THREADS * 4) *reinterpret_cast<u32x4*>(words + i) = u32x4{0u, 0u, 0u, 0u};
+        if (tid == 0) again = 0;
+        __syncthreads();
+        for (int j = tid; j < a.n_bias; j += LOGITS_THREADS) {
+            const long at = ids[j] - c0;
+            if (at >= 0 && at < here) atomicMax(&words[at], (unsigned)(MOST_ENTRIES - j) << ENTRY_SHIFT);
+        }
+        if (a.n_bias > 0) {
+            __syncthreads();
+            for (int j = tid; j < a.n_bias; j += LOGITS_THREADS) {
+                const long at = ids[j] - c0;
+                if (at >= 0 && at < here && words[at] >> ENTRY_SHIFT != (unsigned)(MOST_ENTRIES - j)) again = 1;
+            }
+            __syncthreads();
+        }
+        if (a.tokens != nullptr) {
+            long length = a.history;
+            if (a.lengths != nullptr) {
+                const long given = a.lengths[row];
+                length = given < length ? given : length;
+            }
+            const long prompt = a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
+            const int32_t* mine = a.tokens + row * a.history;
+            for (long i = (long)tid * 4; i < length; i += LOGITS_THREADS * 4) {
+                const u32x4 t = load16<SP_F32>(mine, i, length - i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const long at = (long)(int)t[e] - c0;
+                    if (i + e >= length || at < 0 || at >= here) continue;
+                    if (i + e < prompt) atomicOr(&words[at], SEEN_BIT);
+                    else atomicAdd(&words[at], 1u);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    Best best{-INFINITY, -1};
+    const unsigned* mask = a.mask + row * a.mask_step;
+    for (int i = tid * N; i < here; i += LOGITS_THREADS * N) {
+        const u32x4 raw = load16<DT>(logits, row * cols + c0 + i, here - i);
+        unsigned allowed = ~0u;
+        if (a.mask != nullptr) allowed = mask[(c0 + i) >> 5] >> (i & 31);
+        float v[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = element<DT>(raw, e);
+        if constexpr (SPARSE) {
+            unsigned w[N], any = 0;
+#pragma unroll
+            for (int h = 0; h < N; h += 4) {
+                const u32x4 ww = *reinterpret_cast<const u32x4*>(words + i + h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) any |= w[h + e] = ww[e];
+            }
+            if (any != 0) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    if (w[e] == 0) continue;
+                    const unsigned count = w[e] & COUNT_MASK;
+                    float x = v[e];
+                    if (has_rep && (w[e] & (SEEN_BIT | COUNT_MASK)) != 0) x = x > 0.f ? x / rep : x * rep;
+                    if (count != 0) {
+                        if (has_freq) x = x - freq * (float)count;
+                        if (has_pres) x = x - pres;
+                    }
+                    if (const unsigned entry = w[e] >> ENTRY_SHIFT; entry != 0) {
+                        const int first = MOST_ENTRIES - (int)entry;
+                        float b = biases[first];
+                        if (again != 0)
+                            for (int j = first + 1; j < a.n_bias; ++j)
+                                if (ids[j] == c0 + i + e) b += biases[j];
+                        x = x + b;
+                    }
+                    v[e] = x;
+                }
+            }
+        }
+        if (temp > 0.f)
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = v[e] / temp;
+        if (a.mask != nullptr)
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = (allowed >> e) & 1u ? v[e] : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (i + e < here && v[e] > best.v) best = Best{v[e], (int)c0 + i + e};     // (columns go up: the first one stays)
+#pragma unroll
+        for (int h = 0; h < N; h += 4) {
+            const float o[4] = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+            store16<SP_F32>(a.out, row * cols + c0 + i + h, here - i - h, o);
+        }
+    }
+    if (a.token == nullptr) return;
+    best = best_of_wave(best);
+    if ((tid & 63) == 0) {
+        wave_v[tid >> 6] = best.v;
+        wave_at[tid >> 6] = best.at;
+    }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int w = 1; w < LOGITS_THREADS / 64; ++w) best.take(wave_v[w], wave_at[w]);
+        if (chunks == 1) {
+            a.token[row] = best.at;
+        } else {
+            a.best[blockIdx.x] = best.v;
+            a.best_at[blockIdx.x] = best.at;
+        }
+    }
+}
+
+// The best of a row's chunks, a wave per row.
+__global__ __launch_bounds__(256) void logits_token_kernel(const float* best, const int* best_at, unsigned chunks, long rows, int32_t* token) {
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    Best b{-INFINITY, -1};
+    for (unsigned c = threadIdx.x & 63; c < chunks; c += 64) b.take(best[row * chunks + c], best_at[row * chunks + c]);
+    b = best_of_wave(b);
+    if ((threadIdx.x & 63) == 0) token[row] = b.at;
+}
+
+// ---- host side -------------------------------------------------------------------------------
+
+static int64_t logits_chunks(int64_t cols) { return (cols + CHUNK - 1) / CHUNK; }
+
+template <int DT>
+static void launch_logits(const void* logits, long rows, long cols, const LogitsArgs& a, hipStream_t stream) {
+    const unsigned chunks = (unsigned)logits_chunks(cols);
+    if (a.tokens != nullptr || a.n_bias > 0)
+        hipLaunchKernelGGL((logits_kernel<DT, true>), dim3((unsigned)rows * chunks), dim3(LOGITS_THREADS), 0, stream, logits, cols, chunks, a);
+    else
+        hipLaunchKernelGGL((logits_kernel<DT, false>), dim3((unsigned)rows * chunks), dim3(LOGITS_THREADS), 0, stream, logits, cols, chunks, a);
+}
+
+namespace {
+struct LogitsKernelNames {
+    LogitsKernelNames() {
+        register_kernel("logits", (const void*)logits_kernel<SP_F32, true>, LOGITS_THREADS);
+        register_kernel("logits_bf16", (const void*)logits_kernel<SP_BF16, true>, LOGITS_THREADS);
+    }
+} logits_kernel_names;
+}  // namespace
+
+}  // namespace sp
+
+using namespace sp;
+
+extern "C" int64_t sp_logits_penalize_workspace_bytes(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    return rows * logits_chunks(cols) * 8;
+}
+
+extern "C" int sp_logits_penalize(int dtype, const void* logits, float* out, int32_t* token, const int32_t* tokens, const int32_t* lengths,
+                                  const int32_t* prompt_lengths, int64_t history, const float* repetition, const float* presence,
+                                  const float* frequency, const float* temperature, const int32_t* bias_ids, const float* bias, int64_t n_bias,
+                                  const int32_t* mask, int64_t mask_rows, int64_t rows, int64_t cols, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
+    SP_REQUIRE_PTR(logits);
+    SP_REQUIRE_PTR(out);
+    SP_OPTIONAL_PTR(token);
+    SP_OPTIONAL_PTR(tokens);
+    SP_OPTIONAL_PTR(lengths);
+    SP_OPTIONAL_PTR(prompt_lengths);
+    SP_OPTIONAL_PTR(repetition);
+    SP_OPTIONAL_PTR(presence);
+    SP_OPTIONAL_PTR(frequency);
+    SP_OPTIONAL_PTR(temperature);
+    SP_OPTIONAL_PTR(bias_ids);
+    SP_OPTIONAL_PTR(bias);
+    SP_OPTIONAL_PTR(mask);
+    if (dtype != SP_F32 && dtype != SP_F16 && dtype != SP_BF16) return fail(SP_ERR_DTYPE, "sp_logits_penalize: dtype must be f32, f16 or bf16, got %d", dtype);
+    if (rows <= 0 || cols <= 0) return fail(SP_ERR_SHAPE, "sp_logits_penalize: rows and cols must be positive (got %lld, %lld)", (long long)rows, (long long)cols);
+    if (cols > INT32_MAX || rows > INT32_MAX || rows * logits_chunks(cols) * LOGITS_THREADS >= (int64_t)1 << 32) return fail(SP_ERR_SHAPE, "sp_logits_penalize: too large");
+    if (dtype != SP_F32 && (const void*)out == logits) return fail(SP_ERR_ARG, "sp_logits_penalize: only f32 logits can be overwritten");
+    if (history < 0 || history > (int64_t)COUNT_MASK) return fail(SP_ERR_SHAPE, "sp_logits_penalize: history must be in [0, 2^20), got %lld", (long long)history);
+    if (n_bias < 0 || n_bias > MOST_ENTRIES) return fail(SP_ERR_SHAPE, "sp_logits_penalize: n_bias must be in [0, 2047], got %lld", (long long)n_bias);
+    if (history > 0 && tokens == nullptr) return fail(SP_ERR_NULL, "sp_logits_penalize: tokens is NULL");
+    if (n_bias > 0 && (bias_ids == nullptr || bias == nullptr)) return fail(SP_ERR_NULL, "sp_logits_penalize: bias_ids and bias go together");
+    if (mask != nullptr && mask_rows != 1 && mask_rows != rows) return fail(SP_ERR_SHAPE, "sp_logits_penalize: mask_rows must be 1 or rows, got %lld", (long long)mask_rows);
+    if (token != nullptr) {
+        SP_REQUIRE_PTR(workspace);
+        if (workspace_bytes < sp_logits_penalize_workspace_bytes(rows, cols))
+            return fail(SP_ERR_ARG, "sp_logits_penalize: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes,
+                        (long long)sp_logits_penalize_workspace_bytes(rows, cols));
+    }
+    const int rc = require_gfx950(__func__);
+    if (rc != SP_OK) return rc;
+    LogitsArgs a{};
+    a.out = out; a.token = token; a.tokens = history > 0 ? tokens : nullptr; a.lengths = lengths; a.prompt_lengths = prompt_lengths; a.history = history;
+    a.repetition = repetition; a.presence = presence; a.frequency = frequency; a.temperature = temperature;
+    a.bias_ids = bias_ids; a.bias = bias; a.n_bias = (int)n_bias; a.mask = (const unsigned*)mask;
+    a.mask_step = mask_rows == rows ? (cols + 31) / 32 : 0;
+    const int64_t chunks = logits_chunks(cols);
+    a.best = (float*)workspace; a.best_at = token != nullptr ? (int*)((float*)workspace + rows * chunks) : nullptr;
+    if (dtype == SP_F32) launch_logits<SP_F32>(logits, rows, cols, a, (hipStream_t)stream);
+    else if (dtype == SP_F16) launch_logits<SP_F16>(logits, rows, cols, a, (hipStream_t)stream);
+    else launch_logits<SP_BF16>(logits, rows, cols, a, (hipStream_t)stream);
+    if (const int launched = check_launch(__func__); launched != SP_OK || token == nullptr || chunks == 1) return launched;
+    hipLaunchKernelGGL(logits_token_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a.best, a.best_at, (unsigned)chunks, (long)rows, token);
+    return check_launch(__func__);
+}

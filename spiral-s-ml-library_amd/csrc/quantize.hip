@@ -1,0 +1,230 @@
+// Rows and columns of a matrix in 8-bit blocks of 128 with a scale each: the operands of gemm_scaled.hip.
+//
+// A workgroup takes a tile of 128 x 128 (16 x 128 where only rows are wanted in blocks of one), so every block along either direction lies inside
+// one tile, and x is read once whatever is wanted of it.  A lane holds R rows of 8 columns.  A row's 16 lanes are a DPP row, so the
+// largest magnitude of a row's block takes four DPP steps; a column's takes two cross-lane steps and, over the four waves, LDS.
+// Magnitudes are compared as bits: an infinity is larger than every number and a NaN larger than that, so neither is lost.  The transposed
+// numbers go through LDS so that both forms leave in 128-byte rows.
+//
+// x / scale costs three operations: q = x * (1 / scale) and one step q + (x - q * scale) * (1 / scale), whose remainder is exact (Markstein's
+// correction).  That is x / scale rounded to f32, but for ties of f32, before the 8-bit rounding.
+#include "vec_io.h"
+
+namespace sp {
+
+constexpr int QB = 128;                       // elements of a block
+constexpr float SCALE_LEAST = 0x1p-126f;      // the smallest normal f32: 1 / scale stays finite, and a block of zeros has a scale
+
+template <int F8>
+constexpr float F8_MOST = F8 == SP_F8_E4M3 ? 448.f : 57344.f;
+
+// Four numbers as four bytes.
+template <int F8>
+__device__ __forceinline__ unsigned pack_f8(float a, float b, float c, float d) {
+    int v = 0;
+    if constexpr (F8 == SP_F8_E4M3) {
+        v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, v, false);
+        v = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+    } else {
+        v = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, v, false);
+        v = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, v, true);
+    }
+    return (unsigned)v;
+}
+
+struct BlockScale {
+    float scale, inv;
+    template <int F8>
+    __device__ __forceinline__ void set(unsigned magnitude) {
+        scale = __uint_as_float(magnitude) / F8_MOST<F8>;
+        scale = scale < SCALE_LEAST ? SCALE_LEAST : scale;               // (a NaN stays)
+        inv = 1.f / scale;
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        const float q = x * inv;
+        return __builtin_fmaf(__builtin_fmaf(-q, scale, x), inv, q);
+    }
+};
+
+struct QuantArgs {
+    const void* x;
+    unsigned char *q, *q_t;
+    float *scale, *scale_t;
+    long rows, cols;
+    long pitch, pitch_t;          // of q and q_t: cols and rows rounded up to a multiple of 16
+    long blocks_c, blocks_r;      // blocks of 128 along cols and rows: the widths of scale and scale_t
+};
+
+__device__ __forceinline__ unsigned max_u32(unsigned a, unsigned b) { return a > b ? a : b; }
+
+// WIDE: blocks of 128 x 128.  OUT: 1 = q, 2 = q_t, 3 = both.  R: rows per lane.
+template <int DT, int F8, bool WIDE, int OUT, int R>
+__global__ __launch_bounds__(256) void quantize_kernel(const void* x_first, long rows_first, long cols_first, const QuantArgs args) {
+    constexpr int E = ELEM_BYTES<DT>, PIECES = 8 / PER16<DT>;
+    constexpr bool ROW = (OUT & 1) != 0, COL = (OUT & 2) != 0;
+    static_assert(R == 8 || (!COL && !WIDE), "tiles of fewer rows hold blocks of one row only");
+    constexpr int PITCH = QB + 16;            // bytes of a transposed row in LDS
+    __shared__ __attribute__((aligned(16))) unsigned char turned[COL ? QB * PITCH : 16];
+    __shared__ unsigned most[COL && !WIDE ? 4 * QB : 4];
+    const long rows = rows_first, cols = cols_first;
+    const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4, wave = tid >> 6;
+    const long tiles_c = (cols + QB - 1) / QB;
+    const long tile_r = blockIdx.x / tiles_c, tile_c = blockIdx.x - tile_r * tiles_c;
+    const long r0 = tile_r * (16 * R) + rg * R, c0 = tile_c * QB + cg * 8;
+    u32x4 raw[R][PIECES];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p) {
+            const long col = c0 + p * PER16<DT>;
+            raw[i][p] = load16<DT>(x_first, (r0 + i) * cols + col, r0 + i < rows ? cols - col : 0);
+        }
+    auto value = [&](int i, int j) { return element<DT>(raw[i][j / PER16<DT>], j % PER16<DT>); };
+    auto magnitude = [&](int i, int j) { return __float_as_uint(value(i, j)) & 0x7fffffffu; };
+    auto across_row = [](unsigned v) { return group_allreduce<16>(v, max_u32); };      // over the 16 lanes of a row
+    auto across_wave = [](unsigned v) {                                                  // over the four row groups of a wave
+        v = max_u32(v, __shfl_xor(v, 16, WAVE));
+        return max_u32(v, __shfl_xor(v, 32, WAVE));
+    };
+    BlockScale one;                           // WIDE: of the tile
+    if constexpr (WIDE) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max_u32(m, magnitude(i, j));
+        m = across_wave(across_row(m));
+        if ((tid & 63) == 0) most[wave] = m;
+        __syncthreads();
+        one.template set<F8>(max_u32(max_u32(most[0], most[1]), max_u32(most[2], most[3])));
+        if (tid == 0) {
+            if constexpr (ROW) args.scale[tile_r * args.blocks_c + tile_c] = one.scale;
+            if constexpr (COL) args.scale_t[tile_c * args.blocks_r + tile_r] = one.scale;
+        }
+    }
+    if constexpr (ROW) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            BlockScale s = one;
+            if constexpr (!WIDE) {
+                unsigned m = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max_u32(m, magnitude(i, j));
+                s.template set<F8>(across_row(m));
+                if (cg == 0 && r0 + i < rows) args.scale[(r0 + i) * args.blocks_c + tile_c] = s.scale;
+            }
+            u32x2 o;
+            o.x = pack_f8<F8>(s(value(i, 0)), s(value(i, 1)), s(value(i, 2)), s(value(i, 3)));
+            o.y = pack_f8<F8>(s(value(i, 4)), s(value(i, 5)), s(value(i, 6)), s(value(i, 7)));
+            if (r0 + i < rows && c0 < args.pitch) *reinterpret_cast<u32x2*>(args.q + (r0 + i) * args.pitch + c0) = o;
+        }
+    }
+    if constexpr (COL) {
+        unsigned column[8];                   // !WIDE: the largest magnitude of each of this lane's columns
+        if constexpr (!WIDE) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                unsigned m = 0;
+#pragma unroll
+                for (int i = 0; i < R; ++i) m = max_u32(m, magnitude(i, j));
+                m = across_wave(m);
+                if ((tid & 63) < 16) most[wave * QB + cg * 8 + j] = m;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int c = cg * 8 + j;
+                column[j] = max_u32(max_u32(most[c], most[QB + c]), max_u32(most[2 * QB + c], most[3 * QB + c]));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            BlockScale s = one;
+            if constexpr (!WIDE) {
+                s.template set<F8>(column[j]);
+                if (rg == 0 && c0 + j < cols) args.scale_t[(c0 + j) * args.blocks_r + tile_r] = s.scale;
+            }
+            u32x2 o;
+            o.x = pack_f8<F8>(s(value(0, j)), s(value(1, j)), s(value(2, j)), s(value(3, j)));
+            o.y = pack_f8<F8>(s(value(4, j)), s(value(5, j)), s(value(6, j)), s(value(7, j)));
+            *reinterpret_cast<u32x2*>(turned + (cg * 8 + j) * PITCH + rg * 8) = o;
+        }
+        __syncthreads();
+        // 16 bytes per lane: eight lanes a row of 128 bytes, 32 rows at a time
+        const long at = tile_r * QB + (tid & 7) * 16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = k * 32 + (tid >> 3);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(turned + c * PITCH + (tid & 7) * 16);
+            if (tile_c * QB + c < cols && at < args.pitch_t) *reinterpret_cast<u32x4*>(args.q_t + (tile_c * QB + c) * args.pitch_t + at) = v;
+        }
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------
+
+template <int DT, int F8, bool WIDE, int OUT, int R>
+static int launch_quantize(const QuantArgs& a, hipStream_t stream) {
+    const long tiles = ((a.rows + 16 * R - 1) / (16 * R)) * a.blocks_c;
+    if (tiles * 256 >= 1l << 32) return fail(SP_ERR_SHAPE, "sp_quantize_blocks: too large");
+    hipLaunchKernelGGL((quantize_kernel<DT, F8, WIDE, OUT, R>), dim3((unsigned)tiles), dim3(256), 0, stream, a.x, a.rows, a.cols, a);
+    return check_launch("sp_quantize_blocks");
+}
+
+template <int DT, int F8>
+static int quantize(const QuantArgs& a, bool wide, hipStream_t stream) {
+    const int out = (a.q != nullptr ? 1 : 0) | (a.q_t != nullptr ? 2 : 0);
+    if (wide) {
+        if (out == 1) return launch_quantize<DT, F8, true, 1, 8>(a, stream);
+        if (out == 2) return launch_quantize<DT, F8, true, 2, 8>(a, stream);
+        return launch_quantize<DT, F8, true, 3, 8>(a, stream);
+    }
+    if (out == 1) return launch_quantize<DT, F8, false, 1, 1>(a, stream);
+    if (out == 2) return launch_quantize<DT, F8, false, 2, 8>(a, stream);
+    return launch_quantize<DT, F8, false, 3, 8>(a, stream);
+}
+
+namespace {
+struct QuantizeKernelNames {
+    QuantizeKernelNames() {
+        register_kernel("quantize_rows", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 1, 1>, 256);
+        register_kernel("quantize_both", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 3, 8>, 256);
+        register_kernel("quantize_both_128", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, true, 3, 8>, 256);
+    }
+} quantize_kernel_names;
+}  // namespace
+
+}  // namespace sp
+
+using namespace sp;
+
+extern "C" int sp_quantize_blocks(int dtype, int f8, int32_t block_rows, const void* x, void* q, float* scale, void* q_t, float* scale_t,
+                                  int64_t rows, int64_t cols, void* stream) {
+    SP_REQUIRE_PTR(x);
+    SP_OPTIONAL_PTR(q);
+    SP_OPTIONAL_PTR(scale);
+    SP_OPTIONAL_PTR(q_t);
+    SP_OPTIONAL_PTR(scale_t);
+    if (q == nullptr && q_t == nullptr) return fail(SP_ERR_NULL, "sp_quantize_blocks: q and q_t are NULL");
+    if ((q == nullptr) != (scale == nullptr) || (q_t == nullptr) != (scale_t == nullptr))
+        return fail(SP_ERR_NULL, "sp_quantize_blocks: numbers and their scales go together");
+    if (dtype != SP_F32 && dtype != SP_F16 && dtype != SP_BF16) return fail(SP_ERR_DTYPE, "sp_quantize_blocks: dtype must be f32, f16 or bf16, got %d", dtype);
+    if (f8 != SP_F8_E4M3 && f8 != SP_F8_E5M2) return fail(SP_ERR_DTYPE, "sp_quantize_blocks: f8 must be e4m3 or e5m2, got %d", f8);
+    if (block_rows != 1 && block_rows != QB) return fail(SP_ERR_ARG, "sp_quantize_blocks: blocks have 1 or 128 rows, got %d", block_rows);
+    if (rows <= 0 || cols <= 0) return fail(SP_ERR_SHAPE, "sp_quantize_blocks: rows and cols must be positive (got %lld, %lld)", (long long)rows, (long long)cols);
+    if (rows > (int64_t)1 << 31 || cols > (int64_t)1 << 31) return fail(SP_ERR_SHAPE, "sp_quantize_blocks: too large");
+    const int rc = require_gfx950(__func__);
+    if (rc != SP_OK) return rc;
+    QuantArgs a{};
+    a.x = x; a.q = (unsigned char*)q; a.q_t = (unsigned char*)q_t; a.scale = scale; a.scale_t = scale_t; a.rows = rows; a.cols = cols;
+    a.pitch = (cols + 15) / 16 * 16; a.pitch_t = (rows + 15) / 16 * 16;
+    a.blocks_c = (cols + QB - 1) / QB; a.blocks_r = (rows + QB - 1) / QB;
+    const bool wide = block_rows == QB;
+    auto by_f8 = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return f8 == SP_F8_E4M3 ? quantize<DT, SP_F8_E4M3>(a, wide, (hipStream_t)stream) : quantize<DT, SP_F8_E5M2>(a, wide, (hipStream_t)stream);
+    };
+    if (dtype == SP_F32) return by_f8(std::integral_constant<int, SP_F32>{});
+    if (dtype == SP_F16) return by_f8(std::integral_constant<int, SP_F16>{});
+    return by_f8(std::integral_constant<int, SP_BF16>{});
+}

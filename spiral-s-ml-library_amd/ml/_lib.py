@@ -12,6 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SPIRAL_MI355_LIB") or os.path.join(os.path.dirname(_HERE), "libspiral_mi355.so")
 
 SP_F32, SP_F16, SP_BF16 = 0, 1, 2
+SP_F8_E4M3, SP_F8_E5M2 = 8, 9
 GEMM_RELU, GEMM_FORCE_GENERIC = 0x1, 0x100
 (ROW_IDENTITY, ROW_SOFTMAX, ROW_MASKED_SOFTMAX, ROW_LN_L2, ROW_REGRET_MATCHING, ROW_MASKED_REGRET_MATCHING,
  ROW_INCLUSIVE_SCAN, ROW_EXCLUSIVE_SCAN) = range(8)
@@ -97,6 +98,13 @@ SIGNATURES = {
     "sp_stack_forward_f32": (C.c_int, [_P, _I32, C.POINTER(_P), C.POINTER(C.c_int32), C.POINTER(C.c_int32), _I32, _P,
                                        C.POINTER(PhiloxConfig), _P, _P, _I64, _I32, _I32, _P]),
     "sp_stack_forward_takes": (C.c_int, [_I32, C.POINTER(C.c_int32), _I32, _I64, _I32, _I32]),
+    "sp_layer_norm": (C.c_int, [C.c_int, C.c_int] + [_P] * 6 + [_I64, _I64, _F, _P]),
+    "sp_layer_norm_backward": (C.c_int, [C.c_int, C.c_int] + [_P] * 8 + [_I64, _I64, _P, _I64, _P]),
+    "sp_layer_norm_backward_workspace_bytes": (C.c_int64, [_I64, _I64]),
+    "sp_logits_penalize": (C.c_int, [C.c_int] + [_P] * 6 + [_I64] + [_P] * 6 + [_I64, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    "sp_logits_penalize_workspace_bytes": (C.c_int64, [_I64, _I64]),
+    "sp_quantize_blocks": (C.c_int, [C.c_int, C.c_int, _I32] + [_P] * 5 + [_I64, _I64, _P]),
+    "sp_gemm_abt_scaled": (C.c_int, [C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _F, _U32, _P]),
     "sp_ensemble_binarize": (C.c_int, [C.c_int, _P, _P, _P, _I32, _I64, _I32, _I32, _U32, _P]),
 }
 
@@ -186,6 +194,7 @@ def stream_ptr():
 
 
 DTYPES = {torch.float32: SP_F32, torch.float16: SP_F16, torch.bfloat16: SP_BF16}
+F8_TYPES = {torch.float8_e4m3fn: SP_F8_E4M3, torch.float8_e5m2: SP_F8_E5M2}
 
 
 # ptr(t, dtype=None, name="tensor"): device pointer of a contiguous ROCm tensor, an integer (None passes through as NULL).

@@ -81,6 +81,107 @@ def matmul_abt_batched(a, b, c=None, alpha=1.0, beta=0.0, bias=None, relu=False,
     return c
 
 
+def _blocks(n):
+    return -(-n // 128)
+
+
+def _on_device_of(what, *tensors):
+    """The device index all of `tensors` (None passed over) live on: a launch on another device than theirs would read foreign memory."""
+    index = None
+    for t in tensors:
+        if t is not None and t.is_cuda:
+            if index is None:
+                index = t.device.index
+            elif t.device.index != index:
+                raise ValueError("%s: the tensors live on different devices" % what)
+    return index
+
+
+def quantize_blocks(x, block=(1, 128), dtype=torch.float8_e4m3fn, transpose=False):
+    """x (rows, cols) f32, f16 or bf16 in 8-bit blocks with an f32 scale each (sp_quantize_blocks): (q, scale), the operand of
+    `matmul_abt_scaled`.  `block` is (1, 128), for activations, or (128, 128), for weights; a block's scale is its largest magnitude over the
+    type's largest number.  q is (rows, cols rounded up to a multiple of 16), zeros behind the columns of x; scale (rows or ceil(rows / 128),
+    ceil(cols / 128)).  transpose=True gives the same of the transpose of x, transpose="both" reads x once and gives
+    (q, scale, q_t, scale_t): what a layer's forward product and the gradients of its input (weights) or its weights (activations) take."""
+    if x.dim() != 2:
+        raise ValueError("x must be 2-D")
+    if x.dtype not in _lib.DTYPES:
+        raise TypeError("x must be f32, f16 or bf16, got %s" % x.dtype)
+    if dtype not in _lib.F8_TYPES:
+        raise TypeError("dtype must be torch.float8_e4m3fn or torch.float8_e5m2, got %s" % dtype)
+    block = tuple(block)
+    if block not in ((1, 128), (128, 128)):
+        raise ValueError("block must be (1, 128) or (128, 128), got %r" % (block,))
+    if transpose not in (False, True, "both"):
+        raise ValueError("transpose must be False, True or \"both\", got %r" % (transpose,))
+    rows, cols = x.shape
+    if rows == 0 or cols == 0:
+        raise ValueError("x must not be empty, got %d x %d" % (rows, cols))
+    address = ptr(x, name="x")
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return quantize_blocks(x, block, dtype, transpose)
+    out = []
+    for r, c, wanted in ((rows, cols, transpose is not True), (cols, rows, transpose is not False)):
+        if wanted:
+            out += [torch.empty((r, (c + 15) // 16 * 16), dtype=dtype, device=x.device),
+                    torch.empty((r if block[0] == 1 else _blocks(r), _blocks(c)), dtype=torch.float32, device=x.device)]
+        else:
+            out += [None, None]
+    check(lib.sp_quantize_blocks(_lib.DTYPES[x.dtype], _lib.F8_TYPES[dtype], block[0], address, ptr(out[0]), ptr(out[1]), ptr(out[2]),
+                                 ptr(out[3]), rows, cols, stream_ptr()))
+    return tuple(t for t in out if t is not None)
+
+
+def matmul_abt_scaled(a, scale_a, b, scale_b, c=None, beta=0.0, bias=None, relu=False, out_dtype=None):
+    """C = A . B^T + beta * C (+ bias, ReLU) of 8-bit operands with a scale for each block of 128 along K (sp_gemm_abt_scaled): the
+    numbers a (M, K), b (N, K), e4m3 or e5m2, and their scales as `quantize_blocks` gives them.  scale_a is (M, ceil(K / 128)), scale_b
+    (N, ceil(K / 128)) or, in blocks of 128 x 128, (ceil(N / 128), ceil(K / 128)).  `c` (f32, f16 or bf16) is updated in place and returned; when it
+    is None a new (M, N) tensor of `out_dtype` (default f32) is allocated by torch (beta must then be 0).  Sums are f32.
+
+    A layer y = x . W^T and its gradients, with dy, x and W of M x N, M x K and N x K:
+        x8, sx, xt, sxt = quantize_blocks(x, transpose="both");  w8, sw, wt, swt = quantize_blocks(W, (128, 128), transpose="both")
+        d8, sd, dt, sdt = quantize_blocks(dy, dtype=torch.float8_e5m2, transpose="both")
+        y = matmul_abt_scaled(x8, sx, w8, sw);  dx = matmul_abt_scaled(d8, sd, wt, swt);  dW = matmul_abt_scaled(dt, sdt, xt, sxt)
+    (with N, K and M multiples of 16; otherwise the padding of q shows in the widths of what they are multiplied with)."""
+    if a.dim() != 2 or b.dim() != 2 or scale_a.dim() != 2 or scale_b.dim() != 2:
+        raise ValueError("a, b and their scales must be 2-D")
+    if a.dtype not in _lib.F8_TYPES or b.dtype not in _lib.F8_TYPES:
+        raise TypeError("a and b must be torch.float8_e4m3fn or torch.float8_e5m2, got %s and %s" % (a.dtype, b.dtype))
+    m, k = a.shape
+    n, kb = b.shape
+    assert k == kb, "The K dimension of the A and B tensors must match."
+    if tuple(scale_a.shape) != (m, _blocks(k)):
+        raise ValueError("scale_a must be (M, ceil(K / 128)) = (%d, %d), got %s" % (m, _blocks(k), tuple(scale_a.shape)))
+    if tuple(scale_b.shape) not in ((n, _blocks(k)), (_blocks(n), _blocks(k))):
+        raise ValueError("scale_b must be (N, ceil(K / 128)) = (%d, %d) or (ceil(N / 128), ceil(K / 128)) = (%d, %d), got %s"
+                         % (n, _blocks(k), _blocks(n), _blocks(k), tuple(scale_b.shape)))
+    if c is None:
+        assert beta == 0.0, "beta != 0 needs an existing C"
+        out = out_dtype or torch.float32
+    else:
+        assert tuple(c.shape) == (m, n), "The dimensions of the C tensor must be (M, N)."
+        out = c.dtype
+        if out_dtype is not None and out_dtype != out:
+            raise TypeError("out_dtype is %s, c is %s" % (out_dtype, out))
+    if out not in _lib.DTYPES:
+        raise TypeError("C must be f32, f16 or bf16, got %s" % out)
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError("bias must be (N,) = (%d,), got %s" % (n, tuple(bias.shape)))
+    addresses = (ptr(a, name="a"), ptr(scale_a, torch.float32, "scale_a"), ptr(b, name="b"), ptr(scale_b, torch.float32, "scale_b"))
+    bias_at = ptr(bias, torch.float32, "bias")
+    device = _on_device_of("matmul_abt_scaled", a, scale_a, b, scale_b, c, bias)
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return matmul_abt_scaled(a, scale_a, b, scale_b, c, beta, bias, relu, out_dtype)
+    if c is None:
+        c = torch.empty((m, n), dtype=out, device=a.device)
+    check(lib.sp_gemm_abt_scaled(_lib.F8_TYPES[a.dtype], _lib.F8_TYPES[b.dtype], _lib.DTYPES[out], *addresses,
+                                 1 if scale_b.shape[0] == n else 128, ptr(c, name="c"), bias_at, m, n, k, float(beta),
+                                 _lib.GEMM_RELU if relu else 0, stream_ptr()))
+    return c
+
+
 def _transposed(x):
     """Materialise x^T with the library's transpose kernel (4-byte elements only)."""
     if x.dtype != torch.float32:

@@ -235,6 +235,150 @@ def binarize(x, modulo, out=None):
     return out
 
 
+def _one_device(what, *tensors):
+    """The device index of `tensors` (None passed over), which have to share it: a launch runs on one device."""
+    index = tensors[0].device.index
+    for t in tensors[1:]:
+        if t is not None and t.device.index != index:
+            raise ValueError("%s: the tensors live on different devices" % what)
+    return index
+
+
+def _norm_weights(x, cols, weight, bias):
+    """(the code of their type, weight's address, bias' address): of x's type or f32, (cols,) each."""
+    dtype = None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if tuple(t.shape) != (cols,):
+            raise ValueError("%s must be (%d,), got %s" % (name, cols, tuple(t.shape)))
+        if t.dtype != torch.float32 and t.dtype != x.dtype:
+            raise TypeError("%s must be f32 or %s, got %s" % (name, x.dtype, t.dtype))
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError("weight and bias must have one dtype, got %s and %s" % (dtype, t.dtype))
+        dtype = t.dtype
+    return _lib.DTYPES[dtype or torch.float32], ptr(weight, name="weight"), ptr(bias, name="bias")
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None, want_stats=False):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the innermost dimension (sp_layer_norm), next to `ln_l2`, the norm without a mean
+    (ml/primitives.spi:701-703).  x: f32, f16 or bf16 with rows of any length up to 16384; the result has its type, `out` may be x.  weight,
+    bias: (cols,), f32 or of x's type, or None.  Statistics are f32; want_stats=True also returns each row's mean and 1 / sqrt(var + eps),
+    which `layer_norm_backward` takes: (y, mean, rstd)."""
+    if x.dtype not in _lib.DTYPES:
+        raise TypeError("layer_norm takes f32, f16 or bf16 tensors, got %s" % x.dtype)
+    rows, cols = _rows_cols(x)
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+        raise ValueError("out must have the shape and type of x")
+    code, weight_at, bias_at = _norm_weights(x, cols, weight, bias)
+    x_at = ptr(x, name="x")
+    if _one_device("layer_norm", x, weight, bias, out) != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return layer_norm(x, weight, bias, eps, out, want_stats)
+    y = torch.empty_like(x) if out is None else out
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) for _ in range(2))
+    check(lib.sp_layer_norm(_lib.DTYPES[x.dtype], code, x_at, weight_at, bias_at, ptr(y, name="out"), ptr(mean), ptr(rstd), rows, cols,
+                            float(eps), stream_ptr()))
+    return (y, mean, rstd) if want_stats else y
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None, want_weight_grads=True):
+    """The gradients of `layer_norm` (sp_layer_norm_backward): (dx, dweight, dbias) from dy and the x, mean and rstd of the forward call.
+    dx has x's type (`out` may be dy), dweight and dbias are f32, summed over all rows in an order that depends on the sizes alone; they are None with
+    want_weight_grads=False."""
+    if x.dtype not in _lib.DTYPES:
+        raise TypeError("layer_norm_backward takes f32, f16 or bf16 tensors, got %s" % x.dtype)
+    rows, cols = _rows_cols(x)
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have the shape and type of x")
+    if mean.shape != x.shape[:-1] or rstd.shape != x.shape[:-1]:
+        raise ValueError("mean and rstd must have one entry per row")
+    if out is not None and (out.shape != x.shape or out.dtype != x.dtype):
+        raise ValueError("out must have the shape and type of x")
+    code, weight_at, _ = _norm_weights(x, cols, weight, None)
+    addresses = ptr(dy, name="dy"), ptr(x, name="x"), ptr(mean, torch.float32, "mean"), ptr(rstd, torch.float32, "rstd")
+    if _one_device("layer_norm_backward", x, dy, mean, rstd, weight, out) != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return layer_norm_backward(dy, x, mean, rstd, weight, out, want_weight_grads)
+    dx = torch.empty_like(x) if out is None else out
+    dweight = dbias = workspace = None
+    bytes_ = 0
+    if want_weight_grads:
+        dweight, dbias = (torch.empty((cols,), dtype=torch.float32, device=x.device) for _ in range(2))
+        bytes_ = lib.sp_layer_norm_backward_workspace_bytes(rows, cols)
+        workspace = torch.empty((max(bytes_, 16),), dtype=torch.uint8, device=x.device)   # of this call alone: calls may overlap
+    check(lib.sp_layer_norm_backward(_lib.DTYPES[x.dtype], code, *addresses, weight_at, ptr(dx, name="out"), ptr(dweight), ptr(dbias), rows,
+                                     cols, ptr(workspace), bytes_, stream_ptr()))
+    return dx, dweight, dbias
+
+
+def penalize_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repetition=None, presence=None, frequency=None,
+                    temperature=None, bias_ids=None, bias=None, mask=None, out=None, want_token=False):
+    """Logits (..., cols) of any length before a token is chosen (sp_logits_penalize), next to `masked_softmax` and `argmax`, whose masks are
+    a prefix of a short row.  In f32 and in this order: tokens of the row's history are divided (positive logits) or multiplied by
+    `repetition`; `frequency` times their count and, once, `presence` are subtracted for those behind the prompt; biases are added; what
+    is left is divided by `temperature` (where it is above 0) and becomes -inf where the mask's bit is 0.
+
+    logits: f32, f16 or bf16; the result is f32 (`out` may be f32 logits).  tokens: (..., history) i32, of which the first lengths (...,) i32
+    count and the first prompt_lengths (...,) i32 are the prompt's; ids outside the row are passed over, so -1 pads.
+    repetition, presence, frequency, temperature: (...,) f32.  bias_ids (..., n) i32 with bias (..., n) f32, n <= 2047; of an
+    id that stands twice both count.  mask: (..., ceil(cols / 32)) i32, or one row of it for all; bit j % 32 of word j // 32 allows j.  Every
+    one may be None.  want_token=True also returns the (...,) i32 index of each row's largest result, the lowest of equal ones, -1 for a
+    row that has none above -inf."""
+    if logits.dtype not in _lib.DTYPES:
+        raise TypeError("penalize_logits takes f32, f16 or bf16 logits, got %s" % logits.dtype)
+    rows, cols = _rows_cols(logits)
+    lead = logits.shape[:-1]
+    if out is not None and (out.shape != logits.shape or out.dtype != torch.float32):
+        raise ValueError("out must have the shape of the logits and be f32")
+    if out is not None and logits.dtype != torch.float32 and out.data_ptr() == logits.data_ptr():
+        raise ValueError("only f32 logits can be overwritten")
+    for t, name in ((lengths, "lengths"), (prompt_lengths, "prompt_lengths"), (repetition, "repetition"), (presence, "presence"),
+                    (frequency, "frequency"), (temperature, "temperature")):
+        if t is not None and t.shape != lead:
+            raise ValueError("%s must have one entry per row" % name)
+    if tokens is not None and (tokens.dim() != logits.dim() or tokens.shape[:-1] != lead):
+        raise ValueError("tokens must be (..., history) with the rows of the logits")
+    if tokens is None and (lengths is not None or prompt_lengths is not None):
+        raise ValueError("lengths and prompt_lengths need tokens")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias go together")
+    if bias is not None and (bias_ids.shape != bias.shape or bias.dim() != logits.dim() or bias.shape[:-1] != lead):
+        raise ValueError("bias_ids and bias must be (..., n) with the rows of the logits")
+    words = -(-cols // 32)
+    mask_rows = 0
+    if mask is not None:
+        if mask.dim() == 0 or mask.shape[-1] != words or mask.numel() not in (words, rows * words):
+            raise ValueError("mask must be (..., %d) with the rows of the logits, or one row" % words)
+        mask_rows = mask.numel() // words
+    history = tokens.shape[-1] if tokens is not None else 0
+    n_bias = bias.shape[-1] if bias is not None else 0
+    i32, f32 = torch.int32, torch.float32
+    before = (ptr(tokens, i32, "tokens") if history else None, ptr(lengths, i32, "lengths"), ptr(prompt_lengths, i32, "prompt_lengths"), history,
+              ptr(repetition, f32, "repetition"), ptr(presence, f32, "presence"), ptr(frequency, f32, "frequency"),
+              ptr(temperature, f32, "temperature"), ptr(bias_ids, i32, "bias_ids") if n_bias else None, ptr(bias, f32, "bias") if n_bias else None,
+              n_bias, ptr(mask, i32, "mask"), mask_rows)
+    logits_at = ptr(logits, name="logits")
+    if _one_device("penalize_logits", logits, out, tokens, lengths, prompt_lengths, repetition, presence, frequency, temperature, bias_ids,
+                   bias, mask) != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return penalize_logits(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, temperature, bias_ids, bias,
+                                   mask, out, want_token)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    token = workspace = None
+    bytes_ = 0
+    if want_token:
+        token = torch.empty(lead, dtype=torch.int32, device=logits.device)
+        bytes_ = lib.sp_logits_penalize_workspace_bytes(rows, cols)
+        workspace = torch.empty((bytes_,), dtype=torch.uint8, device=logits.device)       # of this call alone: calls may overlap
+    check(lib.sp_logits_penalize(_lib.DTYPES[logits.dtype], logits_at, ptr(out, name="out"), ptr(token), *before, rows, cols, ptr(workspace),
+                                 bytes_, stream_ptr()))
+    return (out, token) if want_token else out
+
+
 def cem_update_rewards_mask(rewards, mask=None):
     """`grid_update_rewards_mask` (ml/cem.spi:92-96): rewards (ensemble, 2) f32 (reward sum, count) pairs are
     turned into the winners' mask (average reward at or above the ensemble's mean) and zeroed."""
