@@ -127,20 +127,35 @@ __device__ __forceinline__ void scaled_tile_of_block(int pid, int tiles_m, int t
     tn = in / rows;
 }
 
-// 64 scales, four bytes a lane, like dma_to_lds.
-__device__ __forceinline__ void dma4_to_lds(const unsigned char* base, unsigned lane_offset, unsigned lds_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(lane_offset), "s"(base), "s"(lds_addr) : "memory", "m0");
+// Scales come in for eight blocks of K at a time, eight rows per instruction: 32 bytes of a row lie side by side, so that a load asks for eight
+// lines of memory and not for 64 (one block at a time they are as many lines as the operands: 8192^3 517 us against SCALES_US).
+constexpr int SCALE_BLOCKS = 8;
+
+// Lane l's scale is that of row l / 8 and block l % 8 of what `row` and `first` say; to LDS bytes lds_addr + 4 l.
+__device__ __forceinline__ void dma_scales(const float* scales, long row, long last_row, long first, long blocks, int lane, unsigned lds_addr) {
+    const long r = row + (lane >> 3) < last_row ? row + (lane >> 3) : last_row, k = first + (lane & 7) < blocks ? first + (lane & 7) : blocks - 1;
+    const float* at = scales + r * blocks + k;
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(at), "s"(lds_addr) : "memory", "m0");
 }
 
-// Tiles of BM x BN on WM x WN waves, two stages of LDS: tile kt + 1 comes in while tile kt is multiplied.  SHIFT: 7 where a scale of B
-// holds for 128 rows, else 0.
+// 16-byte chunk kc of row `row` of a tile in LDS stands in slot kc ^ f(row) of the row: the 16 rows that one read of a fragment touches lie in
+// different banks, and every fragment has the same pattern, so fragments of an operand are apart by immediates.
+__device__ __forceinline__ int tile_slot(int row, int kc) { return (kc ^ row ^ (row >> 3 & 1)) & 7; }
+
+// Tiles of BM x BN on WM x WN waves, two stages of LDS.  SHIFT: 7 where a scale of B holds for 128 rows, else 0.
+//
+// A wave walks its TM rows of fragments.  While row i is on the matrix pipe, the vector ALU adds the scaled sums of row i - 1 and the fragment of row i + 1 comes
+// in from LDS.  The boundary between two blocks of K stands in front of a block's last row: by then everything of the
+// block is in registers, the next block has landed (it was asked for a whole block earlier), the block after that is asked for, and behind each MFMA of the last row
+// the next block's fragment of B takes the place of the one just used.
 template <int F8A, int F8B, bool FAST, int SHIFT, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM* WN * 64) void gemm_scaled_tile_kernel(const ScaledArgs g) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const ScaledArgs g) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
-    constexpr int NIA = BM / 8 / NW, NI = (BM + BN) / 8 / NW;       // DMA instructions of 8 rows per wave and K-tile; A's first
-    constexpr int SCALES = (BM + BN) / 64;                          // and of 64 scales per workgroup
-    static_assert(SCALES == NW, "one instruction of scales per wave");
-    constexpr int TILE_BYTES = (BM + BN) * ROW_BYTES, STAGE = TILE_BYTES + (BM + BN) * 4;
+    constexpr int NIA = BM / 8 / NW, NI = (BM + BN) / 8 / NW;       // DMA instructions of 8 rows per wave and block; A's first
+    constexpr int GROUPS_A = BM / 8, GROUPS = GROUPS_A + (SHIFT == 7 ? 1 : BN / 8);      // of eight rows of scales; B's behind A's
+    static_assert(GROUPS <= SCALE_BLOCKS * NW && NW % 2 == 0 && TM % 2 == 0, "one instruction of scales per wave and block");
+    constexpr int STAGE = (BM + BN) * ROW_BYTES, SCALE_STAGE = GROUPS * 256;
+    static_assert(2 * (STAGE + SCALE_STAGE) <= 160 * 1024, "LDS");
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, fi = lane & 15, fq = lane >> 4;
@@ -150,183 +165,278 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_scaled_tile_kernel(const Sca
     const int nk = (int)g.blocks;
     const bool k_tail = (g.K & 127) != 0;
 
-    // operands: rows past the end are the last row again, chunks past the end of a row zeros
+    // operands: instruction q of a wave takes rows (q NW + wave) 8 ... of A's or B's part of the tile, a lane 16 bytes of one of them.  Rows past the
+    // end are the last row again: the offset of a row stops at that row's.  Chunks past the end of a row are zeros.
     const unsigned char* pA = uniform_ptr(g.A + m0 * g.K);
     const unsigned char* pB = uniform_ptr(g.B + n0 * g.K);
-    const unsigned lds_base = (unsigned)(size_t)lds;
-    unsigned voff[NI], dst[NI], tail_in = 0;
-#pragma unroll
-    for (int q = 0; q < NI; ++q) {
-        const bool is_a = q < NIA;
-        const int blk = (is_a ? q : q - NIA) * NW + wave, r = lane >> 3, kc = (lane & 7) ^ ((r ^ blk) & 7);
-        const long left = (is_a ? g.M - m0 : g.N - n0) - 1, row = blk * 8 + r < left ? blk * 8 + r : left;
-        voff[q] = (unsigned)(row * g.K) + kc * 16;
-        if ((long)(nk - 1) * ROW_BYTES + kc * 16 < g.K) tail_in |= 1u << q;
-        dst[q] = __builtin_amdgcn_readfirstlane(lds_base + ((is_a ? 0 : BM) + blk * 8) * ROW_BYTES);
-    }
-    // scales: position p of A's is row 16 (p % TM) + p / TM of a wave's rows, so that a lane reads its TM side by side
-    const bool scales_of_a = wave < BM / 64;
-    const int pos = (scales_of_a ? wave : wave - BM / 64) * 64 + lane;
-    const long left = (scales_of_a ? g.M - m0 : g.N - n0) - 1;
-    long srow = scales_of_a ? (long)(pos / WTM) * WTM + 16 * (pos % TM) + pos % WTM / TM : (long)pos;
-    srow = srow < left ? srow : left;
-    const unsigned char* pS;
-    unsigned soff;
-    if (scales_of_a) {
-        pS = uniform_ptr((const unsigned char*)(g.scale_a + m0 * g.blocks));
-        soff = (unsigned)(srow * g.blocks * 4);
-    } else {
-        pS = uniform_ptr((const unsigned char*)(g.scale_b + (n0 >> SHIFT) * g.blocks));
-        soff = (unsigned)((((n0 + srow) >> SHIFT) - (n0 >> SHIFT)) * g.blocks * 4);
-    }
-    const unsigned sdst = __builtin_amdgcn_readfirstlane(lds_base + TILE_BYTES + wave * 256);
-    auto fetch = [&](int kt) {
-        const unsigned stage = (kt & 1) * STAGE;
+    const unsigned K = (unsigned)g.K, lds_base = (unsigned)(size_t)lds;
+    const int r = lane >> 3, kc = tile_slot((wave & 1) * 8 + r, lane & 7);
+    const unsigned voff = (unsigned)(wave * 8 + r) * K + kc * 16;
+    const long left_a = g.M - m0 - 1, left_b = g.N - n0 - 1;
+    const unsigned last_a = (unsigned)(left_a < BM ? left_a : BM) * K + kc * 16, last_b = (unsigned)(left_b < BN ? left_b : BN) * K + kc * 16;
+    const bool tail_in = (long)(nk - 1) * ROW_BYTES + kc * 16 < g.K;
+    const unsigned dst = __builtin_amdgcn_readfirstlane(lds_base + wave * 8 * ROW_BYTES);
+    // scales: of the eight blocks from 8 c on, in stage c % 2; wave w brings its share (group `part` NW + w) once per block, a chunk ahead
+    const unsigned scale_lds = __builtin_amdgcn_readfirstlane(lds_base + 2 * STAGE);
+    const long last_sb = SHIFT == 7 ? (g.N - 1) >> 7 : g.N - 1;
+    auto fetch_scales = [&](int chunk, int part) {
+        const int group = part * NW + wave;
+        if (group >= GROUPS || chunk * SCALE_BLOCKS >= nk) return;
+        const bool of_a = group < GROUPS_A;
+        const unsigned to = scale_lds + (chunk & 1) * SCALE_STAGE + group * 256;
+        dma_scales(of_a ? g.scale_a : g.scale_b, of_a ? m0 + group * 8 : (n0 >> SHIFT) + (group - GROUPS_A) * 8, of_a ? g.M - 1 : last_sb,
+                   (long)chunk * SCALE_BLOCKS, nk, lane, to);
+    };
+    auto fetch = [&](int kt, unsigned stage) {
         const unsigned char *a = pA + (long)kt * ROW_BYTES, *b = pB + (long)kt * ROW_BYTES;
+        auto offset = [&](int q) {
+            const unsigned at = voff + (unsigned)(q < NIA ? q : q - NIA) * (NW * 8) * K, last = q < NIA ? last_a : last_b;
+            return at < last ? at : last;
+        };
+        auto to = [&](int q) { return dst + stage + (q < NIA ? q * NW * 8 : BM + (q - NIA) * NW * 8) * ROW_BYTES; };
         if (k_tail && kt == nk - 1) {
 #pragma unroll
             for (int q = 0; q < NI; ++q) {
-                const unsigned char* inside = (q < NIA ? a : b) + voff[q];
-                dma_to_lds_addr((tail_in >> q) & 1u ? inside : (const unsigned char*)kZeroChunk, dst[q] + stage);
+                const unsigned char* inside = (q < NIA ? a : b) + offset(q);
+                dma_to_lds_addr(tail_in ? inside : (const unsigned char*)kZeroChunk, to(q));
             }
         } else {
 #pragma unroll
-            for (int q = 0; q < NI; ++q) dma_to_lds(q < NIA ? a : b, voff[q], dst[q] + stage);
+            for (int q = 0; q < NI; ++q) dma_to_lds(q < NIA ? a : b, offset(q), to(q));
         }
-        dma4_to_lds(pS + (long)kt * 4, soff, sdst + stage);
     };
 
-    f32x4 acc[TM][TN];
+    // fragments: chunks 2 fq and 2 fq + 1 of a row
+    int at_a[2], at_b[2];
+    const int at_sa = 2 * STAGE + (wm * WTM + fi) * 32, at_sb = 2 * STAGE + GROUPS_A * 256 + (SHIFT == 7 ? (wn * WTN) >> 7 : wn * WTN + 4 * fq) * 32;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int h = 0; h < 2; ++h) {
+        const int in = fi * ROW_BYTES + (tile_slot(fi, 2 * fq + h) << 4);
+        at_a[h] = wm * WTM * ROW_BYTES + in;
+        at_b[h] = (BM + wn * WTN) * ROW_BYTES + in;
+    }
+    u32x4 ra[2][2], rb[TN][2];
+    auto load_a = [&](int i) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    fetch(0);
-    for (int kt = 0; kt < nk; ++kt) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                       // tile kt is there, and everybody has read tile kt - 1
-        if (kt + 1 < nk) fetch(kt + 1);
-        const unsigned char* at = lds + (kt & 1) * STAGE;
-        const float* scales = reinterpret_cast<const float*>(at + TILE_BYTES);
-        auto fragment = [&](auto& f, int row) {
-            u32x4 c[2];
+        for (int h = 0; h < 2; ++h) ra[i & 1][h] = *reinterpret_cast<const u32x4*>(lds + at_a[h] + i * 16 * ROW_BYTES);
+    };
+    auto load_b = [&](int j) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) c[h] = *reinterpret_cast<const u32x4*>(at + lds_offset(row, 2 * fq + h));
-            f.set(c);
-        };
-        Fragment<F8B, FAST> b[TN];
+        for (int h = 0; h < 2; ++h) rb[j][h] = *reinterpret_cast<const u32x4*>(lds + at_b[h] + j * 16 * ROW_BYTES);
+    };
+    float sa[TM], pending = 0.f;                       // pending: the scale of the row whose sums are still to be added
+    f32x4 sb[SHIFT == 7 ? 1 : TN], sb_pending[SHIFT == 7 ? 1 : TN];
+    auto load_scales = [&](int kt) {
+        const unsigned char* at = lds + (kt >> 3 & 1) * SCALE_STAGE + (kt & 7) * 4;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) fragment(b[j], BM + wn * WTN + 16 * j + fi);
-        float sa[TM];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) sa[i] = scales[wm * WTM + fi * TM + i];
-        f32x4 sb[TN];
+        for (int i = 0; i < TM; ++i) sa[i] = *reinterpret_cast<const float*>(at + at_sa + i * 512);
         if constexpr (SHIFT == 7) {
-            const float s = scales[BM + wn * WTN];
-#pragma unroll
-            for (int i = 0; i < TM; ++i) sa[i] *= s;
+            sb[0][0] = *reinterpret_cast<const float*>(at + at_sb);
         } else {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) sb[j] = *reinterpret_cast<const f32x4*>(scales + BM + wn * WTN + 16 * j + 4 * fq);
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sb[j][e] = *reinterpret_cast<const float*>(at + at_sb + (16 * j + e) * 32);
         }
+    };
+    f32x4 acc[TM][TN], sums[2][TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        sums[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (SHIFT != 7) sb_pending[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    auto add = [&](int i, int j, float scale, const f32x4& scale_n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float t = SHIFT == 7 ? sums[i & 1][j][e] : sums[i & 1][j][e] * scale_n[e];
+            acc[i][j][e] = __builtin_fmaf(t, scale, acc[i][j][e]);
+        }
+        asm volatile("" : "+v"(acc[i][j]));            // here, not where the loop ends: that is where the compiler would gather them
+    };
+
+    for (int part = 0; part < SCALE_BLOCKS; ++part) fetch_scales(0, part);
+    fetch(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    fetch_scales(1, 0);
+    fetch(nk > 1 ? 1 : 0, STAGE);                      // (past the last block the last one comes again, into a stage that is not read: no branch)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) load_b(j);
+    load_a(0);
+    load_scales(0);
+    int step = STAGE;
+    Fragment<F8B, FAST> fb[TN];
+    for (int kt = 0; kt < nk; ++kt) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            Fragment<F8A, FAST> a;
-            fragment(a, wm * WTM + 16 * i + fi);
+            const bool boundary = i == TM - 1;
+            if (!boundary) {
+                load_a(i + 1);
+            } else {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __syncthreads();
+                fetch_scales((kt + 1) / SCALE_BLOCKS + 1, (kt + 1) % SCALE_BLOCKS);
+                fetch(kt + 2 < nk ? kt + 2 : nk - 1, step > 0 ? 0 : STAGE);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) at_a[h] += step, at_b[h] += step;
+                step = -step;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            Fragment<F8A, FAST> fa;
+            fa.set(ra[i & 1]);
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-                const f32x4 t = block_sum<F8A, F8B, FAST>(b[j], a);
+                if (i == 0) fb[j].set(rb[j]);
+                sums[i & 1][j] = block_sum<F8A, F8B, FAST>(fb[j], fa);
+                if (i == 0) add(TM - 1, j, pending, sb_pending[SHIFT == 7 ? 0 : j]);
+                else add(i - 1, j, sa[i - 1], sb[SHIFT == 7 ? 0 : j]);
+                if (boundary) load_b(j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (i == 0) {
+                if constexpr (SHIFT == 7)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], SHIFT == 7 ? sa[i] : sa[i] * sb[j][e], acc[i][j][e]);
+                    for (int k = 0; k < TM; ++k) sa[k] *= sb[0][0];
+            }
+            if (boundary) {
+                pending = sa[TM - 1];
+                if constexpr (SHIFT != 7)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) sb_pending[j] = sb[j];
+                load_a(0);
+                load_scales(kt + 1);
             }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < TN; ++j) add(TM - 1, j, pending, sb_pending[SHIFT == 7 ? 0 : j]);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) put_quad(g, m0 + wm * WTM + 16 * i + fi, n0 + wn * WTN + 16 * j + 4 * fq, acc[i][j]);
 }
 
-// One tile of (16 TM) x (16 TN) on KS waves; wave w takes blocks w, w + KS, ... of K, U of them at a time under way.
-template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int KS, int U>
-__global__ __launch_bounds__(KS * 64) void gemm_scaled_split_kernel(const ScaledArgs g) {
+// One tile of (16 TM) x (16 TN) outputs on four waves: each takes a quarter of K through an LDS ring of NS stages of its own, so no
+// wave waits for another inside the loop, and the four partial sums meet in LDS at the end.  All that is read comes in by DMA, the scales too.
+template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int NS>
+__global__ __launch_bounds__(256) void gemm_scaled_split_kernel(const ScaledArgs g) {
+    constexpr int KS = 4;
+    constexpr int NIA = 2 * TM, ND = 2 * (TM + TN);     // DMA instructions per block
+    constexpr int GROUPS_A = 2 * TM, GROUPS = GROUPS_A + (SHIFT == 7 ? 1 : 2 * TN);       // of eight rows of scales
+    constexpr int STAGE = ND * 8 * ROW_BYTES, WAVE_LDS = NS * STAGE + 2 * GROUPS * 256;
+    static_assert((NS - 1) * ND < 64 && NS < SCALE_BLOCKS, "vmcnt counts to 63; scales are asked for a chunk ahead of their operands");
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fi = lane & 15, fq = lane >> 4;
     int tm, tn;
     scaled_tile_of_block(blockIdx.x, g.tiles_m, g.tiles_n, g.group_m, tm, tn);
     const long m0 = (long)tm * (16 * TM), n0 = (long)tn * (16 * TN);
-    const unsigned char *rowA[TM], *rowB[TN];
-    const float *rowSA[TM], *rowSB[TN][SHIFT == 7 ? 1 : 4];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const long row = m0 + 16 * i + fi < g.M ? m0 + 16 * i + fi : g.M - 1;
-        rowA[i] = g.A + row * g.K + fq * 32;
-        rowSA[i] = g.scale_a + row * g.blocks;
-    }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const long row = n0 + 16 * j + fi < g.N ? n0 + 16 * j + fi : g.N - 1;
-        rowB[j] = g.B + row * g.K + fq * 32;
-#pragma unroll
-        for (int e = 0; e < (SHIFT == 7 ? 1 : 4); ++e) {
-            const long mine = SHIFT == 7 ? n0 + 16 * j : n0 + 16 * j + 4 * fq + e;
-            rowSB[j][e] = g.scale_b + ((mine < g.N ? mine : g.N - 1) >> SHIFT) * g.blocks;
-        }
-    }
     const int nk = (int)g.blocks;
+    const bool k_tail = (g.K & 127) != 0;
+    const unsigned char* pA = uniform_ptr(g.A + m0 * g.K);
+    const unsigned char* pB = uniform_ptr(g.B + n0 * g.K);
+    const unsigned my_lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds + wave * WAVE_LDS);
+    const int r = lane >> 3;
+    unsigned voff[ND], tail_in = 0;
+#pragma unroll
+    for (int q = 0; q < ND; ++q) {
+        const int blk = q < NIA ? q : q - NIA, kc = (lane & 7) ^ ((r ^ blk) & 7);
+        const long left = (q < NIA ? g.M - m0 : g.N - n0) - 1, row = blk * 8 + r < left ? blk * 8 + r : left;
+        voff[q] = (unsigned)(row * g.K) + kc * 16;
+        if ((long)(nk - 1) * ROW_BYTES + kc * 16 < g.K) tail_in |= 1u << q;
+    }
+    // this wave's blocks: an even share, one after the other
+    const int first = (int)((long)nk * wave / KS), mine = (int)((long)nk * (wave + 1) / KS) - first;
+    const long last_sb = SHIFT == 7 ? (g.N - 1) >> 7 : g.N - 1;
+    auto fetch_scales = [&](int chunk) {
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) {
+            const bool of_a = q < GROUPS_A;
+            dma_scales(of_a ? g.scale_a : g.scale_b, of_a ? m0 + q * 8 : (n0 >> SHIFT) + (q - GROUPS_A) * 8, of_a ? g.M - 1 : last_sb,
+                       (long)first + chunk * SCALE_BLOCKS, nk, lane, my_lds + NS * STAGE + ((chunk & 1) * GROUPS + q) * 256);
+        }
+    };
+    auto fetch = [&](int kt, unsigned stage) {
+        const unsigned char *a = pA + (long)kt * ROW_BYTES, *b = pB + (long)kt * ROW_BYTES;
+        const unsigned dst = my_lds + stage * STAGE;
+        if (k_tail && kt == nk - 1) {
+#pragma unroll
+            for (int q = 0; q < ND; ++q) {
+                const unsigned char* inside = (q < NIA ? a : b) + voff[q];
+                dma_to_lds_addr((tail_in >> q) & 1u ? inside : (const unsigned char*)kZeroChunk, dst + q * 8 * ROW_BYTES);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < ND; ++q) dma_to_lds(q < NIA ? a : b, voff[q], dst + q * 8 * ROW_BYTES);
+        }
+    };
+
+    if (mine > 0) fetch_scales(0);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        if (s < mine) fetch(first + s, s);
     f32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const u32x4 none = {0u, 0u, 0u, 0u};
-    auto blocks = [&](int first, auto WHOLE_) {
-        constexpr bool WHOLE = decltype(WHOLE_)::value;         // all U blocks exist and are whole
-        u32x4 a[U][TM][2], b[U][TN][2];
-        float sa[U][TM], sb[U][TN][SHIFT == 7 ? 1 : 4];
+    const unsigned char* ring = lds + wave * WAVE_LDS;
+    int stage = 0;
+    for (int t = 0; t < mine; ++t) {
+        // block t has landed, and the scales, which were asked for before it: with NS of them under way that leaves NS - 1 behind it, near the end only "none" says it
+        if (t + NS <= mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * ND) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const unsigned char* at = ring + stage * STAGE;
+        const float* scales = reinterpret_cast<const float*>(ring + NS * STAGE + (t >> 3 & 1) * (GROUPS * 256)) + (t & 7);
+        u32x4 ra[TM][2], rb[TN][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kt = first + u * KS;
-            const bool in = WHOLE || kt < nk;
-            const long k = (long)kt * ROW_BYTES;
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bool there = WHOLE || (in && k + fq * 32 + h * 16 < g.K);
+            for (int i = 0; i < TM; ++i) ra[i][h] = *reinterpret_cast<const u32x4*>(at + lds_offset(16 * i + fi, 2 * fq + h));
 #pragma unroll
-                for (int j = 0; j < TN; ++j) b[u][j][h] = there ? *reinterpret_cast<const u32x4*>(rowB[j] + k + h * 16) : none;
-#pragma unroll
-                for (int i = 0; i < TM; ++i) a[u][i][h] = there ? *reinterpret_cast<const u32x4*>(rowA[i] + k + h * 16) : none;
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i) sa[u][i] = in ? rowSA[i][kt] : 0.f;
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int e = 0; e < (SHIFT == 7 ? 1 : 4); ++e) sb[u][j][e] = in ? rowSB[j][e][kt] : 0.f;
+            for (int j = 0; j < TN; ++j) rb[j][h] = *reinterpret_cast<const u32x4*>(at + NIA * 8 * ROW_BYTES + lds_offset(16 * j + fi, 2 * fq + h));
         }
+        float sa[TM];
+        f32x4 sb[TN];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            Fragment<F8B, FAST> fb[TN];
+        for (int i = 0; i < TM; ++i) sa[i] = scales[(16 * i + fi) * SCALE_BLOCKS];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) fb[j].set(b[u][j]);
+        for (int j = 0; j < TN; ++j) {
+            if constexpr (SHIFT == 7) {
+                sb[j][0] = scales[GROUPS_A * 64];             // (a tile lies inside one block of 128 rows of B)
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sb[j][e] = scales[(16 * (TM + j) + 4 * fq + e) * SCALE_BLOCKS];
+            }
+        }
+        if (t + NS < mine) {
+            // the stage is free once all of it is in registers, and so is, with the first block of a chunk, the chunk before it
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (t % SCALE_BLOCKS == 0 && t + SCALE_BLOCKS < mine) fetch_scales(t / SCALE_BLOCKS + 1);
+            fetch(first + t + NS, stage);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        Fragment<F8A, FAST> fa[TM];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[i].set(ra[i]);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            Fragment<F8B, FAST> fb;
+            fb.set(rb[j]);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                Fragment<F8A, FAST> fa;
-                fa.set(a[u][i]);
+                const f32x4 v = block_sum<F8A, F8B, FAST>(fb, fa[i]);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    const f32x4 t = block_sum<F8A, F8B, FAST>(fb[j], fa);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(t[e], sa[u][i] * sb[u][j][SHIFT == 7 ? 0 : e], acc[i][j][e]);
-                }
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(v[e], sa[i] * sb[j][SHIFT == 7 ? 0 : e], acc[i][j][e]);
             }
         }
-    };
-    const int whole = (int)(g.K >> 7);
-    int kt = wave;
-    for (; kt + (U - 1) * KS < whole; kt += U * KS) blocks(kt, std::true_type{});
-    for (; kt < nk; kt += U * KS) blocks(kt, std::false_type{});
-    // fragment f of wave w at (f * KS + w) * 1 KiB; fragment f is then finished by wave f % KS
+    }
+    // partial tiles: fragment f of wave w at (f * 4 + w) * 1 KiB; fragment f is then finished by wave f % 4
+    __syncthreads();                                       // the rings are not read any more
     f32x4* part = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -340,10 +450,7 @@ __global__ __launch_bounds__(KS * 64) void gemm_scaled_split_kernel(const Scaled
             const int f = i * TN + j;
             if (f % KS != wave) continue;
             const f32x4* p = part + f * KS * 64 + lane;
-            f32x4 s = p[0];
-#pragma unroll
-            for (int w = 1; w < KS; ++w) s += p[w * 64];
-            put_quad(g, m0 + 16 * i + fi, n0 + 16 * j + 4 * fq, s);
+            put_quad(g, m0 + 16 * i + fi, n0 + 16 * j + 4 * fq, (p[0] + p[64]) + (p[128] + p[192]));
         }
 }
 
@@ -360,7 +467,7 @@ static int check_tiles(ScaledArgs& g, int bm, int bn, int threads) {
 template <int F8A, int F8B, bool FAST, int SHIFT, int BM, int BN, int WM, int WN>
 static int launch_tile(ScaledArgs g, hipStream_t stream) {
     auto kernel = gemm_scaled_tile_kernel<F8A, F8B, FAST, SHIFT, BM, BN, WM, WN>;
-    constexpr int lds_bytes = 2 * (BM + BN) * (ROW_BYTES + 4);
+    constexpr int lds_bytes = 2 * ((BM + BN) * ROW_BYTES + (BM / 8 + (SHIFT == 7 ? 1 : BN / 8)) * 256);
     if (const int rc = check_tiles(g, BM, BN, WM * WN * 64); rc != SP_OK) return rc;
     if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
     g.group_m = 4;
@@ -368,32 +475,37 @@ static int launch_tile(ScaledArgs g, hipStream_t stream) {
     return check_launch("sp_gemm_abt_scaled");
 }
 
-template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int KS, int U>
+template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int NS>
 static int launch_split(ScaledArgs g, hipStream_t stream) {
-    auto kernel = gemm_scaled_split_kernel<F8A, F8B, FAST, SHIFT, TM, TN, KS, U>;
-    constexpr int lds_bytes = KS * TM * TN * 1024;
-    if (const int rc = check_tiles(g, 16 * TM, 16 * TN, KS * 64); rc != SP_OK) return rc;
+    auto kernel = gemm_scaled_split_kernel<F8A, F8B, FAST, SHIFT, TM, TN, NS>;
+    constexpr int ring = 4 * (NS * 2 * (TM + TN) * 8 * ROW_BYTES + 2 * (2 * TM + (SHIFT == 7 ? 1 : 2 * TN)) * 256), partial = TM * TN * 4096;
+    constexpr int lds_bytes = ring > partial ? ring : partial;
+    if (const int rc = check_tiles(g, 16 * TM, 16 * TN, 256); rc != SP_OK) return rc;
     if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
     g.group_m = g.tiles_m;        // the tiles of one panel of B stand side by side
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(KS * 64), lds_bytes, stream, g);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(g.tiles_m * g.tiles_n)), dim3(256), lds_bytes, stream, g);
     return check_launch("sp_gemm_abt_scaled");
 }
 
 template <int F8A, int F8B, bool FAST, int SHIFT>
 static int multiply(const ScaledArgs& g, hipStream_t stream) {
     const long cus = device_cu_count();
-    const long tiles128 = ((g.M + 127) / 128) * ((g.N + 127) / 128);
-    if (g.M > 64 && tiles128 * 2 > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 128, 2, 2>(g, stream);
-    if (g.M <= 16) return launch_split<F8A, F8B, FAST, SHIFT, 1, 1, 8, 4>(g, stream);
-    if (g.M <= 32) return launch_split<F8A, F8B, FAST, SHIFT, 2, 2, 8, 2>(g, stream);
-    return launch_split<F8A, F8B, FAST, SHIFT, 4, 2, 4, 2>(g, stream);
+    auto tiles = [&](long bm, long bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
+    if constexpr (FAST && SHIFT == 7)
+        if (g.M > 64 && tiles(256, 256) > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 256, 256, 2, 4>(g, stream);
+    if constexpr (!FAST || SHIFT != 7)
+        if (g.M > 64 && tiles(128, 256) > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 256, 2, 4>(g, stream);
+    if (g.M > 64 && tiles(128, 128) * 2 > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 128, 2, 2>(g, stream);
+    if (g.M <= 16) return launch_split<F8A, F8B, FAST, SHIFT, 1, 1, 4>(g, stream);
+    if (g.M <= 32) return launch_split<F8A, F8B, FAST, SHIFT, 2, 2, 2>(g, stream);
+    return launch_split<F8A, F8B, FAST, SHIFT, 4, 4, 2>(g, stream);
 }
 
 namespace {
 struct GemmScaledKernelNames {
     GemmScaledKernelNames() {
         register_kernel("gemm_scaled_128x128", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 128, 128, 2, 2>, 256);
-        register_kernel("gemm_scaled_split_16x16", (const void*)gemm_scaled_split_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 1, 1, 8, 4>, 512);
+        register_kernel("gemm_scaled_split_16x16", (const void*)gemm_scaled_split_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 1, 1, 4>, 256);
     }
 } gemm_scaled_kernel_names;
 }  // namespace
