@@ -137,7 +137,7 @@ __device__ __forceinline__ void put_piece(const ScaledArgs& g, long row, long co
 }
 
 // A wave's accumulators to C: two rows of fragments at a time go through a strip of LDS of its own, so that whole 16-byte pieces of C leave, side by
-// side along its rows (as 16 rows of 32 bytes per instruction, straight from the registers, 8192 x 4096 x 4096 149 us against EPI_US).
+// side along its rows (as 16 rows of 32 bytes per instruction, straight from the registers, 8192 x 4096 x 4096 took 149 us against 138).
 template <int TN>
 constexpr int STRIP_ROW = 16 * TN * 4 + 16;                // bytes; the pad spreads a column over the banks
 template <int OT, bool HAS_BETA, bool WHOLE, int TM, int TN>
@@ -194,7 +194,7 @@ __device__ __forceinline__ void scaled_tile_of_block(int pid, int tiles_m, int t
 }
 
 // Scales come in for eight blocks of K at a time, eight rows per instruction: 32 bytes of a row lie side by side, so that a load asks for eight
-// lines of memory and not for 64 (one block at a time they are as many lines as the operands: 8192^3 517 us against SCALES_US).
+// lines of memory and not for 64 (one block at a time, as many lines as the operands, 8192^3 took 517 us against 501).
 constexpr int SCALE_BLOCKS = 8;
 
 // Lane l's scale is that of row l / 8 and block l % 8 of what `row` and `first` say; to LDS bytes lds_addr + 4 l.
@@ -212,8 +212,9 @@ __device__ __forceinline__ int tile_slot(int row, int kc) { return (kc ^ row ^ (
 //
 // A wave walks its TM rows of fragments.  While row i is on the matrix pipe, the vector ALU adds the scaled sums of row i - 1 and the fragment of row i + 1 comes
 // in from LDS.  The boundary between two blocks of K stands in front of a block's last row: by then everything of the
-// block is in registers, the next block has landed (it was asked for a whole block earlier), the block after that is asked for, and behind each MFMA of the last row
-// the next block's fragment of B takes the place of the one just used.
+// block is in registers, and the next block has landed.  Behind each MFMA of the last row the next block's fragment of B takes the place of the one just
+// used; then the block after that is asked for.  A wave waits where it asks (the unit takes an instruction of 1 KiB every 16 cycles), so it does that with MFMAs under way: in front of the last row
+// 8192^3 took 480 us, behind it 470, half there and half a row later 456 (4096 x 2048 x 5008 in f32, whose tile has four rows: 95, 89, 90).
 template <int F8A, int F8B, bool FAST, int SHIFT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const ScaledArgs g) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
@@ -253,7 +254,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
         dma_scales(of_a ? g.scale_a : g.scale_b, of_a ? m0 + group * 8 : (n0 >> SHIFT) + (group - GROUPS_A) * 8, of_a ? g.M - 1 : last_sb,
                    (long)chunk * SCALE_BLOCKS, nk, lane, to);
     };
-    auto fetch = [&](int kt, unsigned stage) {
+    auto fetch_part = [&](int kt, unsigned stage, auto FROM_, auto TO_) {
+        constexpr int FROM = decltype(FROM_)::value, TO = decltype(TO_)::value;
         const unsigned char *a = pA + (long)kt * ROW_BYTES, *b = pB + (long)kt * ROW_BYTES;
         auto offset = [&](int q) {
             const unsigned at = voff + (unsigned)(q < NIA ? q : q - NIA) * (NW * 8) * K, last = q < NIA ? last_a : last_b;
@@ -262,15 +264,20 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
         auto to = [&](int q) { return dst + stage + (q < NIA ? q * NW * 8 : BM + (q - NIA) * NW * 8) * ROW_BYTES; };
         if (k_tail && kt == nk - 1) {
 #pragma unroll
-            for (int q = 0; q < NI; ++q) {
+            for (int q = FROM; q < TO; ++q) {
                 const unsigned char* inside = (q < NIA ? a : b) + offset(q);
                 dma_to_lds_addr(tail_in ? inside : (const unsigned char*)kZeroChunk, to(q));
             }
         } else {
 #pragma unroll
-            for (int q = 0; q < NI; ++q) dma_to_lds(q < NIA ? a : b, offset(q), to(q));
+            for (int q = FROM; q < TO; ++q) dma_to_lds(q < NIA ? a : b, offset(q), to(q));
         }
     };
+    // of the fetches behind a boundary FIRST stand behind the last row, the others behind the next block's first row
+    constexpr int FIRST = TM >= 8 ? NI / 2 : NI;
+    typedef std::integral_constant<int, 0> from_start;
+    typedef std::integral_constant<int, FIRST> middle;
+    typedef std::integral_constant<int, NI> to_end;
 
     // fragments: chunks 2 fq and 2 fq + 1 of a row
     int at_a[2], at_b[2];
@@ -323,11 +330,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
     };
 
     for (int part = 0; part < SCALE_BLOCKS; ++part) fetch_scales(0, part);
-    fetch(0, 0);
+    fetch_part(0, 0, from_start{}, to_end{});
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     fetch_scales(1, 0);
-    fetch(nk > 1 ? 1 : 0, STAGE);                      // (past the last block the last one comes again, into a stage that is not read: no branch)
+    fetch_part(nk > 1 ? 1 : 0, STAGE, from_start{}, middle{});                      // (past the last block the last one comes again, into a stage that is not read: no branch)
 #pragma unroll
     for (int j = 0; j < TN; ++j) load_b(j);
     load_a(0);
@@ -343,8 +350,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
             } else {
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __syncthreads();
-                fetch_scales((kt + 1) / SCALE_BLOCKS + 1, (kt + 1) % SCALE_BLOCKS);
-                fetch(kt + 2 < nk ? kt + 2 : nk - 1, step > 0 ? 0 : STAGE);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) at_a[h] += step, at_b[h] += step;
                 step = -step;
@@ -363,11 +368,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (i == 0) {
+                if constexpr (FIRST < NI) fetch_part(kt + 1 < nk ? kt + 1 : nk - 1, step > 0 ? STAGE : 0, middle{}, to_end{});
                 if constexpr (SHIFT == 7)
 #pragma unroll
                     for (int k = 0; k < TM; ++k) sa[k] *= sb[0][0];
             }
             if (boundary) {
+                fetch_scales((kt + 1) / SCALE_BLOCKS + 1, (kt + 1) % SCALE_BLOCKS);
+                fetch_part(kt + 2 < nk ? kt + 2 : nk - 1, step > 0 ? STAGE : 0, from_start{}, middle{});
                 pending = sa[TM - 1];
                 if constexpr (SHIFT != 7)
 #pragma unroll
@@ -551,23 +559,35 @@ static int launch_split(ScaledArgs g, hipStream_t stream) {
     return check_launch("sp_gemm_abt_scaled");
 }
 
+// Which kernel: the largest tile that still gives every compute unit one (and half of them for 128 x 128); else the split ones.
+// Measured, bf16 C and scales of 128 x 128 of B unless said otherwise (us): 4096^3 256 x 256 65, 128 x 256 90, 128 x 128 92;
+// 2048 x 4096 x 4096 56, 43, 43.5; 1024 x 4096 x 4096 128 x 256 35, 128 x 128 28.5, split 64 x 64 50; 512 x 4096 x 4096 128 x 128 26.7, split 64 x 64 26;
+// 256 x 4096 x 4096 26.5, 14.2, split 32 x 32 15.9; 128 x 4096 x 4096 26.4, 14, 10; 64 x 4096 x 4096 split 64 x 64 13.9, 32 x 32 6.9;
+// 49 x 32003 x 4096 split 64 x 64 37, 32 x 32 40; 32 x 32003 x 4096 35, 32; 1 x 4096 x 4096 split 32 x 32 6.8, 16 x 16 5.6;
+// 1 x 16384 x 16384 62, 54; 4096 x 2048 x 5008, f32 C and scales per row of B: 128 x 256 89, 128 x 128 101.  (256 x 256 with C of f32, or scales per row of B,
+// has no room for the f16 fragments, or the scales, in its registers.)
 template <int F8A, int F8B, bool FAST, int SHIFT>
 static int multiply(const ScaledArgs& g, hipStream_t stream) {
     const long cus = device_cu_count();
     auto tiles = [&](long bm, long bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
-    if constexpr (FAST && SHIFT == 7)
-        if (g.M > 64 && tiles(256, 256) > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 256, 256, 2, 4>(g, stream);
-    if constexpr (!FAST || SHIFT != 7)
-        if (g.M > 64 && tiles(128, 256) > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 256, 2, 4>(g, stream);
-    if (g.M > 64 && tiles(128, 128) * 2 > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 128, 2, 2>(g, stream);
+    if (g.M > 64) {
+        if constexpr (FAST && SHIFT == 7) {
+            if (tiles(256, 256) >= cus) return launch_tile<F8A, F8B, FAST, SHIFT, 256, 256, 2, 4>(g, stream);
+        } else {
+            if (tiles(128, 256) >= cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 256, 2, 4>(g, stream);
+        }
+        if (tiles(128, 128) * 2 > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 128, 2, 2>(g, stream);
+    }
     if (g.M <= 16) return launch_split<F8A, F8B, FAST, SHIFT, 1, 1, 4>(g, stream);
-    if (g.M <= 32) return launch_split<F8A, F8B, FAST, SHIFT, 2, 2, 2>(g, stream);
-    return launch_split<F8A, F8B, FAST, SHIFT, 4, 4, 2>(g, stream);
+    if (g.M <= 32 || tiles(32, 32) <= 3 * cus) return launch_split<F8A, F8B, FAST, SHIFT, 2, 2, 2>(g, stream);
+    return launch_split<F8A, F8B, FAST, SHIFT, 4, 4, 1>(g, stream);
 }
 
 namespace {
 struct GemmScaledKernelNames {
     GemmScaledKernelNames() {
+        register_kernel("gemm_scaled_256x256", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 256, 256, 2, 4>, 512);
+        register_kernel("gemm_scaled_f32_128x256", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, false, 7, 128, 256, 2, 4>, 512);
         register_kernel("gemm_scaled_128x128", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 128, 128, 2, 2>, 256);
         register_kernel("gemm_scaled_split_16x16", (const void*)gemm_scaled_split_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 1, 1, 4>, 256);
     }

@@ -165,7 +165,7 @@ def product64(a, sa, b, sb):
 # every kernel: few rows, few tiles, full ones; sides that are no multiple of a tile, K below a block, behind one, and with a tail of one chunk
 PRODUCTS = [(1, 1, 16), (1, 128, 128), (1, 4096, 1040), (2, 130, 112), (7, 33, 272), (16, 256, 4096), (17, 100, 144), (31, 515, 2064), (33, 48, 128), (49, 1003, 528),
             (64, 64, 640), (65, 17, 384), (100, 300, 1168), (128, 128, 128), (129, 257, 272), (1000, 1500, 400), (2304, 1153, 272), (1537, 2050, 144),
-            (2048, 2304, 1024), (4100, 3000, 528)]
+            (2048, 2304, 1024), (4100, 3000, 528), (1, 24700, 272), (20, 24580, 1168), (49, 25001, 2576), (64, 32768, 128)]
 
 
 @pytest.mark.parametrize("wide", [True, False])
@@ -184,7 +184,7 @@ def test_product_of_whole_numbers_is_exact(M, m, n, k, wide):
 
 @pytest.mark.parametrize("types", ["e4m3 e4m3", "e5m2 e4m3", "e4m3 e5m2", "e5m2 e5m2"])
 @pytest.mark.parametrize("m,n,k,wide", [(1, 500, 4096, True), (20, 300, 1040, False), (50, 1000, 528, True), (300, 200, 272, False), (2048, 2100, 656, True),
-                                        (2100, 2048, 400, False)])
+                                        (2100, 2048, 400, False), (17, 25001, 656, False), (3, 24704, 144, True)])
 def test_product(M, m, n, k, wide, types):
     fa, fb = types.split()
     announce("matmul_abt_scaled %s" % ((m, n, k, wide, types),))
@@ -274,7 +274,7 @@ def test_product_of_bad_numbers(M):
 
 def test_a_row_does_not_depend_on_the_others(M):
     announce("matmul_abt_scaled rows")
-    for m, n, k in ((13, 100, 656), (2304, 2304, 272)):
+    for m, n, k in ((13, 100, 656), (2304, 2304, 272), (40, 25000, 272)):
         a, sa, b, sb = (v.cuda() for v in operands(m, n, k, True, "e4m3", "e4m3", 7))
         c = M.matmul_abt_scaled(a, sa, b, sb)
         order = torch.randperm(m, device="cuda")
