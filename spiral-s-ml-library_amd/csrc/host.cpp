@@ -8,6 +8,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/ops/empty.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -20,6 +22,7 @@
 #include <tuple>
 #include <type_traits>
 #include <utility>
+#include <vector>
 
 #include "spiral_mi355.h"
 
@@ -153,6 +156,7 @@ struct Bound {
     PyObject* stream;             // the ctypes structure that stands for sp_philox_t
     const char* name;
     PyObject* function = nullptr; // the function object itself: what the tape records
+    void* more = nullptr;         // a second entry point, for the functions that need one
     Bound(void* fn, PyObject* stream, const char* name) : fn(fn), stream(Py_NewRef(stream)), name(name) {}
     Bound(const Bound&) = delete;
     ~Bound() { Py_DECREF(stream); }
@@ -379,14 +383,254 @@ struct Entry<int(A...)> {
     X(sp_mlp_forward) X(sp_mlp_pack_weights) X(sp_mlp_forward_packed) X(sp_mlp_forward_ensemble) X(sp_ensemble_binarize)            \
     X(sp_stack_forward_f32) X(sp_layer_norm) X(sp_layer_norm_backward) X(sp_logits_penalize) X(sp_quantize_blocks) X(sp_gemm_abt_scaled)
 
-bool bind_one(void* library, PyObject* stream, PyObject* functions, const char* name, PyCFunction call, PyMethodDef& def) {
+// ---- whole calls: checks, outputs and launch of the operators that a decoding step makes of one token at a time ----
+//
+// As the Python functions of the same names (ml.matmul, ml.primitives) do it, for calls that are right and ordinary: contiguous tensors on the current
+// device, nothing recorded.  None for any other call, and where the library refuses: the Python function then goes its own way, and raises what there
+// is to raise.  (us a call with the queue kept full, in Python / here: a norm 7.4 / 4.1, a product
+// of one row 8.1 / 4.0, a row in 8 bits 9.7 / 5.6, the logits of one row, two launches, 18.7 / 9.7; a launch alone takes 3 to 4.)
+PyObject* g_raw_stream = nullptr; // torch's query of the current stream
+
+struct Unusual {};                // thrown to leave a call to Python
+
+struct Whole {
+    int device;
+    void* stream;
+    std::vector<at::Tensor> out;
+
+    static const at::Tensor* given(PyObject* o) {          // nullptr for None
+        if (o == Py_None) return nullptr;
+        if (!THPVariable_Check(o)) throw Unusual();
+        return &THPVariable_Unpack(o);
+    }
+    // The first tensor of a call, whose device has to be the current one.
+    explicit Whole(const at::Tensor* x) {
+        if (g_calls != nullptr || g_raw_stream == nullptr || x == nullptr || !x->is_cuda()) throw Unusual();
+        device = x->get_device();
+        if (c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice().index() != device) throw Unusual();
+        PyObject* index = PyLong_FromLong(device);
+        PyObject* raw = index != nullptr ? PyObject_CallOneArg(g_raw_stream, index) : nullptr;
+        Py_XDECREF(index);
+        stream = raw != nullptr ? PyLong_AsVoidPtr(raw) : nullptr;
+        Py_XDECREF(raw);
+        if (PyErr_Occurred()) throw Unusual();
+    }
+    void* at(const at::Tensor* t, at::ScalarType type) const {     // the address, nullptr for None
+        if (t == nullptr) return nullptr;
+        if (t->scalar_type() != type || !t->is_cuda() || t->get_device() != device || !t->is_contiguous()) throw Unusual();
+        return t->data_ptr();
+    }
+    void* make(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+        out.push_back(at::empty(sizes, like.options().dtype(type)));
+        return out.back().data_ptr();
+    }
+    // The first `n` outputs as a tuple, or the only one.
+    PyObject* result(size_t n) {
+        if (n == 1) return THPVariable_Wrap(std::move(out[0]));
+        PyObject* all = PyTuple_New((Py_ssize_t)n);
+        if (all == nullptr) return nullptr;
+        for (size_t i = 0; i < n; ++i) {
+            PyObject* one = THPVariable_Wrap(std::move(out[i]));
+            if (one == nullptr) {
+                Py_DECREF(all);
+                return nullptr;
+            }
+            PyTuple_SET_ITEM(all, (Py_ssize_t)i, one);
+        }
+        return all;
+    }
+};
+
+int code_of(at::ScalarType t) {
+    switch (t) {
+        case at::kFloat: return SP_F32;
+        case at::kHalf: return SP_F16;
+        case at::kBFloat16: return SP_BF16;
+        default: throw Unusual();
+    }
+}
+int f8_code_of(at::ScalarType t) {
+    if (t == at::kFloat8_e4m3fn) return SP_F8_E4M3;
+    if (t == at::kFloat8_e5m2) return SP_F8_E5M2;
+    throw Unusual();
+}
+bool yes(PyObject* o) { return o == Py_True ? true : o == Py_False ? false : throw Unusual(); }
+double number(PyObject* o) { return PyFloat_Check(o) ? PyFloat_AS_DOUBLE(o) : throw Unusual(); }
+at::ScalarType type_of(PyObject* o) { return THPDtype_Check(o) ? ((THPDtype*)o)->scalar_type : throw Unusual(); }
+void need(bool ok) {
+    if (!ok) throw Unusual();
+}
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+// f(bound, arguments), None for what it throws.
+template <typename F>
+PyObject* whole(PyObject* capsule, Py_ssize_t n, Py_ssize_t want, const F& f) {
+    const Bound* const bound = (const Bound*)PyCapsule_GetPointer(capsule, nullptr);
+    if (bound == nullptr) return nullptr;
+    if (n != want) return PyErr_Format(PyExc_TypeError, "%zd arguments (%zd given)", want, n);
+    try {
+        return f(*bound);
+    } catch (const Unusual&) {
+    } catch (const std::exception&) {
+    }
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+template <typename F, typename... A>
+void launch(F* fn, A... args) {
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = fn(args...);
+    Py_END_ALLOW_THREADS
+    need(rc == 0);
+}
+
+// (x, weight, bias, eps, want_stats)
+PyObject* whole_layer_norm(PyObject* capsule, PyObject* const* a, Py_ssize_t n) {
+    return whole(capsule, n, 5, [&](const Bound& bound) {
+        const at::Tensor *x = Whole::given(a[0]), *weight = Whole::given(a[1]), *bias = Whole::given(a[2]);
+        Whole call(x);
+        need(x->dim() >= 2 && x->numel() > 0);
+        const int64_t cols = x->size(-1), rows = x->numel() / cols;
+        const at::ScalarType type = x->scalar_type(), weights = weight != nullptr ? weight->scalar_type() : bias != nullptr ? bias->scalar_type() : at::kFloat;
+        const int code = code_of(type);
+        need(weights == at::kFloat || weights == type);
+        for (const at::Tensor* t : {weight, bias}) need(t == nullptr || (t->dim() == 1 && t->size(0) == cols));
+        const bool stats = yes(a[4]);
+        const double eps = number(a[3]);
+        void *from = call.at(x, type), *w = call.at(weight, weights), *b = call.at(bias, weights), *y = call.make(x->sizes(), type, *x), *mean = nullptr, *rstd = nullptr;
+        if (stats) {
+            const auto lead = x->sizes().slice(0, x->dim() - 1);
+            mean = call.make(lead, at::kFloat, *x);
+            rstd = call.make(lead, at::kFloat, *x);
+        }
+        launch((decltype(&sp_layer_norm))bound.fn, code, code_of(weights), from, w, b, y, (float*)mean, (float*)rstd, rows, cols, (float)eps, call.stream);
+        return call.result(stats ? 3 : 1);
+    });
+}
+
+// (dy, x, mean, rstd, weight)
+PyObject* whole_layer_norm_backward(PyObject* capsule, PyObject* const* a, Py_ssize_t n) {
+    return whole(capsule, n, 5, [&](const Bound& bound) {
+        const at::Tensor *dy = Whole::given(a[0]), *x = Whole::given(a[1]), *mean = Whole::given(a[2]), *rstd = Whole::given(a[3]), *weight = Whole::given(a[4]);
+        Whole call(x);
+        need(bound.more != nullptr && dy != nullptr && mean != nullptr && rstd != nullptr && x->dim() >= 2 && x->numel() > 0 && dy->sizes() == x->sizes());
+        const int64_t cols = x->size(-1), rows = x->numel() / cols;
+        const auto lead = x->sizes().slice(0, x->dim() - 1);
+        need(mean->sizes() == lead && rstd->sizes() == lead);
+        const at::ScalarType type = x->scalar_type(), weights = weight != nullptr ? weight->scalar_type() : at::kFloat;
+        const int code = code_of(type);
+        need((weights == at::kFloat || weights == type) && (weight == nullptr || (weight->dim() == 1 && weight->size(0) == cols)));
+        void *g = call.at(dy, type), *from = call.at(x, type), *m = call.at(mean, at::kFloat), *r = call.at(rstd, at::kFloat), *w = call.at(weight, weights);
+        void *dx = call.make(x->sizes(), type, *x), *dw = call.make({cols}, at::kFloat, *x), *db = call.make({cols}, at::kFloat, *x);
+        const int64_t bytes = ((decltype(&sp_layer_norm_backward_workspace_bytes))bound.more)(rows, cols);
+        void* workspace = call.make({bytes > 16 ? bytes : 16}, at::kByte, *x);
+        launch((decltype(&sp_layer_norm_backward))bound.fn, code, code_of(weights), g, from, (const float*)m, (const float*)r, w, dx, (float*)dw, (float*)db, rows,
+               cols, workspace, bytes, call.stream);
+        return call.result(3);
+    });
+}
+
+// (x, rows of a block, type, plain, transposed)
+PyObject* whole_quantize_blocks(PyObject* capsule, PyObject* const* a, Py_ssize_t n) {
+    return whole(capsule, n, 5, [&](const Bound& bound) {
+        const at::Tensor* x = Whole::given(a[0]);
+        Whole call(x);
+        need(x->dim() == 2 && x->numel() > 0 && PyLong_Check(a[1]));
+        const int64_t size[2] = {x->size(0), x->size(1)};
+        const long high = PyLong_AsLong(a[1]);
+        const at::ScalarType type = x->scalar_type(), f8 = type_of(a[2]);
+        const int code = code_of(type), f8_code = f8_code_of(f8);
+        void *from = call.at(x, type), *to[4] = {};
+        for (int form = 0; form < 2; ++form) {
+            if (!yes(a[3 + form])) continue;
+            const int64_t r = size[form], c = size[1 - form];
+            to[2 * form] = call.make({r, (c + 15) / 16 * 16}, f8, *x);
+            to[2 * form + 1] = call.make({high == 1 ? r : blocks_of(r), blocks_of(c)}, at::kFloat, *x);
+        }
+        launch((decltype(&sp_quantize_blocks))bound.fn, code, f8_code, (int32_t)high, from, to[0], (float*)to[1], to[2], (float*)to[3], size[0], size[1], call.stream);
+        return call.result(call.out.size());
+    });
+}
+
+// (a, scale_a, b, scale_b, bias, relu, type of C)
+PyObject* whole_matmul_abt_scaled(PyObject* capsule, PyObject* const* o, Py_ssize_t n) {
+    return whole(capsule, n, 7, [&](const Bound& bound) {
+        const at::Tensor *a = Whole::given(o[0]), *sa = Whole::given(o[1]), *b = Whole::given(o[2]), *sb = Whole::given(o[3]), *bias = Whole::given(o[4]);
+        Whole call(a);
+        for (const at::Tensor* t : {a, sa, b, sb}) need(t != nullptr && t->dim() == 2 && t->numel() > 0);
+        const int64_t m = a->size(0), k = a->size(1), rows_b = b->size(0), kb = blocks_of(k), high = sb->size(0) == rows_b ? 1 : 128;
+        need(b->size(1) == k && sa->size(0) == m && sa->size(1) == kb && sb->size(1) == kb && (high == 1 || sb->size(0) == blocks_of(rows_b)));
+        need(bias == nullptr || (bias->dim() == 1 && bias->size(0) == rows_b));
+        const at::ScalarType out = type_of(o[6]);
+        const int fa = f8_code_of(a->scalar_type()), fb = f8_code_of(b->scalar_type()), code = code_of(out);
+        const bool relu = yes(o[5]);
+        void *pa = call.at(a, a->scalar_type()), *psa = call.at(sa, at::kFloat), *pb = call.at(b, b->scalar_type()), *psb = call.at(sb, at::kFloat), *pbias = call.at(bias, at::kFloat);
+        void* c = call.make({m, rows_b}, out, *a);
+        launch((decltype(&sp_gemm_abt_scaled))bound.fn, fa, fb, code, pa, (const float*)psa, pb, (const float*)psb, (int32_t)high, c, (const float*)pbias, m, rows_b, k, 0.f,
+               relu ? SP_GEMM_RELU : 0u, call.stream);
+        return call.result(1);
+    });
+}
+
+// (logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, temperature, bias_ids, bias, mask, want_token)
+PyObject* whole_penalize_logits(PyObject* capsule, PyObject* const* a, Py_ssize_t n) {
+    return whole(capsule, n, 12, [&](const Bound& bound) {
+        const at::Tensor *x = Whole::given(a[0]), *tokens = Whole::given(a[1]), *ids = Whole::given(a[8]), *bias = Whole::given(a[9]), *mask = Whole::given(a[10]);
+        Whole call(x);
+        need(bound.more != nullptr && x->dim() >= 2 && x->numel() > 0);
+        const int64_t cols = x->size(-1), rows = x->numel() / cols, words = (cols + 31) / 32;
+        const auto lead = x->sizes().slice(0, x->dim() - 1);
+        auto rows_of = [&](const at::Tensor* t) { return t->dim() == x->dim() && t->sizes().slice(0, t->dim() - 1) == lead; };
+        const at::Tensor* each[6];                         // one entry per row
+        void* at_each[6];
+        for (int i = 0; i < 6; ++i) {
+            each[i] = Whole::given(a[2 + i]);
+            need(each[i] == nullptr || each[i]->sizes() == lead);
+            at_each[i] = call.at(each[i], i < 2 ? at::kInt : at::kFloat);
+        }
+        need(tokens != nullptr ? rows_of(tokens) : each[0] == nullptr && each[1] == nullptr);
+        need((ids == nullptr) == (bias == nullptr) && (bias == nullptr || (rows_of(bias) && ids->sizes() == bias->sizes())));
+        need(mask == nullptr || (mask->dim() > 0 && mask->size(-1) == words && (mask->numel() == words || mask->numel() == rows * words)));
+        const int64_t history = tokens != nullptr ? tokens->size(-1) : 0, n_bias = bias != nullptr ? bias->size(-1) : 0;
+        const at::ScalarType type = x->scalar_type();
+        const int code = code_of(type);
+        const bool want_token = yes(a[11]);
+        void *from = call.at(x, type), *history_at = call.at(tokens, at::kInt), *ids_at = call.at(ids, at::kInt), *bias_at = call.at(bias, at::kFloat), *mask_at = call.at(mask, at::kInt);
+        void *out = call.make(x->sizes(), at::kFloat, *x), *token = nullptr, *workspace = nullptr;
+        int64_t bytes = 0;
+        if (want_token) {
+            token = call.make(lead, at::kInt, *x);
+            bytes = ((decltype(&sp_logits_penalize_workspace_bytes))bound.more)(rows, cols);
+            workspace = call.make({bytes}, at::kByte, *x);
+        }
+        launch((decltype(&sp_logits_penalize))bound.fn, code, from, (float*)out, (int32_t*)token, (const int32_t*)(history > 0 ? history_at : nullptr), (const int32_t*)at_each[0],
+               (const int32_t*)at_each[1], history, (const float*)at_each[2], (const float*)at_each[3], (const float*)at_each[4], (const float*)at_each[5],
+               (const int32_t*)(n_bias > 0 ? ids_at : nullptr), (const float*)(n_bias > 0 ? bias_at : nullptr), n_bias, (const int32_t*)mask_at,
+               mask != nullptr ? mask->numel() / words : (int64_t)0, rows, cols, workspace, bytes, call.stream);
+        return call.result(want_token ? 2 : 1);
+    });
+}
+
+// (Python's name, the function, the entry point, another one it asks)
+#define SP_WHOLE(X)                                                                                        \
+    X(layer_norm, sp_layer_norm, nullptr)                                                                   \
+    X(layer_norm_backward, sp_layer_norm_backward, "sp_layer_norm_backward_workspace_bytes")                  \
+    X(quantize_blocks, sp_quantize_blocks, nullptr)                                                          \
+    X(matmul_abt_scaled, sp_gemm_abt_scaled, nullptr)                                                        \
+    X(penalize_logits, sp_logits_penalize, "sp_logits_penalize_workspace_bytes")
+
+// `as`: the name the function goes by; `other`: a second entry point for it, where the library has it.
+bool bind_one(void* library, PyObject* stream, PyObject* functions, const char* name, PyCFunction call, PyMethodDef& def, const char* as, const char* other) {
     void* const fn = dlsym(library, name);
+    void* const more = fn != nullptr && other != nullptr ? dlsym(library, other) : nullptr;
     if (fn == nullptr) {
         PyErr_Format(PyExc_RuntimeError, "the library has no %s", name);
         return false;
     }
-    def = PyMethodDef{name, call, METH_FASTCALL, nullptr};
+    def = PyMethodDef{as, call, METH_FASTCALL, nullptr};
     Bound* const bound = new (std::nothrow) Bound(fn, stream, name);
+    if (bound != nullptr) bound->more = more;
     if (bound == nullptr) {
         PyErr_NoMemory();
         return false;
@@ -400,7 +644,7 @@ bool bind_one(void* library, PyObject* stream, PyObject* functions, const char* 
     Py_DECREF(capsule);
     if (function == nullptr) return false;
     bound->function = function;                            // (borrowed: the function holds the capsule)
-    const int failed = PyDict_SetItemString(functions, name, function);
+    const int failed = PyDict_SetItemString(functions, as, function);
     Py_DECREF(function);
     return failed == 0;
 }
@@ -434,6 +678,12 @@ PyObject* bind(PyObject*, PyObject* const* given, Py_ssize_t n) {
     }
     Py_DECREF(ctypes);
     if (!found) return nullptr;
+    if (g_raw_stream == nullptr) {                         // (a torch without a GPU has none: no whole calls then)
+        PyObject* torch_c = PyImport_ImportModule("torch._C");
+        if (torch_c != nullptr) g_raw_stream = PyObject_GetAttrString(torch_c, "_cuda_getCurrentRawStream");
+        Py_XDECREF(torch_c);
+        PyErr_Clear();
+    }
     void* library = dlopen(p, RTLD_NOW | RTLD_LOCAL);
     if (library == nullptr) return PyErr_Format(PyExc_RuntimeError, "%s", dlerror());
     PyObject* functions = PyDict_New();
@@ -441,12 +691,18 @@ PyObject* bind(PyObject*, PyObject* const* given, Py_ssize_t n) {
     bool ok = true;
     enum {
 #define SP_ID(name) ID_##name,
-        SP_LAUNCHES(SP_ID) COUNT
+        SP_LAUNCHES(SP_ID)
+#undef SP_ID
+#define SP_ID(as, name, other) ID_whole_##as,
+        SP_WHOLE(SP_ID) COUNT
 #undef SP_ID
     };
     static PyMethodDef defs[COUNT];
-#define SP_BIND(name) ok = ok && bind_one(library, given[1], functions, #name, (PyCFunction)(void (*)(void))&Entry<std::remove_pointer_t<decltype(&::name)>>::call, defs[ID_##name]);
+#define SP_BIND(name) ok = ok && bind_one(library, given[1], functions, #name, (PyCFunction)(void (*)(void))&Entry<std::remove_pointer_t<decltype(&::name)>>::call, defs[ID_##name], #name, nullptr);
     SP_LAUNCHES(SP_BIND)
+#undef SP_BIND
+#define SP_BIND(as, name, other) ok = ok && bind_one(library, given[1], functions, #name, (PyCFunction)(void (*)(void))&whole_##as, defs[ID_whole_##as], "whole_" #as, other);
+    SP_WHOLE(SP_BIND)
 #undef SP_BIND
     if (!ok) {
         Py_DECREF(functions);

@@ -103,6 +103,10 @@ def quantize_blocks(x, block=(1, 128), dtype=torch.float8_e4m3fn, transpose=Fals
     type's largest number.  q is (rows, cols rounded up to a multiple of 16), zeros behind the columns of x; scale (rows or ceil(rows / 128),
     ceil(cols / 128)).  transpose=True gives the same of the transpose of x, transpose="both" reads x once and gives
     (q, scale, q_t, scale_t): what a layer's forward product and the gradients of its input (weights) or its weights (activations) take."""
+    if (block == (1, 128) or block == (128, 128)) and (transpose in (False, True) or transpose == "both"):
+        done = lib.whole_quantize_blocks(x, block[0], dtype, transpose is not True, transpose is not False)
+        if done is not None:
+            return done
     if x.dim() != 2:
         raise ValueError("x must be 2-D")
     if x.dtype not in _lib.DTYPES:
@@ -144,6 +148,10 @@ def matmul_abt_scaled(a, scale_a, b, scale_b, c=None, beta=0.0, bias=None, relu=
         d8, sd, dt, sdt = quantize_blocks(dy, dtype=torch.float8_e5m2, transpose="both")
         y = matmul_abt_scaled(x8, sx, w8, sw);  dx = matmul_abt_scaled(d8, sd, wt, swt);  dW = matmul_abt_scaled(dt, sdt, xt, sxt)
     (with N, K and M multiples of 16; otherwise the padding of q shows in the widths of what they are multiplied with)."""
+    if c is None and beta == 0.0:
+        done = lib.whole_matmul_abt_scaled(a, scale_a, b, scale_b, bias, relu, out_dtype or torch.float32)
+        if done is not None:
+            return done
     if a.dim() != 2 or b.dim() != 2 or scale_a.dim() != 2 or scale_b.dim() != 2:
         raise ValueError("a, b and their scales must be 2-D")
     if a.dtype not in _lib.F8_TYPES or b.dtype not in _lib.F8_TYPES:

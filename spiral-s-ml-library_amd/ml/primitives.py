@@ -265,6 +265,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None, want_stats=False):
     (ml/primitives.spi:701-703).  x: f32, f16 or bf16 with rows of any length up to 16384; the result has its type, `out` may be x.  weight,
     bias: (cols,), f32 or of x's type, or None.  Statistics are f32; want_stats=True also returns each row's mean and 1 / sqrt(var + eps),
     which `layer_norm_backward` takes: (y, mean, rstd)."""
+    if out is None:
+        done = lib.whole_layer_norm(x, weight, bias, eps, want_stats)
+        if done is not None:
+            return done
     if x.dtype not in _lib.DTYPES:
         raise TypeError("layer_norm takes f32, f16 or bf16 tensors, got %s" % x.dtype)
     rows, cols = _rows_cols(x)
@@ -288,6 +292,10 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None, want_weight_gr
     """The gradients of `layer_norm` (sp_layer_norm_backward): (dx, dweight, dbias) from dy and the x, mean and rstd of the forward call.
     dx has x's type (`out` may be dy), dweight and dbias are f32, summed over all rows in an order that depends on the sizes alone; they are None with
     want_weight_grads=False."""
+    if out is None and want_weight_grads is True:
+        done = lib.whole_layer_norm_backward(dy, x, mean, rstd, weight)
+        if done is not None:
+            return done
     if x.dtype not in _lib.DTYPES:
         raise TypeError("layer_norm_backward takes f32, f16 or bf16 tensors, got %s" % x.dtype)
     rows, cols = _rows_cols(x)
@@ -327,6 +335,11 @@ def penalize_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repe
     id that stands twice both count.  mask: (..., ceil(cols / 32)) i32, or one row of it for all; bit j % 32 of word j // 32 allows j.  Every
     one may be None.  want_token=True also returns the (...,) i32 index of each row's largest result, the lowest of equal ones, -1 for a
     row that has none above -inf."""
+    if out is None:
+        done = lib.whole_penalize_logits(logits, tokens, lengths, prompt_lengths, repetition, presence, frequency, temperature, bias_ids, bias,
+                                         mask, want_token)
+        if done is not None:
+            return done
     if logits.dtype not in _lib.DTYPES:
         raise TypeError("penalize_logits takes f32, f16 or bf16 logits, got %s" % logits.dtype)
     rows, cols = _rows_cols(logits)
