@@ -72,7 +72,7 @@ def test_what_is_not_taken_raises():
     stats = torch.zeros((4,), device="cuda")
     for error, text, f in ((ValueError, "contiguous", lambda: P.layer_norm(x.t())), (ValueError, "GPU", lambda: P.layer_norm(x, w.cpu())), (ValueError, "weight must", lambda: P.layer_norm(x, w[:3])),
                            (TypeError, "f32, f16", lambda: P.layer_norm(x.double())), (RuntimeError, "16384", lambda: P.layer_norm(torch.zeros((1, 16385), device="cuda"))),
-                           (RuntimeError, "eps", lambda: P.layer_norm(x, eps=-1.0)), (RuntimeError, "positive", lambda: P.layer_norm(x[:0])), (RuntimeError, "16-byte", lambda: P.layer_norm(x.view(-1)[1:].view(3, 85))),
+                           (RuntimeError, "eps", lambda: P.layer_norm(x, eps=-1.0)), (RuntimeError, "NULL", lambda: P.layer_norm(x[:0])), (RuntimeError, "16-byte", lambda: P.layer_norm(x.view(-1)[1:].view(3, 85))),
                            (ValueError, "dy must", lambda: P.layer_norm_backward(x.half(), x, stats, stats)), (TypeError, "mean must have dtype", lambda: P.layer_norm_backward(x, x, stats.half(), stats)),
                            (ValueError, "contiguous", lambda: M.quantize_blocks(x.t())), (ValueError, "block", lambda: M.quantize_blocks(x, (64, 64))), (ValueError, "empty", lambda: M.quantize_blocks(x[:, :0])),
                            (AssertionError, "K dimension", lambda: M.matmul_abt_scaled(a8, sa, a8.view(torch.uint8)[:, :32].contiguous().view(F8), sa)),
