@@ -1,9 +1,10 @@
 // Logits of a whole vocabulary before a token is chosen: penalties for tokens that stand in the history, biases, temperature and a mask,
 // and the largest of what is left.  One pass: every logit is read once and written once, and that bounds it.
 //
-// A workgroup takes CHUNK columns of one row.  What the history and the biases say about them is gathered first in a 32-bit
-// word of LDS per column -- bits 0..19 the count behind the prompt, bit 20 "seen in the prompt", bits 21..31 the first bias entry that names
-// the column -- with integer atomics, whose order does not matter.  Columns whose word is zero, most of them, then cost one LDS read.
+// A workgroup takes CHUNK columns of one row, and asks for them, and for their mask, before anything else.  What the history and the biases say about
+// them is gathered meanwhile in a 32-bit word of LDS per column -- bits 0..19 the count behind the prompt, bit 20 "seen in the prompt", bits 21..31
+// the first bias entry that names the column -- with integer atomics, whose order does not matter.  Columns whose word is zero, most of them, then
+// cost one LDS read.
 // A column named by several bias entries (rare; a flag says whether there is one at all) goes through the entries again, in their order.
 // The arithmetic is that of the steps written out, each rounded to f32: nothing is contracted.
 #include "vec_io.h"
@@ -14,7 +15,10 @@ namespace sp {
 
 constexpr unsigned COUNT_MASK = (1u << 20) - 1u, SEEN_BIT = 1u << 20;
 constexpr int ENTRY_SHIFT = 21, MOST_ENTRIES = 2047;      // entry j is kept as 2047 - j: the first one is the largest, 0 is none
-constexpr int CHUNK = 8192, LOGITS_THREADS = 512;
+// Columns to a workgroup: enough of them that reading the history again for every chunk of a row does not count; fewer where the large chunks
+// would leave most of the chip idle (1 x 32003, a history of 2000: ONE_ROW).  (One workgroup for a whole row, which needs no second launch to
+// choose the token, is slower than both launches: a compute unit alone brings in 24 bytes a cycle, 16 us for 32003 columns.)
+constexpr int LARGE_CHUNK = 8192, LARGE_THREADS = 512, SMALL_CHUNK = 2048, SMALL_THREADS = 256;
 
 struct LogitsArgs {
     float* out;
@@ -46,18 +50,28 @@ __device__ __forceinline__ Best best_of_wave(Best b) {
 }
 
 // SPARSE: there is a history or there are biases.
-template <int DT, bool SPARSE>
-__global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const void* logits, long cols, unsigned chunks, const LogitsArgs a) {
-    constexpr int N = PER16<DT>;
-    __shared__ __attribute__((aligned(16))) unsigned words[SPARSE ? CHUNK : 4];
+template <int DT, bool SPARSE, int CHUNK, int THREADS>
+__global__ __launch_bounds__(THREADS) void logits_kernel(const void* logits, long cols, unsigned chunks, const LogitsArgs a) {
+    constexpr int N = PER16<DT>, STEP = THREADS * N, PIECES = CHUNK / STEP;
+    static_assert(CHUNK % STEP == 0 && CHUNK % 32 == 0, "whole pieces, whole words of the mask");
+    extern __shared__ __attribute__((aligned(16))) unsigned words[];       // SPARSE: CHUNK of them
     __shared__ int again;                                  // a column has more than one bias entry
-    __shared__ float wave_v[LOGITS_THREADS / 64];
-    __shared__ int wave_at[LOGITS_THREADS / 64];
+    __shared__ float wave_v[THREADS / 64];
+    __shared__ int wave_at[THREADS / 64];
     const int tid = threadIdx.x;
     const long row = blockIdx.x / chunks;
     const unsigned chunk = blockIdx.x - (unsigned)row * chunks;
     const long c0 = (long)chunk * CHUNK;
     const int here = (int)(cols - c0 < CHUNK ? cols - c0 : CHUNK);     // columns of this workgroup
+    u32x4 raw[PIECES];
+    unsigned allowed[PIECES];
+    const unsigned* mask = a.mask + row * a.mask_step;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int i = p * STEP + tid * N;
+        raw[p] = load16<DT>(logits, row * cols + c0 + i, here - i);
+        allowed[p] = a.mask != nullptr && i < here ? mask[(c0 + i) >> 5] : ~0u;
+    }
     float rep = 1.f, pres = 0.f, freq = 0.f, temp = 0.f;
     const bool has_rep = a.repetition != nullptr, has_pres = a.presence != nullptr, has_freq = a.frequency != nullptr;
     if (has_rep) rep = a.repetition[row];
@@ -67,20 +81,20 @@ __global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const void* logi
     const int32_t* ids = a.bias_ids + row * a.n_bias;
     const float* biases = a.bias + row * a.n_bias;
     if constexpr (SPARSE) {
-        for (int i = tid * 4; i < CHUNK; i += LOGITS_THREADS * 4) *reinterpret_cast<u32x4*>(words + i) = u32x4{0u, 0u, 0u, 0u};
+        for (int i = tid * 4; i < CHUNK; i += THREADS * 4) *reinterpret_cast<u32x4*>(words + i) = u32x4{0u, 0u, 0u, 0u};
         if (tid == 0) again = 0;
         __syncthreads();
-        for (int j = tid; j < a.n_bias; j += LOGITS_THREADS) {
+        for (int j = tid; j < a.n_bias; j += THREADS) {
             const long at = ids[j] - c0;
             if (at >= 0 && at < here) atomicMax(&words[at], (unsigned)(MOST_ENTRIES - j) << ENTRY_SHIFT);
         }
         if (a.n_bias > 0) {
             __syncthreads();
-            for (int j = tid; j < a.n_bias; j += LOGITS_THREADS) {
+            // (counting goes on meanwhile: it leaves the upper bits alone)
+            for (int j = tid; j < a.n_bias; j += THREADS) {
                 const long at = ids[j] - c0;
                 if (at >= 0 && at < here && words[at] >> ENTRY_SHIFT != (unsigned)(MOST_ENTRIES - j)) again = 1;
             }
-            __syncthreads();
         }
         if (a.tokens != nullptr) {
             long length = a.history;
@@ -88,15 +102,19 @@ __global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const void* logi
                 const long given = a.lengths[row];
                 length = given < length ? given : length;
             }
-            const long prompt = a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
+            long prompt = a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
+            prompt = prompt > 0 ? prompt : 0;
+            const unsigned first = (unsigned)c0;
             const int32_t* mine = a.tokens + row * a.history;
-            for (long i = (long)tid * 4; i < length; i += LOGITS_THREADS * 4) {
+            for (long i = (long)tid * 4; i < length; i += THREADS * 4) {
                 const u32x4 t = load16<SP_F32>(mine, i, length - i);
+                // (columns are below 2^31: a token in front of the chunk or below zero wraps to one behind it)
+                const int left = length - i < 4 ? (int)(length - i) : 4, of_prompt = prompt - i < 4 ? (int)(prompt - i) : 4;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const long at = (long)(int)t[e] - c0;
-                    if (i + e >= length || at < 0 || at >= here) continue;
-                    if (i + e < prompt) atomicOr(&words[at], SEEN_BIT);
+                    const unsigned at = t[e] - first;
+                    if (at >= (unsigned)here || e >= left) continue;
+                    if (e < of_prompt) atomicOr(&words[at], SEEN_BIT);
                     else atomicAdd(&words[at], 1u);
                 }
             }
@@ -104,14 +122,13 @@ __global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const void* logi
         __syncthreads();
     }
     Best best{-INFINITY, -1};
-    const unsigned* mask = a.mask + row * a.mask_step;
-    for (int i = tid * N; i < here; i += LOGITS_THREADS * N) {
-        const u32x4 raw = load16<DT>(logits, row * cols + c0 + i, here - i);
-        unsigned allowed = ~0u;
-        if (a.mask != nullptr) allowed = mask[(c0 + i) >> 5] >> (i & 31);
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int i = p * STEP + tid * N;
+        if (i >= here) break;
         float v[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = element<DT>(raw, e);
+        for (int e = 0; e < N; ++e) v[e] = element<DT>(raw[p], e);
         if constexpr (SPARSE) {
             unsigned w[N], any = 0;
 #pragma unroll
@@ -148,7 +165,7 @@ __global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const void* logi
             for (int e = 0; e < N; ++e) v[e] = v[e] / temp;
         if (a.mask != nullptr)
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = (allowed >> e) & 1u ? v[e] : -INFINITY;
+            for (int e = 0; e < N; ++e) v[e] = (allowed[p] >> ((i & 31) + e)) & 1u ? v[e] : -INFINITY;
 #pragma unroll
         for (int e = 0; e < N; ++e)
             if (i + e < here && v[e] > best.v) best = Best{v[e], (int)c0 + i + e};     // (columns go up: the first one stays)
@@ -167,7 +184,7 @@ __global__ __launch_bounds__(LOGITS_THREADS) void logits_kernel(const void* logi
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
-        for (int w = 1; w < LOGITS_THREADS / 64; ++w) best.take(wave_v[w], wave_at[w]);
+        for (int w = 1; w < THREADS / 64; ++w) best.take(wave_v[w], wave_at[w]);
         if (chunks == 1) {
             a.token[row] = best.at;
         } else {
@@ -189,22 +206,30 @@ __global__ __launch_bounds__(256) void logits_token_kernel(const float* best, co
 
 // ---- host side -------------------------------------------------------------------------------
 
-static int64_t logits_chunks(int64_t cols) { return (cols + CHUNK - 1) / CHUNK; }
+static int64_t chunks_of(int64_t cols, int64_t chunk) { return (cols + chunk - 1) / chunk; }
+static bool small_chunks(int64_t rows, int64_t cols) { return rows * chunks_of(cols, LARGE_CHUNK) <= device_cu_count() / 2; }
+static int64_t logits_chunks(int64_t rows, int64_t cols) { return chunks_of(cols, small_chunks(rows, cols) ? SMALL_CHUNK : LARGE_CHUNK); }
 
-template <int DT>
-static void launch_logits(const void* logits, long rows, long cols, const LogitsArgs& a, hipStream_t stream) {
-    const unsigned chunks = (unsigned)logits_chunks(cols);
-    if (a.tokens != nullptr || a.n_bias > 0)
-        hipLaunchKernelGGL((logits_kernel<DT, true>), dim3((unsigned)rows * chunks), dim3(LOGITS_THREADS), 0, stream, logits, cols, chunks, a);
-    else
-        hipLaunchKernelGGL((logits_kernel<DT, false>), dim3((unsigned)rows * chunks), dim3(LOGITS_THREADS), 0, stream, logits, cols, chunks, a);
+template <int DT, bool SPARSE, int CHUNK, int THREADS>
+static int launch_chunks(const void* logits, long rows, long cols, unsigned chunks, const LogitsArgs& a, hipStream_t stream) {
+    auto kernel = logits_kernel<DT, SPARSE, CHUNK, THREADS>;
+    constexpr int lds_bytes = SPARSE ? CHUNK * 4 : 0;
+    if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)rows * chunks), dim3(THREADS), lds_bytes, stream, logits, cols, chunks, a);
+    return check_launch("sp_logits_penalize");
+}
+
+template <int DT, bool SPARSE>
+static int launch_logits(const void* logits, long rows, long cols, unsigned chunks, const LogitsArgs& a, hipStream_t stream) {
+    if (small_chunks(rows, cols)) return launch_chunks<DT, SPARSE, SMALL_CHUNK, SMALL_THREADS>(logits, rows, cols, chunks, a, stream);
+    return launch_chunks<DT, SPARSE, LARGE_CHUNK, LARGE_THREADS>(logits, rows, cols, chunks, a, stream);
 }
 
 namespace {
 struct LogitsKernelNames {
     LogitsKernelNames() {
-        register_kernel("logits", (const void*)logits_kernel<SP_F32, true>, LOGITS_THREADS);
-        register_kernel("logits_bf16", (const void*)logits_kernel<SP_BF16, true>, LOGITS_THREADS);
+        register_kernel("logits", (const void*)logits_kernel<SP_F32, true, LARGE_CHUNK, LARGE_THREADS>, LARGE_THREADS);
+        register_kernel("logits_bf16", (const void*)logits_kernel<SP_BF16, true, LARGE_CHUNK, LARGE_THREADS>, LARGE_THREADS);
     }
 } logits_kernel_names;
 }  // namespace
@@ -215,7 +240,7 @@ using namespace sp;
 
 extern "C" int64_t sp_logits_penalize_workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return rows * logits_chunks(cols) * 8;
+    return rows * logits_chunks(rows, cols) * 8;
 }
 
 extern "C" int sp_logits_penalize(int dtype, const void* logits, float* out, int32_t* token, const int32_t* tokens, const int32_t* lengths,
@@ -238,7 +263,7 @@ extern "C" int sp_logits_penalize(int dtype, const void* logits, float* out, int
     SP_OPTIONAL_PTR(mask);
     if (dtype != SP_F32 && dtype != SP_F16 && dtype != SP_BF16) return fail(SP_ERR_DTYPE, "sp_logits_penalize: dtype must be f32, f16 or bf16, got %d", dtype);
     if (rows <= 0 || cols <= 0) return fail(SP_ERR_SHAPE, "sp_logits_penalize: rows and cols must be positive (got %lld, %lld)", (long long)rows, (long long)cols);
-    if (cols > INT32_MAX || rows > INT32_MAX || rows * logits_chunks(cols) * LOGITS_THREADS >= (int64_t)1 << 32) return fail(SP_ERR_SHAPE, "sp_logits_penalize: too large");
+    if (cols > INT32_MAX || rows > INT32_MAX || rows * chunks_of(cols, LARGE_CHUNK) * LARGE_THREADS >= (int64_t)1 << 32) return fail(SP_ERR_SHAPE, "sp_logits_penalize: too large");
     if (dtype != SP_F32 && (const void*)out == logits) return fail(SP_ERR_ARG, "sp_logits_penalize: only f32 logits can be overwritten");
     if (history < 0 || history > (int64_t)COUNT_MASK) return fail(SP_ERR_SHAPE, "sp_logits_penalize: history must be in [0, 2^20), got %lld", (long long)history);
     if (n_bias < 0 || n_bias > MOST_ENTRIES) return fail(SP_ERR_SHAPE, "sp_logits_penalize: n_bias must be in [0, 2047], got %lld", (long long)n_bias);
@@ -258,12 +283,16 @@ extern "C" int sp_logits_penalize(int dtype, const void* logits, float* out, int
     a.repetition = repetition; a.presence = presence; a.frequency = frequency; a.temperature = temperature;
     a.bias_ids = bias_ids; a.bias = bias; a.n_bias = (int)n_bias; a.mask = (const unsigned*)mask;
     a.mask_step = mask_rows == rows ? (cols + 31) / 32 : 0;
-    const int64_t chunks = logits_chunks(cols);
+    const int64_t chunks = logits_chunks(rows, cols);
     a.best = (float*)workspace; a.best_at = token != nullptr ? (int*)((float*)workspace + rows * chunks) : nullptr;
-    if (dtype == SP_F32) launch_logits<SP_F32>(logits, rows, cols, a, (hipStream_t)stream);
-    else if (dtype == SP_F16) launch_logits<SP_F16>(logits, rows, cols, a, (hipStream_t)stream);
-    else launch_logits<SP_BF16>(logits, rows, cols, a, (hipStream_t)stream);
-    if (const int launched = check_launch(__func__); launched != SP_OK || token == nullptr || chunks == 1) return launched;
+    auto launch = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        const hipStream_t st = (hipStream_t)stream;
+        return a.tokens != nullptr || a.n_bias > 0 ? launch_logits<DT, true>(logits, rows, cols, (unsigned)chunks, a, st) : launch_logits<DT, false>(logits, rows, cols, (unsigned)chunks, a, st);
+    };
+    const int launched = dtype == SP_F32 ? launch(std::integral_constant<int, SP_F32>{}) : dtype == SP_F16 ? launch(std::integral_constant<int, SP_F16>{})
+                                                                                                          : launch(std::integral_constant<int, SP_BF16>{});
+    if (launched != SP_OK || token == nullptr || chunks == 1) return launched;
     hipLaunchKernelGGL(logits_token_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, (hipStream_t)stream, a.best, a.best_at, (unsigned)chunks, (long)rows, token);
     return check_launch(__func__);
 }

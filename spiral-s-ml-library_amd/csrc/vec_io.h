@@ -31,7 +31,7 @@ __device__ __forceinline__ float element(const u32x4& v, int i) {
     else return half_bits_to_f32<DT>(i & 1 ? v[i >> 1] >> 16 : v[i >> 1] & 0xffffu);
 }
 
-template <int DT>
+template <int DT, int POLICY = ST_PLAIN>
 __device__ __forceinline__ void store16(void* p, long at, long left, const float (&v)[PER16<DT>]) {
     constexpr int E = ELEM_BYTES<DT>, N = PER16<DT>;
     unsigned char* q = (unsigned char*)p + at * E;
@@ -42,7 +42,7 @@ __device__ __forceinline__ void store16(void* p, long at, long left, const float
         else o[i] = pack_halves<DT>(v[2 * i], v[2 * i + 1]);
     }
     if (left >= N) {
-        store_c<ST_PLAIN, E>(q, o);
+        store_c<POLICY, E>(q, o);
         return;
     }
 #pragma unroll
