@@ -19,6 +19,7 @@ constexpr int ENTRY_SHIFT = 21, MOST_ENTRIES = 2047;      // entry j is kept as 
 // would leave most of the chip idle (1 x 32003, a history of 2000: ONE_ROW).  (One workgroup for a whole row, which needs no second launch to
 // choose the token, is slower than both launches: a compute unit alone brings in 24 bytes a cycle, 16 us for 32003 columns.)
 constexpr int LARGE_CHUNK = 8192, LARGE_THREADS = 512, SMALL_CHUNK = 2048, SMALL_THREADS = 256;
+constexpr int AHEAD = 2;                                  // 16-byte pieces of the history per lane that are asked for at once
 
 struct LogitsArgs {
     float* out;
@@ -81,44 +82,51 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const void* logits, lon
     const int32_t* ids = a.bias_ids + row * a.n_bias;
     const float* biases = a.bias + row * a.n_bias;
     if constexpr (SPARSE) {
+        // the history's first tokens and the first biases' columns are asked for before anything waits
+        const int32_t* mine = a.tokens + row * a.history;
+        long length = a.tokens != nullptr ? a.history : 0;
+        auto tokens_at = [&](int v) { return ((long)v * THREADS + tid) * 4; };
+        u32x4 ahead[AHEAD];
+#pragma unroll
+        for (int v = 0; v < AHEAD; ++v) ahead[v] = load16<SP_F32>(mine, tokens_at(v), length - tokens_at(v));
+        const int id = tid < a.n_bias ? ids[tid] : -1;
+        if (a.lengths != nullptr) {
+            const long given = a.lengths[row];
+            length = given < length ? given : length;
+        }
+        long prompt = a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
+        prompt = prompt > 0 ? prompt : 0;
+        // (columns are below 2^31: a token in front of the chunk, or below zero, wraps to a column behind it)
+        const unsigned first = (unsigned)c0;
         for (int i = tid * 4; i < CHUNK; i += THREADS * 4) *reinterpret_cast<u32x4*>(words + i) = u32x4{0u, 0u, 0u, 0u};
         if (tid == 0) again = 0;
         __syncthreads();
-        for (int j = tid; j < a.n_bias; j += THREADS) {
-            const long at = ids[j] - c0;
-            if (at >= 0 && at < here) atomicMax(&words[at], (unsigned)(MOST_ENTRIES - j) << ENTRY_SHIFT);
-        }
+        auto each_bias = [&](auto f) {
+            for (int j = tid; j < a.n_bias; j += THREADS) {
+                const unsigned at = (unsigned)(j == tid ? id : ids[j]) - first;
+                if (at < (unsigned)here) f(at, (unsigned)(MOST_ENTRIES - j));
+            }
+        };
         if (a.n_bias > 0) {
+            each_bias([&](unsigned at, unsigned entry) { atomicMax(&words[at], entry << ENTRY_SHIFT); });
             __syncthreads();
             // (counting goes on meanwhile: it leaves the upper bits alone)
-            for (int j = tid; j < a.n_bias; j += THREADS) {
-                const long at = ids[j] - c0;
-                if (at >= 0 && at < here && words[at] >> ENTRY_SHIFT != (unsigned)(MOST_ENTRIES - j)) again = 1;
-            }
+            each_bias([&](unsigned at, unsigned entry) { if (words[at] >> ENTRY_SHIFT != entry) again = 1; });
         }
-        if (a.tokens != nullptr) {
-            long length = a.history;
-            if (a.lengths != nullptr) {
-                const long given = a.lengths[row];
-                length = given < length ? given : length;
-            }
-            long prompt = a.prompt_lengths != nullptr ? a.prompt_lengths[row] : 0;
-            prompt = prompt > 0 ? prompt : 0;
-            const unsigned first = (unsigned)c0;
-            const int32_t* mine = a.tokens + row * a.history;
-            for (long i = (long)tid * 4; i < length; i += THREADS * 4) {
-                const u32x4 t = load16<SP_F32>(mine, i, length - i);
-                // (columns are below 2^31: a token in front of the chunk or below zero wraps to one behind it)
-                const int left = length - i < 4 ? (int)(length - i) : 4, of_prompt = prompt - i < 4 ? (int)(prompt - i) : 4;
+        auto take = [&](const u32x4& t, long i) {
+            const int left = length - i < 4 ? (int)(length - i) : 4, of_prompt = prompt - i < 4 ? (int)(prompt - i) : 4;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const unsigned at = t[e] - first;
-                    if (at >= (unsigned)here || e >= left) continue;
-                    if (e < of_prompt) atomicOr(&words[at], SEEN_BIT);
-                    else atomicAdd(&words[at], 1u);
-                }
+            for (int e = 0; e < 4; ++e) {
+                const unsigned at = t[e] - first;
+                if (at >= (unsigned)here || e >= left) continue;
+                if (e < of_prompt) atomicOr(&words[at], SEEN_BIT);
+                else atomicAdd(&words[at], 1u);
             }
-        }
+        };
+#pragma unroll
+        for (int v = 0; v < AHEAD; ++v)
+            if (tokens_at(v) < length) take(ahead[v], tokens_at(v));
+        for (long i = tokens_at(AHEAD); i < length; i += THREADS * 4) take(load16<SP_F32>(mine, i, length - i), i);
         __syncthreads();
     }
     Best best{-INFINITY, -1};
