@@ -1,7 +1,7 @@
 // Rows and columns of a matrix in 8-bit blocks of 128 with a scale each: the operands of gemm_scaled.hip.
 //
 // A workgroup takes a tile of 128 x 128 (16 x 128 where only rows are wanted in blocks of one), so every block along either direction lies inside
-// one tile, and x is read once whatever is wanted of it.  A lane holds R rows of 8 columns.  A row's 16 lanes are a DPP row, so the
+// one tile, and x is read once whatever is wanted of it.  A lane holds 1, 4 or 8 rows of 8 columns.  A row's 16 lanes are a DPP row, so the
 // largest magnitude of a row's block takes four DPP steps; a column's takes two cross-lane steps and, over the four waves, LDS.
 // Magnitudes are compared as bits: an infinity is larger than every number and a NaN larger than that, so neither is lost.  The transposed
 // numbers go through LDS so that both forms leave in 128-byte rows.
@@ -57,20 +57,23 @@ struct QuantArgs {
 
 __device__ __forceinline__ unsigned max_u32(unsigned a, unsigned b) { return a > b ? a : b; }
 
-// WIDE: blocks of 128 x 128.  OUT: 1 = q, 2 = q_t, 3 = both.  R: rows per lane.
-template <int DT, int F8, bool WIDE, int OUT, int R>
-__global__ __launch_bounds__(256) void quantize_kernel(const void* x_first, long rows_first, long cols_first, const QuantArgs args) {
+// WIDE: blocks of 128 x 128.  OUT: 1 = q, 2 = q_t, 3 = both.  R: rows per lane, ROWS: of the tile.  POLICY: of the stores (a branch at each
+// store, the compiler folds both sides into a plain one).
+template <int DT, int F8, bool WIDE, int OUT, int R, int ROWS, int POLICY>
+__global__ __launch_bounds__(ROWS / R * 16) void quantize_kernel(const void* x_first, long rows_first, long cols_first, const QuantArgs args) {
     constexpr int E = ELEM_BYTES<DT>, PIECES = 8 / PER16<DT>;
     constexpr bool ROW = (OUT & 1) != 0, COL = (OUT & 2) != 0;
-    static_assert(R == 8 || (!COL && !WIDE), "tiles of fewer rows hold blocks of one row only");
+    constexpr int THREADS = ROWS / R * 16, WAVES = THREADS / 64;
+    static_assert(ROWS == QB || (!COL && !WIDE), "tiles of fewer rows hold blocks of one row only");
+    static_assert(!COL || R == 8 || R == 4, "a lane's rows of a column are one store");
     constexpr int PITCH = QB + 16;            // bytes of a transposed row in LDS
     __shared__ __attribute__((aligned(16))) unsigned char turned[COL ? QB * PITCH : 16];
-    __shared__ unsigned most[COL && !WIDE ? 4 * QB : 4];
+    __shared__ unsigned most[COL && !WIDE ? WAVES * QB : WAVES];
     const long rows = rows_first, cols = cols_first;
     const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4, wave = tid >> 6;
     const long tiles_c = (cols + QB - 1) / QB;
     const long tile_r = blockIdx.x / tiles_c, tile_c = blockIdx.x - tile_r * tiles_c;
-    const long r0 = tile_r * (16 * R) + rg * R, c0 = tile_c * QB + cg * 8;
+    const long r0 = tile_r * ROWS + rg * R, c0 = tile_c * QB + cg * 8;
     u32x4 raw[R][PIECES];
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -79,6 +82,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* x_first, long
             const long col = c0 + p * PER16<DT>;
             raw[i][p] = load16<DT>(x_first, (r0 + i) * cols + col, r0 + i < rows ? cols - col : 0);
         }
+    auto put = [&](auto* to, auto v) { store_c<POLICY, sizeof(v)>(to, v); };
     auto value = [&](int i, int j) { return element<DT>(raw[i][j / PER16<DT>], j % PER16<DT>); };
     auto magnitude = [&](int i, int j) { return __float_as_uint(value(i, j)) & 0x7fffffffu; };
     auto across_row = [](unsigned v) { return group_allreduce<16>(v, max_u32); };      // over the 16 lanes of a row
@@ -96,7 +100,10 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* x_first, long
         m = across_wave(across_row(m));
         if ((tid & 63) == 0) most[wave] = m;
         __syncthreads();
-        one.template set<F8>(max_u32(max_u32(most[0], most[1]), max_u32(most[2], most[3])));
+        m = most[0];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) m = max_u32(m, most[w]);
+        one.template set<F8>(m);
         if (tid == 0) {
             if constexpr (ROW) args.scale[tile_r * args.blocks_c + tile_c] = one.scale;
             if constexpr (COL) args.scale_t[tile_c * args.blocks_r + tile_r] = one.scale;
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* x_first, long
             u32x2 o;
             o.x = pack_f8<F8>(s(value(i, 0)), s(value(i, 1)), s(value(i, 2)), s(value(i, 3)));
             o.y = pack_f8<F8>(s(value(i, 4)), s(value(i, 5)), s(value(i, 6)), s(value(i, 7)));
-            if (r0 + i < rows && c0 < args.pitch) *reinterpret_cast<u32x2*>(args.q + (r0 + i) * args.pitch + c0) = o;
+            if (r0 + i < rows && c0 < args.pitch) put(args.q + (r0 + i) * args.pitch + c0, o);
         }
     }
     if constexpr (COL) {
@@ -133,8 +140,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* x_first, long
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int c = cg * 8 + j;
-                column[j] = max_u32(max_u32(most[c], most[QB + c]), max_u32(most[2 * QB + c], most[3 * QB + c]));
+                column[j] = most[cg * 8 + j];
+#pragma unroll
+                for (int w = 1; w < WAVES; ++w) column[j] = max_u32(column[j], most[w * QB + cg * 8 + j]);
             }
         }
 #pragma unroll
@@ -144,52 +152,56 @@ __global__ __launch_bounds__(256) void quantize_kernel(const void* x_first, long
                 s.template set<F8>(column[j]);
                 if (rg == 0 && c0 + j < cols) args.scale_t[(c0 + j) * args.blocks_r + tile_r] = s.scale;
             }
-            u32x2 o;
-            o.x = pack_f8<F8>(s(value(0, j)), s(value(1, j)), s(value(2, j)), s(value(3, j)));
-            o.y = pack_f8<F8>(s(value(4, j)), s(value(5, j)), s(value(6, j)), s(value(7, j)));
-            *reinterpret_cast<u32x2*>(turned + (cg * 8 + j) * PITCH + rg * 8) = o;
+#pragma unroll
+            for (int i = 0; i < R; i += 4)
+                *reinterpret_cast<unsigned*>(turned + (cg * 8 + j) * PITCH + rg * R + i) =
+                    pack_f8<F8>(s(value(i, j)), s(value(i + 1, j)), s(value(i + 2, j)), s(value(i + 3, j)));
         }
         __syncthreads();
-        // 16 bytes per lane: eight lanes a row of 128 bytes, 32 rows at a time
+        // 16 bytes per lane: eight lanes a row of 128 bytes
         const long at = tile_r * QB + (tid & 7) * 16;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int c = k * 32 + (tid >> 3);
+        for (int k = 0; k < QB * 8 / THREADS; ++k) {
+            const int c = k * (THREADS / 8) + (tid >> 3);
             const u32x4 v = *reinterpret_cast<const u32x4*>(turned + c * PITCH + (tid & 7) * 16);
-            if (tile_c * QB + c < cols && at < args.pitch_t) *reinterpret_cast<u32x4*>(args.q_t + (tile_c * QB + c) * args.pitch_t + at) = v;
+            if (tile_c * QB + c < cols && at < args.pitch_t) put(args.q_t + (tile_c * QB + c) * args.pitch_t + at, v);
         }
     }
 }
 
 // ---- host side -------------------------------------------------------------------------------
 
-template <int DT, int F8, bool WIDE, int OUT, int R>
+template <int DT, int F8, bool WIDE, int OUT, int R, int ROWS, int POLICY>
 static int launch_quantize(const QuantArgs& a, hipStream_t stream) {
-    const long tiles = ((a.rows + 16 * R - 1) / (16 * R)) * a.blocks_c;
-    if (tiles * 256 >= 1l << 32) return fail(SP_ERR_SHAPE, "sp_quantize_blocks: too large");
-    hipLaunchKernelGGL((quantize_kernel<DT, F8, WIDE, OUT, R>), dim3((unsigned)tiles), dim3(256), 0, stream, a.x, a.rows, a.cols, a);
+    constexpr int THREADS = ROWS / R * 16;
+    const long tiles = ((a.rows + ROWS - 1) / ROWS) * a.blocks_c;
+    if (tiles * THREADS >= 1l << 32) return fail(SP_ERR_SHAPE, "sp_quantize_blocks: too large");
+    hipLaunchKernelGGL((quantize_kernel<DT, F8, WIDE, OUT, R, ROWS, POLICY>), dim3((unsigned)tiles), dim3(THREADS), 0, stream, a.x, a.rows, a.cols, a);
     return check_launch("sp_quantize_blocks");
 }
 
-template <int DT, int F8>
+// Rows per lane of the 128 x 128 tiles: 4 (eight waves) where a tile has one scale, 8 where every row or column has its own, whose steps across
+// lanes count then.  (us, 8 / 4 rows: 8192 x 4096 bf16 both ways in 128 x 128 blocks 23.8 / 22.2; 16384 x 4096 both ways in rows of 128
+// 59.3 / 66.2, transposed alone 43.5 / 48.5.  Written back instead of streamed 27.5 / 25.8, 62.8 / 67.7, 44.9 / 49.)
+template <int DT, int F8, int POLICY>
 static int quantize(const QuantArgs& a, bool wide, hipStream_t stream) {
     const int out = (a.q != nullptr ? 1 : 0) | (a.q_t != nullptr ? 2 : 0);
     if (wide) {
-        if (out == 1) return launch_quantize<DT, F8, true, 1, 8>(a, stream);
-        if (out == 2) return launch_quantize<DT, F8, true, 2, 8>(a, stream);
-        return launch_quantize<DT, F8, true, 3, 8>(a, stream);
+        if (out == 1) return launch_quantize<DT, F8, true, 1, 4, QB, POLICY>(a, stream);
+        if (out == 2) return launch_quantize<DT, F8, true, 2, 4, QB, POLICY>(a, stream);
+        return launch_quantize<DT, F8, true, 3, 4, QB, POLICY>(a, stream);
     }
-    if (out == 1) return launch_quantize<DT, F8, false, 1, 1>(a, stream);
-    if (out == 2) return launch_quantize<DT, F8, false, 2, 8>(a, stream);
-    return launch_quantize<DT, F8, false, 3, 8>(a, stream);
+    if (out == 1) return launch_quantize<DT, F8, false, 1, 1, 16, POLICY>(a, stream);
+    if (out == 2) return launch_quantize<DT, F8, false, 2, 8, QB, POLICY>(a, stream);
+    return launch_quantize<DT, F8, false, 3, 8, QB, POLICY>(a, stream);
 }
 
 namespace {
 struct QuantizeKernelNames {
     QuantizeKernelNames() {
-        register_kernel("quantize_rows", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 1, 1>, 256);
-        register_kernel("quantize_both", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 3, 8>, 256);
-        register_kernel("quantize_both_128", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, true, 3, 8>, 256);
+        register_kernel("quantize_rows", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 1, 1, 16, ST_STREAM>, 256);
+        register_kernel("quantize_both", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 3, 8, QB, ST_STREAM>, 256);
+        register_kernel("quantize_both_128", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, true, 3, 4, QB, ST_STREAM>, 512);
     }
 } quantize_kernel_names;
 }  // namespace
@@ -219,10 +231,15 @@ extern "C" int sp_quantize_blocks(int dtype, int f8, int32_t block_rows, const v
     a.x = x; a.q = (unsigned char*)q; a.q_t = (unsigned char*)q_t; a.scale = scale; a.scale_t = scale_t; a.rows = rows; a.cols = cols;
     a.pitch = (cols + 15) / 16 * 16; a.pitch_t = (rows + 15) / 16 * 16;
     a.blocks_c = (cols + QB - 1) / QB; a.blocks_r = (rows + QB - 1) / QB;
+    // results that do not stay in the caches (32 MiB of L2) are streamed past them
+    const bool large = ((q != nullptr ? rows * a.pitch : 0) + (q_t != nullptr ? cols * a.pitch_t : 0)) > (int64_t)32 << 20;
     const bool wide = block_rows == QB;
+    auto by_policy = [&](auto dt, auto type) {
+        constexpr int DT = decltype(dt)::value, F8 = decltype(type)::value;
+        return large ? quantize<DT, F8, ST_STREAM>(a, wide, (hipStream_t)stream) : quantize<DT, F8, ST_PLAIN>(a, wide, (hipStream_t)stream);
+    };
     auto by_f8 = [&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-        return f8 == SP_F8_E4M3 ? quantize<DT, SP_F8_E4M3>(a, wide, (hipStream_t)stream) : quantize<DT, SP_F8_E5M2>(a, wide, (hipStream_t)stream);
+        return f8 == SP_F8_E4M3 ? by_policy(dt, std::integral_constant<int, SP_F8_E4M3>{}) : by_policy(dt, std::integral_constant<int, SP_F8_E5M2>{});
     };
     if (dtype == SP_F32) return by_f8(std::integral_constant<int, SP_F32>{});
     if (dtype == SP_F16) return by_f8(std::integral_constant<int, SP_F16>{});
