@@ -23,14 +23,14 @@ __device__ __forceinline__ void put16(bool stream, void* p, long at, long left, 
     else store16<DT>(p, at, left, v);
 }
 
-// The sum of v over a group of T lanes, T a multiple of 64 up to the workgroup: through `slots` (T / 64 floats of LDS of this group).
-// A group wider than a wave is joined by a barrier of the whole workgroup; `slots` must not be used again before another one.
+// The sums of v over a group of T lanes, a power of two.  A group wider than a wave goes through `slots` (T / 64 floats per sum of LDS of this group) and
+// is joined by a barrier of the whole workgroup; `slots` must not be used again before another one.
 template <int T, int N>
 __device__ __forceinline__ void group_sums(float (&v)[N], float* slots) {
     constexpr int W = T / 64;
     auto add = [](float a, float b) { return a + b; };
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = group_reduce<64>(v[i], add);
+    for (int i = 0; i < N; ++i) v[i] = group_reduce<T < 64 ? T : 64>(v[i], add);
     if constexpr (W > 1) {
         const int wave = (threadIdx.x % T) >> 6;
         if ((threadIdx.x & 63) == 0)
@@ -47,12 +47,58 @@ __device__ __forceinline__ void group_sums(float (&v)[N], float* slots) {
     }
 }
 
+// The N columns that piece `at` of a row stands for: from `col` on, of which the first `skip` are its neighbour's.  The last piece of a row that is no
+// multiple of N begins where its 16 bytes end with the row, so that it is one load and one store like the others (element by
+// element 33554432 / 2500 rows of 2500 bf16, forward and backward, took 143 us, whole 70): what it has twice counts once, and is stored twice with
+// the same bits.  A row of fewer than N columns is one piece, loaded element by element.
+// WHOLE: rows are a multiple of N, and there is none of that to keep track of (16384 x 4096 bf16, forward and backward, 134 us without it, 129 with).
+template <int N, bool WHOLE>
+struct Piece {
+    int col, skip;
+    __device__ __forceinline__ Piece(int at, int cols) {
+        const int wanted = at * N, last = cols - N;
+        if constexpr (WHOLE) {
+            col = wanted;
+            skip = wanted < cols ? 0 : N;
+        } else {
+            col = wanted <= last || cols < N ? wanted : last;
+            skip = wanted < cols ? wanted - col : N;
+            col = skip < N ? col : 0;
+        }
+    }
+    __device__ __forceinline__ bool mine() const { return skip < N; }
+    // Whether element i is a column that this piece counts.
+    __device__ __forceinline__ bool counts(int i, int cols) const { return WHOLE ? mine() : i >= skip && col + i < cols; }
+    template <int DT>
+    __device__ __forceinline__ u32x4 load(const void* p, long row_at, int cols, bool ok) const {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (!WHOLE && cols < N) v = load16<DT>(p, row_at + col, ok && mine() ? cols - col : 0);
+        else if (ok && mine()) v = load_aligned<WHOLE ? 16 : ELEM_BYTES<DT>, u32x4>((const unsigned char*)p + (row_at + col) * ELEM_BYTES<DT>);
+        return v;
+    }
+};
+// N weights from column `col` on (all of them exist where the row has N columns).
+template <int WT, int N, bool WHOLE>
+__device__ __forceinline__ void load_weights(const void* weight, float otherwise, const Piece<N, WHOLE>& piece, int cols, float (&w)[N]) {
+    const int col = piece.col;
+#pragma unroll
+    for (int h = 0; h < N; h += PER16<WT>) {
+        u32x4 v = {0u, 0u, 0u, 0u};
+        if (weight != nullptr && (!WHOLE || piece.mine())) {
+            if (!WHOLE && cols < N) v = load16<WT>(weight, col + h, cols - col - h);
+            else v = load_aligned<WHOLE ? 16 : ELEM_BYTES<WT>, u32x4>((const unsigned char*)weight + (col + h) * ELEM_BYTES<WT>);
+        }
+#pragma unroll
+        for (int i = 0; i < PER16<WT>; ++i) w[h + i] = weight != nullptr ? element<WT>(v, i) : otherwise;
+    }
+}
+
 // T lanes per row, C 16-byte pieces of it per lane; a workgroup takes ROWS rows at a time.
-template <int DT, int WT, int T, int C>
+template <int DT, int WT, int T, int C, bool WHOLE>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const void* x, const void* weight, const void* bias, void* y, long rows,
                                                                       int cols, float eps, float* mean_out, float* rstd_out) {
     constexpr int N = PER16<DT>, ROWS = T < 256 ? 256 / T : 1;
-    __shared__ float slots[2][T / 64 * ROWS];
+    __shared__ float slots[2][T < 64 ? 1 : T / 64 * ROWS];
     const int t = threadIdx.x % T, group = threadIdx.x / T;
     const float count = (float)cols;
     const bool stream = streamed(rows, cols, ELEM_BYTES<DT>);
@@ -61,25 +107,24 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const voi
         const bool ok = row < rows;                        // (one row per workgroup: always)
         u32x4 raw[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int col = (c * T + t) * N;
-            raw[c] = load16<DT>(x, row * cols + col, ok ? cols - col : 0);
-        }
+        for (int c = 0; c < C; ++c) raw[c] = Piece<N, WHOLE>(c * T + t, cols).template load<DT>(x, row * cols, cols, ok);
         float s[1] = {0.f};
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c) {
+            const Piece<N, WHOLE> piece(c * T + t, cols);
 #pragma unroll
-            for (int i = 0; i < N; ++i) s[0] += element<DT>(raw[c], i);
+            for (int i = 0; i < N; ++i) s[0] += piece.counts(i, cols) ? element<DT>(raw[c], i) : 0.f;
+        }
         group_sums<T>(s, slots[0] + group * (T / 64));
         const float mean = s[0] / count;       // (the mean of equal numbers is that number)
         float q[1] = {0.f};
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int left = cols - (c * T + t) * N;
+            const Piece<N, WHOLE> piece(c * T + t, cols);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float d = element<DT>(raw[c], i) - mean;
-                q[0] += i < left ? d * d : 0.f;
+                q[0] += piece.counts(i, cols) ? d * d : 0.f;
             }
         }
         group_sums<T>(q, slots[1] + group * (T / 64));
@@ -90,49 +135,31 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const voi
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int col = (c * T + t) * N;
-            if (!ok || col >= cols) continue;
+            const Piece<N, WHOLE> piece(c * T + t, cols);
+            if (!ok || !piece.mine()) continue;
             float w[N], b[N], o[N];
-#pragma unroll
-            for (int h = 0; h < N; h += PER16<WT>) {
-                u32x4 wv = {0u, 0u, 0u, 0u}, bv = wv;
-                if (weight != nullptr) wv = load16<WT>(weight, col + h, cols - col - h);
-                if (bias != nullptr) bv = load16<WT>(bias, col + h, cols - col - h);
-#pragma unroll
-                for (int i = 0; i < PER16<WT>; ++i) {
-                    w[h + i] = weight != nullptr ? element<WT>(wv, i) : 1.f;
-                    b[h + i] = element<WT>(bv, i);
-                }
-            }
+            load_weights<WT>(weight, 1.f, piece, cols, w);
+            load_weights<WT>(bias, 0.f, piece, cols, b);
 #pragma unroll
             for (int i = 0; i < N; ++i) o[i] = (element<DT>(raw[c], i) - mean) * rstd * w[i] + b[i];
-            put16<DT>(stream, y, row * cols + col, cols - col, o);
+            put16<DT>(stream, y, row * cols + piece.col, cols - piece.col, o);
         }
     }
 }
 
 // T lanes per row, C pieces of it per lane, 1024 / T rows at a time in a workgroup; SUMS: dweight and dbias are wanted.
 // With 8 columns per lane the weights and the next row fit its 128 registers as well; with 16 (rows of more than 8192) they do not.
-template <int DT, int WT, int T, int C, bool SUMS>
+template <int DT, int WT, int T, int C, bool SUMS, bool WHOLE>
 __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* dy, const void* x, const float* mean, const float* rstd, long rows,
                                                                   int cols, const void* weight, void* dx, float* partial) {
-    constexpr int N = PER16<DT>, GROUPS = 1024 / T, W = T / 64;
+    constexpr int N = PER16<DT>, GROUPS = 1024 / T, W = T < 64 ? 1 : T / 64;
     constexpr bool AHEAD = C * N <= 8;
     extern __shared__ __attribute__((aligned(16))) float sums[];          // SUMS: 512 lanes x C N floats
     __shared__ float slots[2][GROUPS * 2 * W];
     const int t = threadIdx.x % T, group = threadIdx.x / T;
     const float count = (float)cols;
     const bool stream = streamed(rows, cols, ELEM_BYTES<DT>);
-    auto load_weight = [&](int c, float(&w)[N]) {
-        const int col = (c * T + t) * N;
-#pragma unroll
-        for (int h = 0; h < N; h += PER16<WT>) {
-            u32x4 v = {0u, 0u, 0u, 0u};
-            if (weight != nullptr) v = load16<WT>(weight, col + h, cols - col - h);
-#pragma unroll
-            for (int i = 0; i < PER16<WT>; ++i) w[h + i] = weight != nullptr ? element<WT>(v, i) : 1.f;
-        }
-    };
+    auto load_weight = [&](int c, float(&w)[N]) { load_weights<WT>(weight, 1.f, Piece<N, WHOLE>(c * T + t, cols), cols, w); };
     float kept[AHEAD ? C : 1][N], dw[C][N], db[C][N];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -146,9 +173,9 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
         const bool ok = row < rows;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int col = (c * T + t) * N;
-            xr[c] = load16<DT>(x, row * cols + col, ok ? cols - col : 0);
-            gr[c] = load16<DT>(dy, row * cols + col, ok ? cols - col : 0);
+            const Piece<N, WHOLE> piece(c * T + t, cols);
+            xr[c] = piece.template load<DT>(x, row * cols, cols, ok);
+            gr[c] = piece.template load<DT>(dy, row * cols, cols, ok);
         }
         m = ok ? mean[row] : 0.f;
         r = ok ? rstd[row] : 0.f;
@@ -168,12 +195,13 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int left = cols - (c * T + t) * N;
+            const Piece<N, WHOLE> piece(c * T + t, cols);
             float now[N];
             if constexpr (!AHEAD) load_weight(c, now);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float d = element<DT>(gv[c], i), h = i < left ? (element<DT>(xv[c], i) - mu) * rs : 0.f, g = d * (AHEAD ? kept[AHEAD ? c : 0][i] : now[i]);
+                const bool counts = piece.counts(i, cols);
+                const float d = counts ? element<DT>(gv[c], i) : 0.f, h = counts ? (element<DT>(xv[c], i) - mu) * rs : 0.f, g = d * (AHEAD ? kept[AHEAD ? c : 0][i] : now[i]);
                 s[0] += g;
                 s[1] += g * h;
                 dw[c][i] += d * h;
@@ -185,8 +213,8 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
         const float a = s[0] / count, b = s[1] / count;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int col = (c * T + t) * N;
-            if (row >= rows || col >= cols) continue;
+            const Piece<N, WHOLE> piece(c * T + t, cols);
+            if (row >= rows || !piece.mine()) continue;
             float o[N], now[N];
             if constexpr (!AHEAD) load_weight(c, now);
 #pragma unroll
@@ -194,7 +222,7 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
                 const float g = element<DT>(gv[c], i) * (AHEAD ? kept[AHEAD ? c : 0][i] : now[i]), h = (element<DT>(xv[c], i) - mu) * rs;
                 o[i] = rs * (g - a - h * b);
             }
-            put16<DT>(stream, dx, row * cols + col, cols - col, o);
+            put16<DT>(stream, dx, row * cols + piece.col, cols - piece.col, o);
         }
     }
     if constexpr (SUMS) {
@@ -221,17 +249,15 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
         if (group == 0) {
             float* out = partial + (long)blockIdx.x * 2 * cols;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c) {
+                const Piece<N, WHOLE> piece(c * T + t, cols);
 #pragma unroll
-                for (int h = 0; h < N; h += 4) {
-                    const int col = (c * T + t) * N + h;
-                    const float ow[4] = {dw[c][h], dw[c][h + 1], dw[c][h + 2], dw[c][h + 3]};
-                    const float ob[4] = {db[c][h], db[c][h + 1], db[c][h + 2], db[c][h + 3]};
-                    if (col < cols) {
-                        store16<SP_F32>(out, col, cols - col, ow);
-                        store16<SP_F32>(out, cols + col, cols - col, ob);
+                for (int i = 0; i < N; ++i)
+                    if (piece.counts(i, cols)) {
+                        out[piece.col + i] = dw[c][i];
+                        out[cols + piece.col + i] = db[c][i];
                     }
-                }
+            }
         }
     }
 }
@@ -276,25 +302,36 @@ struct NormArgs {
     hipStream_t stream;
 };
 
+template <int DT>
+static bool whole_pieces(const NormArgs& a) { return a.cols % PER16<DT> == 0; }
+
 template <int DT, int WT, int T, int C>
 static int launch_forward(const NormArgs& a) {
     constexpr int THREADS = T < 256 ? 256 : T, ROWS = THREADS / T;
     const long blocks = (a.rows + ROWS - 1) / ROWS, most = 1l << 20;       // (a launch counts its work items in 32 bits)
-    hipLaunchKernelGGL((layer_norm_kernel<DT, WT, T, C>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(THREADS), 0, a.stream, a.x,
+    auto kernel = whole_pieces<DT>(a) ? layer_norm_kernel<DT, WT, T, C, true> : layer_norm_kernel<DT, WT, T, C, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(THREADS), 0, a.stream, a.x,
                        a.weight, a.bias, a.y, a.rows, a.cols, a.eps, a.mean, a.rstd);
     return check_launch("sp_layer_norm");
 }
 
 template <int DT, int WT>
 static int forward(const NormArgs& a) {
+    // few lanes per row as long as a wave can hold it; three pieces per lane where four would leave a quarter of them idle
     const int pieces = (a.cols + PER16<DT> - 1) / PER16<DT>;
+    if (pieces <= 8) return launch_forward<DT, WT, 8, 1>(a);
+    if (pieces <= 16) return launch_forward<DT, WT, 16, 1>(a);
+    if (pieces <= 32) return launch_forward<DT, WT, 32, 1>(a);
     if (pieces <= 64) return launch_forward<DT, WT, 64, 1>(a);
     if (pieces <= 128) return launch_forward<DT, WT, 64, 2>(a);
     if (pieces <= 256) return launch_forward<DT, WT, 64, 4>(a);
     if (pieces <= 512) return a.rows <= 2 * device_cu_count() ? launch_forward<DT, WT, 512, 1>(a) : launch_forward<DT, WT, 256, 2>(a);   // (16 x 4096 bf16 3.1 us, 3.4; 16384 rows 80, 68)
+    if (pieces <= 768) return launch_forward<DT, WT, 256, 3>(a);
     if (pieces <= 1024) return launch_forward<DT, WT, 256, 4>(a);
-    if (pieces <= 2048) return launch_forward<DT, WT, 1024, 2>(a);
-    return launch_forward<DT, WT, 1024, 4>(a);
+    if (pieces <= 1536) return launch_forward<DT, WT, 512, 3>(a);
+    if constexpr (DT == SP_F32)
+        if (pieces > 2048) return launch_forward<DT, WT, 1024, 4>(a);
+    return launch_forward<DT, WT, 512, 4>(a);
 }
 
 static int backward_blocks(int64_t rows) {
@@ -306,7 +343,7 @@ template <int DT, int WT, int T, int C, bool SUMS>
 static int launch_backward(const NormArgs& a) {
     constexpr int GROUPS = 1024 / T;
     const int blocks = (int)std::min<long>(backward_blocks(a.rows), (a.rows + GROUPS - 1) / GROUPS);
-    auto kernel = layer_norm_backward_kernel<DT, WT, T, C, SUMS>;
+    auto kernel = whole_pieces<DT>(a) ? layer_norm_backward_kernel<DT, WT, T, C, SUMS, true> : layer_norm_backward_kernel<DT, WT, T, C, SUMS, false>;
     const int lds_bytes = SUMS && GROUPS > 1 ? 512 * C * PER16<DT> * 4 : 0;
     if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(1024), lds_bytes, a.stream, a.dy, a.x, a.mean_in, a.rstd_in, a.rows, a.cols, a.weight, a.dx, a.partial);
@@ -318,6 +355,9 @@ static int launch_backward(const NormArgs& a) {
 template <int DT, int WT, bool SUMS>
 static int backward(const NormArgs& a) {
     constexpr int C = 8 / PER16<DT>;                       // 8 columns per lane
+    if (a.cols <= 8 * 8) return launch_backward<DT, WT, 8, C, SUMS>(a);
+    if (a.cols <= 16 * 8) return launch_backward<DT, WT, 16, C, SUMS>(a);
+    if (a.cols <= 32 * 8) return launch_backward<DT, WT, 32, C, SUMS>(a);
     if (a.cols <= 64 * 8) return launch_backward<DT, WT, 64, C, SUMS>(a);
     if (a.cols <= 128 * 8) return launch_backward<DT, WT, 128, C, SUMS>(a);
     if (a.cols <= 256 * 8) return launch_backward<DT, WT, 256, C, SUMS>(a);
@@ -352,8 +392,8 @@ static int check_norm(const char* fn, int dtype, int weight_dtype, int64_t rows,
 namespace {
 struct NormKernelNames {
     NormKernelNames() {
-        register_kernel("layer_norm", (const void*)layer_norm_kernel<SP_BF16, SP_F32, 256, 2>, 256);
-        register_kernel("layer_norm_backward", (const void*)layer_norm_backward_kernel<SP_BF16, SP_F32, 256, 2, true>, 1024);
+        register_kernel("layer_norm", (const void*)layer_norm_kernel<SP_BF16, SP_F32, 256, 2, true>, 256);
+        register_kernel("layer_norm_backward", (const void*)layer_norm_backward_kernel<SP_BF16, SP_F32, 512, 1, true, true>, 1024);
     }
 } norm_kernel_names;
 }  // namespace

@@ -14,8 +14,8 @@ U = 2.0 ** -24
 CHAIN = 64 + 6 + 15 + 1                  # and the product by 1 / cols; 1 / cols itself is off by u
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 # one lane, one wave, several; a piece of 16 bytes more or less; every width of group and the widest row
-SHAPES = [(1, 1), (1, 2), (3, 7), (5, 8), (257, 9), (4, 64), (7, 255), (300, 512), (2, 513), (9, 1003), (33, 1024), (513, 1025), (16, 2047),
-          (1, 4096), (5, 4097), (6, 8192), (3, 8200), (2, 16383), (3, 16384)]
+SHAPES = [(1, 1), (1, 2), (3, 7), (5, 8), (257, 9), (1000, 24), (70, 33), (4, 64), (131, 65), (515, 128), (35, 200), (7, 255), (300, 512), (2, 513), (9, 1003), (33, 1024), (513, 1025), (16, 2047),
+          (1, 4096), (5, 4097), (600, 2500), (4, 6000), (6, 8192), (3, 8200), (2, 12001), (2, 16383), (3, 16384)]
 
 
 @pytest.fixture(scope="module")
@@ -121,6 +121,20 @@ def test_leading_dimensions_and_in_place(P):
     dx, dw, db = P.layer_norm_backward(dy, x, mean, rstd, w)
     dz = dy.clone()
     assert P.layer_norm_backward(dz, x, mean, rstd, w, out=dz)[0] is dz and torch.equal(dx, dz)
+
+
+@pytest.mark.parametrize("cols", [3, 9, 203, 1003, 2501, 5003, 9001])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_in_place_at_widths_that_end_inside_a_piece(P, cols, dtype):
+    """The last piece of such a row overlaps the one before it."""
+    announce("layer_norm in place %d %s" % (cols, dtype))
+    x, w, b, dy = (v.cuda() for v in make(131, cols, TYPES[dtype], torch.float32, 10))
+    y, mean, rstd = P.layer_norm(x, w, b, want_stats=True)
+    z, dz = x.clone(), dy.clone()
+    P.layer_norm(z, w, b, out=z)
+    dx = P.layer_norm_backward(dy, x, mean, rstd, w)[0]
+    P.layer_norm_backward(dz, x, mean, rstd, w, out=dz)
+    assert torch.equal(y, z) and torch.equal(dx, dz)
 
 
 def backward64(dy, x, mean, rstd, w):
