@@ -193,13 +193,15 @@ __device__ __forceinline__ void scaled_tile_of_block(int pid, int tiles_m, int t
     tn = in / rows;
 }
 
-// Scales come in for eight blocks of K at a time, eight rows per instruction: 32 bytes of a row lie side by side, so that a load asks for eight
-// lines of memory and not for 64 (one block at a time, as many lines as the operands, 8192^3 took 517 us against 501).
-constexpr int SCALE_BLOCKS = 8;
+// Scales come in for several blocks of K at a time, a chunk: SB = 8 of them of eight rows, or 4 of sixteen, per instruction.  The scales of a row's blocks lie side
+// by side, so that a load asks for eight or sixteen lines of memory and not for 64 (one block at a time, as many lines as the operands, 8192^3 took
+// 517 us against 501).
+constexpr int SCALE_BLOCKS = 8, SPLIT_BLOCKS = 4;
 
-// Lane l's scale is that of row l / 8 and block l % 8 of what `row` and `first` say; to LDS bytes lds_addr + 4 l.
+// Lane l's scale is that of row l / SB and block l % SB of what `row` and `first` say; to LDS bytes lds_addr + 4 l.
+template <int SB>
 __device__ __forceinline__ void dma_scales(const float* scales, long row, long last_row, long first, long blocks, int lane, unsigned lds_addr) {
-    const long r = row + (lane >> 3) < last_row ? row + (lane >> 3) : last_row, k = first + (lane & 7) < blocks ? first + (lane & 7) : blocks - 1;
+    const long r = row + lane / SB < last_row ? row + lane / SB : last_row, k = first + lane % SB < blocks ? first + lane % SB : blocks - 1;
     const float* at = scales + r * blocks + k;
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(at), "s"(lds_addr) : "memory", "m0");
 }
@@ -251,7 +253,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
         if (group >= GROUPS || chunk * SCALE_BLOCKS >= nk) return;
         const bool of_a = group < GROUPS_A;
         const unsigned to = scale_lds + (chunk & 1) * SCALE_STAGE + group * 256;
-        dma_scales(of_a ? g.scale_a : g.scale_b, of_a ? m0 + group * 8 : (n0 >> SHIFT) + (group - GROUPS_A) * 8, of_a ? g.M - 1 : last_sb,
+        dma_scales<SCALE_BLOCKS>(of_a ? g.scale_a : g.scale_b, of_a ? m0 + group * 8 : (n0 >> SHIFT) + (group - GROUPS_A) * 8, of_a ? g.M - 1 : last_sb,
                    (long)chunk * SCALE_BLOCKS, nk, lane, to);
     };
     auto fetch_part = [&](int kt, unsigned stage, auto FROM_, auto TO_) {
@@ -397,9 +399,9 @@ template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int NS>
 __global__ __launch_bounds__(256) void gemm_scaled_split_kernel(const ScaledArgs g) {
     constexpr int KS = 4;
     constexpr int NIA = 2 * TM, ND = 2 * (TM + TN);     // DMA instructions per block
-    constexpr int GROUPS_A = 2 * TM, GROUPS = GROUPS_A + (SHIFT == 7 ? 1 : 2 * TN);       // of eight rows of scales
+    constexpr int GROUPS_A = TM, GROUPS = GROUPS_A + (SHIFT == 7 ? 1 : TN);               // of sixteen rows of scales
     constexpr int STAGE = ND * 8 * ROW_BYTES, WAVE_LDS = NS * STAGE + 2 * GROUPS * 256;
-    static_assert((NS - 1) * ND < 64 && NS < SCALE_BLOCKS, "vmcnt counts to 63; scales are asked for a chunk ahead of their operands");
+    static_assert((NS - 1) * ND < 64 && NS <= SPLIT_BLOCKS, "vmcnt counts to 63; scales are asked for a chunk ahead of their operands");
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fi = lane & 15, fq = lane >> 4;
     int tm, tn;
@@ -426,8 +428,8 @@ __global__ __launch_bounds__(256) void gemm_scaled_split_kernel(const ScaledArgs
 #pragma unroll
         for (int q = 0; q < GROUPS; ++q) {
             const bool of_a = q < GROUPS_A;
-            dma_scales(of_a ? g.scale_a : g.scale_b, of_a ? m0 + q * 8 : (n0 >> SHIFT) + (q - GROUPS_A) * 8, of_a ? g.M - 1 : last_sb,
-                       (long)first + chunk * SCALE_BLOCKS, nk, lane, my_lds + NS * STAGE + ((chunk & 1) * GROUPS + q) * 256);
+            dma_scales<SPLIT_BLOCKS>(of_a ? g.scale_a : g.scale_b, of_a ? m0 + q * 16 : (n0 >> SHIFT) + (q - GROUPS_A) * 16, of_a ? g.M - 1 : last_sb,
+                       (long)first + chunk * SPLIT_BLOCKS, nk, lane, my_lds + NS * STAGE + ((chunk & 1) * GROUPS + q) * 256);
         }
     };
     auto fetch = [&](int kt, unsigned stage) {
@@ -461,7 +463,7 @@ __global__ __launch_bounds__(256) void gemm_scaled_split_kernel(const ScaledArgs
         if (t + NS <= mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * ND) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         const unsigned char* at = ring + stage * STAGE;
-        const float* scales = reinterpret_cast<const float*>(ring + NS * STAGE + (t >> 3 & 1) * (GROUPS * 256)) + (t & 7);
+        const float* scales = reinterpret_cast<const float*>(ring + NS * STAGE + (t / SPLIT_BLOCKS & 1) * (GROUPS * 256)) + t % SPLIT_BLOCKS;
         u32x4 ra[TM][2], rb[TN][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -473,21 +475,21 @@ __global__ __launch_bounds__(256) void gemm_scaled_split_kernel(const ScaledArgs
         float sa[TM];
         f32x4 sb[TN];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) sa[i] = scales[(16 * i + fi) * SCALE_BLOCKS];
+        for (int i = 0; i < TM; ++i) sa[i] = scales[(16 * i + fi) * SPLIT_BLOCKS];
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             if constexpr (SHIFT == 7) {
                 sb[j][0] = scales[GROUPS_A * 64];             // (a tile lies inside one block of 128 rows of B)
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sb[j][e] = scales[(16 * (TM + j) + 4 * fq + e) * SCALE_BLOCKS];
+                for (int e = 0; e < 4; ++e) sb[j][e] = scales[(16 * (TM + j) + 4 * fq + e) * SPLIT_BLOCKS];
             }
         }
         if (t + NS < mine) {
             // the stage is free once all of it is in registers, and so is, with the first block of a chunk, the chunk before it
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (t % SCALE_BLOCKS == 0 && t + SCALE_BLOCKS < mine) fetch_scales(t / SCALE_BLOCKS + 1);
+            if (t % SPLIT_BLOCKS == 0 && t + SPLIT_BLOCKS < mine) fetch_scales(t / SPLIT_BLOCKS + 1);
             fetch(first + t + NS, stage);
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -550,7 +552,7 @@ static int launch_tile(ScaledArgs g, hipStream_t stream) {
 template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int NS>
 static int launch_split(ScaledArgs g, hipStream_t stream) {
     auto kernel = gemm_scaled_split_kernel<F8A, F8B, FAST, SHIFT, TM, TN, NS>;
-    constexpr int ring = 4 * (NS * 2 * (TM + TN) * 8 * ROW_BYTES + 2 * (2 * TM + (SHIFT == 7 ? 1 : 2 * TN)) * 256), partial = TM * TN * 4096;
+    constexpr int ring = 4 * (NS * 2 * (TM + TN) * 8 * ROW_BYTES + 2 * (TM + (SHIFT == 7 ? 1 : TN)) * 256), partial = TM * TN * 4096;
     constexpr int lds_bytes = ring > partial ? ring : partial;
     if (const int rc = check_tiles(g, 16 * TM, 16 * TN, 256); rc != SP_OK) return rc;
     if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
@@ -563,7 +565,7 @@ static int launch_split(ScaledArgs g, hipStream_t stream) {
 // Measured, bf16 C and scales of 128 x 128 of B unless said otherwise (us): 4096^3 256 x 256 65, 128 x 256 90, 128 x 128 92;
 // 2048 x 4096 x 4096 56, 43, 43.5; 1024 x 4096 x 4096 128 x 256 35, 128 x 128 28.5, split 64 x 64 50; 512 x 4096 x 4096 128 x 128 26.7, split 64 x 64 26;
 // 256 x 4096 x 4096 26.5, 14.2, split 32 x 32 15.9; 128 x 4096 x 4096 26.4, 14, 10; 64 x 4096 x 4096 split 64 x 64 13.9, 32 x 32 6.9;
-// 49 x 32003 x 4096 split 64 x 64 37, 32 x 32 40; 32 x 32003 x 4096 35, 32; 1 x 4096 x 4096 split 32 x 32 6.8, 16 x 16 5.6;
+// 49 x 32003 x 4096 split 64 x 64 33, 32 x 32 41 (f32 C 36, 42: two workgroups of 64 x 64 on a unit; with more LDS for scales, one, 37 and 39); 32 x 32003 x 4096 35, 32; 1 x 4096 x 4096 split 32 x 32 6.8, 16 x 16 5.6;
 // 1 x 16384 x 16384 62, 54; 4096 x 2048 x 5008, f32 C and scales per row of B: 128 x 256 89, 128 x 128 101.  (256 x 256 with C of f32, or scales per row of B,
 // has no room for the f16 fragments, or the scales, in its registers.)
 template <int F8A, int F8B, bool FAST, int SHIFT>
