@@ -16,8 +16,9 @@ namespace sp {
 constexpr unsigned COUNT_MASK = (1u << 20) - 1u, SEEN_BIT = 1u << 20;
 constexpr int ENTRY_SHIFT = 21, MOST_ENTRIES = 2047;      // entry j is kept as 2047 - j: the first one is the largest, 0 is none
 // Columns to a workgroup: enough of them that reading the history again for every chunk of a row does not count; fewer where the large chunks
-// would leave most of the chip idle (1 x 32003, a history of 2000: 4 chunks 13.3 us with the token, 16 chunks 8.5).  (One workgroup for a whole row, which needs no second launch to
-// choose the token, is slower than both launches: a compute unit alone brings in 24 bytes a cycle, 16 us for 32003 columns.)
+// would leave most of the chip idle (1 x 32003, a history of 2000, with the token: 4 chunks 13.3 us, 16 chunks 8.5).  (One workgroup for a whole
+// row, which needs no second launch to choose the token, is slower than both launches: a compute unit alone brings in 24 bytes a cycle, 16 us for
+// 32003 columns.)
 constexpr int LARGE_CHUNK = 8192, LARGE_THREADS = 512, SMALL_CHUNK = 2048, SMALL_THREADS = 256;
 constexpr int AHEAD = 2;                                  // 16-byte pieces of the history per lane that are asked for at once
 
