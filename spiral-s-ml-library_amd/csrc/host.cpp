@@ -591,7 +591,7 @@ PyObject* whole_penalize_logits(PyObject* capsule, PyObject* const* a, Py_ssize_
         }
         need(tokens != nullptr ? rows_of(tokens) : each[0] == nullptr && each[1] == nullptr);
         need((ids == nullptr) == (bias == nullptr) && (bias == nullptr || (rows_of(bias) && ids->sizes() == bias->sizes())));
-        need(mask == nullptr || (mask->dim() > 0 && mask->size(-1) == words && (mask->numel() == words || mask->numel() == rows * words)));
+        need(mask == nullptr || (mask->dim() > 0 && mask->size(-1) == words && (mask->numel() == words || mask->sizes().slice(0, mask->dim() - 1) == lead)));
         const int64_t history = tokens != nullptr ? tokens->size(-1) : 0, n_bias = bias != nullptr ? bias->size(-1) : 0;
         const at::ScalarType type = x->scalar_type();
         const int code = code_of(type);

@@ -103,6 +103,8 @@ def quantize_blocks(x, block=(1, 128), dtype=torch.float8_e4m3fn, transpose=Fals
     type's largest number.  q is (rows, cols rounded up to a multiple of 16), zeros behind the columns of x; scale (rows or ceil(rows / 128),
     ceil(cols / 128)).  transpose=True gives the same of the transpose of x, transpose="both" reads x once and gives
     (q, scale, q_t, scale_t): what a layer's forward product and the gradients of its input (weights) or its weights (activations) take."""
+    if transpose in (False, True):
+        transpose = bool(transpose)                                # (0 and 1 are taken for them)
     if (block == (1, 128) or block == (128, 128)) and (transpose in (False, True) or transpose == "both"):
         done = lib.whole_quantize_blocks(x, block[0], dtype, transpose is not True, transpose is not False)
         if done is not None:

@@ -363,7 +363,7 @@ def penalize_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repe
     words = -(-cols // 32)
     mask_rows = 0
     if mask is not None:
-        if mask.dim() == 0 or mask.shape[-1] != words or mask.numel() not in (words, rows * words):
+        if mask.dim() == 0 or mask.shape[-1] != words or (mask.numel() != words and mask.shape[:-1] != lead):
             raise ValueError("mask must be (..., %d) with the rows of the logits, or one row" % words)
         mask_rows = mask.numel() // words
     history = tokens.shape[-1] if tokens is not None else 0

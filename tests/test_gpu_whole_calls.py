@@ -83,6 +83,18 @@ def test_what_is_not_taken_raises():
         with pytest.raises(error, match=text):
             f()
     assert torch.equal(P.layer_norm(x, eps=1), P.layer_norm(x, eps=1.0))          # (an integer goes the long way)
+    for mask in (torch.full((4, 2), -1, device="cuda", dtype=torch.int32), torch.full((2, 2, 3), -1, device="cuda", dtype=torch.int32)):      # (rows in another shape than the logits')
+        with pytest.raises(ValueError, match="mask must"):
+            P.penalize_logits(x.view(2, 2, 64), mask=mask)
+
+
+def test_a_transpose_of_0_or_1_is_false_or_true():
+    from ml import matmul as M
+    announce("quantize_blocks transpose=0, 1")
+    x = torch.randn((40, 200), device="cuda")
+    for flag in (0, 1):
+        for got, want in zip(M.quantize_blocks(x, transpose=flag), M.quantize_blocks(x, transpose=bool(flag)), strict=True):
+            assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
 
 
 def test_gradients_are_not_asked_of_the_outputs():

@@ -101,6 +101,7 @@ def test_python_refusals():
             (TypeError, "logits", lambda: Lo(x.double())), (ValueError, "out must", lambda: Lo(x, out=x[:2])), (ValueError, "one entry", lambda: Lo(x, repetition=stat[:2])),
             (ValueError, "tokens must", lambda: Lo(x, tokens=i32(3, 5))), (ValueError, "need tokens", lambda: Lo(x, lengths=i32(4))), (ValueError, "go together", lambda: Lo(x, bias=x)),
             (ValueError, "bias_ids and bias", lambda: Lo(x, bias=x, bias_ids=i32(4, 3))), (ValueError, "mask must", lambda: Lo(x, mask=i32(4, 3))), (ValueError, "mask must", lambda: Lo(x, mask=i32(3, 2))),
+            (ValueError, "mask must", lambda: Lo(x.view(2, 2, 64), mask=i32(4, 2))), (ValueError, "mask must", lambda: Lo(torch.zeros((2, 3, 64)), mask=i32(3, 2, 2))),
             (ValueError, "GPU", lambda: Lo(x)), (ValueError, "GPU", lambda: Lo(x, tokens=i32(4, 5)))):
         with pytest.raises(error, match=text):
             f()
