@@ -1,8 +1,8 @@
 // Rows and columns of a matrix in 8-bit blocks of 128 with a scale each: the operands of gemm_scaled.hip.
 //
-// A workgroup takes a tile of 128 x 128 (16 x 128 where only rows are wanted in blocks of one), so every block along either direction lies inside
+// A workgroup takes a tile of 128 x 128 (16 x 128 where only rows are wanted in blocks of one, 128 x 64 for few blocks of one column), so every block along either direction lies inside
 // one tile, and x is read once whatever is wanted of it.  A lane holds 1, 4 or 8 rows of 8 columns.  A row's 16 lanes are a DPP row, so the
-// largest magnitude of a row's block takes four DPP steps; a column's takes two cross-lane steps and, over the four waves, LDS.
+// largest magnitude of a row's block takes four DPP steps; a column's takes two or three cross-lane steps and, over the waves, LDS.
 // Magnitudes are compared as bits: an infinity is larger than every number and a NaN larger than that, so neither is lost.  The transposed
 // numbers go through LDS so that both forms leave in 128-byte rows.
 //
@@ -57,23 +57,24 @@ struct QuantArgs {
 
 __device__ __forceinline__ unsigned max_u32(unsigned a, unsigned b) { return a > b ? a : b; }
 
-// WIDE: blocks of 128 x 128.  OUT: 1 = q, 2 = q_t, 3 = both.  R: rows per lane, ROWS: of the tile.  POLICY: of the stores (a branch at each
+// WIDE: blocks of 128 x 128.  OUT: 1 = q, 2 = q_t, 3 = both.  R: rows per lane, ROWS: of the tile, LANES: of 8 columns, its width.  POLICY: of the stores (a branch at each
 // store, the compiler folds both sides into a plain one).
-template <int DT, int F8, bool WIDE, int OUT, int R, int ROWS, int POLICY>
-__global__ __launch_bounds__(ROWS / R * 16) void quantize_kernel(const void* x_first, long rows_first, long cols_first, const QuantArgs args) {
+template <int DT, int F8, bool WIDE, int OUT, int R, int ROWS, int LANES, int POLICY>
+__global__ __launch_bounds__(ROWS / R * LANES) void quantize_kernel(const void* x_first, long rows_first, long cols_first, const QuantArgs args) {
     constexpr int E = ELEM_BYTES<DT>, PIECES = 8 / PER16<DT>;
     constexpr bool ROW = (OUT & 1) != 0, COL = (OUT & 2) != 0;
-    constexpr int THREADS = ROWS / R * 16, WAVES = THREADS / 64;
+    constexpr int COLS = LANES * 8, THREADS = ROWS / R * LANES, WAVES = THREADS / 64;
     static_assert(ROWS == QB || (!COL && !WIDE), "tiles of fewer rows hold blocks of one row only");
+    static_assert(LANES == 16 || (!ROW && !WIDE), "tiles of fewer columns hold blocks of one column only");
     static_assert(!COL || R == 8 || R == 4, "a lane's rows of a column are one store");
     constexpr int PITCH = QB + 16;            // bytes of a transposed row in LDS
-    __shared__ __attribute__((aligned(16))) unsigned char turned[COL ? QB * PITCH : 16];
-    __shared__ unsigned most[COL && !WIDE ? WAVES * QB : WAVES];
+    __shared__ __attribute__((aligned(16))) unsigned char turned[COL ? COLS * PITCH : 16];
+    __shared__ unsigned most[COL && !WIDE ? WAVES * COLS : WAVES];
     const long rows = rows_first, cols = cols_first;
-    const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4, wave = tid >> 6;
-    const long tiles_c = (cols + QB - 1) / QB;
+    const int tid = threadIdx.x, cg = tid % LANES, rg = tid / LANES, wave = tid >> 6;
+    const long tiles_c = (cols + COLS - 1) / COLS;
     const long tile_r = blockIdx.x / tiles_c, tile_c = blockIdx.x - tile_r * tiles_c;
-    const long r0 = tile_r * ROWS + rg * R, c0 = tile_c * QB + cg * 8;
+    const long r0 = tile_r * ROWS + rg * R, c0 = tile_c * COLS + cg * 8;
     u32x4 raw[R][PIECES];
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -86,9 +87,10 @@ __global__ __launch_bounds__(ROWS / R * 16) void quantize_kernel(const void* x_f
     auto value = [&](int i, int j) { return element<DT>(raw[i][j / PER16<DT>], j % PER16<DT>); };
     auto magnitude = [&](int i, int j) { return __float_as_uint(value(i, j)) & 0x7fffffffu; };
     auto across_row = [](unsigned v) { return group_allreduce<16>(v, max_u32); };      // over the 16 lanes of a row
-    auto across_wave = [](unsigned v) {                                                  // over the four row groups of a wave
-        v = max_u32(v, __shfl_xor(v, 16, WAVE));
-        return max_u32(v, __shfl_xor(v, 32, WAVE));
+    auto across_wave = [](unsigned v) {                                                  // over the row groups of a wave
+#pragma unroll
+        for (int d = LANES; d < WAVE; d *= 2) v = max_u32(v, __shfl_xor(v, d, WAVE));
+        return v;
     };
     BlockScale one;                           // WIDE: of the tile
     if constexpr (WIDE) {
@@ -135,14 +137,14 @@ __global__ __launch_bounds__(ROWS / R * 16) void quantize_kernel(const void* x_f
 #pragma unroll
                 for (int i = 0; i < R; ++i) m = max_u32(m, magnitude(i, j));
                 m = across_wave(m);
-                if ((tid & 63) < 16) most[wave * QB + cg * 8 + j] = m;
+                if ((tid & 63) < LANES) most[wave * COLS + cg * 8 + j] = m;
             }
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 column[j] = most[cg * 8 + j];
 #pragma unroll
-                for (int w = 1; w < WAVES; ++w) column[j] = max_u32(column[j], most[w * QB + cg * 8 + j]);
+                for (int w = 1; w < WAVES; ++w) column[j] = max_u32(column[j], most[w * COLS + cg * 8 + j]);
             }
         }
 #pragma unroll
@@ -161,47 +163,53 @@ __global__ __launch_bounds__(ROWS / R * 16) void quantize_kernel(const void* x_f
         // 16 bytes per lane: eight lanes a row of 128 bytes
         const long at = tile_r * QB + (tid & 7) * 16;
 #pragma unroll
-        for (int k = 0; k < QB * 8 / THREADS; ++k) {
+        for (int k = 0; k < COLS * 8 / THREADS; ++k) {
             const int c = k * (THREADS / 8) + (tid >> 3);
             const u32x4 v = *reinterpret_cast<const u32x4*>(turned + c * PITCH + (tid & 7) * 16);
-            if (tile_c * QB + c < cols && at < args.pitch_t) put(args.q_t + (tile_c * QB + c) * args.pitch_t + at, v);
+            if (tile_c * COLS + c < cols && at < args.pitch_t) put(args.q_t + (tile_c * COLS + c) * args.pitch_t + at, v);
         }
     }
 }
 
 // ---- host side -------------------------------------------------------------------------------
 
-template <int DT, int F8, bool WIDE, int OUT, int R, int ROWS, int POLICY>
+template <int DT, int F8, bool WIDE, int OUT, int R, int ROWS, int LANES, int POLICY>
 static int launch_quantize(const QuantArgs& a, hipStream_t stream) {
-    constexpr int THREADS = ROWS / R * 16;
-    const long tiles = ((a.rows + ROWS - 1) / ROWS) * a.blocks_c;
+    constexpr int THREADS = ROWS / R * LANES, COLS = LANES * 8;
+    const long tiles = ((a.rows + ROWS - 1) / ROWS) * ((a.cols + COLS - 1) / COLS);
     if (tiles * THREADS >= 1l << 32) return fail(SP_ERR_SHAPE, "sp_quantize_blocks: too large");
-    hipLaunchKernelGGL((quantize_kernel<DT, F8, WIDE, OUT, R, ROWS, POLICY>), dim3((unsigned)tiles), dim3(THREADS), 0, stream, a.x, a.rows, a.cols, a);
+    hipLaunchKernelGGL((quantize_kernel<DT, F8, WIDE, OUT, R, ROWS, LANES, POLICY>), dim3((unsigned)tiles), dim3(THREADS), 0, stream, a.x, a.rows, a.cols, a);
     return check_launch("sp_quantize_blocks");
 }
 
 // Rows per lane of the 128 x 128 tiles: 4 (eight waves) where a tile has one scale, 8 where every row or column has its own, whose steps across
 // lanes count then.  (us, 8 / 4 rows: 8192 x 4096 bf16 both ways in 128 x 128 blocks 23.8 / 22.2; 16384 x 4096 both ways in rows of 128
 // 59.3 / 66.2, transposed alone 43.5 / 48.5.  Written back instead of streamed 27.5 / 25.8, 62.8 / 67.7, 44.9 / 49.)
+// Transposed alone, in tiles of 64 columns and 4 rows per lane where the chip has less than two tiles of 128 x 128 a unit: 5001 x 1003 f32 11.1 / 10.1,
+// 512 x 1024 bf16 5.3 / 4.7; 2048 x 4096 bf16, two a unit, 9.0 / 9.15, 8192 x 4096 21.6 / 22.8.
 template <int DT, int F8, int POLICY>
 static int quantize(const QuantArgs& a, bool wide, hipStream_t stream) {
     const int out = (a.q != nullptr ? 1 : 0) | (a.q_t != nullptr ? 2 : 0);
     if (wide) {
-        if (out == 1) return launch_quantize<DT, F8, true, 1, 4, QB, POLICY>(a, stream);
-        if (out == 2) return launch_quantize<DT, F8, true, 2, 4, QB, POLICY>(a, stream);
-        return launch_quantize<DT, F8, true, 3, 4, QB, POLICY>(a, stream);
+        if (out == 1) return launch_quantize<DT, F8, true, 1, 4, QB, 16, POLICY>(a, stream);
+        if (out == 2) return launch_quantize<DT, F8, true, 2, 4, QB, 16, POLICY>(a, stream);
+        return launch_quantize<DT, F8, true, 3, 4, QB, 16, POLICY>(a, stream);
     }
-    if (out == 1) return launch_quantize<DT, F8, false, 1, 1, 16, POLICY>(a, stream);
-    if (out == 2) return launch_quantize<DT, F8, false, 2, 8, QB, POLICY>(a, stream);
-    return launch_quantize<DT, F8, false, 3, 8, QB, POLICY>(a, stream);
+    if (out == 1) return launch_quantize<DT, F8, false, 1, 1, 16, 16, POLICY>(a, stream);
+    if (out == 2) {
+        if constexpr (POLICY == ST_PLAIN)
+            if (a.blocks_r * a.blocks_c < 2 * device_cu_count()) return launch_quantize<DT, F8, false, 2, 4, QB, 8, POLICY>(a, stream);
+        return launch_quantize<DT, F8, false, 2, 8, QB, 16, POLICY>(a, stream);
+    }
+    return launch_quantize<DT, F8, false, 3, 8, QB, 16, POLICY>(a, stream);
 }
 
 namespace {
 struct QuantizeKernelNames {
     QuantizeKernelNames() {
-        register_kernel("quantize_rows", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 1, 1, 16, ST_STREAM>, 256);
-        register_kernel("quantize_both", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 3, 8, QB, ST_STREAM>, 256);
-        register_kernel("quantize_both_128", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, true, 3, 4, QB, ST_STREAM>, 512);
+        register_kernel("quantize_rows", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 1, 1, 16, 16, ST_STREAM>, 256);
+        register_kernel("quantize_both", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, false, 3, 8, QB, 16, ST_STREAM>, 256);
+        register_kernel("quantize_both_128", (const void*)quantize_kernel<SP_BF16, SP_F8_E4M3, true, 3, 4, QB, 16, ST_STREAM>, 512);
     }
 } quantize_kernel_names;
 }  // namespace

@@ -72,6 +72,18 @@ def test_quantize(M, shape, dtype, high, f8):
         assert torch.equal(p.view(torch.uint8), w.view(torch.uint8))
 
 
+@pytest.mark.parametrize("rows,cols", [(2053, 4099), (8200, 4500)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_quantize_transposed_in_many_tiles(M, rows, cols, dtype):
+    announce("quantize_blocks transposed %d x %d %s" % (rows, cols, dtype))
+    x = torch.randn((rows, cols), generator=torch.Generator().manual_seed(2)).to(TYPES[dtype])
+    d = x.cuda()
+    q, s = M.quantize_blocks(d, transpose=True)
+    check_form(q, s, x.t().contiguous().double(), 1, "e4m3")
+    both = M.quantize_blocks(d, transpose="both")
+    assert torch.equal(both[2].view(torch.uint8), q.view(torch.uint8)) and torch.equal(both[3], s)
+
+
 def test_quantize_every_8_bit_number_and_every_tie(M):
     """Numbers of the type times a power of two come back, and those half-way between two go to the even one."""
     announce("quantize_blocks ties")
