@@ -212,6 +212,13 @@ def test_captured_and_on_another_stream(P):
         assert all(torch.equal(p, q) for got in kept for p, q in zip(want, got)), k
 
 
+@pytest.mark.parametrize("rows,cols,history", [(40, 32003, 900), (129, 8191, 0), (300, 33001, 4097)])       # (large chunks; the last results are streamed)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_rows_of_several_chunks(P, rows, cols, history, dtype):
+    announce("penalize_logits %s" % ((rows, cols, history, dtype),))
+    check(P, *inputs(rows, cols, history, 5, 3, dtype))
+
+
 def test_offsets_past_32_bits(P):
     """More than 2^31 logits: the last rows are those of a call on them alone."""
     announce("penalize_logits 16400 x 131072 bf16")
