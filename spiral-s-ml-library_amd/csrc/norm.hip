@@ -72,7 +72,7 @@ struct Piece {
     template <int DT>
     __device__ __forceinline__ u32x4 load(const void* p, long row_at, int cols, bool ok) const {
         u32x4 v = {0u, 0u, 0u, 0u};
-        if (!WHOLE && cols < N) v = load16<DT>(p, row_at + col, ok && mine() ? cols - col : 0);
+        if (!WHOLE && cols < N) v = load_each<DT>(p, row_at + col, ok && mine() ? cols - col : 0);
         else if (ok && mine()) v = load_aligned<WHOLE ? 16 : ELEM_BYTES<DT>, u32x4>((const unsigned char*)p + (row_at + col) * ELEM_BYTES<DT>);
         return v;
     }
@@ -85,7 +85,7 @@ __device__ __forceinline__ void load_weights(const void* weight, float otherwise
     for (int h = 0; h < N; h += PER16<WT>) {
         u32x4 v = {0u, 0u, 0u, 0u};
         if (weight != nullptr && (!WHOLE || piece.mine())) {
-            if (!WHOLE && cols < N) v = load16<WT>(weight, col + h, cols - col - h);
+            if (!WHOLE && cols < N) v = load_each<WT>(weight, col + h, cols - col - h);
             else v = load_aligned<WHOLE ? 16 : ELEM_BYTES<WT>, u32x4>((const unsigned char*)weight + (col + h) * ELEM_BYTES<WT>);
         }
 #pragma unroll
@@ -148,25 +148,48 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void layer_norm_kernel(const voi
 }
 
 // T lanes per row, C pieces of it per lane, 1024 / T rows at a time in a workgroup; SUMS: dweight and dbias are wanted.
-// With 8 columns per lane the weights and the next row fit its 128 registers as well; with 16 (rows of more than 8192) they do not.
+// With 8 columns per lane the weights and the next row fit its 128 registers as well; with 16 (rows of more than 8192) they do not, and the
+// sums over rows, which would not either, are in LDS, every lane's own (in registers,
+// spilled: 2048 x 16384 bf16, forward and backward, 103 us, in LDS 93; 37 x 12887 30, 18).
 template <int DT, int WT, int T, int C, bool SUMS, bool WHOLE>
 __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* dy, const void* x, const float* mean, const float* rstd, long rows,
                                                                   int cols, const void* weight, void* dx, float* partial) {
     constexpr int N = PER16<DT>, GROUPS = 1024 / T, W = T < 64 ? 1 : T / 64;
-    constexpr bool AHEAD = C * N <= 8;
-    extern __shared__ __attribute__((aligned(16))) float sums[];          // SUMS: 512 lanes x C N floats
+    constexpr bool AHEAD = C * N <= 8, IN_LDS = SUMS && !AHEAD;
+    static_assert(AHEAD || GROUPS == 1, "nothing to join where the sums are in LDS");
+    extern __shared__ __attribute__((aligned(16))) float sums[];          // SUMS: 512 lanes x C N floats; IN_LDS: 1024 lanes x 2 C N
     __shared__ float slots[2][GROUPS * 2 * W];
     const int t = threadIdx.x % T, group = threadIdx.x / T;
     const float count = (float)cols;
     const bool stream = streamed(rows, cols, ELEM_BYTES<DT>);
     auto load_weight = [&](int c, float(&w)[N]) { load_weights<WT>(weight, 1.f, Piece<N, WHOLE>(c * T + t, cols), cols, w); };
     float kept[AHEAD ? C : 1][N], dw[C][N], db[C][N];
+    f32x4* const mine = reinterpret_cast<f32x4*>(sums) + threadIdx.x;     // IN_LDS: 4 of dw at mine[1024 (c N / 4 + i / 4)], db behind them
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         if constexpr (AHEAD) load_weight(c, kept[c]);
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[c][i] = db[c][i] = 0.f;
     }
+    if constexpr (IN_LDS)
+#pragma unroll
+        for (int q = 0; q < C * N / 2; ++q) mine[1024 * q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // what is in LDS of a piece's sums, into registers and back
+    auto bring = [&](int c, bool back) {
+        if constexpr (IN_LDS)
+#pragma unroll
+            for (int h = 0; h < N; h += 4)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    f32x4* at = mine + 1024 * (((k * C + c) * N + h) / 4);
+                    float* v = (k == 0 ? dw[c] : db[c]) + h;
+                    if (back) *at = f32x4{v[0], v[1], v[2], v[3]};
+                    else {
+                        const f32x4 q = *at;
+                        v[0] = q[0], v[1] = q[1], v[2] = q[2], v[3] = q[3];
+                    }
+                }
+    };
     u32x4 xr[C], gr[C];
     float m = 0.f, r = 0.f;
     auto fetch = [&](long row) {
@@ -198,6 +221,7 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
             const Piece<N, WHOLE> piece(c * T + t, cols);
             float now[N];
             if constexpr (!AHEAD) load_weight(c, now);
+            bring(c, false);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const bool counts = piece.counts(i, cols);
@@ -207,6 +231,7 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
                 dw[c][i] += d * h;
                 db[c][i] += d;
             }
+            bring(c, true);
         }
         group_sums<T>(s, slots[turn] + group * 2 * W);
         turn ^= 1;
@@ -251,6 +276,16 @@ __global__ __launch_bounds__(1024) void layer_norm_backward_kernel(const void* d
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const Piece<N, WHOLE> piece(c * T + t, cols);
+                bring(c, false);
+                if ((WHOLE || GROUPS == 1) && piece.skip == 0 && (WHOLE || cols >= N)) {           // (all of them counted: in whole pieces; one by one 5 x 7909 f16, forward and backward, took 18.8 us, 13.1)
+#pragma unroll
+                    for (int h = 0; h < N; h += 4) {
+                        const float w[4] = {dw[c][h], dw[c][h + 1], dw[c][h + 2], dw[c][h + 3]}, b[4] = {db[c][h], db[c][h + 1], db[c][h + 2], db[c][h + 3]};
+                        store16<SP_F32>(out, piece.col + h, 4, w);
+                        store16<SP_F32>(out, cols + piece.col + h, 4, b);
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     if (piece.counts(i, cols)) {
@@ -344,7 +379,8 @@ static int launch_backward(const NormArgs& a) {
     constexpr int GROUPS = 1024 / T;
     const int blocks = (int)std::min<long>(backward_blocks(a.rows), (a.rows + GROUPS - 1) / GROUPS);
     auto kernel = whole_pieces<DT>(a) ? layer_norm_backward_kernel<DT, WT, T, C, SUMS, true> : layer_norm_backward_kernel<DT, WT, T, C, SUMS, false>;
-    const int lds_bytes = SUMS && GROUPS > 1 ? 512 * C * PER16<DT> * 4 : 0;
+    constexpr int columns = C * PER16<DT>;               // of a lane
+    const int lds_bytes = !SUMS ? 0 : columns > 8 ? 1024 * 2 * columns * 4 : GROUPS > 1 ? 512 * columns * 4 : 0;
     if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(1024), lds_bytes, a.stream, a.dy, a.x, a.mean_in, a.rstd_in, a.rows, a.cols, a.weight, a.dx, a.partial);
     if (const int rc = check_launch("sp_layer_norm_backward"); rc != SP_OK || !SUMS) return rc;

@@ -169,7 +169,7 @@ def check_backward(P, dy, x, mean, rstd, w):
     return dx, dw, db
 
 
-@pytest.mark.parametrize("shape", SHAPES + [(5001, 96), (2049, 4096)])
+@pytest.mark.parametrize("shape", SHAPES + [(5001, 96), (2049, 4096), (600, 8208), (530, 12001), (520, 16384)])
 @pytest.mark.parametrize("types", ["f32 f32", "bf16 f32", "bf16 bf16", "f16 f32", "f16 f16"])
 def test_backward(P, shape, types):
     t, wt = (TYPES[n] for n in types.split())
