@@ -177,7 +177,7 @@ def product64(a, sa, b, sb):
 # every kernel: few rows, few tiles, full ones; sides that are no multiple of a tile, K below a block, behind one, and with a tail of one chunk
 PRODUCTS = [(1, 1, 16), (1, 128, 128), (1, 4096, 1040), (2, 130, 112), (7, 33, 272), (16, 256, 4096), (17, 100, 144), (31, 515, 2064), (33, 48, 128), (49, 1003, 528),
             (64, 64, 640), (65, 17, 384), (100, 300, 1168), (128, 128, 128), (129, 257, 272), (1000, 1500, 400), (2304, 1153, 272), (1537, 2050, 144),
-            (2048, 2304, 1024), (4100, 3000, 528), (1, 24700, 272), (20, 24580, 1168), (49, 25001, 2576), (64, 32768, 128)]
+            (2048, 2304, 1024), (4100, 3000, 528), (1, 24700, 272), (20, 24580, 1168), (49, 25001, 2576), (64, 32768, 128), (4224, 4112, 144)]
 
 
 @pytest.mark.parametrize("wide", [True, False])
