@@ -334,6 +334,7 @@ int sp_row_reduce_f32(int op, int map_in, int map_out, const float* x, float* ou
  * y = (x - mean) * rstd * weight + bias row by row, with mean and var = the mean of (x - mean)^2 over the row in f32 and
  * rstd = 1 / sqrt(var + eps).  x, y (rows, cols) of `dtype` (SP_F32, SP_F16, SP_BF16), any cols from 1 to 16384; weight, bias (cols,)
  * of `weight_dtype` (SP_F32 or dtype), either may be NULL (1 and 0).  mean_out, rstd_out: (rows,) f32, or NULL.  y may be x.
+ * How a row is added up depends on the sizes: in a call of another number of rows it may come out another rounding away.
  * Stands beside SP_ROW_LN_L2 (ml/primitives.spi:701-703), which divides by the root of the sum of squares.
  */
 int sp_layer_norm(int dtype, int weight_dtype, const void* x, const void* weight, const void* bias, void* y, float* mean_out,

@@ -360,7 +360,13 @@ static int forward(const NormArgs& a) {
     if (pieces <= 64) return launch_forward<DT, WT, 64, 1>(a);
     if (pieces <= 128) return launch_forward<DT, WT, 64, 2>(a);
     if (pieces <= 256) return launch_forward<DT, WT, 64, 4>(a);
-    if (pieces <= 512) return a.rows <= 2 * device_cu_count() ? launch_forward<DT, WT, 512, 1>(a) : launch_forward<DT, WT, 256, 2>(a);   // (16 x 4096 bf16 3.1 us, 3.4; 16384 rows 80, 68)
+    // rows for two workgroups a unit or less: the shortest way through one (us, this / the rules below: 16 x 4096 bf16 3.1 / 3.4, 5 x 7909 f16 4.3 / 6.3,
+    // 256 x 8192 bf16 4.5 / 5.1; 16384 x 4096 80 / 68; with two pieces a lane 100 x 12887 6.9 / 7.5, but 512 x 16384 11.1 / 10.4)
+    if (a.rows <= 2 * device_cu_count()) {
+        if (pieces <= 512) return launch_forward<DT, WT, 512, 1>(a);
+        if (pieces <= 1024) return launch_forward<DT, WT, 1024, 1>(a);
+    }
+    if (pieces <= 512) return launch_forward<DT, WT, 256, 2>(a);
     if (pieces <= 768) return launch_forward<DT, WT, 256, 3>(a);
     if (pieces <= 1024) return launch_forward<DT, WT, 256, 4>(a);
     if (pieces <= 1536) return launch_forward<DT, WT, 512, 3>(a);

@@ -185,7 +185,9 @@ static int launch_quantize(const QuantArgs& a, hipStream_t stream) {
 // Rows per lane of the 128 x 128 tiles: 4 (eight waves) where a tile has one scale, 8 where every row or column has its own, whose steps across
 // lanes count then.  (us, 8 / 4 rows: 8192 x 4096 bf16 both ways in 128 x 128 blocks 23.8 / 22.2; 16384 x 4096 both ways in rows of 128
 // 59.3 / 66.2, transposed alone 43.5 / 48.5.  Written back instead of streamed 27.5 / 25.8, 62.8 / 67.7, 44.9 / 49.)
-// Transposed alone, in tiles of 64 columns and 4 rows per lane where the chip has less than two tiles of 128 x 128 a unit: 5001 x 1003 f32 11.1 / 10.1,
+// Where the chip has less than two tiles a unit the way through one counts, 4 rows per lane: 16 x 4096 bf16 both ways in rows of 128 6.9 / 5.8,
+// 512 x 1024 6.7 / 6.3, 2047 x 3000 12.2 / 12.0; 2048 x 4096, two a unit, is on 8.
+// Transposed alone, in tiles of 64 columns and 4 rows per lane there: 5001 x 1003 f32 11.1 / 10.1,
 // 512 x 1024 bf16 5.3 / 4.7; 2048 x 4096 bf16, two a unit, 9.0 / 9.15, 8192 x 4096 21.6 / 22.8.
 template <int DT, int F8, int POLICY>
 static int quantize(const QuantArgs& a, bool wide, hipStream_t stream) {
@@ -201,6 +203,8 @@ static int quantize(const QuantArgs& a, bool wide, hipStream_t stream) {
             if (a.blocks_r * a.blocks_c < 2 * device_cu_count()) return launch_quantize<DT, F8, false, 2, 4, QB, 8, POLICY>(a, stream);
         return launch_quantize<DT, F8, false, 2, 8, QB, 16, POLICY>(a, stream);
     }
+    if constexpr (POLICY == ST_PLAIN)
+        if (a.blocks_r * a.blocks_c < 2 * device_cu_count()) return launch_quantize<DT, F8, false, 3, 4, QB, 16, POLICY>(a, stream);
     return launch_quantize<DT, F8, false, 3, 8, QB, 16, POLICY>(a, stream);
 }
 
