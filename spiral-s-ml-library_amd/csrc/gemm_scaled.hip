@@ -1,8 +1,8 @@
 // C = A . B^T of 8-bit operands with a scale for each block of 128 along K: per row of A, per row of B or per 128 of its rows.
 //
-// A block of 128 is 128 bytes of a row: one MFMA of K = 128, or four of K = 32, which start from zero.  The vector ALU multiplies their sum by
+// A block of 128 is 128 bytes of a row: four f16 MFMAs of K = 32, which start from zero.  The vector ALU multiplies their sum by
 // the block's two scales and adds it to the accumulators (so the sum over the blocks is rounded to nearest f32): four multiply-adds
-// of 4 cycles per 16 x 16 block, against 32 or 64 cycles on the matrix pipe.
+// of 4 cycles per 16 x 16 block, against 64 cycles on the matrix pipe.
 //
 // The B fragment is the MFMA's first operand: register r of lane l of a 16 x 16 fragment holds C[m = l % 16][n = 4 (l / 16) + r], so a lane
 // needs one scale of A per fragment and stores four consecutive columns.
@@ -12,8 +12,6 @@
 #include "vec_io.h"
 
 namespace sp {
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct ScaledArgs {
     const unsigned char *A, *B;
@@ -28,22 +26,10 @@ struct ScaledArgs {
     int stream;                   // C does not stay in the caches
 };
 
-// A lane's 32 numbers of a block of one row.  A and B agree on which 16-byte chunks of the block they are; in which order does not matter.
-template <int F8, bool FAST>
-struct Fragment;
-
+// A lane's 32 numbers of a block of one row, as f16, which holds every number of both types.  A and B agree on which 16-byte chunks of the block they
+// are; in which order does not matter.
 template <int F8>
-struct Fragment<F8, true> {
-    i32x8 v;
-    __device__ __forceinline__ void set(const u32x4 (&c)[2]) {
-        struct Pair { u32x4 v[2]; };
-        v = __builtin_bit_cast(i32x8, Pair{{c[0], c[1]}});
-    }
-};
-
-// As f16, which holds every number of both types.
-template <int F8>
-struct Fragment<F8, false> {
+struct Fragment {
     f16x8 v[4];
     __device__ __forceinline__ void set(const u32x4 (&c)[2]) {
 #pragma unroll
@@ -63,21 +49,15 @@ struct Fragment<F8, false> {
     }
 };
 
-// The sum of one block.  The 8-bit MFMAs add eight products at a time and cut off what lies below 2^-13 of the largest's power of two before they go on in f32 (measured:
-// 2^16 + 8 is exact, 2^16 + 4 is 2^16 with both in one group of eight, and exact otherwise; sums of 4096 N(0, 1) products are 1.5e-5 off in the 2-norm).  FAST
-// takes them, for C of 16 bits, whose own rounding is 1.7e-3 (bf16) or 2.1e-4 (f16).  C of f32 takes the f16 MFMAs, at half their rate,
-// where products are exact and sums f32.
-template <int F8A, int F8B, bool FAST>
-__device__ __forceinline__ f32x4 block_sum(const Fragment<F8B, FAST>& b, const Fragment<F8A, FAST>& a) {
+// The sum of one block.  The f16 MFMAs have exact products and keep 24 bits below the largest of a sum (measured: 128 N(0, 1) products are 0.5 U of the sum of their magnitudes off at
+// most, numbers of every exponent 4 U, U = 2^-24).  The 8-bit MFMAs, of K = 128 at twice the rate and of K = 32 at the same, add eight products at a time and cut off what
+// lies below 2^-13 of the largest's power of two before they go on in f32 (2^16 + 4 - 2^16 is 0; 280 to 3000 U off): no type of C takes them.
+template <int F8A, int F8B>
+__device__ __forceinline__ f32x4 block_sum(const Fragment<F8B>& b, const Fragment<F8A>& a) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (FAST) {
-        constexpr int FA = F8A == SP_F8_E4M3 ? 0 : 1, FB = F8B == SP_F8_E4M3 ? 0 : 1;
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, t, FB, FA, 0, 0, 0, 0);
-    } else {
 #pragma unroll
-        for (int h = 0; h < 4; ++h) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.v[h], a.v[h], t, 0, 0, 0);
-        return t;
-    }
+    for (int h = 0; h < 4; ++h) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.v[h], a.v[h], t, 0, 0, 0);
+    return t;
 }
 
 // Four columns of a row of C from col on.
@@ -138,7 +118,7 @@ __device__ __forceinline__ void put_piece(const ScaledArgs& g, long row, long co
 }
 
 // A wave's accumulators to C: two rows of fragments at a time go through a strip of LDS of its own, so that whole 16-byte pieces of C leave, side by
-// side along its rows (as 16 rows of 32 bytes per instruction, straight from the registers, 8192 x 4096 x 4096 took 149 us against 138).
+// side along its rows (as 16 rows of 32 bytes per instruction, straight from the registers, 8192 x 4096 x 4096 bf16 takes 248 us against 235, 8192 x 8192 x 2048 280 against 253).
 template <int TN>
 constexpr int STRIP_ROW = 16 * TN * 4 + 16;                // bytes; the pad spreads a column over the banks
 template <int OT, bool HAS_BETA, bool WHOLE, int POLICY, int TM, int TN>
@@ -172,8 +152,8 @@ __device__ __forceinline__ void put_rows(const ScaledArgs& g, const f32x4 (&acc)
 }
 template <int TM, int TN>
 __device__ __forceinline__ void put_tile(const ScaledArgs& g, const f32x4 (&acc)[TM][TN], unsigned char* strip, long row0, long col0, int lane) {
-    // a C that does not stay in the caches anyway is streamed past them where its tiles are whole: 8192 x 8192 x 2048 bf16 139 -> 134 us, 4096 x 4096 x 2048 f32
-    // 72 -> 68
+    // a C that does not stay in the caches anyway is streamed past them where its tiles are whole: 8192 x 8192 x 2048 bf16 260 -> 254 us, 8192 x 4096 x 4096 bf16
+    // 245 -> 239
     const bool whole = row0 + 16 * TM <= g.M && col0 + 16 * TN <= g.N;
     auto put = [&](auto ot) {
         constexpr int OT = decltype(ot)::value;
@@ -198,8 +178,7 @@ __device__ __forceinline__ void scaled_tile_of_block(int pid, int tiles_m, int t
 }
 
 // Scales come in for several blocks of K at a time, a chunk: SB = 8 of them of eight rows, or 4 of sixteen, per instruction.  The scales of a row's blocks lie side
-// by side, so that a load asks for eight or sixteen lines of memory and not for 64 (one block at a time, as many lines as the operands, 8192^3 took
-// 517 us against 501).
+// by side, so that a load asks for eight or sixteen lines of memory and not for 64, as many as the operands of a whole block.
 constexpr int SCALE_BLOCKS = 8, SPLIT_BLOCKS = 4;
 
 // Lane l's scale is that of row l / SB and block l % SB of what `row` and `first` say; to LDS bytes lds_addr + 4 l.
@@ -220,8 +199,8 @@ __device__ __forceinline__ int tile_slot(int row, int kc) { return (kc ^ row ^ (
 // in from LDS.  The boundary between two blocks of K stands in front of a block's last row: by then everything of the
 // block is in registers, and the next block has landed.  Behind each MFMA of the last row the next block's fragment of B takes the place of the one just
 // used; then the block after that is asked for.  A wave waits where it asks (the unit takes an instruction of 1 KiB every 16 cycles), so it does that with MFMAs under way: in front of the last row
-// 8192^3 took 480 us, behind it 470, half there and half a row later 456 (4096 x 2048 x 5008 in f32, whose tile has four rows: 95, 89, 90).
-template <int F8A, int F8B, bool FAST, int SHIFT, int BM, int BN, int WM, int WN>
+// 4096 x 2048 x 5008 took 95 us, behind it 89, half there and half a row later 90.
+template <int F8A, int F8B, int SHIFT, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const ScaledArgs g) {
     constexpr int NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     constexpr int NIA = BM / 8 / NW, NI = (BM + BN) / 8 / NW;       // DMA instructions of 8 rows per wave and block; A's first
@@ -260,8 +239,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
         dma_scales<SCALE_BLOCKS>(of_a ? g.scale_a : g.scale_b, of_a ? m0 + group * 8 : (n0 >> SHIFT) + (group - GROUPS_A) * 8, of_a ? g.M - 1 : last_sb,
                    (long)chunk * SCALE_BLOCKS, nk, lane, to);
     };
-    auto fetch_part = [&](int kt, unsigned stage, auto FROM_, auto TO_) {
-        constexpr int FROM = decltype(FROM_)::value, TO = decltype(TO_)::value;
+    auto fetch = [&](int kt, unsigned stage) {
         const unsigned char *a = pA + (long)kt * ROW_BYTES, *b = pB + (long)kt * ROW_BYTES;
         auto offset = [&](int q) {
             const unsigned at = voff + (unsigned)(q < NIA ? q : q - NIA) * (NW * 8) * K, last = q < NIA ? last_a : last_b;
@@ -270,21 +248,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
         auto to = [&](int q) { return dst + stage + (q < NIA ? q * NW * 8 : BM + (q - NIA) * NW * 8) * ROW_BYTES; };
         if (k_tail && kt == nk - 1) {
 #pragma unroll
-            for (int q = FROM; q < TO; ++q) {
+            for (int q = 0; q < NI; ++q) {
                 const unsigned char* inside = (q < NIA ? a : b) + offset(q);
                 dma_to_lds_addr(tail_in ? inside : (const unsigned char*)kZeroChunk, to(q));
             }
         } else {
 #pragma unroll
-            for (int q = FROM; q < TO; ++q) dma_to_lds(q < NIA ? a : b, offset(q), to(q));
+            for (int q = 0; q < NI; ++q) dma_to_lds(q < NIA ? a : b, offset(q), to(q));
         }
     };
-    // of the fetches behind a boundary FIRST stand behind the last row, the others behind the next block's first row
-    constexpr int FIRST = TM >= 8 ? NI / 2 : NI;
-    typedef std::integral_constant<int, 0> from_start;
-    typedef std::integral_constant<int, FIRST> middle;
-    typedef std::integral_constant<int, NI> to_end;
-
     // fragments: chunks 2 fq and 2 fq + 1 of a row
     int at_a[2], at_b[2];
     const int at_sa = 2 * STAGE + (wm * WTM + fi) * 32, at_sb = 2 * STAGE + GROUPS_A * 256 + (SHIFT == 7 ? (wn * WTN) >> 7 : wn * WTN + 4 * fq) * 32;
@@ -336,17 +308,17 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
     };
 
     for (int part = 0; part < SCALE_BLOCKS; ++part) fetch_scales(0, part);
-    fetch_part(0, 0, from_start{}, to_end{});
+    fetch(0, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     fetch_scales(1, 0);
-    fetch_part(nk > 1 ? 1 : 0, STAGE, from_start{}, middle{});                      // (past the last block the last one comes again, into a stage that is not read: no branch)
+    fetch(nk > 1 ? 1 : 0, STAGE);                      // (past the last block the last one comes again, into a stage that is not read: no branch)
 #pragma unroll
     for (int j = 0; j < TN; ++j) load_b(j);
     load_a(0);
     load_scales(0);
     int step = STAGE;
-    Fragment<F8B, FAST> fb[TN];
+    Fragment<F8B> fb[TN];
     for (int kt = 0; kt < nk; ++kt) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
@@ -362,26 +334,24 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
                 load_a(0);
             }
             __builtin_amdgcn_sched_barrier(0);
-            Fragment<F8A, FAST> fa;
+            Fragment<F8A> fa;
             fa.set(ra[i & 1]);
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 if (i == 0) fb[j].set(rb[j]);
-                sums[i & 1][j] = block_sum<F8A, F8B, FAST>(fb[j], fa);
+                sums[i & 1][j] = block_sum<F8A, F8B>(fb[j], fa);
                 if (i == 0) add(TM - 1, j, pending, sb_pending[SHIFT == 7 ? 0 : j]);
                 else add(i - 1, j, sa[i - 1], sb[SHIFT == 7 ? 0 : j]);
                 if (boundary) load_b(j);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (i == 0) {
-                if constexpr (FIRST < NI) fetch_part(kt + 1 < nk ? kt + 1 : nk - 1, step > 0 ? STAGE : 0, middle{}, to_end{});
-                if constexpr (SHIFT == 7)
+            if constexpr (SHIFT == 7)
+                if (i == 0)
 #pragma unroll
                     for (int k = 0; k < TM; ++k) sa[k] *= sb[0][0];
-            }
             if (boundary) {
                 fetch_scales((kt + 1) / SCALE_BLOCKS + 1, (kt + 1) % SCALE_BLOCKS);
-                fetch_part(kt + 2 < nk ? kt + 2 : nk - 1, step > 0 ? STAGE : 0, from_start{}, middle{});
+                fetch(kt + 2 < nk ? kt + 2 : nk - 1, step > 0 ? STAGE : 0);
                 pending = sa[TM - 1];
                 if constexpr (SHIFT != 7)
 #pragma unroll
@@ -399,7 +369,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
 
 // One tile of (16 TM) x (16 TN) outputs on four waves: each takes a quarter of K through an LDS ring of NS stages of its own, so no
 // wave waits for another inside the loop, and the four partial sums meet in LDS at the end.  All that is read comes in by DMA, the scales too.
-template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int NS>
+template <int F8A, int F8B, int SHIFT, int TM, int TN, int NS>
 __global__ __launch_bounds__(256) void gemm_scaled_split_kernel(const ScaledArgs g) {
     constexpr int KS = 4;
     constexpr int NIA = 2 * TM, ND = 2 * (TM + TN);     // DMA instructions per block
@@ -498,16 +468,16 @@ __global__ __launch_bounds__(256) void gemm_scaled_split_kernel(const ScaledArgs
             __builtin_amdgcn_sched_barrier(0);
         }
         stage = stage + 1 == NS ? 0 : stage + 1;
-        Fragment<F8A, FAST> fa[TM];
+        Fragment<F8A> fa[TM];
 #pragma unroll
         for (int i = 0; i < TM; ++i) fa[i].set(ra[i]);
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            Fragment<F8B, FAST> fb;
+            Fragment<F8B> fb;
             fb.set(rb[j]);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                const f32x4 v = block_sum<F8A, F8B, FAST>(fb, fa[i]);
+                const f32x4 v = block_sum<F8A, F8B>(fb, fa[i]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(v[e], sa[i] * sb[j][SHIFT == 7 ? 0 : e], acc[i][j][e]);
             }
@@ -542,9 +512,9 @@ static int check_tiles(ScaledArgs& g, int bm, int bn, int threads) {
     return SP_OK;
 }
 
-template <int F8A, int F8B, bool FAST, int SHIFT, int BM, int BN, int WM, int WN>
+template <int F8A, int F8B, int SHIFT, int BM, int BN, int WM, int WN>
 static int launch_tile(ScaledArgs g, hipStream_t stream) {
-    auto kernel = gemm_scaled_tile_kernel<F8A, F8B, FAST, SHIFT, BM, BN, WM, WN>;
+    auto kernel = gemm_scaled_tile_kernel<F8A, F8B, SHIFT, BM, BN, WM, WN>;
     constexpr int lds_bytes = 2 * ((BM + BN) * ROW_BYTES + (BM / 8 + (SHIFT == 7 ? 1 : BN / 8)) * 256);
     if (const int rc = check_tiles(g, BM, BN, WM * WN * 64); rc != SP_OK) return rc;
     if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
@@ -553,9 +523,9 @@ static int launch_tile(ScaledArgs g, hipStream_t stream) {
     return check_launch("sp_gemm_abt_scaled");
 }
 
-template <int F8A, int F8B, bool FAST, int SHIFT, int TM, int TN, int NS>
+template <int F8A, int F8B, int SHIFT, int TM, int TN, int NS>
 static int launch_split(ScaledArgs g, hipStream_t stream) {
-    auto kernel = gemm_scaled_split_kernel<F8A, F8B, FAST, SHIFT, TM, TN, NS>;
+    auto kernel = gemm_scaled_split_kernel<F8A, F8B, SHIFT, TM, TN, NS>;
     constexpr int ring = 4 * (NS * 2 * (TM + TN) * 8 * ROW_BYTES + 2 * (TM + (SHIFT == 7 ? 1 : TN)) * 256), partial = TM * TN * 4096;
     constexpr int lds_bytes = ring > partial ? ring : partial;
     if (const int rc = check_tiles(g, 16 * TM, 16 * TN, 256); rc != SP_OK) return rc;
@@ -566,36 +536,29 @@ static int launch_split(ScaledArgs g, hipStream_t stream) {
 }
 
 // Which kernel: the largest tile that still gives every compute unit one (and half of them for 128 x 128); else the split ones.
-// Measured, bf16 C and scales of 128 x 128 of B unless said otherwise (us): 4096^3 256 x 256 65, 128 x 256 90, 128 x 128 92;
-// 2048 x 4096 x 4096 56, 43, 43.5; 1024 x 4096 x 4096 128 x 256 35, 128 x 128 28.5, split 64 x 64 50; 512 x 4096 x 4096 128 x 128 26.7, split 64 x 64 26;
-// 256 x 4096 x 4096 26.5, 14.2, split 32 x 32 15.9; 128 x 4096 x 4096 26.4, 14, 10; 64 x 4096 x 4096 split 64 x 64 13.9, 32 x 32 6.9;
-// 49 x 32003 x 4096 split 64 x 64 33, 32 x 32 41 (f32 C 36, 42: two workgroups of 64 x 64 on a unit; with more LDS for scales, one, 37 and 39); 32 x 32003 x 4096 35, 32; 1 x 4096 x 4096 split 32 x 32 6.8, 16 x 16 5.6;
-// 1 x 16384 x 16384 62, 54; 4096 x 2048 x 5008, f32 C and scales per row of B: 128 x 256 89, 128 x 128 101.  (256 x 256 with C of f32, or scales per row of B,
-// has no room for the f16 fragments, or the scales, in its registers.)
-template <int F8A, int F8B, bool FAST, int SHIFT>
+// Measured (us), bf16 C, scales of 128 x 128 of B, N = K = 4096: 4096 rows 128 x 256 122, 128 x 128 129; 2048 rows 61, 65.5; 1024 rows 54, 42, split 64 x 64 46; 512 rows
+// 128 x 128 41, split 64 x 64 25, 32 x 32 34.5; 256 rows 40.5, 18.4, 19.7; 128 rows split 64 x 64 17.3, 32 x 32 11.3, 16 x 16 19.9; 64 rows 16.9, 8.0, 11.9; 16 rows
+// split 32 x 32 7.6, 16 x 16 6.3; one row 7.6, 6.0.  49 x 32003 x 4096 split 64 x 64 35.4, 32 x 32 42.9 (f32 C 35.6, 43.1); 32 x 32003 x 4096 33.3, 32.2; 1 x 16384 x 16384
+// split 32 x 32 64, 16 x 16 55; 4096 x 2048 x 5008, f32 C and scales per row of B: 128 x 256 95.7, 128 x 128 99.
+template <int F8A, int F8B, int SHIFT>
 static int multiply(const ScaledArgs& g, hipStream_t stream) {
     const long cus = device_cu_count();
     auto tiles = [&](long bm, long bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
     if (g.M > 64) {
-        if constexpr (FAST && SHIFT == 7) {
-            if (tiles(256, 256) >= cus) return launch_tile<F8A, F8B, FAST, SHIFT, 256, 256, 2, 4>(g, stream);
-        } else {
-            if (tiles(128, 256) >= cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 256, 2, 4>(g, stream);
-        }
-        if (tiles(128, 128) * 2 > cus) return launch_tile<F8A, F8B, FAST, SHIFT, 128, 128, 2, 2>(g, stream);
+        if (tiles(128, 256) >= cus) return launch_tile<F8A, F8B, SHIFT, 128, 256, 2, 4>(g, stream);
+        if (tiles(128, 128) * 2 > cus) return launch_tile<F8A, F8B, SHIFT, 128, 128, 2, 2>(g, stream);
     }
-    if (g.M <= 16) return launch_split<F8A, F8B, FAST, SHIFT, 1, 1, 4>(g, stream);
-    if (g.M <= 32 || tiles(32, 32) <= 3 * cus) return launch_split<F8A, F8B, FAST, SHIFT, 2, 2, 2>(g, stream);
-    return launch_split<F8A, F8B, FAST, SHIFT, 4, 4, 1>(g, stream);
+    if (g.M <= 16) return launch_split<F8A, F8B, SHIFT, 1, 1, 4>(g, stream);
+    if (g.M <= 32 || tiles(32, 32) <= 3 * cus) return launch_split<F8A, F8B, SHIFT, 2, 2, 2>(g, stream);
+    return launch_split<F8A, F8B, SHIFT, 4, 4, 1>(g, stream);
 }
 
 namespace {
 struct GemmScaledKernelNames {
     GemmScaledKernelNames() {
-        register_kernel("gemm_scaled_256x256", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 256, 256, 2, 4>, 512);
-        register_kernel("gemm_scaled_f32_128x256", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, false, 7, 128, 256, 2, 4>, 512);
-        register_kernel("gemm_scaled_128x128", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 128, 128, 2, 2>, 256);
-        register_kernel("gemm_scaled_split_16x16", (const void*)gemm_scaled_split_kernel<SP_F8_E4M3, SP_F8_E4M3, true, 7, 1, 1, 4>, 256);
+        register_kernel("gemm_scaled_128x256", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, 7, 128, 256, 2, 4>, 512);
+        register_kernel("gemm_scaled_128x128", (const void*)gemm_scaled_tile_kernel<SP_F8_E4M3, SP_F8_E4M3, 7, 128, 128, 2, 2>, 256);
+        register_kernel("gemm_scaled_split_16x16", (const void*)gemm_scaled_split_kernel<SP_F8_E4M3, SP_F8_E4M3, 7, 1, 1, 4>, 256);
     }
 } gemm_scaled_kernel_names;
 }  // namespace
@@ -632,8 +595,7 @@ extern "C" int sp_gemm_abt_scaled(int f8_a, int f8_b, int dtype_out, const void*
     auto by_block = [&](auto fa, auto fb) {
         constexpr int FA = decltype(fa)::value, FB = decltype(fb)::value;
         const hipStream_t st = (hipStream_t)stream;
-        if (dtype_out == SP_F32) return block_n == 128 ? multiply<FA, FB, false, 7>(g, st) : multiply<FA, FB, false, 0>(g, st);
-        return block_n == 128 ? multiply<FA, FB, true, 7>(g, st) : multiply<FA, FB, true, 0>(g, st);
+        return block_n == 128 ? multiply<FA, FB, 7>(g, st) : multiply<FA, FB, 0>(g, st);
     };
     typedef std::integral_constant<int, SP_F8_E4M3> e4m3;
     typedef std::integral_constant<int, SP_F8_E5M2> e5m2;

@@ -353,3 +353,41 @@ def test_weight_gradients_add_up(M):
         part = lambda v, s: (v.view(torch.uint8)[:, at:at + 256].contiguous().view(v.dtype), s[:, at // 128:at // 128 + 2].contiguous())
         M.matmul_abt_scaled(*part(a, sa), *part(b, sb), c=dw, beta=1.0)
     assert torch.equal(dw, whole)
+
+
+def test_small_products_beside_large_ones_that_cancel(M):
+    """Of every eight products along K two are 2^16 and -2^16, the others integers of at most 9: what is left is exact in f32, so every type of C is its
+    rounding.  A sum that keeps fewer bits than f32 (13 below the largest of eight, say) has none of it."""
+    for m, n in ((5, 64), (40, 130), (200, 301), (49, 25001), (2304, 2304), (4224, 4112)):
+        for fa, fb, wide in (("e4m3", "e4m3", True), ("e5m2", "e4m3", False)):
+            announce("matmul_abt_scaled cancelling products %s" % ((m, n, fa, fb, wide),))
+            g = torch.Generator().manual_seed(13)
+            k = 272
+            a, b = (torch.randint(-3, 4, (r, k), generator=g).float() for r in (m, n))
+            for at in range(0, k, 8):
+                p, q = (at + torch.randperm(8, generator=g)[:2]).tolist()
+                sign = torch.randint(0, 2, (m,), generator=g) * 512. - 256.
+                a[:, p], a[:, q], b[:, p], b[:, q] = sign, -sign, 256., 256.
+            power = lambda *shape: torch.exp2(torch.randint(-1, 2, shape, generator=g).float())
+            a, sa, b, sb = a.to(F8[fa]), power(m, 3), b.to(F8[fb]), power(blocks(n) if wide else n, 3)
+            want, _ = product64(a, sa, b, sb)
+            a, sa, b, sb = (v.cuda() for v in (a, sa, b, sb))
+            for out in (torch.float32, torch.bfloat16, torch.float16):
+                c = M.matmul_abt_scaled(a, sa, b, sb, out_dtype=out)
+                assert torch.equal(c, want.float().to(out)), (m, n, out, float((c.double() - want).abs().max()))
+
+
+@pytest.mark.parametrize("types", ["e4m3 e4m3", "e5m2 e4m3", "e5m2 e5m2"])
+@pytest.mark.parametrize("m,n,k,wide", [(1, 500, 4096, True), (50, 1000, 528, True), (300, 200, 272, False), (2048, 2304, 656, True), (4224, 4112, 400, False)])
+def test_16_bit_results_are_roundings_of_f32_sums(M, m, n, k, wide, types):
+    fa, fb = types.split()
+    announce("matmul_abt_scaled 16 bits %s" % ((m, n, k, wide, types),))
+    a, sa, b, sb = operands(m, n, k, wide, fa, fb, 14)
+    want, size = product64(a, sa, b, sb)
+    bound = (128 * 2 + 2 + blocks(k) + 8) * U * size            # of the f32 sums, as in test_product
+    a, sa, b, sb = (v.cuda() for v in (a, sa, b, sb))
+    for t in (torch.bfloat16, torch.float16):
+        off = (M.matmul_abt_scaled(a, sa, b, sb, out_dtype=t).double() - want).abs()
+        fine = want.abs() < 60000
+        allowed = bound + torch.finfo(t).eps / 2 * (want.abs() + bound) + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+        assert (off <= allowed)[fine].all(), float((off / allowed)[fine].max())
