@@ -301,8 +301,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_scaled_tile_kernel(const 
     auto add = [&](int i, int j, float scale, const f32x4& scale_n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float t = SHIFT == 7 ? sums[i & 1][j][e] : sums[i & 1][j][e] * scale_n[e];
-            acc[i][j][e] = __builtin_fmaf(t, scale, acc[i][j][e]);
+            // (the scales first, as in the other kernel: the sum times one of them may be no f32 where the product of both is)
+            acc[i][j][e] = __builtin_fmaf(sums[i & 1][j][e], SHIFT == 7 ? scale : scale * scale_n[e], acc[i][j][e]);
         }
         asm volatile("" : "+v"(acc[i][j]));            // here, not where the loop ends: that is where the compiler would gather them
     };

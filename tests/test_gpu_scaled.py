@@ -391,3 +391,17 @@ def test_16_bit_results_are_roundings_of_f32_sums(M, m, n, k, wide, types):
         fine = want.abs() < 60000
         allowed = bound + torch.finfo(t).eps / 2 * (want.abs() + bound) + torch.finfo(t).smallest_normal * torch.finfo(t).eps
         assert (off <= allowed)[fine].all(), float((off / allowed)[fine].max())
+
+
+@pytest.mark.parametrize("wide", [True, False])
+def test_scales_far_apart(M, wide):
+    """Only the product of two scales has to be a number of f32: neither times the sum alone does.  Everything here is exact."""
+    for m, n in ((5, 64), (40, 130), (200, 301), (49, 25001), (2304, 2304), (4224, 4112)):
+        announce("matmul_abt_scaled scales far apart %s" % ((m, n, wide),))
+        a, sa, b, sb = operands(m, n, 272, wide, "e5m2", "e5m2", 15, whole=True)
+        for step, up in ((1.0, 125), (1.0, -125), (2.0 ** -16, 125), (2.0 ** -16, -125)):
+            x, y = (a.float() * step).to(a.dtype), (b.float() * step).to(b.dtype)
+            far, near = sa * 2.0 ** up, sb * 2.0 ** -up
+            want, _ = product64(x, far, y, near)
+            c = M.matmul_abt_scaled(x.cuda(), far.cuda(), y.cuda(), near.cuda())
+            assert torch.equal(c.double(), want), (m, n, step, up)
