@@ -32,6 +32,9 @@ __device__ __forceinline__ unsigned pack_f8(float a, float b, float c, float d) 
     return (unsigned)v;
 }
 
+// The first `left` of four bytes, and zeros: what lies behind a row is zeros whatever its block's scale is (0 / inf and 0 / NaN are NaNs).
+__device__ __forceinline__ unsigned first_bytes(unsigned v, long left) { return left >= 4 ? v : left <= 0 ? 0u : v & ((1u << (8 * (int)left)) - 1u); }
+
 struct BlockScale {
     float scale, inv;
     template <int F8>
@@ -112,6 +115,7 @@ __global__ __launch_bounds__(ROWS / R * LANES) void quantize_kernel(const void* 
         }
     }
     if constexpr (ROW) {
+        const bool ends = ((int)cols & 15) != 0 && (tile_c + 1) * COLS > cols;             // the rows end inside this tile, with padding behind them
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             BlockScale s = one;
@@ -125,10 +129,15 @@ __global__ __launch_bounds__(ROWS / R * LANES) void quantize_kernel(const void* 
             u32x2 o;
             o.x = pack_f8<F8>(s(value(i, 0)), s(value(i, 1)), s(value(i, 2)), s(value(i, 3)));
             o.y = pack_f8<F8>(s(value(i, 4)), s(value(i, 5)), s(value(i, 6)), s(value(i, 7)));
+            if (ends) {
+                o.x = first_bytes(o.x, cols - c0);
+                o.y = first_bytes(o.y, cols - c0 - 4);
+            }
             if (r0 + i < rows && c0 < args.pitch) put(args.q + (r0 + i) * args.pitch + c0, o);
         }
     }
     if constexpr (COL) {
+        const bool ends = ((int)rows & 15) != 0 && (tile_r + 1) * ROWS > rows;
         unsigned column[8];                   // !WIDE: the largest magnitude of each of this lane's columns
         if constexpr (!WIDE) {
 #pragma unroll
@@ -155,9 +164,11 @@ __global__ __launch_bounds__(ROWS / R * LANES) void quantize_kernel(const void* 
                 if (rg == 0 && c0 + j < cols) args.scale_t[(c0 + j) * args.blocks_r + tile_r] = s.scale;
             }
 #pragma unroll
-            for (int i = 0; i < R; i += 4)
-                *reinterpret_cast<unsigned*>(turned + (cg * 8 + j) * PITCH + rg * R + i) =
-                    pack_f8<F8>(s(value(i, j)), s(value(i + 1, j)), s(value(i + 2, j)), s(value(i + 3, j)));
+            for (int i = 0; i < R; i += 4) {
+                unsigned o = pack_f8<F8>(s(value(i, j)), s(value(i + 1, j)), s(value(i + 2, j)), s(value(i + 3, j)));
+                if (ends) o = first_bytes(o, rows - r0 - i);
+                *reinterpret_cast<unsigned*>(turned + (cg * 8 + j) * PITCH + rg * R + i) = o;
+            }
         }
         __syncthreads();
         // 16 bytes per lane: eight lanes a row of 128 bytes

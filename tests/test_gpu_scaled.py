@@ -405,3 +405,23 @@ def test_scales_far_apart(M, wide):
             want, _ = product64(x, far, y, near)
             c = M.matmul_abt_scaled(x.cuda(), far.cuda(), y.cuda(), near.cuda())
             assert torch.equal(c.double(), want), (m, n, step, up)
+
+
+@pytest.mark.parametrize("bad", ["inf", "-inf", "nan"])
+@pytest.mark.parametrize("f8", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("high", [1, 128])
+def test_padding_is_zeros_beside_bad_numbers(M, high, f8, bad):
+    """An infinity or a NaN in the last block of a row makes its numbers NaNs, zeros among them, and leaves the columns behind them zeros."""
+    for dtype in TYPES:
+        for rows, cols in ((1, 1), (3, 7), (140, 300), (131, 1003), (2, 12), (260, 133)):
+            announce("quantize_blocks padding %s" % ((rows, cols, high, f8, bad, dtype),))
+            x = torch.randn((rows, cols), generator=torch.Generator().manual_seed(17)).to(TYPES[dtype])
+            x[rows // 2, cols // 2] = 0
+            x[rows - 1, cols - 1] = float(bad)
+            for transpose in (False, True, "both"):
+                forms = [v.cpu() for v in M.quantize_blocks(x.cuda(), (high, 128), F8[f8], transpose=transpose)]
+                for i, form in enumerate(zip(forms[::2], forms[1::2])):
+                    q, scale, y = form[0].view(torch.uint8), form[1], x if transpose is False or (transpose == "both" and i == 0) else x.t()
+                    assert (q[:, y.shape[1]:] == 0).all() and not scale[-1, -1].isfinite()
+                    last = slice((y.shape[0] - 1) // 128 * 128, None) if high == 128 else slice(y.shape[0] - 1, None)
+                    assert form[0].float()[last, (y.shape[1] - 1) // 128 * 128:y.shape[1]].isnan().all()
