@@ -425,3 +425,19 @@ def test_padding_is_zeros_beside_bad_numbers(M, high, f8, bad):
                     assert (q[:, y.shape[1]:] == 0).all() and not scale[-1, -1].isfinite()
                     last = slice((y.shape[0] - 1) // 128 * 128, None) if high == 128 else slice(y.shape[0] - 1, None)
                     assert form[0].float()[last, (y.shape[1] - 1) // 128 * 128:y.shape[1]].isnan().all()
+
+
+# Loops long enough that every stage of LDS, those of the scales among them, is filled again and again, with a tail of K; on 256 compute units these
+# are the 16 x 16, 32 x 32 and 64 x 64 split tiles, then 128 x 128 and 128 x 256
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 8208), (9, 300, 12304), (20, 3000, 8208), (100, 515, 12304), (49, 12850, 8208), (2048, 2304, 1040), (2048, 2304, 2320),
+                                   (2100, 2241, 4176), (4224, 4112, 1040), (4100, 2200, 2320), (4096, 2304, 4112)])
+def test_product_of_many_blocks_is_exact(M, m, n, k, wide):
+    announce("matmul_abt_scaled many blocks %s" % ((m, n, k, wide),))
+    a, sa, b, sb = operands(m, n, k, wide, "e4m3", "e5m2", 16, whole=True)
+    want, size = product64(a, sa, b, sb)
+    assert float(size.max()) < 2 ** 22                  # in quarters: below 2^24 of them
+    a, sa, b, sb = (v.cuda() for v in (a, sa, b, sb))
+    for out in (torch.float32, torch.bfloat16):
+        c = M.matmul_abt_scaled(a, sa, b, sb, out_dtype=out)
+        assert torch.equal(c, want.float().to(out)), (out, (c.double() - want).abs().max())
