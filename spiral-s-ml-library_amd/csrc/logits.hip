@@ -5,7 +5,9 @@
 // them is gathered meanwhile in a 32-bit word of LDS per column -- bits 0..19 the count behind the prompt, bit 20 "seen in the prompt", bits 21..31
 // the first bias entry that names the column -- with integer atomics, whose order does not matter.  Columns whose word is zero, most of them, then
 // cost one LDS read.
-// A column named by several bias entries (rare; a flag says whether there is one at all) goes through the entries again, in their order.
+// Columns named by several bias entries (rare; a flag says whether there is one at all) have theirs added up in their order, in an LDS sum at the place of the first of them: the
+// waves go through the entries once more, each for columns of its own.  1 x 32003, 2047 entries, none twice 11 us, one twice 17, half of them one id (a padded list)
+// 51; with every named column going through the entries by itself, once one stood there twice, 10, 1230, 1220.
 // The arithmetic is that of the steps written out, each rounded to f32: nothing is contracted.
 #include "vec_io.h"
 
@@ -80,7 +82,7 @@ template <int DT, bool SPARSE, int CHUNK, int THREADS, int POLICY>
 __global__ __launch_bounds__(THREADS) void logits_kernel(const void* logits, long cols, unsigned chunks, const LogitsArgs a) {
     constexpr int N = 4, STEP = THREADS * N, PIECES = CHUNK / STEP;
     static_assert(CHUNK % STEP == 0 && CHUNK % 32 == 0, "whole pieces, whole words of the mask");
-    extern __shared__ __attribute__((aligned(16))) unsigned words[];       // SPARSE: CHUNK of them
+    extern __shared__ __attribute__((aligned(16))) unsigned words[];       // SPARSE: CHUNK of them, and behind them a sum per bias entry
     __shared__ int again;                                  // a column has more than one bias entry
     __shared__ float wave_v[THREADS / 64];
     __shared__ int wave_at[THREADS / 64];
@@ -153,6 +155,28 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const void* logits, lon
             if (tokens_at(v) < length) take(ahead[v], tokens_at(v));
         for (long i = tokens_at(AHEAD); i < length; i += THREADS * 4) take(load16<SP_F32>(mine, i, length - i), i);
         __syncthreads();
+        if (a.n_bias > 0 && again != 0) {
+            float* sums = reinterpret_cast<float*>(words + CHUNK);
+            for (int j = tid; j < a.n_bias; j += THREADS) sums[j] = biases[j];
+            __syncthreads();
+            const int wave = tid >> 6;
+            for (int j0 = 0; j0 < a.n_bias; j0 += 64) {
+                const int j = j0 + (tid & 63);
+                const unsigned at = j < a.n_bias ? (unsigned)ids[j] - first : ~0u;
+                const int to = at < (unsigned)here ? MOST_ENTRIES - (int)(words[at] >> ENTRY_SHIFT) : j;      // the column's first entry
+                const bool adds = to != j && to % (THREADS / 64) == wave;
+                const float b = adds ? biases[j] : 0.f;
+                for (unsigned long todo = __ballot(adds); todo != 0;) {
+                    const int column = __builtin_amdgcn_readlane(to, __builtin_ctzl(todo));
+                    unsigned long same = __ballot(to == column) & todo;
+                    todo &= ~same;
+                    float s = sums[column];
+                    for (; same != 0; same &= same - 1) s = s + __int_as_float(__builtin_amdgcn_readlane(__float_as_int(b), __builtin_ctzl(same)));
+                    sums[column] = s;                      // (of all lanes the same)
+                }
+            }
+            __syncthreads();
+        }
     }
     Best best{-INFINITY, -1};
 #pragma unroll
@@ -177,11 +201,7 @@ __global__ __launch_bounds__(THREADS) void logits_kernel(const void* logits, lon
                     }
                     if (const unsigned entry = w[e] >> ENTRY_SHIFT; entry != 0) {
                         const int first = MOST_ENTRIES - (int)entry;
-                        float b = biases[first];
-                        if (again != 0)
-                            for (int j = first + 1; j < a.n_bias; ++j)
-                                if (ids[j] == c0 + i + e) b += biases[j];
-                        x = x + b;
+                        x = x + (again != 0 ? reinterpret_cast<const float*>(words + CHUNK)[first] : biases[first]);
                     }
                     v[e] = x;
                 }
@@ -236,8 +256,8 @@ static int64_t logits_chunks(int64_t rows, int64_t cols) { return chunks_of(cols
 template <int DT, bool SPARSE, int CHUNK, int THREADS, int POLICY>
 static int launch_chunks(const void* logits, long rows, long cols, unsigned chunks, const LogitsArgs& a, hipStream_t stream) {
     auto kernel = logits_kernel<DT, SPARSE, CHUNK, THREADS, POLICY>;
-    constexpr int lds_bytes = SPARSE ? CHUNK * 4 : 0;
-    if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
+    if (const int rc = ensure_dynamic_lds((const void*)kernel, SPARSE ? (CHUNK + MOST_ENTRIES + 1) * 4 : 0); rc != SP_OK) return rc;
+    const int lds_bytes = SPARSE ? (CHUNK + (a.n_bias + 3) / 4 * 4) * 4 : 0;
     hipLaunchKernelGGL(kernel, dim3((unsigned)rows * chunks), dim3(THREADS), lds_bytes, stream, logits, cols, chunks, a);
     return check_launch("sp_logits_penalize");
 }

@@ -276,3 +276,28 @@ def test_from_a_hidden_state_to_a_token(P):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(want, kept)), k
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 32003), (3, 2100), (40, 32003), (2, 9000)])
+@pytest.mark.parametrize("kind", ["padding", "pairs", "runs", "few", "all", "one"])
+def test_biases_of_ids_that_repeat(P, rows, cols, kind):
+    """Their sum in their order: numbers of which most orders round differently."""
+    for n in (2, 64, 65, 300, 2047):
+        announce("penalize_logits repeated ids %s" % ((rows, cols, kind, n),))
+        g = torch.Generator().manual_seed(12)
+        ids = torch.stack([torch.randperm(cols, generator=g)[:n] if n <= cols else torch.randint(0, cols, (n,), generator=g) for _ in range(rows)])
+        if kind == "padding":
+            ids[:, n // 2:] = ids[:, :1]
+        elif kind == "pairs":
+            ids[:, n // 2:n // 2 * 2] = ids[:, :n // 2].flip(1)
+        elif kind == "runs":
+            ids = ids.sort(1).values // 7 * 7
+        elif kind == "few":
+            ids = ids % 5 * (cols // 5)
+        elif kind == "all":
+            ids[:] = cols - 1
+        else:
+            ids[:, -1] = ids[:, 0]
+        kw = dict(bias_ids=ids.int(), bias=torch.randn((rows, n), generator=g) * torch.exp2(torch.randint(-12, 13, (rows, n), generator=g).float()))
+        kw["bias_ids"][:, 1::9] = -1
+        check(P, torch.randn((rows, cols), generator=g), kw)
