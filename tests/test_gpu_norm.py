@@ -250,3 +250,22 @@ def test_offsets_past_32_bits(P):
     y = P.layer_norm(x)
     assert torch.equal(y[-8:], P.layer_norm(x[-8:].clone())) and torch.equal(y[:8], P.layer_norm(x[:8].clone()))
     assert (y[rows // 2] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_rows_of_one_number(P, dtype):
+    """Sums of equal numbers of 16 bits are exact in f32, bf16 of any width and f16 up to 8192 columns: such rows are exactly zero behind the mean.  f32 rows
+    are as far from it as the sum's roundings put the mean."""
+    t = TYPES[dtype]
+    for rows, cols in ((200, 1003), (40, 96), (3, 8192), (600, 5001), (2, 7909), (5, 7), (2, 16384 if dtype == "bf16" else 4099)):
+        announce("layer_norm rows of one number %d x %d %s" % (rows, cols, dtype))
+        g = torch.Generator().manual_seed(11)
+        value = (torch.randn((rows, 1), generator=g) * 100).to(t)
+        b = torch.randn((cols,), generator=g)
+        y, mean, rstd = (v.cpu() for v in P.layer_norm(value.expand(rows, cols).contiguous().cuda(), None, b.cuda(), eps=0.25, want_stats=True))
+        if dtype == "f32":
+            off = (CHAIN + 2) * U * value.double().abs()
+            assert ((mean.double() - value[:, 0].double()).abs() <= off[:, 0]).all()
+            assert ((y.double() - b.double()).abs() <= off * 2 * 1.001 + 2 * U * (b.double().abs() + off * 2)).all()      # (x - mean, times a rstd of at most 2, plus b)
+        else:
+            assert torch.equal(mean, value[:, 0].float()) and (rstd == 2).all() and torch.equal(y, b.to(t).expand(rows, cols))
