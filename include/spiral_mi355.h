@@ -171,7 +171,7 @@ int sp_quantize_blocks(int dtype, int f8, int32_t block_rows, const void* x, voi
  * NULL; beta == 0: C is not read.  flags: SP_GEMM_RELU.  scale_a * scale_b has to be a finite f32, and
  * holds fewer bits below 2^-126.  A result depends on its row of A, its
  * row of B, the shape and the type of C alone.
- * Products are exact and sums f32, whatever the type of C.
+ * Products are exact and sums f32, whatever the type of C.  ReLU makes a NaN 0, as in sp_gemm_abt.
  * Stands beside sp_gemm_abt (ml/matmul/run.spi:21-26), which multiplies 16- and 32-bit operands.
  */
 int sp_gemm_abt_scaled(int f8_a, int f8_b, int dtype_out, const void* A, const float* scale_a, const void* B, const float* scale_b,

@@ -143,13 +143,14 @@ def matmul_abt_scaled(a, scale_a, b, scale_b, c=None, beta=0.0, bias=None, relu=
     """C = A . B^T + beta * C (+ bias, ReLU) of 8-bit operands with a scale for each block of 128 along K (sp_gemm_abt_scaled): the
     numbers a (M, K), b (N, K), e4m3 or e5m2, and their scales as `quantize_blocks` gives them.  scale_a is (M, ceil(K / 128)), scale_b
     (N, ceil(K / 128)) or, in blocks of 128 x 128, (ceil(N / 128), ceil(K / 128)).  `c` (f32, f16 or bf16) is updated in place and returned; when it
-    is None a new (M, N) tensor of `out_dtype` (default f32) is allocated by torch (beta must then be 0).  Sums are f32.
+    is None a new (M, N) tensor of `out_dtype` (default f32) is allocated by torch (beta must then be 0).  Sums are f32, whatever the type of C;
+    ReLU makes a NaN 0, as in `matmul_abt`.
 
     A layer y = x . W^T and its gradients, with dy, x and W of M x N, M x K and N x K:
         x8, sx, xt, sxt = quantize_blocks(x, transpose="both");  w8, sw, wt, swt = quantize_blocks(W, (128, 128), transpose="both")
         d8, sd, dt, sdt = quantize_blocks(dy, dtype=torch.float8_e5m2, transpose="both")
         y = matmul_abt_scaled(x8, sx, w8, sw);  dx = matmul_abt_scaled(d8, sd, wt, swt);  dW = matmul_abt_scaled(dt, sdt, xt, sxt)
-    (with N, K and M multiples of 16; otherwise the padding of q shows in the widths of what they are multiplied with)."""
+    for any M, N and K: both operands of a product have the same padding."""
     if c is None and beta == 0.0:
         done = lib.whole_matmul_abt_scaled(a, scale_a, b, scale_b, bias, relu, out_dtype or torch.float32)
         if done is not None:

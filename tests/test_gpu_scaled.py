@@ -1,4 +1,6 @@
 """8-bit blocks and their product on the GPU against float64, with bounds counted from the roundings."""
+import math
+
 import pytest
 import torch
 
@@ -441,3 +443,36 @@ def test_product_of_many_blocks_is_exact(M, m, n, k, wide):
     for out in (torch.float32, torch.bfloat16):
         c = M.matmul_abt_scaled(a, sa, b, sb, out_dtype=out)
         assert torch.equal(c, want.float().to(out)), (out, (c.double() - want).abs().max())
+
+
+def test_a_layer_and_its_gradients_at_odd_sizes(M):
+    """What both operands of a product are padded with are zeros of the same width: the three products have the shapes and values of the plain ones."""
+    announce("a layer in 8 bits, odd sizes")
+    m, n, k = 261, 133, 515
+    g = torch.Generator().manual_seed(18)
+    x, w, dy = (torch.randint(-3, 4, s, generator=g).float() for s in ((m, k), (n, k), (m, n)))
+    for v in (x, w, dy):                                        # scales of 1 or powers of two: 448 or 57344 in every block
+        v[::64, ::64] = 448.
+    dy[dy == 448.] = 57344.
+    x8, sx, xt, sxt = M.quantize_blocks(x.cuda(), (1, 128), transpose="both")
+    w8, sw, wt, swt = M.quantize_blocks(w.cuda(), (128, 128), transpose="both")
+    d8, sd, dt, sdt = M.quantize_blocks(dy.cuda(), dtype=torch.float8_e5m2, transpose="both")
+    back = lambda q, s, rows, cols: q.cpu().double()[:, :cols] * spread(s.cpu(), rows, cols, 1 if s.shape[0] == rows else 128).double()
+    for got, a, b in ((M.matmul_abt_scaled(x8, sx, w8, sw), back(x8, sx, m, k), back(w8, sw, n, k)),
+                      (M.matmul_abt_scaled(d8, sd, wt, swt), back(d8, sd, m, n), back(wt, swt, k, n)),
+                      (M.matmul_abt_scaled(dt, sdt, xt, sxt), back(dt, sdt, n, m), back(xt, sxt, k, m))):
+        assert got.shape == (a.shape[0], b.shape[0])
+        size = a.abs() @ b.abs().t()
+        assert ((got.cpu().double() - a @ b.t()).abs() <= (128 * 2 + 2 + 5 + 8) * U * size).all()      # (as in test_product)
+
+
+def test_relu_makes_a_nan_zero(M):
+    announce("matmul_abt_scaled NaN and ReLU")
+    for m, n in ((9, 70), (40, 130), (300, 2301), (2304, 2304)):
+        a, sa, b, sb = operands(m, n, 272, True, "e4m3", "e4m3", 19)
+        codes = a.view(torch.uint8).clone()
+        codes[m // 2, 271] = 0x7f
+        a, sa, b, sb = codes.view(a.dtype).cuda(), sa.cuda(), b.cuda(), sb.cuda()
+        for out in (torch.float32, torch.bfloat16, torch.float16):
+            c = M.matmul_abt_scaled(a, sa, b, sb, relu=True, out_dtype=out)
+            assert (c[m // 2] == 0).all() and torch.equal(c, M.matmul_abt_scaled(a, sa, b, sb, out_dtype=out).nan_to_num(0, math.inf).clamp(min=0))
