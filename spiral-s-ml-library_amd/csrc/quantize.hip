@@ -194,12 +194,12 @@ static int launch_quantize(const QuantArgs& a, hipStream_t stream) {
 }
 
 // Rows per lane of the 128 x 128 tiles: 4 (eight waves) where a tile has one scale, 8 where every row or column has its own, whose steps across
-// lanes count then.  (us, 8 / 4 rows: 8192 x 4096 bf16 both ways in 128 x 128 blocks 23.8 / 22.2; 16384 x 4096 both ways in rows of 128
-// 59.3 / 66.2, transposed alone 43.5 / 48.5.  Written back instead of streamed 27.5 / 25.8, 62.8 / 67.7, 44.9 / 49.)
-// Where the chip has less than two tiles a unit the way through one counts, 4 rows per lane: 16 x 4096 bf16 both ways in rows of 128 6.9 / 5.8,
-// 512 x 1024 6.7 / 6.3, 2047 x 3000 12.2 / 12.0; 2048 x 4096, two a unit, is on 8.
+// lanes count then.  (us, 8 / 4 rows: 8192 x 4096 bf16 both ways in 128 x 128 blocks 22.6 / 22.2; 16384 x 4096 both ways in rows of 128
+// 60.1 / 69.5, transposed alone 43.8 / 50.2.  Written back instead of streamed 27.5 / 25.8, 62.8 / 67.7, 44.9 / 49.)
+// Where the chip has less than two tiles a unit the way through one counts, 4 rows per lane: 16 x 4096 bf16 both ways in rows of 128 7.4 / 6.5,
+// 512 x 1024 7.3 / 6.7, 2047 x 3000 12.7 / 12.4; 2048 x 4096, two a unit, is on 8.
 // Transposed alone, in tiles of 64 columns and 4 rows per lane there: 5001 x 1003 f32 11.1 / 10.1,
-// 512 x 1024 bf16 5.3 / 4.7; 2048 x 4096 bf16, two a unit, 9.0 / 9.15, 8192 x 4096 21.6 / 22.8.
+// 512 x 1024 bf16 5.6 / 4.8; 2048 x 4096 bf16, two a unit, 9.0 / 9.15, 8192 x 4096 21.6 / 22.8.
 template <int DT, int F8, int POLICY>
 static int quantize(const QuantArgs& a, bool wide, hipStream_t stream) {
     const int out = (a.q != nullptr ? 1 : 0) | (a.q_t != nullptr ? 2 : 0);
