@@ -476,3 +476,19 @@ def test_relu_makes_a_nan_zero(M):
         for out in (torch.float32, torch.bfloat16, torch.float16):
             c = M.matmul_abt_scaled(a, sa, b, sb, relu=True, out_dtype=out)
             assert (c[m // 2] == 0).all() and torch.equal(c, M.matmul_abt_scaled(a, sa, b, sb, out_dtype=out).nan_to_num(0, math.inf).clamp(min=0))
+
+
+@pytest.mark.parametrize("m,n,k", [(70016, 32771, 32), (5, 140011, 16400), (140011, 130, 16400), (40, 140011, 16400)])
+def test_product_offsets_past_32_bits(M, m, n, k):
+    """More than 2^31 elements of C, of B or of A: the corners are those of a product of them alone, in whole numbers."""
+    announce("matmul_abt_scaled %d x %d x %d" % (m, n, k))
+    g = torch.Generator(device="cuda").manual_seed(20)
+    draw = lambda r: torch.randint(-3, 4, (r, k), generator=g, device="cuda", dtype=torch.int8).to(torch.float8_e4m3fn)
+    scale = lambda r: torch.exp2(torch.randint(-1, 2, (r, blocks(k)), generator=g, device="cuda").float())
+    a, sa, b, sb = draw(m), scale(m), draw(n), scale(n)
+    c = M.matmul_abt_scaled(a, sa, b, sb, out_dtype=torch.bfloat16)
+    ends = lambda r: torch.arange(r, device="cuda").unique() if r <= 300 else torch.cat([torch.arange(130, device="cuda"), torch.arange(r - 130, r, device="cuda")])
+    rows, cols = ends(m), ends(n)
+    part = lambda v, at: v.view(torch.uint8)[at].view(v.dtype)
+    want, _ = product64(part(a, rows), sa[rows], part(b, cols), sb[cols])
+    assert torch.equal(c[rows][:, cols], want.float().bfloat16())
