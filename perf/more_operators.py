@@ -248,7 +248,8 @@ def _own_gated(s):
 def _own_tokens(s):
     case, (_, primitives) = s["case"], _ml()
     if case["kind"] == "tokens":
-        return primitives.token_log_probs(s["x"], s["tokens"], top=min(case["top"], case["cols"]), want_entropy=case["entropy"])
+        out = primitives.token_log_probs(s["x"], s["tokens"], top=min(case["top"], case["cols"]), want_entropy=case["entropy"])
+        return out if isinstance(out, tuple) else (out,)
     out = primitives.token_log_probs(s["x"], s["tokens"], want_entropy=case["entropy"], want_lse=True)
     return tuple(out) + (primitives.token_log_probs_backward(s["d_logp"], s["x"], s["tokens"], out[-1], d_entropy=s["d_entropy"],
                                                              entropy=out[1] if case["entropy"] else None),)
