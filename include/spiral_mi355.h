@@ -178,6 +178,30 @@ int sp_gemm_abt_scaled(int f8_a, int f8_b, int dtype_out, const void* A, const f
                        int32_t block_n, void* C, const float* bias, int64_t M, int64_t N, int64_t K, float beta, uint32_t flags,
                        void* stream);
 
+/*
+ * A gated feed-forward block: C = act(A . B_gate^T) * (A . B_up^T), element by element.  A (M, K), B_gate, B_up (N, K), C (M, N), all of `dtype` (SP_F32, SP_F16,
+ * SP_BF16), row-major; K a multiple of 16 bytes (8; 4 for f32), any M and N.  Sums, activation and product are f32, rounded once; C must not overlap the operands.
+ *   SP_ACT_SILU g / (1 + exp(-g)),  SP_ACT_GELU g (1 + erf(g / sqrt 2)) / 2,  SP_ACT_RELU max(0, g)
+ * gate, up: NULL, or what the backward pass takes, g = A . B_gate^T and u = A . B_up^T, of kept_dtype: dtype, (M, N) each; or SP_F8_E4M3, in the blocks of 1 x 128 of sp_quantize_blocks,
+ * (M, N rounded up to 16) each with gate_scale, up_scale (M, ceil(N / 128)) f32.  Either way they are rounded once, from f32.
+ * Stands beside sp_gemm_abt with its ReLU (ml/layers.spi:194-240 multiplies and activates in two passes).
+ */
+typedef enum { SP_ACT_SILU = 0, SP_ACT_GELU = 1, SP_ACT_RELU = 2 } sp_activation;
+int sp_gemm_abt_gated(int dtype, int activation, const void* A, const void* B_gate, const void* B_up, void* C, int kept_dtype, void* gate,
+                      float* gate_scale, void* up, float* up_scale, int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
+ * Its gradients from dC (M, N), at the g and u that were kept:  dg = dC u act'(g), du = dC act(g), rounded to dtype, and
+ *   dA = dg . B_gate + du . B_up (M, K),   dB_gate = dg^T . A, dB_up = du^T . A (N, K)
+ * in dtype, of f32 sums.  dA may be NULL, and dB_gate with dB_up.  The ReLU's slope at 0 is 0.  Every sum has one order: results repeat bit for bit.
+ * `workspace`: sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N) bytes of device memory that hold dg and du during the call (what they held before does not matter).  Calls
+ * that may run at the same time need one each.
+ */
+int sp_gemm_abt_gated_backward(int dtype, int activation, const void* dC, const void* A, const void* B_gate, const void* B_up, int kept_dtype,
+                               const void* gate, const float* gate_scale, const void* up, const float* up_scale, void* dA, void* dB_gate,
+                               void* dB_up, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t sp_gemm_abt_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t N);
+
 /* ------------------------------------------------------------------------------------------ */
 /* Row primitives                                                                              */
 /* ------------------------------------------------------------------------------------------ */
@@ -375,6 +399,30 @@ int sp_logits_penalize(int dtype, const void* logits, float* out, int32_t* token
                        const int32_t* mask, int64_t mask_rows, int64_t rows, int64_t cols, void* workspace, int64_t workspace_bytes,
                        void* stream);
 int64_t sp_logits_penalize_workspace_bytes(int64_t rows, int64_t cols);
+
+/*
+ * Log probabilities of one token per row of logits (rows, cols) of `dtype` (SP_F32, SP_F16, SP_BF16), any cols, in f32:
+ *   lse = ln sum exp x,   logp = x[token] - lse,   entropy = -sum p ln p with p = exp(x - lse)
+ * logp (rows,) f32; entropy, lse (rows,) f32, each may be NULL.  tokens (rows,) i32: a row whose token is outside [0, cols) has logp 0 (pad with -1).
+ * top: 0 to 32; top_logp, top_ids (rows, top) receive the log probabilities and columns of the row's largest logits, largest first, of equal ones
+ * the lowest column first; -inf and -1 where the row has no more above -inf (a NaN is never among them).
+ * -inf has probability 0.  A row with nothing above -inf: lse and logp -inf, entropy 0.  A row with a NaN or +inf: NaN.
+ * `workspace`: sp_token_log_probs_workspace_bytes(rows, cols, top) bytes of device memory (their former contents do not matter), may be NULL where that is 0; calls that
+ * may run at the same time need one each.  A row's sums have one order for given sizes; in a call of another number of rows they may come out a rounding away.
+ * Stands beside sp_logits_penalize, sp_row_get_prob and SP_ROW_SOFTMAX (ml/primitives.spi:711-716).
+ */
+int sp_token_log_probs(int dtype, const void* logits, const int32_t* tokens, float* logp, float* entropy, float* lse, int32_t top,
+                       float* top_logp, int32_t* top_ids, int64_t rows, int64_t cols, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t sp_token_log_probs_workspace_bytes(int64_t rows, int64_t cols, int32_t top);
+
+/*
+ * The gradient of the logits, from those of logp, entropy and lse (each (rows,) f32 or NULL):
+ *   d_logits[j] = d_logp ([j = token] - p_j) - d_entropy p_j (ln p_j + entropy) + d_lse p_j
+ * logits, tokens as in the forward call, lse (and, with d_entropy, entropy) as it wrote them.  d_logits: like the logits, whose memory it may be.  A row whose token does not count has
+ * no d_logp; one with nothing above -inf has zeros.  p is exp(x - lse) of the f32 lse: of a row of nothing but numbers as low as the type's lowest, whose lse has lost ln(count), it is 1.
+ */
+int sp_token_log_probs_backward(int dtype, const void* logits, const int32_t* tokens, const float* lse, const float* entropy, const float* d_logp,
+                                const float* d_entropy, const float* d_lse, void* d_logits, int64_t rows, int64_t cols, void* stream);
 
 typedef enum { SP_MAP_COPY = 0, SP_MAP_RELU = 1, SP_MAP_TANH = 2, SP_MAP_SIGMOID = 3 } sp_map_op;
 

@@ -381,7 +381,8 @@ struct Entry<int(A...)> {
     X(sp_row_get_prob) X(sp_cem_resample) X(sp_cem_resample_philox) X(sp_row_reduce_f32) X(sp_cem_update_mask) X(sp_row_binarize)   \
     X(sp_map_f32) X(sp_reduce_sum) X(sp_reduce) X(sp_row_l1_normalize) X(sp_reduce_sum_static) X(sp_transpose_inner_b32)            \
     X(sp_mlp_forward) X(sp_mlp_pack_weights) X(sp_mlp_forward_packed) X(sp_mlp_forward_ensemble) X(sp_ensemble_binarize)            \
-    X(sp_stack_forward_f32) X(sp_layer_norm) X(sp_layer_norm_backward) X(sp_logits_penalize) X(sp_quantize_blocks) X(sp_gemm_abt_scaled)
+    X(sp_stack_forward_f32) X(sp_layer_norm) X(sp_layer_norm_backward) X(sp_logits_penalize) X(sp_quantize_blocks) X(sp_gemm_abt_scaled) \
+    X(sp_gemm_abt_gated) X(sp_gemm_abt_gated_backward) X(sp_token_log_probs) X(sp_token_log_probs_backward)
 
 // ---- whole calls: checks, outputs and launch of the operators that a decoding step makes of one token at a time ----
 //
@@ -612,13 +613,132 @@ PyObject* whole_penalize_logits(PyObject* capsule, PyObject* const* a, Py_ssize_
     });
 }
 
+// (a, b_gate, b_up, activation, type that is kept)
+PyObject* whole_matmul_abt_gated(PyObject* capsule, PyObject* const* o, Py_ssize_t n) {
+    return whole(capsule, n, 5, [&](const Bound& bound) {
+        const at::Tensor *a = Whole::given(o[0]), *gate = Whole::given(o[1]), *up = Whole::given(o[2]);
+        Whole call(a);
+        for (const at::Tensor* t : {a, gate, up}) need(t != nullptr && t->dim() == 2 && t->numel() > 0);
+        need(gate->sizes() == up->sizes() && gate->size(1) == a->size(1) && PyLong_Check(o[3]));
+        const int64_t m = a->size(0), k = a->size(1), cols = gate->size(0);
+        const at::ScalarType type = a->scalar_type();
+        const int code = code_of(type), activation = (int)PyLong_AsLong(o[3]);
+        const bool keeps = o[4] != Py_None, f8 = keeps && type_of(o[4]) == at::kFloat8_e4m3fn;
+        need(!keeps || f8 || type_of(o[4]) == type);
+        void *pa = call.at(a, type), *pg = call.at(gate, type), *pu = call.at(up, type), *c = call.make({m, cols}, type, *a), *kept[4] = {};
+        for (int i = 0; keeps && i < 2; ++i) {
+            kept[2 * i] = call.make({m, f8 ? (cols + 15) / 16 * 16 : cols}, f8 ? at::kFloat8_e4m3fn : type, *a);
+            if (f8) kept[2 * i + 1] = call.make({m, blocks_of(cols)}, at::kFloat, *a);
+        }
+        launch((decltype(&sp_gemm_abt_gated))bound.fn, code, activation, pa, pg, pu, c, f8 ? (int)SP_F8_E4M3 : code, kept[0], (float*)kept[1], kept[2], (float*)kept[3], m, cols, k,
+               call.stream);
+        if (!keeps) return call.result(1);
+        PyObject* first = THPVariable_Wrap(std::move(call.out[0]));
+        if (first == nullptr) return first;
+        call.out.erase(call.out.begin());
+        PyObject *rest = call.result(call.out.size()), *both = rest != nullptr ? PyTuple_Pack(2, first, rest) : nullptr;
+        Py_DECREF(first);
+        Py_XDECREF(rest);
+        return both;
+    });
+}
+
+// (dc, a, b_gate, b_up, gate, its scales, up, its scales, activation)
+PyObject* whole_matmul_abt_gated_backward(PyObject* capsule, PyObject* const* o, Py_ssize_t n) {
+    return whole(capsule, n, 9, [&](const Bound& bound) {
+        const at::Tensor *dc = Whole::given(o[0]), *a = Whole::given(o[1]), *gate = Whole::given(o[2]), *up = Whole::given(o[3]);
+        const at::Tensor* kept[4] = {Whole::given(o[4]), Whole::given(o[5]), Whole::given(o[6]), Whole::given(o[7])};
+        Whole call(a);
+        for (const at::Tensor* t : {dc, a, gate, up, kept[0], kept[2]}) need(t != nullptr && t->dim() == 2 && t->numel() > 0);
+        need(bound.more != nullptr && gate->sizes() == up->sizes() && gate->size(1) == a->size(1) && PyLong_Check(o[8]));
+        const int64_t m = a->size(0), k = a->size(1), cols = gate->size(0);
+        const at::ScalarType type = a->scalar_type(), as = kept[0]->scalar_type();
+        const bool f8 = as == at::kFloat8_e4m3fn;
+        const int code = code_of(type), activation = (int)PyLong_AsLong(o[8]);
+        need(dc->size(0) == m && dc->size(1) == cols && (f8 || as == type) && (kept[1] != nullptr) == f8 && (kept[3] != nullptr) == f8);
+        for (int i = 0; i < 4; ++i) {
+            const int64_t wide = i % 2 != 0 ? blocks_of(cols) : f8 ? (cols + 15) / 16 * 16 : cols;
+            need(kept[i] == nullptr || (kept[i]->dim() == 2 && kept[i]->size(0) == m && kept[i]->size(1) == wide));
+        }
+        void *pd = call.at(dc, type), *pa = call.at(a, type), *pg = call.at(gate, type), *pu = call.at(up, type);
+        void *k0 = call.at(kept[0], as), *k1 = call.at(kept[1], at::kFloat), *k2 = call.at(kept[2], as), *k3 = call.at(kept[3], at::kFloat);
+        void *da = call.make({m, k}, type, *a), *dg = call.make({cols, k}, type, *a), *du = call.make({cols, k}, type, *a);
+        const int64_t bytes = ((decltype(&sp_gemm_abt_gated_backward_workspace_bytes))bound.more)(code, m, cols);
+        void* workspace = call.make({bytes}, at::kByte, *a);
+        launch((decltype(&sp_gemm_abt_gated_backward))bound.fn, code, activation, pd, pa, pg, pu, f8 ? (int)SP_F8_E4M3 : code, k0, (const float*)k1, k2, (const float*)k3, da, dg, du,
+               m, cols, k, workspace, bytes, call.stream);
+        return call.result(3);
+    });
+}
+
+// (logits, tokens, top, want_entropy, want_lse)
+PyObject* whole_token_log_probs(PyObject* capsule, PyObject* const* a, Py_ssize_t n) {
+    return whole(capsule, n, 5, [&](const Bound& bound) {
+        const at::Tensor *x = Whole::given(a[0]), *tokens = Whole::given(a[1]);
+        Whole call(x);
+        need(bound.more != nullptr && tokens != nullptr && x->dim() >= 2 && x->numel() > 0 && PyLong_Check(a[2]));
+        const int64_t cols = x->size(-1), rows = x->numel() / cols;
+        const auto lead = x->sizes().slice(0, x->dim() - 1);
+        const long top = PyLong_AsLong(a[2]);
+        need(tokens->sizes() == lead && top >= 0 && top <= 32);
+        const at::ScalarType type = x->scalar_type();
+        const int code = code_of(type);
+        const bool want_entropy = yes(a[3]), want_lse = yes(a[4]);
+        void *from = call.at(x, type), *ids = call.at(tokens, at::kInt), *logp = call.make(lead, at::kFloat, *x), *top_logp = nullptr, *top_ids = nullptr, *workspace = nullptr;
+        void* entropy = want_entropy ? call.make(lead, at::kFloat, *x) : nullptr;
+        void* lse = want_lse ? call.make(lead, at::kFloat, *x) : nullptr;
+        if (top > 0) {
+            std::vector<int64_t> each(lead.begin(), lead.end());
+            each.push_back(top);
+            top_logp = call.make(each, at::kFloat, *x);
+            top_ids = call.make(each, at::kInt, *x);
+        }
+        const size_t results = call.out.size();
+        const int64_t bytes = ((decltype(&sp_token_log_probs_workspace_bytes))bound.more)(rows, cols, (int32_t)top);
+        if (bytes > 0) workspace = call.make({bytes}, at::kByte, *x);
+        launch((decltype(&sp_token_log_probs))bound.fn, code, from, (const int32_t*)ids, (float*)logp, (float*)entropy, (float*)lse, (int32_t)top, (float*)top_logp, (int32_t*)top_ids,
+               rows, cols, workspace, bytes, call.stream);
+        return call.result(results);
+    });
+}
+
+// (d_log_probs, logits, tokens, lse, d_entropy, entropy, d_lse)
+PyObject* whole_token_log_probs_backward(PyObject* capsule, PyObject* const* a, Py_ssize_t n) {
+    return whole(capsule, n, 7, [&](const Bound& bound) {
+        const at::Tensor *x = Whole::given(a[1]), *tokens = Whole::given(a[2]);
+        Whole call(x);
+        need(tokens != nullptr && x->dim() >= 2 && x->numel() > 0);
+        const int64_t cols = x->size(-1), rows = x->numel() / cols;
+        const auto lead = x->sizes().slice(0, x->dim() - 1);
+        need(tokens->sizes() == lead);
+        const int at_each[5] = {0, 3, 4, 5, 6};            // d_log_probs, lse, d_entropy, entropy, d_lse
+        void* each[5];
+        for (int i = 0; i < 5; ++i) {
+            const at::Tensor* t = Whole::given(a[at_each[i]]);
+            need(t == nullptr || t->sizes() == lead);
+            each[i] = call.at(t, at::kFloat);
+        }
+        need(each[1] != nullptr);
+        const at::ScalarType type = x->scalar_type();
+        const int code = code_of(type);
+        void *from = call.at(x, type), *ids = call.at(tokens, at::kInt), *dx = call.make(x->sizes(), type, *x);
+        launch((decltype(&sp_token_log_probs_backward))bound.fn, code, from, (const int32_t*)ids, (const float*)each[1], (const float*)each[3], (const float*)each[0],
+               (const float*)each[2], (const float*)each[4], dx, rows, cols, call.stream);
+        return call.result(1);
+    });
+}
+
 // (Python's name, the function, the entry point, another one it asks)
 #define SP_WHOLE(X)                                                                                        \
     X(layer_norm, sp_layer_norm, nullptr)                                                                   \
     X(layer_norm_backward, sp_layer_norm_backward, "sp_layer_norm_backward_workspace_bytes")                  \
     X(quantize_blocks, sp_quantize_blocks, nullptr)                                                          \
     X(matmul_abt_scaled, sp_gemm_abt_scaled, nullptr)                                                        \
-    X(penalize_logits, sp_logits_penalize, "sp_logits_penalize_workspace_bytes")
+    X(penalize_logits, sp_logits_penalize, "sp_logits_penalize_workspace_bytes")                              \
+    X(matmul_abt_gated, sp_gemm_abt_gated, nullptr)                                                          \
+    X(matmul_abt_gated_backward, sp_gemm_abt_gated_backward, "sp_gemm_abt_gated_backward_workspace_bytes")    \
+    X(token_log_probs, sp_token_log_probs, "sp_token_log_probs_workspace_bytes")                              \
+    X(token_log_probs_backward, sp_token_log_probs_backward, nullptr)
 
 // `as`: the name the function goes by; `other`: a second entry point for it, where the library has it.
 bool bind_one(void* library, PyObject* stream, PyObject* functions, const char* name, PyCFunction call, PyMethodDef& def, const char* as, const char* other) {

@@ -8,46 +8,9 @@
 //
 // x / scale costs three operations: q = x * (1 / scale) and one step q + (x - q * scale) * (1 / scale), whose remainder is exact (Markstein's
 // correction).  That is x / scale rounded to f32, but for ties of f32, before the 8-bit rounding.
-#include "vec_io.h"
+#include "f8_blocks.h"
 
 namespace sp {
-
-constexpr int QB = 128;                       // elements of a block
-constexpr float SCALE_LEAST = 0x1p-126f;      // the smallest normal f32: 1 / scale stays finite, and a block of zeros has a scale
-
-template <int F8>
-constexpr float F8_MOST = F8 == SP_F8_E4M3 ? 448.f : 57344.f;
-
-// Four numbers as four bytes.
-template <int F8>
-__device__ __forceinline__ unsigned pack_f8(float a, float b, float c, float d) {
-    int v = 0;
-    if constexpr (F8 == SP_F8_E4M3) {
-        v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, v, false);
-        v = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
-    } else {
-        v = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, v, false);
-        v = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, v, true);
-    }
-    return (unsigned)v;
-}
-
-// The first `left` of four bytes, and zeros: what lies behind a row is zeros whatever its block's scale is (0 / inf and 0 / NaN are NaNs).
-__device__ __forceinline__ unsigned first_bytes(unsigned v, long left) { return left >= 4 ? v : left <= 0 ? 0u : v & ((1u << (8 * (int)left)) - 1u); }
-
-struct BlockScale {
-    float scale, inv;
-    template <int F8>
-    __device__ __forceinline__ void set(unsigned magnitude) {
-        scale = __uint_as_float(magnitude) / F8_MOST<F8>;
-        scale = scale < SCALE_LEAST ? SCALE_LEAST : scale;               // (a NaN stays)
-        inv = 1.f / scale;
-    }
-    __device__ __forceinline__ float operator()(float x) const {
-        const float q = x * inv;
-        return __builtin_fmaf(__builtin_fmaf(-q, scale, x), inv, q);
-    }
-};
 
 struct QuantArgs {
     const void* x;
@@ -57,8 +20,6 @@ struct QuantArgs {
     long pitch, pitch_t;          // of q and q_t: cols and rows rounded up to a multiple of 16
     long blocks_c, blocks_r;      // blocks of 128 along cols and rows: the widths of scale and scale_t
 };
-
-__device__ __forceinline__ unsigned max_u32(unsigned a, unsigned b) { return a > b ? a : b; }
 
 // WIDE: blocks of 128 x 128.  OUT: 1 = q, 2 = q_t, 3 = both.  R: rows per lane, ROWS: of the tile, LANES: of 8 columns, its width.  POLICY: of the stores (a branch at each
 // store, the compiler folds both sides into a plain one).

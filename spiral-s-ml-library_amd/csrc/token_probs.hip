@@ -1,0 +1,544 @@
+// Log probabilities of one token per row of logits, the entropy of the row and its most likely tokens; and the gradient of the logits.
+//
+// With m the largest logit, s = sum exp(x - m) and w = sum exp(x - m) (x - m): lse = m + ln s, log p_t = (x_t - m) - ln s, and the entropy
+// -sum p ln p = ln s - w / s, two numbers that are not negative, so nothing cancels.  A row is read once: a lane keeps m, s and w of what it has seen
+// and scales s and w where m grows; lanes, waves and chunks of a row then join in an order of the sizes alone.
+// Backward: dx_j = d_logp [j = t] - p_j (d_logp + d_entropy (ln p_j + H) - d_lse), one read and one write.
+//
+// What rows may hold: -inf has probability 0 (its terms are left out); a row with nothing above -inf has lse -inf, log probability -inf and entropy 0, and
+// gradients of 0; the lowest finite number is a logit like any other (x - m is taken before it is scaled, so that it does not
+// overflow to a NaN); +inf or a NaN make the sums NaN.
+#include "vec_io.h"
+
+namespace sp {
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float FAR_BELOW = -1e4f;            // of y = (x - m) log2 e: 2^y is 0 there, and 0 * y stays 0 where y alone would be -inf
+constexpr int MOST_TOP = 32;                  // alternatives
+constexpr int MOST_CHUNKS = 64;               // of a row: one lane each where they join
+constexpr int LIST = 2048;                    // candidates for them that a workgroup can hold
+
+struct TokenArgs {
+    const int32_t* tokens;
+    float *logp, *entropy, *lse, *top_logp;
+    int32_t* top_ids;
+    int top;
+    float* part;                  // of every (row, chunk): m, s, w, and behind all of them `top` values each, and their columns
+    float* part_top;
+    int32_t* part_ids;
+};
+
+// The sums of some of a row's logits, of e = 2^y with y = (x - m) log2 e.
+struct Sums {
+    float m, s, w;                // w: of e y
+};
+__device__ __forceinline__ float finite_reference(float m) { return m == -INFINITY ? 0.f : m; }
+// What s and w are from another m, which is no smaller.
+__device__ __forceinline__ void move_to(Sums& a, float m) {
+    const float y = (a.m - finite_reference(m)) * LOG2E, f = __builtin_amdgcn_exp2f(y);
+    a.w = f * __builtin_fmaf(a.s, fmaxf(y, FAR_BELOW), a.w);
+    a.s *= f;
+    a.m = m;
+}
+__device__ __forceinline__ float add_f32(float a, float b) { return a + b; }
+template <int N, bool ENTROPY>
+__device__ __forceinline__ void take(Sums& a, const float (&x)[N]) {
+    float most = a.m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = fmaxf(most, x[i]);
+    move_to(a, most);
+    const float from = finite_reference(most);
+    float s = 0.f, w = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float y = (x[i] - from) * LOG2E, e = __builtin_amdgcn_exp2f(y);
+        s += e;
+        if constexpr (ENTROPY) w = __builtin_fmaf(e, fmaxf(y, FAR_BELOW), w);
+    }
+    a.s += s;
+    a.w += w;
+}
+
+// A row's results from its sums.
+struct RowResult {
+    bool none;
+    float m, ln_s;
+    __device__ __forceinline__ explicit RowResult(const Sums& a) : none(a.m == -INFINITY && a.s == 0.f), m(a.m), ln_s(logf(a.s)) {}
+    __device__ __forceinline__ float logp(float x) const { return none ? -INFINITY : (x - m) - ln_s; }
+};
+template <int DT>
+__device__ __forceinline__ float logit_at(const void* logits, long at) {
+    if constexpr (DT == SP_F32) return ((const float*)logits)[at];
+    else return half_bits_to_f32<DT>(((const unsigned short*)logits)[at]);
+}
+template <int DT>
+__device__ __forceinline__ void put_row(const TokenArgs& a, const void* logits, long cols, long row, const Sums& sums) {
+    const RowResult r(sums);
+    const int token = a.tokens[row];
+    const bool counts = (unsigned)token < (unsigned)cols;
+    a.logp[row] = counts ? r.logp(logit_at<DT>(logits, row * cols + token)) : 0.f;
+    if (a.lse != nullptr) a.lse[row] = r.none ? -INFINITY : r.m + r.ln_s;
+    if (a.entropy != nullptr) a.entropy[row] = r.none ? 0.f : r.ln_s - LN2 * (sums.w / sums.s);
+}
+
+// ---- the most likely tokens ----
+// A logit and its column as one number: larger for the larger logit, of equal ones for the lower column; 0 for what is never taken, -inf and NaN.
+typedef unsigned long long Key;
+__device__ __forceinline__ Key key_of(float x, int column) {
+    if (!(x > -INFINITY)) return 0;
+    const unsigned u = __float_as_uint(x + 0.f);                       // (-0 is +0)
+    return (Key)(u ^ ((u >> 31) != 0 ? 0xffffffffu : 0x80000000u)) << 32 | (unsigned)~column;
+}
+__device__ __forceinline__ float logit_of(Key k) {
+    const unsigned u = (unsigned)(k >> 32);
+    return __uint_as_float(u ^ ((u >> 31) != 0 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ int column_of(Key k) { return (int)~(unsigned)k; }
+__device__ __forceinline__ Key larger(Key a, Key b) { return a > b ? a : b; }
+
+struct TopLds {
+    Key list[LIST];
+    Key lanes[64];
+    Key least;
+    int count;
+};
+
+// The `top` largest keys of a workgroup's part of a row, in their order, to put(place, key); places behind the last one get key 0.  each(f): f of every
+// key of this lane; mine: the largest of them.
+// The 64 largest of lanes apart by 64 hold `top` keys (or all there are) that are no smaller than the top-th of them, so nothing below that one is taken: what is left, some two
+// dozen of a row for 20 alternatives, goes to a list, where every key counts the larger ones.  Where the list is too short (thousands of the largest logits in a few lanes) the
+// workgroup looks for one key after the other.
+template <int T, typename Each, typename Put>
+__device__ __forceinline__ void largest_keys(TopLds& lds, Key* keys, Key mine, int top, const Each& each, const Put& put) {
+    const int tid = threadIdx.x;
+    keys[tid] = mine;
+    if (tid == 0) {
+        lds.count = 0;
+        lds.least = 1;
+    }
+    __syncthreads();
+    Key best = 0;
+    if (tid < 64) {
+        for (int t = tid; t < T; t += 64) best = larger(best, keys[t]);
+        lds.lanes[tid] = best;
+    }
+    __syncthreads();
+    if (tid < 64 && best != 0) {
+        int above = 0;
+        for (int j = 0; j < 64; ++j) above += lds.lanes[j] > best ? 1 : 0;
+        if (above == top - 1) lds.least = best;
+    }
+    __syncthreads();
+    const Key least = lds.least;
+    if (mine >= least)
+        each([&](Key k) {
+            if (k < least) return;
+            const int at = atomicAdd(&lds.count, 1);
+            if (at < LIST) lds.list[at] = k;
+        });
+    __syncthreads();
+    const int n = lds.count;
+    if (n <= LIST) {
+        for (int i = tid; i < n; i += T) {
+            const Key k = lds.list[i];
+            int above = 0;
+            for (int j = 0; j < n; ++j) above += lds.list[j] > k ? 1 : 0;
+            if (above < top) put(above, k);
+        }
+        for (int i = n + tid; i < top; i += T) put(i, (Key)0);
+        return;
+    }
+    Key last = ~(Key)0;
+    for (int place = 0; place < top; ++place) {
+        best = 0;
+        each([&](Key k) {
+            if (k < last) best = larger(best, k);
+        });
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) best = larger(best, __shfl_xor(best, d, WAVE));
+        __syncthreads();                                   // (the last round's are read)
+        if ((tid & 63) == 0) keys[tid >> 6] = best;
+        __syncthreads();
+        best = keys[0];
+#pragma unroll
+        for (int w = 1; w < T / 64; ++w) best = larger(best, keys[w]);
+        if (tid == 0) put(place, best);
+        last = best;
+    }
+}
+
+// ---- long rows: a workgroup for a chunk of a row ----
+constexpr int AT_ONCE = 4;        // 16-byte pieces of a lane between two looks at m
+
+template <int DT, int T, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(T) void token_probs_kernel(const void* logits, long cols, unsigned chunks, long chunk_cols, const TokenArgs a) {
+    constexpr int P = PER16<DT>, STEP = T * P, N = AT_ONCE * P;
+    const int tid = threadIdx.x;
+    const long row = blockIdx.x / chunks;
+    const unsigned chunk = blockIdx.x - (unsigned)row * chunks;
+    const long c0 = (long)chunk * chunk_cols;
+    const int here = (int)(cols - c0 < chunk_cols ? cols - c0 : chunk_cols);
+    const long base = row * cols + c0;
+    auto load = [&](int i0, u32x4 (&raw)[AT_ONCE]) {
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int i = i0 + u * STEP + tid * P;
+            raw[u] = load16<DT>(logits, base + i, here - i);
+        }
+    };
+    auto values = [&](int i0, const u32x4 (&raw)[AT_ONCE], float (&x)[N]) {
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+            for (int e = 0; e < P; ++e) x[u * P + e] = element<DT>(raw[u], e);
+        if (i0 + AT_ONCE * STEP > here)                    // (of the whole workgroup)
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+                for (int e = 0; e < P; ++e)
+                    if (i0 + u * STEP + tid * P + e >= here) x[u * P + e] = -INFINITY;
+    };
+    Sums mine{-INFINITY, 0.f, 0.f};
+    int best_at = 0;                                       // where the step with this lane's largest logit begins
+    u32x4 ahead[AT_ONCE];
+    load(0, ahead);
+    for (int i0 = 0; i0 < here; i0 += AT_ONCE * STEP) {
+        u32x4 raw[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) raw[u] = ahead[u];
+        if (i0 + AT_ONCE * STEP < here) load(i0 + AT_ONCE * STEP, ahead);
+        float x[N];
+        values(i0, raw, x);
+        const float before = mine.m;
+        take<N, ENTROPY>(mine, x);
+        if constexpr (TOP)
+            if (mine.m > before) best_at = i0;
+    }
+    const float most_here = mine.m;
+    __shared__ Sums waves[T / 64];
+    __shared__ Sums all;
+    const float wave_most = group_max<64>(mine.m);
+    move_to(mine, wave_most);
+    mine.s = group_reduce<64>(mine.s, add_f32);
+    mine.w = group_reduce<64>(mine.w, add_f32);
+    if ((tid & 63) == 0) waves[tid >> 6] = mine;
+    __syncthreads();
+    if (tid == 0) {
+        float most = waves[0].m;
+#pragma unroll
+        for (int w = 1; w < T / 64; ++w) most = fmaxf(most, waves[w].m);
+        Sums sums{most, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) {
+            Sums one = waves[w];
+            move_to(one, most);
+            sums.s += one.s;
+            sums.w += one.w;
+        }
+        if (chunks == 1) {
+            put_row<DT>(a, logits, cols, row, sums);
+        } else {
+            a.part[3l * blockIdx.x] = sums.m;
+            a.part[3l * blockIdx.x + 1] = sums.s;
+            a.part[3l * blockIdx.x + 2] = sums.w;
+        }
+        all = sums;
+    }
+    if constexpr (TOP) {
+        __shared__ TopLds lds;
+        __shared__ Key keys[T];
+        auto keys_of_step = [&](int i0, const auto& f) {
+            u32x4 raw[AT_ONCE];
+            load(i0, raw);
+            float x[N];
+            values(i0, raw, x);
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+                for (int e = 0; e < P; ++e) f(key_of(x[u * P + e], (int)c0 + i0 + u * STEP + tid * P + e));
+        };
+        Key best = 0;
+        if (most_here > -INFINITY) keys_of_step(best_at, [&](Key k) { best = larger(best, k); });
+        const long to = (long)blockIdx.x * a.top;
+        __syncthreads();
+        const RowResult r(all);
+        largest_keys<T>(lds, keys, best, a.top,
+                        [&](const auto& f) {
+                            for (int i0 = 0; i0 < here; i0 += AT_ONCE * STEP) keys_of_step(i0, f);
+                        },
+                        [&](int place, Key k) {
+                            if (chunks == 1) {
+                                a.top_logp[to + place] = k != 0 ? r.logp(logit_of(k)) : -INFINITY;
+                                a.top_ids[to + place] = k != 0 ? column_of(k) : -1;
+                            } else {
+                                a.part_top[to + place] = k != 0 ? logit_of(k) : -INFINITY;
+                                a.part_ids[to + place] = k != 0 ? column_of(k) : -1;
+                            }
+                        });
+    }
+}
+
+// A row's chunks, a lane each, a wave per row.
+template <int DT>
+__global__ __launch_bounds__(256) void token_probs_join_kernel(const void* logits, long cols, long rows, int chunks, const TokenArgs a) {
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    const long mine_at = row * chunks + lane;
+    Sums sums{-INFINITY, 0.f, 0.f};
+    if (lane < chunks) sums = Sums{a.part[3 * mine_at], a.part[3 * mine_at + 1], a.part[3 * mine_at + 2]};
+    move_to(sums, group_max<64>(sums.m));
+    sums.s = group_reduce<64>(sums.s, add_f32);
+    sums.w = group_reduce<64>(sums.w, add_f32);
+    if (lane == 0) put_row<DT>(a, logits, cols, row, sums);
+    if (a.top == 0) return;
+    // the chunks' alternatives stand in their order: the largest of all is the first of some chunk, whose next one then takes its place
+    const RowResult r(sums);
+    int next = 0;
+    auto first = [&]() {
+        if (lane >= chunks || next >= a.top) return (Key)0;
+        return key_of(a.part_top[mine_at * a.top + next], a.part_ids[mine_at * a.top + next]);
+    };
+    Key head = first();
+    for (int place = 0; place < a.top; ++place) {
+        Key best = head;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) best = larger(best, __shfl_xor(best, d, WAVE));
+        if (lane == 0) {
+            a.top_logp[row * a.top + place] = best != 0 ? r.logp(logit_of(best)) : -INFINITY;
+            a.top_ids[row * a.top + place] = best != 0 ? column_of(best) : -1;
+        }
+        if (head == best && best != 0) {                   // (columns differ: one lane)
+            ++next;
+            head = first();
+        }
+    }
+}
+
+// ---- short rows: T lanes hold one in C pieces each ----
+template <int DT, int T, int C, bool ENTROPY>
+__global__ __launch_bounds__(256) void token_probs_rows_kernel(const void* logits, long cols, long rows, const TokenArgs a) {
+    constexpr int P = PER16<DT>, N = C * P;
+    const int lane = threadIdx.x % T;
+    const long row = (long)blockIdx.x * (256 / T) + threadIdx.x / T;
+    if (row >= rows) return;                               // (all lanes of a row)
+    float x[N];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int i = (c * T + lane) * P;
+        const u32x4 raw = load16<DT>(logits, row * cols + i, cols - i);
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[c * P + e] = i + e < cols ? element<DT>(raw, e) : -INFINITY;
+    }
+    float most = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
+    most = group_max<T>(fmaxf(most, -INFINITY));           // (a NaN alone in its lane is not handed on)
+    Sums sums{most, 0.f, 0.f};
+    take<N, ENTROPY>(sums, x);
+    sums.s = group_reduce<T>(sums.s, add_f32);
+    if constexpr (ENTROPY) sums.w = group_reduce<T>(sums.w, add_f32);
+    if (lane == 0) put_row<DT>(a, logits, cols, row, sums);
+}
+
+// ---- the gradient ----
+struct TokenGradArgs {
+    const int32_t* tokens;
+    const float *lse, *entropy, *d_logp, *d_entropy, *d_lse;
+    void* dx;
+};
+
+// T lanes to a row or a chunk of one, U pieces each.
+template <int DT, int T, int U, bool ENTROPY, int POLICY>
+__global__ __launch_bounds__(256) void token_grad_kernel(const void* logits, long cols, long rows, unsigned chunks, const TokenGradArgs a) {
+    constexpr int P = PER16<DT>;
+    const int lane = threadIdx.x % T;
+    const long part = (long)blockIdx.x * (256 / T) + threadIdx.x / T;
+    const long row = part / chunks;
+    if (row >= rows) return;
+    const long c0 = (part - row * chunks) * (T * U * P);
+    u32x4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long i = c0 + (u * T + lane) * P;
+        raw[u] = load16<DT>(logits, row * cols + i, cols - i);
+    }
+    const float lse = a.lse[row];
+    const int token = a.tokens[row];
+    const bool counts = (unsigned)token < (unsigned)cols, none = lse == -INFINITY;
+    const float of_token = a.d_logp != nullptr && counts && !none ? a.d_logp[row] : 0.f;
+    float slope = 0.f, all = of_token;                     // dx = [j = t] of_token - p (all + slope ln p)
+    if (a.d_lse != nullptr) all -= a.d_lse[row];
+    if constexpr (ENTROPY) {
+        slope = a.d_entropy[row];
+        all = __builtin_fmaf(slope, a.entropy[row], all);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long i = c0 + (u * T + lane) * P;
+        if (i >= cols) break;
+        float d[P];
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            const float ln_p = element<DT>(raw[u], e) - lse, p = none ? 0.f : __builtin_amdgcn_exp2f(ln_p * LOG2E);
+            const float f = ENTROPY ? __builtin_fmaf(slope, fmaxf(ln_p, FAR_BELOW), all) : all;
+            d[e] = __builtin_fmaf(-p, f, i + e == token ? of_token : 0.f);
+        }
+        store16<DT, POLICY>(a.dx, row * cols + i, cols - i, d);
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------
+
+static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int TOKEN_THREADS = 512;
+constexpr int64_t LEAST_CHUNK = 4096;
+constexpr int GRAD_PIECES = 4;                // 16-byte pieces of a lane, long rows
+
+// Chunks of a row: as many as it takes to give every compute unit two workgroups.
+static int64_t token_chunks(int64_t rows, int64_t cols) {
+    const int64_t wanted = ceil_div(2 * device_cu_count(), rows), possible = ceil_div(cols, LEAST_CHUNK);
+    const int64_t n = wanted < possible ? wanted : possible;
+    return n < MOST_CHUNKS ? n : MOST_CHUNKS;
+}
+static bool short_rows(int dtype, int64_t cols, int32_t top) { return top == 0 && cols <= 64 * 4 * (dtype == SP_F32 ? 4 : 8); }
+
+template <int DT, bool ENTROPY>
+static int launch_rows(const void* logits, long cols, long rows, const TokenArgs& a, hipStream_t stream) {
+    constexpr int P = PER16<DT>;
+    auto launch = [&](auto t, auto c) {
+        constexpr int T = decltype(t)::value, C = decltype(c)::value;
+        hipLaunchKernelGGL((token_probs_rows_kernel<DT, T, C, ENTROPY>), dim3((unsigned)ceil_div(rows, 256 / T)), dim3(256), 0, stream, logits, cols, rows, a);
+        return check_launch("sp_token_log_probs");
+    };
+    typedef std::integral_constant<int, 1> one;
+    if (cols <= 16 * P) return launch(std::integral_constant<int, 16>{}, one{});
+    if (cols <= 64 * P) return launch(std::integral_constant<int, 64>{}, one{});
+    if (cols <= 128 * P) return launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    return launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+}
+
+template <int DT, bool ENTROPY, bool TOP>
+static int launch_long(const void* logits, long cols, long rows, const TokenArgs& a, hipStream_t stream) {
+    const long chunks = token_chunks(rows, cols), piece = PER16<DT>;
+    const long chunk_cols = ceil_div(ceil_div(cols, chunks), piece) * piece;
+    hipLaunchKernelGGL((token_probs_kernel<DT, TOKEN_THREADS, ENTROPY, TOP>), dim3((unsigned)(rows * chunks)), dim3(TOKEN_THREADS), 0, stream, logits, cols, (unsigned)chunks,
+                       chunk_cols, a);
+    if (const int rc = check_launch("sp_token_log_probs"); rc != SP_OK || chunks == 1) return rc;
+    hipLaunchKernelGGL(token_probs_join_kernel<DT>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream, logits, cols, rows, (int)chunks, a);
+    return check_launch("sp_token_log_probs");
+}
+
+template <int DT, bool ENTROPY>
+static int launch_grad(const void* logits, long cols, long rows, const TokenGradArgs& a, hipStream_t stream) {
+    constexpr int P = PER16<DT>;
+    auto launch = [&](auto t, auto u) {
+        constexpr int T = decltype(t)::value, U = decltype(u)::value;
+        const long chunks = ceil_div(cols, T * U * P), blocks = ceil_div(rows * chunks, 256 / T);
+        // a gradient that does not stay in the caches (32 MiB of L2) is streamed past them
+        if (rows * cols * ELEM_BYTES<DT> > 32l << 20)
+            hipLaunchKernelGGL((token_grad_kernel<DT, T, U, ENTROPY, ST_STREAM>), dim3((unsigned)blocks), dim3(256), 0, stream, logits, cols, rows, (unsigned)chunks, a);
+        else
+            hipLaunchKernelGGL((token_grad_kernel<DT, T, U, ENTROPY, ST_PLAIN>), dim3((unsigned)blocks), dim3(256), 0, stream, logits, cols, rows, (unsigned)chunks, a);
+        return check_launch("sp_token_log_probs_backward");
+    };
+    typedef std::integral_constant<int, 1> one;
+    if (cols <= 16 * P) return launch(std::integral_constant<int, 16>{}, one{});
+    if (cols <= 64 * P) return launch(std::integral_constant<int, 64>{}, one{});
+    return launch(std::integral_constant<int, 256>{}, std::integral_constant<int, GRAD_PIECES>{});
+}
+
+namespace {
+struct TokenKernelNames {
+    TokenKernelNames() {
+        register_kernel("token_probs", (const void*)token_probs_kernel<SP_BF16, TOKEN_THREADS, true, false>, TOKEN_THREADS);
+        register_kernel("token_probs_top", (const void*)token_probs_kernel<SP_BF16, TOKEN_THREADS, true, true>, TOKEN_THREADS);
+        register_kernel("token_grad", (const void*)token_grad_kernel<SP_BF16, 256, 4, true, ST_STREAM>, 256);
+    }
+} token_kernel_names;
+}  // namespace
+
+}  // namespace sp
+
+using namespace sp;
+
+static int token_sizes(const char* fn, int dtype, int64_t rows, int64_t cols) {
+    if (dtype != SP_F32 && dtype != SP_F16 && dtype != SP_BF16) return fail(SP_ERR_DTYPE, "%s: dtype must be f32, f16 or bf16, got %d", fn, dtype);
+    if (rows <= 0 || cols <= 0) return fail(SP_ERR_SHAPE, "%s: rows and cols must be positive (got %lld, %lld)", fn, (long long)rows, (long long)cols);
+    if (rows > INT32_MAX || cols > (int64_t)1 << 30) return fail(SP_ERR_SHAPE, "%s: too large", fn);     // (columns are counted in 32 bits)
+    return SP_OK;
+}
+
+extern "C" int64_t sp_token_log_probs_workspace_bytes(int64_t rows, int64_t cols, int32_t top) {
+    if (rows <= 0 || cols <= 0 || top < 0 || top > MOST_TOP) return 0;
+    const int64_t chunks = token_chunks(rows, cols);
+    return chunks > 1 ? rows * chunks * 4 * (3 + 2 * top) : 0;
+}
+
+extern "C" int sp_token_log_probs(int dtype, const void* logits, const int32_t* tokens, float* logp, float* entropy, float* lse, int32_t top, float* top_logp, int32_t* top_ids,
+                                  int64_t rows, int64_t cols, void* workspace, int64_t workspace_bytes, void* stream) {
+    SP_REQUIRE_PTR(logits);
+    SP_REQUIRE_PTR(tokens);
+    SP_REQUIRE_PTR(logp);
+    SP_OPTIONAL_PTR(entropy);
+    SP_OPTIONAL_PTR(lse);
+    SP_OPTIONAL_PTR(top_logp);
+    SP_OPTIONAL_PTR(top_ids);
+    if (const int rc = token_sizes(__func__, dtype, rows, cols); rc != SP_OK) return rc;
+    if (top < 0 || top > MOST_TOP) return fail(SP_ERR_ARG, "sp_token_log_probs: top must be in [0, 32], got %d", top);
+    if (top > 0 && (top_logp == nullptr || top_ids == nullptr)) return fail(SP_ERR_NULL, "sp_token_log_probs: top_logp and top_ids are needed for %d alternatives", top);
+    const bool in_registers = short_rows(dtype, cols, top);
+    // a launch holds fewer than 2^32 work items (chunks of a row: only where there are few rows)
+    if (rows >= ((int64_t)1 << 32) / (in_registers ? 64 : TOKEN_THREADS)) return fail(SP_ERR_SHAPE, "sp_token_log_probs: too large");
+    const int64_t need = sp_token_log_probs_workspace_bytes(rows, cols, top);
+    if (need > 0) {
+        SP_REQUIRE_PTR(workspace);
+        if (workspace_bytes < need) return fail(SP_ERR_ARG, "sp_token_log_probs: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+    }
+    if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
+    TokenArgs a{};
+    a.tokens = tokens; a.logp = logp; a.entropy = entropy; a.lse = lse; a.top = top; a.top_logp = top_logp; a.top_ids = top_ids;
+    if (need > 0) {
+        const int64_t parts = rows * token_chunks(rows, cols);
+        a.part = (float*)workspace; a.part_top = a.part + 3 * parts; a.part_ids = (int32_t*)(a.part_top + parts * top);
+    }
+    const hipStream_t st = (hipStream_t)stream;
+    auto by_entropy = [&](auto dt, auto with) {
+        constexpr int DT = decltype(dt)::value;
+        constexpr bool ENTROPY = decltype(with)::value;
+        if (in_registers) return launch_rows<DT, ENTROPY>(logits, cols, rows, a, st);
+        return top > 0 ? launch_long<DT, ENTROPY, true>(logits, cols, rows, a, st) : launch_long<DT, ENTROPY, false>(logits, cols, rows, a, st);
+    };
+    auto by_type = [&](auto dt) { return entropy != nullptr ? by_entropy(dt, std::true_type{}) : by_entropy(dt, std::false_type{}); };
+    if (dtype == SP_F32) return by_type(std::integral_constant<int, SP_F32>{});
+    if (dtype == SP_F16) return by_type(std::integral_constant<int, SP_F16>{});
+    return by_type(std::integral_constant<int, SP_BF16>{});
+}
+
+extern "C" int sp_token_log_probs_backward(int dtype, const void* logits, const int32_t* tokens, const float* lse, const float* entropy, const float* d_logp,
+                                           const float* d_entropy, const float* d_lse, void* d_logits, int64_t rows, int64_t cols, void* stream) {
+    SP_REQUIRE_PTR(logits);
+    SP_REQUIRE_PTR(tokens);
+    SP_REQUIRE_PTR(lse);
+    SP_REQUIRE_PTR(d_logits);
+    SP_OPTIONAL_PTR(entropy);
+    SP_OPTIONAL_PTR(d_logp);
+    SP_OPTIONAL_PTR(d_entropy);
+    SP_OPTIONAL_PTR(d_lse);
+    if (const int rc = token_sizes(__func__, dtype, rows, cols); rc != SP_OK) return rc;
+    if (d_entropy != nullptr && entropy == nullptr) return fail(SP_ERR_NULL, "sp_token_log_probs_backward: d_entropy needs the entropy");
+    const int64_t p = dtype == SP_F32 ? 4 : 8, lanes = cols <= 16 * p ? 16 : cols <= 64 * p ? 64 : 256 * ceil_div(cols, GRAD_PIECES * 256 * p);
+    if (rows * lanes > ((int64_t)1 << 32) - 256) return fail(SP_ERR_SHAPE, "sp_token_log_probs_backward: too large");      // (work items of a launch)
+    if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
+    TokenGradArgs a{};
+    a.tokens = tokens; a.lse = lse; a.entropy = entropy; a.d_logp = d_logp; a.d_entropy = d_entropy; a.d_lse = d_lse; a.dx = d_logits;
+    const hipStream_t st = (hipStream_t)stream;
+    auto by_type = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        return d_entropy != nullptr ? launch_grad<DT, true>(logits, cols, rows, a, st) : launch_grad<DT, false>(logits, cols, rows, a, st);
+    };
+    if (dtype == SP_F32) return by_type(std::integral_constant<int, SP_F32>{});
+    if (dtype == SP_F16) return by_type(std::integral_constant<int, SP_F16>{});
+    return by_type(std::integral_constant<int, SP_BF16>{});
+}

@@ -22,6 +22,7 @@ REDUCE_SUM, REDUCE_PROD, REDUCE_MAX, REDUCE_MIN, REDUCE_AVERAGE = 0, 1, 2, 3, 4
 MAP_IN_IDENTITY, MAP_IN_SQUARE, MAP_IN_ABS = 0, 1, 2
 MAP_OUT_IDENTITY, MAP_OUT_SQRT = 0, 1
 STACK_LN_L2 = 0x100
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
 HEAD_NONE, HEAD_SOFTMAX, HEAD_REGRET_MATCHING, HEAD_SOFTMAX_RM = 0, 1, 2, 3
 
 ERR_SHAPE, ERR_UNSUPPORTED = -2, -6
@@ -105,6 +106,12 @@ SIGNATURES = {
     "sp_logits_penalize_workspace_bytes": (C.c_int64, [_I64, _I64]),
     "sp_quantize_blocks": (C.c_int, [C.c_int, C.c_int, _I32] + [_P] * 5 + [_I64, _I64, _P]),
     "sp_gemm_abt_scaled": (C.c_int, [C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _F, _U32, _P]),
+    "sp_gemm_abt_gated": (C.c_int, [C.c_int, C.c_int] + [_P] * 4 + [C.c_int] + [_P] * 4 + [_I64, _I64, _I64, _P]),
+    "sp_gemm_abt_gated_backward": (C.c_int, [C.c_int, C.c_int] + [_P] * 4 + [C.c_int] + [_P] * 7 + [_I64, _I64, _I64, _P, _I64, _P]),
+    "sp_gemm_abt_gated_backward_workspace_bytes": (C.c_int64, [C.c_int, _I64, _I64]),
+    "sp_token_log_probs": (C.c_int, [C.c_int] + [_P] * 5 + [_I32, _P, _P, _I64, _I64, _P, _I64, _P]),
+    "sp_token_log_probs_backward": (C.c_int, [C.c_int] + [_P] * 8 + [_I64, _I64, _P]),
+    "sp_token_log_probs_workspace_bytes": (C.c_int64, [_I64, _I64, _I32]),
     "sp_ensemble_binarize": (C.c_int, [C.c_int, _P, _P, _P, _I32, _I64, _I32, _I32, _U32, _P]),
 }
 

@@ -193,6 +193,92 @@ def matmul_abt_scaled(a, scale_a, b, scale_b, c=None, beta=0.0, bias=None, relu=
     return c
 
 
+def _gated_operands(a, b_gate, b_up, activation):
+    """(M, N, K) of a gated block's operands, which have one type."""
+    if a.dim() != 2 or b_gate.dim() != 2 or b_up.dim() != 2:
+        raise ValueError("a, b_gate and b_up must be 2-D")
+    if a.dtype not in _lib.DTYPES or b_gate.dtype != a.dtype or b_up.dtype != a.dtype:
+        raise TypeError("a, b_gate and b_up must share one of the dtypes f32/f16/bf16, got %s, %s and %s" % (a.dtype, b_gate.dtype, b_up.dtype))
+    if b_gate.shape != b_up.shape:
+        raise ValueError("b_gate and b_up must have one shape, got %s and %s" % (tuple(b_gate.shape), tuple(b_up.shape)))
+    assert a.shape[1] == b_gate.shape[1], "The K dimension of the A and B tensors must match."
+    if not isinstance(activation, str) or activation not in _lib.ACTIVATIONS:
+        raise ValueError("activation must be \"silu\", \"gelu\" or \"relu\", got %r" % (activation,))
+    return a.shape[0], b_gate.shape[0], a.shape[1]
+
+
+def matmul_abt_gated(a, b_gate, b_up, activation="silu", keep=None):
+    """The gated feed-forward block C = act(A . B_gate^T) * (A . B_up^T) in one launch (sp_gemm_abt_gated), next to `matmul_abt` with its ReLU.  a (M, K), b_gate and
+    b_up (N, K): f32, f16 or bf16, the type of C (M, N); sums, activation ("silu", "gelu", the one with erf, or "relu") and product are f32.
+
+    keep: what `matmul_abt_gated_backward` is to find of the two products, (c, kept) then.  keep=a.dtype: kept is (gate, up), (M, N) each; keep=torch.float8_e4m3fn, a quarter to half of
+    that: (gate, gate_scale, up, up_scale), in the (1, 128) blocks of `quantize_blocks`."""
+    done = lib.whole_matmul_abt_gated(a, b_gate, b_up, _lib.ACTIVATIONS.get(activation) if isinstance(activation, str) else None, keep)
+    if done is not None:
+        return done
+    m, n, k = _gated_operands(a, b_gate, b_up, activation)
+    f8 = keep == torch.float8_e4m3fn
+    if keep is not None and keep != a.dtype and not f8:
+        raise TypeError("keep must be None, %s or torch.float8_e4m3fn, got %s" % (a.dtype, keep))
+    addresses = ptr(a, name="a"), ptr(b_gate, name="b_gate"), ptr(b_up, name="b_up")
+    if _on_device_of("matmul_abt_gated", a, b_gate, b_up) != torch.cuda.current_device():
+        with torch.cuda.device(a.device):
+            return matmul_abt_gated(a, b_gate, b_up, activation, keep)
+    new = lambda r, c, dtype: torch.empty((r, c), dtype=dtype, device=a.device)
+    c = new(m, n, a.dtype)
+    gate = gate_scale = up = up_scale = None
+    kept = ()
+    if f8:
+        gate, up = (new(m, (n + 15) // 16 * 16, keep) for _ in range(2))
+        gate_scale, up_scale = (new(m, _blocks(n), torch.float32) for _ in range(2))
+        kept = gate, gate_scale, up, up_scale
+    elif keep is not None:
+        kept = gate, up = new(m, n, keep), new(m, n, keep)
+    check(lib.sp_gemm_abt_gated(_lib.DTYPES[a.dtype], _lib.ACTIVATIONS[activation], *addresses, ptr(c), _lib.SP_F8_E4M3 if f8 else _lib.DTYPES[a.dtype], ptr(gate),
+                                ptr(gate_scale), ptr(up), ptr(up_scale), m, n, k, stream_ptr()))
+    return c if keep is None else (c, kept)
+
+
+def matmul_abt_gated_backward(dc, a, b_gate, b_up, kept, activation="silu", want_input_grad=True, want_weight_grads=True):
+    """The gradients of `matmul_abt_gated` (sp_gemm_abt_gated_backward): (da, db_gate, db_up), of the type of a, from dc (M, N), the operands and what the forward call kept.  They
+    are those at the numbers that were kept.  da is None with want_input_grad=False, db_gate and db_up with want_weight_grads=False."""
+    if want_input_grad is True and want_weight_grads is True and type(kept) is tuple and len(kept) in (2, 4):
+        done = lib.whole_matmul_abt_gated_backward(dc, a, b_gate, b_up, kept[0], kept[1] if len(kept) == 4 else None, kept[-2] if len(kept) == 4 else kept[1],
+                                                   kept[3] if len(kept) == 4 else None, _lib.ACTIVATIONS.get(activation) if isinstance(activation, str) else None)
+        if done is not None:
+            return done
+    m, n, k = _gated_operands(a, b_gate, b_up, activation)
+    if dc.shape != (m, n) or dc.dtype != a.dtype:
+        raise ValueError("dc must be (M, N) = (%d, %d) of %s, got %s of %s" % (m, n, a.dtype, tuple(dc.shape), dc.dtype))
+    if not isinstance(kept, (tuple, list)) or len(kept) not in (2, 4):
+        raise ValueError("kept must be what matmul_abt_gated returned beside its result: (gate, up) or (gate, gate_scale, up, up_scale)")
+    gate, gate_scale, up, up_scale = kept if len(kept) == 4 else (kept[0], None, kept[1], None)
+    f8 = len(kept) == 4
+    shape, dtype = ((m, (n + 15) // 16 * 16), torch.float8_e4m3fn) if f8 else ((m, n), a.dtype)
+    for t, name in ((gate, "gate"), (up, "up")):
+        if tuple(t.shape) != shape or t.dtype != dtype:
+            raise ValueError("the kept %s must be %s of %s, got %s of %s" % (name, shape, dtype, tuple(t.shape), t.dtype))
+    if f8:
+        for t, name in ((gate_scale, "gate_scale"), (up_scale, "up_scale")):
+            if tuple(t.shape) != (m, _blocks(n)):
+                raise ValueError("the kept %s must be %s, got %s" % (name, (m, _blocks(n)), tuple(t.shape)))
+    if not want_input_grad and not want_weight_grads:
+        raise ValueError("no gradient is wanted")
+    f32 = torch.float32
+    addresses = ptr(dc, name="dc"), ptr(a, name="a"), ptr(b_gate, name="b_gate"), ptr(b_up, name="b_up")
+    kept_at = ptr(gate, name="gate"), ptr(gate_scale, f32, "gate_scale"), ptr(up, name="up"), ptr(up_scale, f32, "up_scale")
+    if _on_device_of("matmul_abt_gated_backward", dc, a, b_gate, b_up, gate, gate_scale, up, up_scale) != torch.cuda.current_device():
+        with torch.cuda.device(a.device):
+            return matmul_abt_gated_backward(dc, a, b_gate, b_up, kept, activation, want_input_grad, want_weight_grads)
+    da = torch.empty_like(a) if want_input_grad else None
+    db_gate, db_up = (torch.empty_like(b_gate) if want_weight_grads else None for _ in range(2))
+    bytes_ = lib.sp_gemm_abt_gated_backward_workspace_bytes(_lib.DTYPES[a.dtype], m, n)
+    workspace = torch.empty((bytes_,), dtype=torch.uint8, device=a.device)                  # of this call alone: calls may overlap
+    check(lib.sp_gemm_abt_gated_backward(_lib.DTYPES[a.dtype], _lib.ACTIVATIONS[activation], *addresses, _lib.SP_F8_E4M3 if f8 else _lib.DTYPES[a.dtype], *kept_at,
+                                         ptr(da), ptr(db_gate), ptr(db_up), m, n, k, ptr(workspace), bytes_, stream_ptr()))
+    return da, db_gate, db_up
+
+
 def _transposed(x):
     """Materialise x^T with the library's transpose kernel (4-byte elements only)."""
     if x.dtype != torch.float32:

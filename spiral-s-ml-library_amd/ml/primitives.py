@@ -392,6 +392,80 @@ def penalize_logits(logits, tokens=None, lengths=None, prompt_lengths=None, repe
     return (out, token) if want_token else out
 
 
+def _token_rows(what, logits, tokens):
+    if logits.dtype not in _lib.DTYPES:
+        raise TypeError("%s takes f32, f16 or bf16 logits, got %s" % (what, logits.dtype))
+    if logits.dim() < 2 or logits.numel() == 0:
+        raise ValueError("logits must have at least 2 dimensions and one entry, got %s" % (tuple(logits.shape),))
+    if tokens.shape != logits.shape[:-1]:
+        raise ValueError("tokens must have one entry per row")
+    return _rows_cols(logits)
+
+
+def token_log_probs(logits, tokens, top=0, want_entropy=False, want_lse=False):
+    """Log probabilities of one token per row of logits (..., cols) of any length (sp_token_log_probs), next to `get_prob` and `softmax`, which take short rows:
+    logits[token] - lse with lse = ln sum exp logits, (...,) f32.  logits: f32, f16 or bf16; tokens: (...,) i32, where a token outside the row (pad with -1) has 0.
+
+    want_entropy=True also returns each row's entropy, -sum p ln p, want_lse=True its lse, which `token_log_probs_backward` takes; top=k <= 32 the log probabilities and the
+    i32 indices of the k largest logits, (..., k) each, largest first and of equal ones the lowest index, -inf and -1 where a row has fewer above -inf.  In this
+    order: (log_probs, entropy, lse, top_log_probs, top_ids), without what is not wanted; the log probabilities alone are no tuple.
+    A logit of -inf has probability 0; a row of nothing else has log probability -inf and entropy 0."""
+    done = lib.whole_token_log_probs(logits, tokens, top, want_entropy, want_lse)
+    if done is not None:
+        return done
+    rows, cols = _token_rows("token_log_probs", logits, tokens)
+    if not 0 <= top <= 32:
+        raise ValueError("top must be in [0, 32], got %r" % (top,))
+    logits_at, tokens_at = ptr(logits, name="logits"), ptr(tokens, torch.int32, "tokens")
+    if _one_device("token_log_probs", logits, tokens) != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return token_log_probs(logits, tokens, top, want_entropy, want_lse)
+    lead = logits.shape[:-1]
+    new = lambda shape, dtype: torch.empty(shape, dtype=dtype, device=logits.device)
+    logp = new(lead, torch.float32)
+    entropy = new(lead, torch.float32) if want_entropy else None
+    lse = new(lead, torch.float32) if want_lse else None
+    top_logp = top_ids = workspace = None
+    if top:
+        top_logp, top_ids = new((*lead, top), torch.float32), new((*lead, top), torch.int32)
+    bytes_ = lib.sp_token_log_probs_workspace_bytes(rows, cols, top)
+    if bytes_:
+        workspace = new((bytes_,), torch.uint8)                           # of this call alone: calls may overlap
+    check(lib.sp_token_log_probs(_lib.DTYPES[logits.dtype], logits_at, tokens_at, ptr(logp), ptr(entropy), ptr(lse), top, ptr(top_logp), ptr(top_ids), rows, cols,
+                                 ptr(workspace), bytes_, stream_ptr()))
+    out = tuple(t for t in (logp, entropy, lse, top_logp, top_ids) if t is not None)
+    return out[0] if len(out) == 1 else out
+
+
+def token_log_probs_backward(d_log_probs, logits, tokens, lse, d_entropy=None, entropy=None, d_lse=None, out=None):
+    """The gradient of the logits of `token_log_probs` (sp_token_log_probs_backward), of their type, from those of its log probabilities, entropies (with the entropies
+    themselves) and lse, (...,) f32 each, any of them None; lse as the forward call returned it.  `out` may be the logits.  Rows whose token does not count have no gradient from
+    d_log_probs; the alternatives of `top` hand on none."""
+    if out is None:
+        done = lib.whole_token_log_probs_backward(d_log_probs, logits, tokens, lse, d_entropy, entropy, d_lse)
+        if done is not None:
+            return done
+    rows, cols = _token_rows("token_log_probs_backward", logits, tokens)
+    for t, name in ((lse, "lse"), (d_log_probs, "d_log_probs"), (d_entropy, "d_entropy"), (entropy, "entropy"), (d_lse, "d_lse")):
+        if t is not None and t.shape != logits.shape[:-1]:
+            raise ValueError("%s must have one entry per row" % name)
+    if lse is None:
+        raise ValueError("lse is needed: token_log_probs(..., want_lse=True)")
+    if d_entropy is not None and entropy is None:
+        raise ValueError("d_entropy needs the entropy")
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype):
+        raise ValueError("out must have the shape and type of the logits")
+    f32 = torch.float32
+    addresses = (ptr(logits, name="logits"), ptr(tokens, torch.int32, "tokens"), ptr(lse, f32, "lse"), ptr(entropy, f32, "entropy"), ptr(d_log_probs, f32, "d_log_probs"),
+                 ptr(d_entropy, f32, "d_entropy"), ptr(d_lse, f32, "d_lse"))
+    if _one_device("token_log_probs_backward", logits, tokens, lse, entropy, d_log_probs, d_entropy, d_lse, out) != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return token_log_probs_backward(d_log_probs, logits, tokens, lse, d_entropy, entropy, d_lse, out)
+    dx = torch.empty_like(logits) if out is None else out
+    check(lib.sp_token_log_probs_backward(_lib.DTYPES[logits.dtype], *addresses, ptr(dx, name="out"), rows, cols, stream_ptr()))
+    return dx
+
+
 def cem_update_rewards_mask(rewards, mask=None):
     """`grid_update_rewards_mask` (ml/cem.spi:92-96): rewards (ensemble, 2) f32 (reward sum, count) pairs are
     turned into the winners' mask (average reward at or above the ensemble's mean) and zeroed."""
