@@ -194,13 +194,13 @@ int sp_gemm_abt_gated(int dtype, int activation, const void* A, const void* B_ga
  * Its gradients from dC (M, N), at the g and u that were kept:  dg = dC u act'(g), du = dC act(g), rounded to dtype, and
  *   dA = dg . B_gate + du . B_up (M, K),   dB_gate = dg^T . A, dB_up = du^T . A (N, K)
  * in dtype, of f32 sums.  dA may be NULL, and dB_gate with dB_up.  The ReLU's slope at 0 is 0.  Every sum has one order: results repeat bit for bit.
- * `workspace`: sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N) bytes of device memory that hold dg and du during the call (what they held before does not matter).  Calls
+ * `workspace`: sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K) bytes of device memory that hold dg, du and partial sums during the call (what they held before does not matter).  Calls
  * that may run at the same time need one each.
  */
 int sp_gemm_abt_gated_backward(int dtype, int activation, const void* dC, const void* A, const void* B_gate, const void* B_up, int kept_dtype,
                                const void* gate, const float* gate_scale, const void* up, const float* up_scale, void* dA, void* dB_gate,
                                void* dB_up, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
-int64_t sp_gemm_abt_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t N);
+int64_t sp_gemm_abt_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 
 /* ------------------------------------------------------------------------------------------ */
 /* Row primitives                                                                              */

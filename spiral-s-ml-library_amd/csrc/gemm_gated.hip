@@ -8,7 +8,7 @@
 // G, U, A and the workspace are then read across their rows: tiles of K rows go to LDS as they lie in memory, and a fragment is read transposed
 // (ds_read_b64_tr_b16: 16 lanes take 4 x 16 numbers, each lane a column's four; f32: four reads of 4 bytes).
 //
-// All products: tiles of LDS in two stages that DMA fills, 128 bytes of K (of a row, or of K rows) a stage.  A wave walks its TM rows of fragments; the fragment of a
+// All products: tiles of LDS in a ring of stages that DMA fills, 128 bytes of K (of a row, or of K rows) a stage.  A wave walks its TM rows of fragments; the fragment of a
 // row is replaced by the next half stage's once its MFMAs are issued, the B fragments have two sets.  The boundary between two stages stands in the middle: everything
 // of a stage is in registers then, and the next one has landed.
 // K may end anywhere: what is missing of the last K-tile comes from zeros, and that tile goes first, so that the loop has whole ones only.
@@ -18,6 +18,7 @@ namespace sp {
 
 enum { MM_FORWARD, MM_INPUT, MM_WEIGHTS };
 enum { KEEP_NONE, KEEP_WHOLE, KEEP_F8 };
+constexpr unsigned ROTATE = 7;      // odd: it meets every one of a power of two of K-tiles
 
 struct GatedArgs {
     // forward: A, G, U; gradient of A: workspace, G, U; of the weights: workspace, A
@@ -30,6 +31,7 @@ struct GatedArgs {
     int activation, keep;
     int tiles_m, tiles_n, group_m;
     int stream;                   // C does not stay in the caches
+    float* parts;                 // backward: partial sums of several workgroups, all of a result (of both weights' gradients) each
 };
 
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f)); }
@@ -86,6 +88,7 @@ __device__ __forceinline__ void gated_tile_of_block(int pid, int tiles_m, int ti
 __device__ __forceinline__ int along_slot(int row, int kc) { return (kc ^ row ^ (row >> 3 & 1)) & 7; }
 template <int ES, int W>
 __device__ __forceinline__ int across_swizzle(int k) {
+    static_assert(W >= 64, "four units a row");
     if constexpr (ES == 4) return k >> 3 & 3;
     else if constexpr (W >= 128) return (k & 3) | (k >> 4 & 1) << 2;
     else return (k >> 1 & 1) | (k >> 4 & 1) << 1;
@@ -135,11 +138,11 @@ struct Fragments {
 template <int ES, bool ACROSS, int R, int NW>
 struct Loader {
     static constexpr int NI = R / 8 / NW;
-    static_assert(R / 8 % NW == 0 && NW % 4 == 0, "blocks split evenly over the waves");
+    static_assert(R / 8 % NW == 0, "blocks split evenly over the waves");
     unsigned off[NI];
     unsigned tail_in = 0;                                  // bit q: this lane's 16 bytes of the partial K-tile exist
     // pitch: bytes from row to row; left: rows (along) or 16-byte chunks of columns (across) from the tile's first one to the last; tail: K of the partial tile.
-    // PAIR: rows of two matrices in turn, 16 and 16; a wave's blocks are all of one of them.
+    // PAIR: rows of two matrices in turn, 16 and 16; block b is of number b / 2 % 2 (a wave's blocks are all of one of them where NW is a multiple of 4).
     template <bool PAIR>
     __device__ __forceinline__ void set(int lane, int wave, long pitch, long left, int tail) {
 #pragma unroll
@@ -183,7 +186,8 @@ __device__ __forceinline__ void put_strip(const unsigned char* strip, void* C, l
     }
 }
 
-template <int DT, int MODE, int BM, int BN, int WM, int WN>
+// PARTS: the K-tiles are shared out over gridDim.y workgroups, whose sums go to a workspace in f32 (gated_join_kernel adds them up).
+template <int DT, int MODE, int BM, int BN, int WM, int WN, int NS, bool PARTS>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArgs g) {
     constexpr int ES = ELEM_BYTES<DT>, BK = ROW_BYTES / ES, NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     constexpr bool A_ACROSS = MODE == MM_WEIGHTS, B_ACROSS = MODE != MM_FORWARD;
@@ -210,7 +214,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
     const long to_up = MODE == MM_INPUT ? g.B1 - g.B0 : 0;
 
     // the K-tiles in their order, partial ones first: where number s begins in A and in B
-    const int whole = (int)(inner / BK), partial = tail != 0 ? (MODE == MM_INPUT ? 2 : 1) : 0, nk = whole * (MODE == MM_INPUT ? 2 : 1) + partial;
+    const int whole = (int)(inner / BK), partial = tail != 0 ? (MODE == MM_INPUT ? 2 : 1) : 0, all = whole * (MODE == MM_INPUT ? 2 : 1) + partial;
+    const int first = PARTS ? (int)((long)all * blockIdx.y / gridDim.y) : 0, nk = PARTS ? (int)((long)all * (blockIdx.y + 1) / gridDim.y) - first : all;
     const unsigned char *at_a, *at_b;
     auto locate = [&](int s) {
         long t;
@@ -230,13 +235,14 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
     const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds + wave * 1024);
     constexpr int NIA = la.NI, NI = la.NI + lb.NI;
     auto to = [&](int q) { return lds_base + (q < NIA ? q * NW * 1024 : A_BYTES + (q - NIA) * NW * 1024); };
-    auto fetch_first = [&](int s) {                        // K-tile s into stage s, whole or not
+    auto fetch_first = [&](int st) {                       // K-tile `st` of this workgroup into stage st, whole or not
+        const int s = first + st;
         locate(s);
 #pragma unroll
         for (int q = 0; q < NI; ++q) {
             const unsigned char* inside = q < NIA ? at_a + la.off[q < NIA ? q : 0] : at_b + lb.off[q < NIA ? 0 : q - NIA];
             const bool exists = s >= partial || ((q < NIA ? la.tail_in >> q : lb.tail_in >> (q - NIA)) & 1u) != 0;
-            dma_to_lds_addr(exists ? inside : (const unsigned char*)kZeroChunk, to(q) + s * STAGE);
+            dma_to_lds_addr(exists ? inside : (const unsigned char*)kZeroChunk, to(q) + st * STAGE);
         }
     };
     auto fetch = [&](int q, unsigned stage) {
@@ -253,25 +259,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     u32x4 fa[TM], fb[2][TN];
 
-    fetch_first(0);
-    if (nk > 1) {
-        fetch_first(1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
-    } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
+#pragma unroll
+    for (int st = 0; st < NS; ++st)
+        if (st < nk) fetch_first(st);
+    if (nk >= NS) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < TN; ++j) fb[0][j] = rb.load(lds, 0, j);
 #pragma unroll
     for (int i = 0; i < TM; ++i) fa[i] = ra.load(lds, 0, i);
-    int step = STAGE;
+    unsigned stage = 0;                                    // where the K-tile that is being multiplied begins
     // One K-tile: its first half's MFMAs while the second half's fragments come in, the boundary, its second half's while the next tile's come in (behind the last
-    // tile they are of a stage that is not looked at any more) and, with MORE, the one after that is asked for.
+    // tile they are of a stage that is not looked at any more) and, with MORE, the one NS tiles on is asked for.
     auto tile = [&](int kt, auto more) {
         constexpr bool MORE = decltype(more)::value;
-        const unsigned stage = step > 0 ? 0 : STAGE;
-        if constexpr (MORE) locate(kt + 2);
+        const unsigned released = stage;
+        if constexpr (MORE) locate(first + kt + NS);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
@@ -284,20 +288,23 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
                 for (int j = i * TN / TM; j < (i + 1) * TN / TM; ++j) fb[ks ^ 1][j] = rb.load(lds, ks ^ 1, j);
                 if (MORE && ks == 1)
 #pragma unroll
-                    for (int q = i * NI / TM; q < (i + 1) * NI / TM; ++q) fetch(q, stage);
+                    for (int q = i * NI / TM; q < (i + 1) * NI / TM; ++q) fetch(q, released);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (ks == 0) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                // tile kt + 1 has landed: the NS - 2 behind it may be on their way; near the end only "none" says it
+                if constexpr (MORE) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * NI) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __syncthreads();
+                const int step = stage == (NS - 1) * STAGE ? -(NS - 1) * STAGE : STAGE;
                 ra.step(step);
                 rb.step(step);
-                step = -step;
+                stage += step;
             }
         }
     };
     int kt = 0;
-    for (; kt + 2 < nk; ++kt) tile(kt, std::true_type{});
+    for (; kt + NS < nk; ++kt) tile(kt, std::true_type{});
     for (; kt < nk; ++kt) tile(kt, std::false_type{});
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();                                       // the stages are not read any more
@@ -307,15 +314,16 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
         constexpr int STRIDE = GATED_STRIP_ROW<TN>;
         static_assert(NW * 32 * STRIDE <= 2 * STAGE, "strips");
         unsigned char* strip = lds + wave * (32 * STRIDE);
-        void* const C = of_up != 0 ? g.C1 : g.C0;
         const long rows = MODE == MM_INPUT ? g.M : g.N, col0 = n0 + wn * WTN;
+        void* const C = PARTS ? g.parts + ((MODE == MM_INPUT ? blockIdx.y : 2 * blockIdx.y + of_up) * rows) * g.K : of_up != 0 ? g.C1 : g.C0;
 #pragma unroll
         for (int i = 0; i < TM; i += 2) {
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(strip + (16 * k + fi) * STRIDE + (16 * j + 4 * fq) * 4) = acc[i + k][j];
-            if (g.stream) put_strip<DT, 16 * TN, STRIDE, ST_STREAM>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
+            if constexpr (PARTS) put_strip<SP_F32, 16 * TN, STRIDE, ST_PLAIN>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
+            else if (g.stream) put_strip<DT, 16 * TN, STRIDE, ST_STREAM>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
             else put_strip<DT, 16 * TN, STRIDE, ST_PLAIN>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
         }
     } else {
@@ -405,6 +413,174 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
     }
 }
 
+// ---- few rows, or few tiles ----
+// One tile of (16 TM) x (16 TN) sums on four waves: wave w takes K-tiles w, w + 4, ... through an LDS ring of NS stages of its own, so no wave waits for another inside the loop, and the four
+// partial sums meet in LDS, in a fixed order.  Forward and the gradient of A; of the weights there are always many.
+// PARTS: the K-tiles are shared out over gridDim.y workgroups, too, whose sums go to a workspace in f32 (gated_join_kernel adds them up).
+template <int DT, int MODE, int TM, int TN, int NS, bool PARTS>
+__global__ __launch_bounds__(256) void gated_split_kernel(const GatedArgs g) {
+    constexpr int KS = 4, ES = ELEM_BYTES<DT>, BK = ROW_BYTES / ES, BM = 16 * TM, BN = 16 * TN;
+    constexpr bool B_ACROSS = MODE == MM_INPUT;
+    constexpr int A_BYTES = BM * ROW_BYTES, STAGE = (BM + BN) * ROW_BYTES;
+    static_assert(MODE == MM_FORWARD ? TN % 2 == 0 : MODE == MM_INPUT, "a gate's fragment and an up's");
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fi = lane & 15, fq = lane >> 4;
+    int tm, tn;
+    gated_tile_of_block(blockIdx.x, g.tiles_m, g.tiles_n, g.group_m, tm, tn);
+    const long m0 = (long)tm * BM, n0 = (long)tn * (MODE == MM_FORWARD ? BN / 2 : BN);
+    const long pitch_a = (MODE == MM_FORWARD ? g.K : 2 * g.half) * ES, pitch_b = g.K * ES;
+    const long inner = MODE == MM_FORWARD ? g.K : g.N;
+    const int tail = (int)(inner % BK), per_half = (int)((inner + BK - 1) / BK), all = per_half * (MODE == MM_INPUT ? 2 : 1);
+    const int first = PARTS ? (int)((long)all * blockIdx.y / gridDim.y) : 0, nk = PARTS ? (int)((long)all * (blockIdx.y + 1) / gridDim.y) - first : all;
+    Loader<ES, false, BM, 1> la;
+    Loader<ES, B_ACROSS, BN, 1> lb;
+    la.template set<false>(lane, 0, pitch_a, g.M - m0, MODE == MM_INPUT ? BK : tail);
+    lb.template set<MODE == MM_FORWARD>(lane, 0, pitch_b, B_ACROSS ? (g.K - n0) * ES / 16 : g.N - n0, tail);
+    constexpr int NIA = la.NI, NI = la.NI + lb.NI;
+    static_assert((NS - 1) * NI < 64, "vmcnt counts to 63");
+    const unsigned char* const pA = uniform_ptr(g.A + m0 * pitch_a);
+    const unsigned char* const pB = uniform_ptr(g.B0 + n0 * (MODE == MM_FORWARD ? pitch_b : ES));
+    const long to_up = g.B1 - g.B0;
+    const unsigned my_lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds + wave * (NS * STAGE));
+    auto fetch = [&](int t, unsigned stage) {
+        const int second = MODE == MM_INPUT && t >= per_half ? 1 : 0, in_half = t - second * per_half;
+        const unsigned char* const a = uniform_ptr(pA + (MODE == MM_INPUT ? in_half + second * (g.half / BK) : t) * ROW_BYTES);
+        const unsigned char* const b = uniform_ptr(pB + (MODE == MM_INPUT ? second * to_up + in_half * (BK * pitch_b) : t * (long)ROW_BYTES));
+        const unsigned char* const b_up = MODE == MM_FORWARD ? uniform_ptr(b + to_up) : b;
+        const unsigned dst = my_lds + stage * STAGE;
+        if (tail != 0 && in_half == per_half - 1) {
+#pragma unroll
+            for (int q = 0; q < NI; ++q) {
+                const unsigned char* inside = q < NIA ? a + la.off[q < NIA ? q : 0] : ((q - NIA) >> 1 & 1 ? b_up : b) + lb.off[q < NIA ? 0 : q - NIA];
+                const bool exists = ((q < NIA ? la.tail_in >> q : lb.tail_in >> (q - NIA)) & 1u) != 0;
+                dma_to_lds_addr(exists ? inside : (const unsigned char*)kZeroChunk, dst + q * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < NI; ++q) dma_to_lds(q < NIA ? a : (q - NIA) >> 1 & 1 ? b_up : b, q < NIA ? la.off[q < NIA ? q : 0] : lb.off[q < NIA ? 0 : q - NIA], dst + q * 1024);
+        }
+    };
+    // this wave's K-tiles: wave, wave + KS, ...; where only the weights count, from another one on in every workgroup: if all began with the first, they would ask the memory system for
+    // the same columns of all rows at a time (1 x 4096 x 8192 bf16 30.3 us, so 24.8; with more rows, whose panels of A the workgroups share, 32 x 4096 x 8192 25.0 and 26.6)
+    const int mine = (nk - wave + KS - 1) / KS;
+    int next = MODE == MM_FORWARD && TM == 1 && mine > 0 ? (int)(blockIdx.x * ROTATE % (unsigned)mine) : 0;
+    auto fetch_next = [&](unsigned stage) {
+        fetch(first + wave + next * KS, stage);
+        next = next + 1 == mine ? 0 : next + 1;
+    };
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        if (s < mine) fetch_next(s);
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const Fragments<ES, false, BM, TM> ra(wave * (NS * STAGE), 0, fi, fq);
+    const Fragments<ES, B_ACROSS, BN, TN> rb(wave * (NS * STAGE) + A_BYTES, 0, fi, fq);
+    int stage = 0;
+    for (int t = 0; t < mine; ++t) {
+        // tile t has landed: with NS tiles under way that leaves NS - 1 behind it, near the end only "none" says it
+        if (t + NS <= mine) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * NI) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        unsigned char* const at = lds + stage * STAGE;
+        u32x4 fa[2][TM], fb[2][TN];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[ks][i] = ra.load(at, ks, i);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[ks][j] = rb.load(at, ks, j);
+        }
+        if (t + NS < mine) {
+            // the stage is free once its fragments are in registers
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            fetch_next(stage);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage = stage + 1 == NS ? 0 : stage + 1;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = gated_mma<DT>(fb[ks][j], fa[ks][i], acc[i][j]);
+    }
+    // partial tiles: fragment f of wave w at (f KS + w) KiB; a fragment, or a pair of them, is then finished by one wave
+    __syncthreads();                                       // the rings are not read any more
+    f32x4* const part = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) part[((i * TN + j) * KS + wave) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    auto sum = [&](int f) {
+        const f32x4* p = part + f * KS * 64 + lane;
+        return (p[0] + p[64]) + (p[128] + p[192]);
+    };
+    auto put = [&](void* C, long pitch, long row, long col, const f32x4& v) {
+        if (row >= g.M || col >= pitch) return;
+        const long at = row * pitch + col;
+        if (col + 3 < pitch) {
+            if constexpr (DT == SP_F32) store_c<ST_PLAIN, 4>((float*)C + at, v);
+            else store_c<ST_PLAIN, 2>((unsigned short*)C + at, u32x2{pack_halves<DT>(v[0], v[1]), pack_halves<DT>(v[2], v[3])});
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (col + e < pitch) {
+                    if constexpr (DT == SP_F32) ((float*)C)[at + e] = v[e];
+                    else ((unsigned short*)C)[at + e] = (unsigned short)pack_halves<DT>(v[e], 0.f);
+                }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const long row = m0 + 16 * i + fi;
+        if constexpr (MODE == MM_FORWARD) {
+#pragma unroll
+            for (int p = 0; p < TN / 2; ++p) {
+                if ((i * (TN / 2) + p) % KS != wave) continue;
+                const f32x4 a = sum(i * TN + 2 * p), u = sum(i * TN + 2 * p + 1);
+                const long col = n0 + 16 * p + 4 * fq;
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = gated_activation(a[e], g.activation) * u[e];
+                put(g.C0, g.N, row, col, v);
+                if (g.keep == KEEP_WHOLE) {
+                    put(g.gate, g.N, row, col, a);
+                    put(g.up, g.N, row, col, u);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                if ((i * TN + j) % KS == wave) {
+                    const long col = n0 + 16 * j + 4 * fq;
+                    if constexpr (PARTS) {                 // (K is a multiple of four)
+                        if (row < g.M && col < g.K) *reinterpret_cast<f32x4*>(g.parts + ((long)blockIdx.y * g.M + row) * g.K + col) = sum(i * TN + j);
+                    } else {
+                        put(g.C0, g.K, row, col, sum(i * TN + j));
+                    }
+                }
+        }
+    }
+}
+
+// The partial sums of n workgroups, in their order, to one result or two of `each` numbers; four numbers a lane.
+template <int DT>
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* parts, int n, void* C0, void* C1, long each) {
+    const long all = C1 != nullptr ? 2 * each : each;
+    long at = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= all) return;
+    f32x4 v = *reinterpret_cast<const f32x4*>(parts + at);
+    for (int p = 1; p < n; ++p) v += *reinterpret_cast<const f32x4*>(parts + p * all + at);
+    void* const C = at < each ? C0 : C1;
+    at -= at < each ? 0 : each;
+    if constexpr (DT == SP_F32) *reinterpret_cast<f32x4*>((float*)C + at) = v;
+    else *reinterpret_cast<u32x2*>((unsigned short*)C + at) = u32x2{pack_halves<DT>(v[0], v[1]), pack_halves<DT>(v[2], v[3])};
+}
+
 // ---- dg and du ----
 struct GatedGradArgs {
     const void *dC, *gate, *up;
@@ -477,37 +653,156 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const GatedGradArgs g) 
 
 static long gated_ceil(long a, long b) { return (a + b - 1) / b; }
 
-template <int DT, int MODE, int BM, int BN, int WM, int WN>
-static int launch_mm(const char* what, GatedArgs g, hipStream_t stream) {
-    auto kernel = gated_mm_kernel<DT, MODE, BM, BN, WM, WN>;
-    constexpr int lds_bytes = 2 * (BM + BN) * ROW_BYTES;
+template <int DT>
+static int launch_join(const char* what, const GatedArgs& g, long rows, int parts, hipStream_t stream) {
+    const long each = rows * g.K;
+    hipLaunchKernelGGL(gated_join_kernel<DT>, dim3((unsigned)gated_ceil(each * (g.C1 != nullptr ? 2 : 1), 1024)), dim3(256), 0, stream, g.parts, parts, g.C0, g.C1, each);
+    return check_launch(what);
+}
+
+template <int DT, int MODE, int BM, int BN, int WM, int WN, int NS>
+static int launch_mm(const char* what, GatedArgs g, int parts, hipStream_t stream) {
+    constexpr int lds_bytes = NS * (BM + BN) * ROW_BYTES;
     const long tiles_m = MODE == MM_WEIGHTS ? 2 * gated_ceil(g.N, BM) : gated_ceil(g.M, BM);
     const long tiles_n = MODE == MM_FORWARD ? gated_ceil(g.N, BN / 2) : gated_ceil(g.K, BN);
     if (tiles_m >= 1l << 31 || tiles_n >= 1l << 31 || tiles_m * tiles_n >= 1l << 31 || tiles_m * tiles_n * (WM * WN * 64) >= 1l << 32) return fail(SP_ERR_SHAPE, "%s: too large", what);
-    if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
     g.tiles_m = (int)tiles_m;
     g.tiles_n = (int)tiles_n;
     g.group_m = 4;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n)), dim3(WM * WN * 64), lds_bytes, stream, g);
-    return check_launch(what);
+    auto launch = [&](auto kernel) {
+        if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(WM * WN * 64), lds_bytes, stream, g);
+        return check_launch(what);
+    };
+    if constexpr (MODE != MM_FORWARD)
+        if (parts > 1) {
+            if (const int rc = launch(gated_mm_kernel<DT, MODE, BM, BN, WM, WN, NS, true>); rc != SP_OK) return rc;
+            return launch_join<DT>(what, g, MODE == MM_INPUT ? g.M : g.N, parts, stream);
+        }
+    return launch(gated_mm_kernel<DT, MODE, BM, BN, WM, WN, NS, false>);
+}
+
+template <int DT, int MODE, int TM, int TN, int NS>
+static int launch_split(const char* what, GatedArgs g, int parts, hipStream_t stream) {
+    constexpr int ring = 4 * NS * 16 * (TM + TN) * ROW_BYTES, partial = TM * TN * 4096, lds_bytes = ring > partial ? ring : partial;
+    const long tiles_m = gated_ceil(g.M, 16 * TM), tiles_n = MODE == MM_FORWARD ? gated_ceil(g.N, 8 * TN) : gated_ceil(g.K, 16 * TN);
+    if (tiles_m * tiles_n * 256 >= 1l << 32) return fail(SP_ERR_SHAPE, "%s: too large", what);
+    g.tiles_m = (int)tiles_m;
+    g.tiles_n = (int)tiles_n;
+    g.group_m = (int)tiles_m;      // the tiles of one panel of weights stand side by side
+    auto launch = [&](auto kernel) {
+        if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(256), lds_bytes, stream, g);
+        return check_launch(what);
+    };
+    if constexpr (MODE == MM_INPUT)
+        if (parts > 1) {
+            if (const int rc = launch(gated_split_kernel<DT, MODE, TM, TN, NS, true>); rc != SP_OK) return rc;
+            return launch_join<DT>(what, g, g.M, parts, stream);
+        }
+    return launch(gated_split_kernel<DT, MODE, TM, TN, NS, false>);
+}
+
+// ---- which kernel ----
+// Estimated time of a product in us, without the launch: workgroups in rounds of as many as a unit's LDS holds at a time, each nk K-tiles (a quarter of them, where four waves share
+// them) plus an overhead; n workgroups on a unit take n times the work of a K-tile, and never less than what a lone one waits for.  Partial sums are written, read and joined.
+// Fitted on what every kernel took on 99 forward, 62 and 62 backward shapes, from 1 x 512 x 1365 to 16384 x 4096 x 512; the one it picks is on the mean 2 % behind the fastest forward
+// (3 with 8-bit blocks), 4 for the gradient of A and 2 for the weights'.  More tiles (64 x 128, 128 x 256 in two stages, 16 x 64 and 64 x 64 in four parts) were worth less than a hundredth.
+struct MmCost {
+    int id, bm, bn;               // bn: columns of the result
+    int per_unit;
+    bool split;
+    float lone, work, overhead;
+};
+enum { SPLIT_16, SPLIT_32, TILE_64, TILE_64_BLOCKS, TILE_128, TILE_128_WIDE, TILE_256 };
+static const MmCost kForward16[] = {{SPLIT_16, 16, 16, 3, true, 0.156f, 0.278f, 2.55f}, {SPLIT_32, 32, 16, 2, true, 0.336f, 0.387f, 2.65f}, {TILE_64, 64, 32, 2, false, 0.227f, 0.183f, 2.57f},
+                                    {TILE_128, 128, 64, 1, false, 0.437f, 0.386f, 3.84f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 4.67f}, {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 5.95f}};
+static const MmCost kForward32[] = {{SPLIT_16, 16, 16, 3, true, 0.587f, 0.354f, 2.47f}, {SPLIT_32, 32, 16, 2, true, 0.587f, 0.632f, 3.2f}, {TILE_64, 64, 32, 2, false, 0.633f, 0.572f, 1.39f},
+                                    {TILE_128, 128, 64, 1, false, 1.918f, 0.386f, 3.7f}};
+// tiles that hold whole blocks of 128 columns of both factors
+static const MmCost kBlocks16[] = {{TILE_64_BLOCKS, 64, 128, 1, false, 0.541f, 0.541f, 3.75f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 4.67f}, {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 5.95f}};
+static const MmCost kBlocks32[] = {{TILE_64_BLOCKS, 64, 128, 1, false, 1.972f, 1.039f, 4.06f}};
+static const MmCost kInput16[] = {{SPLIT_32, 32, 64, 1, true, 0.572f, 0.318f, 2.47f}, {TILE_64, 64, 64, 2, false, 0.225f, 0.201f, 2.96f}, {TILE_128, 128, 128, 1, false, 0.464f, 0.464f, 3.77f},
+                                  {TILE_128_WIDE, 128, 256, 1, false, 0.652f, 0.652f, 4.51f}, {TILE_256, 256, 256, 1, false, 1.112f, 0.4f, 5.2f}};
+static const MmCost kWeights16[] = {{TILE_64, 64, 64, 2, false, 0.171f, 0.218f, 2.64f}, {TILE_128, 128, 128, 1, false, 0.538f, 0.424f, 4.11f}, {TILE_128_WIDE, 128, 256, 1, false, 0.766f, 0.1f, 5.53f},
+                                    {TILE_256, 256, 256, 1, false, 1.282f, 0.1f, 7.04f}};
+static const MmCost kInput32[] = {{SPLIT_32, 32, 64, 1, true, 1.167f, 0.4f, 3.04f}, {TILE_64, 64, 64, 5, false, 0.594f, 0.528f, 2.36f}, {TILE_128, 128, 128, 2, false, 1.999f, 1.918f, 2.23f}};
+static const MmCost kWeights32[] = {{TILE_64, 64, 64, 5, false, 0.603f, 0.538f, 3.78f}, {TILE_128, 128, 128, 2, false, 1.896f, 2.022f, 5.08f}};
+
+struct MmChoice {
+    int id, parts;
+};
+
+template <size_t N>
+static MmChoice cheapest(const MmCost (&menu)[N], int mode, bool f32, long M, long N_, long K) {
+    const long cus = device_cu_count(), bk = f32 ? 32 : 64;
+    const long rows = mode == MM_WEIGHTS ? N_ : M, cols = mode == MM_FORWARD ? N_ : K, twice = mode == MM_WEIGHTS ? 2 : 1;
+    const long nk = mode == MM_FORWARD ? gated_ceil(K, bk) : mode == MM_INPUT ? 2 * gated_ceil(N_, bk) : gated_ceil(M, bk);
+    MmChoice best{menu[0].id, 1};
+    double best_us = 0;
+    bool any = false;
+    for (const MmCost& c : menu) {
+        const double tiles = (double)gated_ceil(rows, c.bm) * (double)gated_ceil(cols, c.bn) * twice;
+        if (tiles * 512 >= 4294967296.0) continue;         // (a launch holds fewer than 2^32 work items)
+        for (int parts = 1; parts <= 16; parts *= 2) {
+            if (parts > 1 && (mode == MM_FORWARD || tiles * parts > 2.0 * cus || nk < 4 * parts)) break;
+            const double groups = tiles * parts, round = (double)cus * c.per_unit;
+            const long mine = gated_ceil(gated_ceil(nk, parts), c.split ? 4 : 1);
+            auto of = [&](double n) { return mine * (n * c.work > c.lone ? n * c.work : (double)c.lone) + c.overhead; };
+            const double full = (double)(int64_t)(groups / round), rest = groups - full * round;
+            double us = full * of(c.per_unit) + (rest > 0 ? of((double)(int64_t)((rest + cus - 1) / cus)) : 0);
+            if (parts > 1) us += 6 + (double)rows * cols * twice * (8.0 * parts + (f32 ? 4 : 2)) * 1e-6 / 8;
+            if (!any || us < best_us) {
+                any = true;
+                best_us = us;
+                best = {c.id, parts};
+            }
+        }
+    }
+    return best;
+}
+static MmChoice choose_backward(int mode, bool f32, long M, long N, long K) {
+    if (mode == MM_INPUT) return f32 ? cheapest(kInput32, mode, f32, M, N, K) : cheapest(kInput16, mode, f32, M, N, K);
+    return f32 ? cheapest(kWeights32, mode, f32, M, N, K) : cheapest(kWeights16, mode, f32, M, N, K);
 }
 
 template <int DT>
 static int gated_forward(const GatedArgs& g, hipStream_t stream) {
-    const long cus = device_cu_count();
-    auto tiles = [&](long bm) { return gated_ceil(g.M, bm) * gated_ceil(g.N, 128); };
-    if (tiles(256) * 5 >= cus * 4) return launch_mm<DT, MM_FORWARD, 256, 256, 4, 2>("sp_gemm_abt_gated", g, stream);
-    if (tiles(128) * 5 >= cus * 4) return launch_mm<DT, MM_FORWARD, 128, 256, 4, 2>("sp_gemm_abt_gated", g, stream);
-    return launch_mm<DT, MM_FORWARD, 64, 256, 2, 2>("sp_gemm_abt_gated", g, stream);
+    constexpr bool F32 = DT == SP_F32;
+    const char* const what = "sp_gemm_abt_gated";
+    int id;
+    if (g.keep == KEEP_F8) id = F32 ? cheapest(kBlocks32, MM_FORWARD, F32, g.M, g.N, g.K).id : cheapest(kBlocks16, MM_FORWARD, F32, g.M, g.N, g.K).id;
+    else id = F32 ? cheapest(kForward32, MM_FORWARD, F32, g.M, g.N, g.K).id : cheapest(kForward16, MM_FORWARD, F32, g.M, g.N, g.K).id;
+    switch (id) {
+        case SPLIT_16: return launch_split<DT, MM_FORWARD, 1, 2, 2>(what, g, 1, stream);
+        case SPLIT_32: return launch_split<DT, MM_FORWARD, 2, 2, 2>(what, g, 1, stream);
+        case TILE_64: return launch_mm<DT, MM_FORWARD, 64, 64, 2, 2, 4>(what, g, 1, stream);
+        case TILE_64_BLOCKS: return launch_mm<DT, MM_FORWARD, 64, 256, 2, 2, 3>(what, g, 1, stream);
+        case TILE_128: return launch_mm<DT, MM_FORWARD, 128, 128, 2, 2, 4>(what, g, 1, stream);
+    }
+    if constexpr (!F32) {
+        if (id == TILE_128_WIDE) return launch_mm<DT, MM_FORWARD, 128, 256, 4, 2, 3>(what, g, 1, stream);
+        return launch_mm<DT, MM_FORWARD, 256, 256, 4, 2, 2>(what, g, 1, stream);
+    }
+    return fail(SP_ERR_UNSUPPORTED, "%s: no kernel", what);
 }
 
 template <int DT, int MODE>
 static int gated_backward_product(const GatedArgs& g, hipStream_t stream) {
-    const long cus = device_cu_count(), rows = MODE == MM_INPUT ? g.M : g.N;
-    auto tiles = [&](long b) { return gated_ceil(rows, b) * (MODE == MM_WEIGHTS ? 2 : 1) * gated_ceil(g.K, b); };
-    if (tiles(256) * 5 >= cus * 4) return launch_mm<DT, MODE, 256, 256, 2, 4>("sp_gemm_abt_gated_backward", g, stream);
-    if (tiles(128) * 5 >= cus * 4) return launch_mm<DT, MODE, 128, 128, 2, 2>("sp_gemm_abt_gated_backward", g, stream);
-    return launch_mm<DT, MODE, 64, 64, 2, 2>("sp_gemm_abt_gated_backward", g, stream);
+    constexpr bool F32 = DT == SP_F32;
+    const char* const what = "sp_gemm_abt_gated_backward";
+    const MmChoice c = choose_backward(MODE, F32, g.M, g.N, g.K);
+    if constexpr (MODE == MM_INPUT)
+        if (c.id == SPLIT_32) return launch_split<DT, MODE, 2, 4, 2>(what, g, c.parts, stream);
+    if constexpr (F32) {
+        if (c.id == TILE_64) return launch_mm<DT, MODE, 64, 64, 2, 2, 2>(what, g, c.parts, stream);
+        return launch_mm<DT, MODE, 128, 128, 2, 2, 2>(what, g, c.parts, stream);
+    } else {
+        if (c.id == TILE_64) return launch_mm<DT, MODE, 64, 64, 2, 2, 4>(what, g, c.parts, stream);
+        if (c.id == TILE_128) return launch_mm<DT, MODE, 128, 128, 2, 2, 4>(what, g, c.parts, stream);
+        if (c.id == TILE_128_WIDE) return launch_mm<DT, MODE, 128, 256, 2, 4, 3>(what, g, c.parts, stream);
+        return launch_mm<DT, MODE, 256, 256, 2, 4, 2>(what, g, c.parts, stream);
+    }
 }
 
 template <int DT>
@@ -525,9 +820,9 @@ static int gated_backward(const GatedArgs& input, const GatedArgs& weights, cons
 namespace {
 struct GatedKernelNames {
     GatedKernelNames() {
-        register_kernel("gated_forward_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_FORWARD, 256, 256, 4, 2>, 512);
-        register_kernel("gated_input_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_INPUT, 256, 256, 2, 4>, 512);
-        register_kernel("gated_weights_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_WEIGHTS, 256, 256, 2, 4>, 512);
+        register_kernel("gated_forward_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_FORWARD, 256, 256, 4, 2, 2, false>, 512);
+        register_kernel("gated_input_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_INPUT, 256, 256, 2, 4, 2, false>, 512);
+        register_kernel("gated_weights_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_WEIGHTS, 256, 256, 2, 4, 2, false>, 512);
     }
 } gated_kernel_names;
 }  // namespace
@@ -578,9 +873,17 @@ extern "C" int sp_gemm_abt_gated(int dtype, int activation, const void* A, const
     return gated_forward<SP_BF16>(g, st);
 }
 
-extern "C" int64_t sp_gemm_abt_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t N) {
-    if (M <= 0 || N <= 0 || M > INT32_MAX || N > (int64_t)1 << 24) return 0;
-    return M * 2 * gated_half(N) * (dtype == SP_F32 ? 4 : 2);
+// Partial sums of the backward products, one after the other in the same place.
+static int64_t gated_parts_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+    const int64_t input = choose_backward(MM_INPUT, dtype == SP_F32, M, N, K).parts, weights = choose_backward(MM_WEIGHTS, dtype == SP_F32, M, N, K).parts;
+    const int64_t a = input > 1 ? input * M * K * 4 : 0, b = weights > 1 ? weights * 2 * N * K * 4 : 0;
+    return a > b ? a : b;
+}
+static int64_t gated_halves_bytes(int dtype, int64_t M, int64_t N) { return M * 2 * gated_half(N) * (dtype == SP_F32 ? 4 : 2); }
+
+extern "C" int64_t sp_gemm_abt_gated_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > (int64_t)1 << 24 || K > (int64_t)1 << 24) return 0;
+    return gated_halves_bytes(dtype, M, N) + gated_parts_bytes(dtype, M, N, K);
 }
 
 extern "C" int sp_gemm_abt_gated_backward(int dtype, int activation, const void* dC, const void* A, const void* B_gate, const void* B_up, int kept_dtype, const void* gate,
@@ -605,9 +908,9 @@ extern "C" int sp_gemm_abt_gated_backward(int dtype, int activation, const void*
     if (dA == nullptr && dB_gate == nullptr) return fail(SP_ERR_NULL, "sp_gemm_abt_gated_backward: no gradient is wanted");
     const int64_t half = gated_half(N);
     if (M * (half / 8) > ((int64_t)1 << 32) - 256) return fail(SP_ERR_SHAPE, "sp_gemm_abt_gated_backward: too large");
-    if (workspace_bytes < sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N))
+    if (workspace_bytes < sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K))
         return fail(SP_ERR_ARG, "sp_gemm_abt_gated_backward: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes,
-                    (long long)sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N));
+                    (long long)sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K));
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     GatedGradArgs grad{};
     grad.dC = dC; grad.gate = gate; grad.up = up; grad.gate_scale = gate_scale; grad.up_scale = up_scale; grad.out = workspace; grad.M = M; grad.N = N; grad.half = half;
@@ -615,7 +918,7 @@ extern "C" int sp_gemm_abt_gated_backward(int dtype, int activation, const void*
     const int es = dtype == SP_F32 ? 4 : 2;
     GatedArgs input{}, weights{};
     input.A = (const unsigned char*)workspace; input.B0 = (const unsigned char*)B_gate; input.B1 = (const unsigned char*)B_up; input.C0 = dA; input.M = M; input.N = N; input.K = K;
-    input.half = half; input.stream = M * K * es > (int64_t)32 << 20;
+    input.half = half; input.parts = (float*)((unsigned char*)workspace + gated_halves_bytes(dtype, M, N)); input.stream = M * K * es > (int64_t)32 << 20;
     weights = input;
     weights.B0 = (const unsigned char*)A; weights.B1 = nullptr; weights.C0 = dB_gate; weights.C1 = dB_up; weights.stream = 2 * N * K * es > (int64_t)32 << 20;
     const hipStream_t st = (hipStream_t)stream;

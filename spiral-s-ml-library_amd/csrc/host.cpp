@@ -663,7 +663,7 @@ PyObject* whole_matmul_abt_gated_backward(PyObject* capsule, PyObject* const* o,
         void *pd = call.at(dc, type), *pa = call.at(a, type), *pg = call.at(gate, type), *pu = call.at(up, type);
         void *k0 = call.at(kept[0], as), *k1 = call.at(kept[1], at::kFloat), *k2 = call.at(kept[2], as), *k3 = call.at(kept[3], at::kFloat);
         void *da = call.make({m, k}, type, *a), *dg = call.make({cols, k}, type, *a), *du = call.make({cols, k}, type, *a);
-        const int64_t bytes = ((decltype(&sp_gemm_abt_gated_backward_workspace_bytes))bound.more)(code, m, cols);
+        const int64_t bytes = ((decltype(&sp_gemm_abt_gated_backward_workspace_bytes))bound.more)(code, m, cols, k);
         void* workspace = call.make({bytes}, at::kByte, *a);
         launch((decltype(&sp_gemm_abt_gated_backward))bound.fn, code, activation, pd, pa, pg, pu, f8 ? (int)SP_F8_E4M3 : code, k0, (const float*)k1, k2, (const float*)k3, da, dg, du,
                m, cols, k, workspace, bytes, call.stream);

@@ -71,14 +71,18 @@ __device__ __forceinline__ float logit_at(const void* logits, long at) {
     if constexpr (DT == SP_F32) return ((const float*)logits)[at];
     else return half_bits_to_f32<DT>(((const unsigned short*)logits)[at]);
 }
-template <int DT>
-__device__ __forceinline__ void put_row(const TokenArgs& a, const void* logits, long cols, long row, const Sums& sums) {
+// x: the token's logit, where it counts.
+__device__ __forceinline__ void put_sums(const TokenArgs& a, long row, bool counts, float x, const Sums& sums) {
     const RowResult r(sums);
-    const int token = a.tokens[row];
-    const bool counts = (unsigned)token < (unsigned)cols;
-    a.logp[row] = counts ? r.logp(logit_at<DT>(logits, row * cols + token)) : 0.f;
+    a.logp[row] = counts ? r.logp(x) : 0.f;
     if (a.lse != nullptr) a.lse[row] = r.none ? -INFINITY : r.m + r.ln_s;
     if (a.entropy != nullptr) a.entropy[row] = r.none ? 0.f : r.ln_s - LN2 * (sums.w / sums.s);
+}
+template <int DT>
+__device__ __forceinline__ void put_row(const TokenArgs& a, const void* logits, long cols, long row, const Sums& sums) {
+    const int token = a.tokens[row];
+    const bool counts = (unsigned)token < (unsigned)cols;
+    put_sums(a, row, counts, counts ? logit_at<DT>(logits, row * cols + token) : 0.f, sums);
 }
 
 // ---- the most likely tokens ----
@@ -96,42 +100,47 @@ __device__ __forceinline__ float logit_of(Key k) {
 __device__ __forceinline__ int column_of(Key k) { return (int)~(unsigned)k; }
 __device__ __forceinline__ Key larger(Key a, Key b) { return a > b ? a : b; }
 
+template <int T>
 struct TopLds {
     Key list[LIST];
-    Key lanes[64];
+    Key lanes[T];
+    Key subsets[64];
     Key least;
-    int count;
+    int count, found;
+    unsigned short who[T];
 };
 
-// The `top` largest keys of a workgroup's part of a row, in their order, to put(place, key); places behind the last one get key 0.  each(f): f of every
-// key of this lane; mine: the largest of them.
-// The 64 largest of lanes apart by 64 hold `top` keys (or all there are) that are no smaller than the top-th of them, so nothing below that one is taken: what is left, some two
-// dozen of a row for 20 alternatives, goes to a list, where every key counts the larger ones.  Where the list is too short (thousands of the largest logits in a few lanes) the
-// workgroup looks for one key after the other.
-template <int T, typename Each, typename Put>
-__device__ __forceinline__ void largest_keys(TopLds& lds, Key* keys, Key mine, int top, const Each& each, const Put& put) {
+// The `top` largest keys of a workgroup's part of a row, in their order, to put(place, key); places behind the last one get key 0.  mine: the largest key of this lane, pieces: how
+// many pieces a lane has, keys(lane, piece, f): f of every key of that lane's piece.
+// The 64 largest of lanes apart by 64 hold `top` keys (or all there are) that are no smaller than the top-th of them, so nothing below that one is taken.  The few lanes that have
+// something left are listed, their pieces shared out over all lanes, and what is left of them, some two dozen keys for 20 alternatives, goes to a list, where every key counts the larger
+// ones.  Where that list is too short (thousands of the largest logits in a few lanes) the workgroup looks for one key after the other.
+template <int T, typename Keys, typename Put>
+__device__ __forceinline__ void largest_keys(TopLds<T>& lds, Key mine, int top, int pieces, const Keys& keys, const Put& put) {
     const int tid = threadIdx.x;
-    keys[tid] = mine;
+    lds.lanes[tid] = mine;
     if (tid == 0) {
-        lds.count = 0;
+        lds.count = lds.found = 0;
         lds.least = 1;
     }
     __syncthreads();
-    Key best = 0;
     if (tid < 64) {
-        for (int t = tid; t < T; t += 64) best = larger(best, keys[t]);
-        lds.lanes[tid] = best;
-    }
-    __syncthreads();
-    if (tid < 64 && best != 0) {
+        Key best = 0;
+#pragma unroll
+        for (int t = 0; t < T; t += 64) best = larger(best, lds.lanes[t + tid]);
+        lds.subsets[tid] = best;                           // (one wave: what it writes it reads in order)
         int above = 0;
-        for (int j = 0; j < 64; ++j) above += lds.lanes[j] > best ? 1 : 0;
-        if (above == top - 1) lds.least = best;
+#pragma unroll 8
+        for (int j = 0; j < 64; ++j) above += lds.subsets[j] > best ? 1 : 0;
+        if (best != 0 && above == top - 1) lds.least = best;
     }
     __syncthreads();
     const Key least = lds.least;
-    if (mine >= least)
-        each([&](Key k) {
+    if (mine >= least) lds.who[atomicAdd(&lds.found, 1)] = (unsigned short)tid;
+    __syncthreads();
+    const int all = lds.found * pieces;
+    for (int i = tid; i < all; i += T)
+        keys(lds.who[i / pieces], i % pieces, [&](Key k) {
             if (k < least) return;
             const int at = atomicAdd(&lds.count, 1);
             if (at < LIST) lds.list[at] = k;
@@ -150,18 +159,19 @@ __device__ __forceinline__ void largest_keys(TopLds& lds, Key* keys, Key mine, i
     }
     Key last = ~(Key)0;
     for (int place = 0; place < top; ++place) {
-        best = 0;
-        each([&](Key k) {
-            if (k < last) best = larger(best, k);
-        });
+        Key best = 0;
+        for (int i = 0; i < pieces; ++i)
+            keys(tid, i, [&](Key k) {
+                if (k < last) best = larger(best, k);
+            });
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) best = larger(best, __shfl_xor(best, d, WAVE));
         __syncthreads();                                   // (the last round's are read)
-        if ((tid & 63) == 0) keys[tid >> 6] = best;
+        if ((tid & 63) == 0) lds.subsets[tid >> 6] = best;
         __syncthreads();
-        best = keys[0];
+        best = lds.subsets[0];
 #pragma unroll
-        for (int w = 1; w < T / 64; ++w) best = larger(best, keys[w]);
+        for (int w = 1; w < T / 64; ++w) best = larger(best, lds.subsets[w]);
         if (tid == 0) put(place, best);
         last = best;
     }
@@ -172,69 +182,90 @@ constexpr int AT_ONCE = 4;        // 16-byte pieces of a lane between two looks 
 
 template <int DT, int T, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(T) void token_probs_kernel(const void* logits, long cols, unsigned chunks, long chunk_cols, const TokenArgs a) {
-    constexpr int P = PER16<DT>, STEP = T * P, N = AT_ONCE * P;
+    constexpr int P = PER16<DT>, PIECES = T * P, STEP = AT_ONCE * PIECES, N = AT_ONCE * P;
     const int tid = threadIdx.x;
     const long row = blockIdx.x / chunks;
     const unsigned chunk = blockIdx.x - (unsigned)row * chunks;
     const long c0 = (long)chunk * chunk_cols;
-    const int here = (int)(cols - c0 < chunk_cols ? cols - c0 : chunk_cols);
-    const long base = row * cols + c0;
+    // pieces are those of memory, 16-byte aligned: the first one may begin up to P - 1 logits in front of the chunk, whose columns count from there
+    const int front = (int)((row * cols) & (P - 1)), here = (int)(cols - c0 < chunk_cols ? cols - c0 : chunk_cols) + front;
+    const long base = row * cols + c0 - front;
+    auto inside = [&](int i) { return i >= front && i < here; };
+    // piece u of the step from column i0 on
     auto load = [&](int i0, u32x4 (&raw)[AT_ONCE]) {
+        if (i0 + STEP <= here) {                           // (of the whole workgroup)
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            const int i = i0 + u * STEP + tid * P;
-            raw[u] = load16<DT>(logits, base + i, here - i);
+            for (int u = 0; u < AT_ONCE; ++u) raw[u] = *reinterpret_cast<const u32x4*>((const unsigned char*)logits + (base + i0 + u * PIECES + tid * P) * ELEM_BYTES<DT>);
+        } else {
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int i = i0 + u * PIECES + tid * P;
+                raw[u] = load16<DT>(logits, base + i, here - i);
+            }
         }
     };
-    auto values = [&](int i0, const u32x4 (&raw)[AT_ONCE], float (&x)[N]) {
+    Sums mine{-INFINITY, 0.f, 0.f};
+    int best_piece = 0;                                    // the first piece with this lane's largest logit
+    auto consume = [&](int i0, const u32x4 (&raw)[AT_ONCE], auto whole) {
+        float x[N];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
-            for (int e = 0; e < P; ++e) x[u * P + e] = element<DT>(raw[u], e);
-        if (i0 + AT_ONCE * STEP > here)                    // (of the whole workgroup)
+            for (int e = 0; e < P; ++e) {
+                x[u * P + e] = element<DT>(raw[u], e);
+                if (!decltype(whole)::value && !inside(i0 + u * PIECES + tid * P + e)) x[u * P + e] = -INFINITY;
+            }
+        if constexpr (TOP) {
+            float most = mine.m;
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u)
+            for (int u = 0; u < AT_ONCE; ++u) {
+                float of_piece = x[u * P];
 #pragma unroll
-                for (int e = 0; e < P; ++e)
-                    if (i0 + u * STEP + tid * P + e >= here) x[u * P + e] = -INFINITY;
+                for (int e = 1; e < P; ++e) of_piece = fmaxf(of_piece, x[u * P + e]);
+                best_piece = of_piece > most ? i0 / PIECES + u : best_piece;
+                most = fmaxf(most, of_piece);
+            }
+        }
+        take<N, ENTROPY>(mine, x);
     };
-    Sums mine{-INFINITY, 0.f, 0.f};
-    int best_at = 0;                                       // where the step with this lane's largest logit begins
     u32x4 ahead[AT_ONCE];
     load(0, ahead);
-    for (int i0 = 0; i0 < here; i0 += AT_ONCE * STEP) {
+    for (int i0 = 0; i0 < here; i0 += STEP) {
         u32x4 raw[AT_ONCE];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) raw[u] = ahead[u];
-        if (i0 + AT_ONCE * STEP < here) load(i0 + AT_ONCE * STEP, ahead);
-        float x[N];
-        values(i0, raw, x);
-        const float before = mine.m;
-        take<N, ENTROPY>(mine, x);
-        if constexpr (TOP)
-            if (mine.m > before) best_at = i0;
+        if (i0 + STEP < here) load(i0 + STEP, ahead);
+        if (i0 + STEP <= here && (i0 > 0 || front == 0)) consume(i0, raw, std::true_type{});
+        else consume(i0, raw, std::false_type{});
     }
-    const float most_here = mine.m;
+    auto keys_of_piece = [&](int lane, int piece, const auto& f) {
+        const int i = piece * PIECES + lane * P;
+        const u32x4 raw = load16<DT>(logits, base + i, here - i);
+#pragma unroll
+        for (int e = 0; e < P; ++e) f(inside(i + e) ? key_of(element<DT>(raw, e), (int)c0 + i + e - front) : (Key)0);
+    };
+    Key best = 0;
+    if constexpr (TOP)
+        if (mine.m > -INFINITY) keys_of_piece(tid, best_piece, [&](Key k) { best = larger(best, k); });
     __shared__ Sums waves[T / 64];
-    __shared__ Sums all;
-    const float wave_most = group_max<64>(mine.m);
-    move_to(mine, wave_most);
+    move_to(mine, group_max<64>(mine.m));
     mine.s = group_reduce<64>(mine.s, add_f32);
-    mine.w = group_reduce<64>(mine.w, add_f32);
+    if constexpr (ENTROPY) mine.w = group_reduce<64>(mine.w, add_f32);
     if ((tid & 63) == 0) waves[tid >> 6] = mine;
     __syncthreads();
+    if (!TOP && tid != 0) return;
+    float most = waves[0].m;
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) most = fmaxf(most, waves[w].m);
+    Sums sums{most, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+        Sums one = waves[w];
+        move_to(one, most);
+        sums.s += one.s;
+        sums.w += one.w;
+    }
     if (tid == 0) {
-        float most = waves[0].m;
-#pragma unroll
-        for (int w = 1; w < T / 64; ++w) most = fmaxf(most, waves[w].m);
-        Sums sums{most, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < T / 64; ++w) {
-            Sums one = waves[w];
-            move_to(one, most);
-            sums.s += one.s;
-            sums.w += one.w;
-        }
         if (chunks == 1) {
             put_row<DT>(a, logits, cols, row, sums);
         } else {
@@ -242,77 +273,64 @@ __global__ __launch_bounds__(T) void token_probs_kernel(const void* logits, long
             a.part[3l * blockIdx.x + 1] = sums.s;
             a.part[3l * blockIdx.x + 2] = sums.w;
         }
-        all = sums;
     }
     if constexpr (TOP) {
-        __shared__ TopLds lds;
-        __shared__ Key keys[T];
-        auto keys_of_step = [&](int i0, const auto& f) {
-            u32x4 raw[AT_ONCE];
-            load(i0, raw);
-            float x[N];
-            values(i0, raw, x);
-#pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u)
-#pragma unroll
-                for (int e = 0; e < P; ++e) f(key_of(x[u * P + e], (int)c0 + i0 + u * STEP + tid * P + e));
-        };
-        Key best = 0;
-        if (most_here > -INFINITY) keys_of_step(best_at, [&](Key k) { best = larger(best, k); });
+        __shared__ TopLds<T> lds;
         const long to = (long)blockIdx.x * a.top;
-        __syncthreads();
-        const RowResult r(all);
-        largest_keys<T>(lds, keys, best, a.top,
-                        [&](const auto& f) {
-                            for (int i0 = 0; i0 < here; i0 += AT_ONCE * STEP) keys_of_step(i0, f);
-                        },
-                        [&](int place, Key k) {
-                            if (chunks == 1) {
-                                a.top_logp[to + place] = k != 0 ? r.logp(logit_of(k)) : -INFINITY;
-                                a.top_ids[to + place] = k != 0 ? column_of(k) : -1;
-                            } else {
-                                a.part_top[to + place] = k != 0 ? logit_of(k) : -INFINITY;
-                                a.part_ids[to + place] = k != 0 ? column_of(k) : -1;
-                            }
-                        });
+        const RowResult r(sums);
+        largest_keys<T>(lds, best, a.top, (here + PIECES - 1) / PIECES, keys_of_piece, [&](int place, Key k) {
+            if (chunks == 1) {
+                a.top_logp[to + place] = k != 0 ? r.logp(logit_of(k)) : -INFINITY;
+                a.top_ids[to + place] = k != 0 ? column_of(k) : -1;
+            } else {
+                a.part_top[to + place] = k != 0 ? logit_of(k) : -INFINITY;
+                a.part_ids[to + place] = k != 0 ? column_of(k) : -1;
+            }
+        });
     }
 }
 
-// A row's chunks, a lane each, a wave per row.
-template <int DT>
-__global__ __launch_bounds__(256) void token_probs_join_kernel(const void* logits, long cols, long rows, int chunks, const TokenArgs a) {
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
-    const long mine_at = row * chunks + lane;
+// A row's chunks, a lane of a wave each.
+__device__ __forceinline__ Sums join_chunks(const TokenArgs& a, long row, int chunks, int lane) {
     Sums sums{-INFINITY, 0.f, 0.f};
-    if (lane < chunks) sums = Sums{a.part[3 * mine_at], a.part[3 * mine_at + 1], a.part[3 * mine_at + 2]};
+    if (lane < chunks) {
+        const float* at = a.part + 3 * (row * chunks + lane);
+        sums = Sums{at[0], at[1], at[2]};
+    }
     move_to(sums, group_max<64>(sums.m));
     sums.s = group_reduce<64>(sums.s, add_f32);
     sums.w = group_reduce<64>(sums.w, add_f32);
-    if (lane == 0) put_row<DT>(a, logits, cols, row, sums);
-    if (a.top == 0) return;
-    // the chunks' alternatives stand in their order: the largest of all is the first of some chunk, whose next one then takes its place
-    const RowResult r(sums);
-    int next = 0;
-    auto first = [&]() {
-        if (lane >= chunks || next >= a.top) return (Key)0;
-        return key_of(a.part_top[mine_at * a.top + next], a.part_ids[mine_at * a.top + next]);
+    return sums;
+}
+template <int DT>
+__global__ __launch_bounds__(256) void token_probs_join_kernel(const void* logits, long cols, long rows, int chunks, const TokenArgs a) {
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const Sums sums = join_chunks(a, row, chunks, threadIdx.x & 63);
+    if ((threadIdx.x & 63) == 0) put_row<DT>(a, logits, cols, row, sums);
+}
+// The same with the alternatives, a workgroup for a row: every chunk has left its own, and the row's are among them.
+template <int DT>
+__global__ __launch_bounds__(256) void token_probs_join_top_kernel(const void* logits, long cols, int chunks, const TokenArgs a) {
+    constexpr int T = 256;
+    const int tid = threadIdx.x;
+    const long row = blockIdx.x;
+    const int n = chunks * a.top;
+    auto keys = [&](int lane, int piece, const auto& f) {
+        const int i = piece * T + lane;
+        f(i < n ? key_of(a.part_top[row * n + i], a.part_ids[row * n + i]) : (Key)0);
     };
-    Key head = first();
-    for (int place = 0; place < a.top; ++place) {
-        Key best = head;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) best = larger(best, __shfl_xor(best, d, WAVE));
-        if (lane == 0) {
-            a.top_logp[row * a.top + place] = best != 0 ? r.logp(logit_of(best)) : -INFINITY;
-            a.top_ids[row * a.top + place] = best != 0 ? column_of(best) : -1;
-        }
-        if (head == best && best != 0) {                   // (columns differ: one lane)
-            ++next;
-            head = first();
-        }
-    }
+    const int pieces = (n + T - 1) / T;
+    Key best = 0;
+    for (int p = 0; p < pieces; ++p) keys(tid, p, [&](Key k) { best = larger(best, k); });
+    const Sums sums = join_chunks(a, row, chunks, tid & 63);           // (every wave for itself)
+    if (tid == 0) put_row<DT>(a, logits, cols, row, sums);
+    const RowResult r(sums);
+    __shared__ TopLds<T> lds;
+    largest_keys<T>(lds, best, a.top, pieces, keys, [&](int place, Key k) {
+        a.top_logp[row * a.top + place] = k != 0 ? r.logp(logit_of(k)) : -INFINITY;
+        a.top_ids[row * a.top + place] = k != 0 ? column_of(k) : -1;
+    });
 }
 
 // ---- short rows: T lanes hold one in C pieces each ----
@@ -322,14 +340,20 @@ __global__ __launch_bounds__(256) void token_probs_rows_kernel(const void* logit
     const int lane = threadIdx.x % T;
     const long row = (long)blockIdx.x * (256 / T) + threadIdx.x / T;
     if (row >= rows) return;                               // (all lanes of a row)
-    float x[N];
+    const int token = a.tokens[row];
+    u32x4 raw[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int i = (c * T + lane) * P;
-        const u32x4 raw = load16<DT>(logits, row * cols + i, cols - i);
-#pragma unroll
-        for (int e = 0; e < P; ++e) x[c * P + e] = i + e < cols ? element<DT>(raw, e) : -INFINITY;
+        raw[c] = load16<DT>(logits, row * cols + i, cols - i);
     }
+    const bool counts = (unsigned)token < (unsigned)cols;
+    const float mine = counts && lane == 0 ? logit_at<DT>(logits, row * cols + token) : 0.f;
+    float x[N];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < P; ++e) x[c * P + e] = (c * T + lane) * P + e < cols ? element<DT>(raw[c], e) : -INFINITY;
     float most = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
@@ -338,7 +362,7 @@ __global__ __launch_bounds__(256) void token_probs_rows_kernel(const void* logit
     take<N, ENTROPY>(sums, x);
     sums.s = group_reduce<T>(sums.s, add_f32);
     if constexpr (ENTROPY) sums.w = group_reduce<T>(sums.w, add_f32);
-    if (lane == 0) put_row<DT>(a, logits, cols, row, sums);
+    if (lane == 0) put_sums(a, row, counts, mine, sums);
 }
 
 // ---- the gradient ----
@@ -392,41 +416,62 @@ __global__ __launch_bounds__(256) void token_grad_kernel(const void* logits, lon
 
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int TOKEN_THREADS = 512;
-constexpr int64_t LEAST_CHUNK = 4096;
+// Workgroups of 512 lanes for a row (or chunk) of more than 16384 columns, of 256 for shorter ones (us, 512 / 256: 2048 x 8192 bf16 12.9 / 7.3, 256 x 131072 with five alternatives 18.2 / 22.5);
+// rows in chunks where there are fewer of them than compute units, one workgroup a unit (two: 256 x 131072 with alternatives 23.7, one 18.2), of 2048 columns at least.
+constexpr int LONG_THREADS = 512, SHORT_THREADS = 256;
+constexpr int64_t LONG_COLS = 16384, LEAST_CHUNK = 2048;
 constexpr int GRAD_PIECES = 4;                // 16-byte pieces of a lane, long rows
 
-// Chunks of a row: as many as it takes to give every compute unit two workgroups.
 static int64_t token_chunks(int64_t rows, int64_t cols) {
-    const int64_t wanted = ceil_div(2 * device_cu_count(), rows), possible = ceil_div(cols, LEAST_CHUNK);
+    const int64_t wanted = ceil_div(device_cu_count(), rows), possible = ceil_div(cols, LEAST_CHUNK);
     const int64_t n = wanted < possible ? wanted : possible;
     return n < MOST_CHUNKS ? n : MOST_CHUNKS;
 }
-static bool short_rows(int dtype, int64_t cols, int32_t top) { return top == 0 && cols <= 64 * 4 * (dtype == SP_F32 ? 4 : 8); }
+// Whether lanes of one wave hold a row: up to 512 of its 16-byte pieces, 1024 where there are waves enough.  (us, so / a workgroup per row: bf16 16384 x 4000 28.6 / 53, 8192 x 8000 33 / 36.8,
+// 2048 x 8192 12.5 / 9.1, 16 x 4091 4.2 / 3.5 and 2.5 for the join of two chunks, 256 x 8192 6.2 / 3.5; f32 16384 x 2000 23.6 / 32.9, 8192 x 4000 24.2 / 28.4.)
+static bool short_rows(int dtype, int64_t rows, int64_t cols, int32_t top) {
+    const int64_t pieces = ceil_div(cols, dtype == SP_F32 ? 4 : 8);
+    return top == 0 && (pieces <= 512 || (pieces <= 1024 && rows >= 4096));
+}
+
+// Lanes to a row of so many 16-byte pieces, and pieces to a lane: few lanes, so that a wave's reductions are of many rows (us, forward and backward of 65536 x 256 f32 on 64 lanes of one
+// piece 17.3 + 27.6, on 16 of four 11.6 + 21.2; 65536 x 1024 bf16 on 64 of two 32.8 + 50.4, on 16 of eight 30.1 + 46.4).
+template <typename F>
+static int by_pieces(long pieces, const F& f) {
+    typedef std::integral_constant<int, 1> c1;
+    typedef std::integral_constant<int, 4> c4;
+    typedef std::integral_constant<int, 16> c16;
+    typedef std::integral_constant<int, 64> c64;
+    if (pieces <= 4) return f(c4{}, c1{});
+    if (pieces <= 16) return f(c4{}, c4{});
+    if (pieces <= 32) return f(c16{}, std::integral_constant<int, 2>{});
+    if (pieces <= 64) return f(c16{}, c4{});
+    typedef std::integral_constant<int, 8> c8;
+    if (pieces <= 128) return f(c16{}, c8{});
+    if (pieces <= 256) return f(c64{}, c4{});
+    if (pieces <= 512) return f(c64{}, c8{});
+    return f(c64{}, c16{});
+}
 
 template <int DT, bool ENTROPY>
 static int launch_rows(const void* logits, long cols, long rows, const TokenArgs& a, hipStream_t stream) {
-    constexpr int P = PER16<DT>;
-    auto launch = [&](auto t, auto c) {
+    return by_pieces(ceil_div(cols, PER16<DT>), [&](auto t, auto c) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         hipLaunchKernelGGL((token_probs_rows_kernel<DT, T, C, ENTROPY>), dim3((unsigned)ceil_div(rows, 256 / T)), dim3(256), 0, stream, logits, cols, rows, a);
         return check_launch("sp_token_log_probs");
-    };
-    typedef std::integral_constant<int, 1> one;
-    if (cols <= 16 * P) return launch(std::integral_constant<int, 16>{}, one{});
-    if (cols <= 64 * P) return launch(std::integral_constant<int, 64>{}, one{});
-    if (cols <= 128 * P) return launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    return launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    });
 }
 
 template <int DT, bool ENTROPY, bool TOP>
 static int launch_long(const void* logits, long cols, long rows, const TokenArgs& a, hipStream_t stream) {
     const long chunks = token_chunks(rows, cols), piece = PER16<DT>;
     const long chunk_cols = ceil_div(ceil_div(cols, chunks), piece) * piece;
-    hipLaunchKernelGGL((token_probs_kernel<DT, TOKEN_THREADS, ENTROPY, TOP>), dim3((unsigned)(rows * chunks)), dim3(TOKEN_THREADS), 0, stream, logits, cols, (unsigned)chunks,
-                       chunk_cols, a);
+    const dim3 blocks((unsigned)(rows * chunks));
+    if (chunk_cols > LONG_COLS) hipLaunchKernelGGL((token_probs_kernel<DT, LONG_THREADS, ENTROPY, TOP>), blocks, dim3(LONG_THREADS), 0, stream, logits, cols, (unsigned)chunks, chunk_cols, a);
+    else hipLaunchKernelGGL((token_probs_kernel<DT, SHORT_THREADS, ENTROPY, TOP>), blocks, dim3(SHORT_THREADS), 0, stream, logits, cols, (unsigned)chunks, chunk_cols, a);
     if (const int rc = check_launch("sp_token_log_probs"); rc != SP_OK || chunks == 1) return rc;
-    hipLaunchKernelGGL(token_probs_join_kernel<DT>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream, logits, cols, rows, (int)chunks, a);
+    if (TOP) hipLaunchKernelGGL(token_probs_join_top_kernel<DT>, dim3((unsigned)rows), dim3(256), 0, stream, logits, cols, (int)chunks, a);
+    else hipLaunchKernelGGL(token_probs_join_kernel<DT>, dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, stream, logits, cols, rows, (int)chunks, a);
     return check_launch("sp_token_log_probs");
 }
 
@@ -443,17 +488,16 @@ static int launch_grad(const void* logits, long cols, long rows, const TokenGrad
             hipLaunchKernelGGL((token_grad_kernel<DT, T, U, ENTROPY, ST_PLAIN>), dim3((unsigned)blocks), dim3(256), 0, stream, logits, cols, rows, (unsigned)chunks, a);
         return check_launch("sp_token_log_probs_backward");
     };
-    typedef std::integral_constant<int, 1> one;
-    if (cols <= 16 * P) return launch(std::integral_constant<int, 16>{}, one{});
-    if (cols <= 64 * P) return launch(std::integral_constant<int, 64>{}, one{});
+    const long pieces = ceil_div(cols, P);
+    if (pieces <= 256) return by_pieces(pieces, launch);
     return launch(std::integral_constant<int, 256>{}, std::integral_constant<int, GRAD_PIECES>{});
 }
 
 namespace {
 struct TokenKernelNames {
     TokenKernelNames() {
-        register_kernel("token_probs", (const void*)token_probs_kernel<SP_BF16, TOKEN_THREADS, true, false>, TOKEN_THREADS);
-        register_kernel("token_probs_top", (const void*)token_probs_kernel<SP_BF16, TOKEN_THREADS, true, true>, TOKEN_THREADS);
+        register_kernel("token_probs", (const void*)token_probs_kernel<SP_BF16, LONG_THREADS, true, false>, LONG_THREADS);
+        register_kernel("token_probs_top", (const void*)token_probs_kernel<SP_BF16, LONG_THREADS, true, true>, LONG_THREADS);
         register_kernel("token_grad", (const void*)token_grad_kernel<SP_BF16, 256, 4, true, ST_STREAM>, 256);
     }
 } token_kernel_names;
@@ -488,9 +532,9 @@ extern "C" int sp_token_log_probs(int dtype, const void* logits, const int32_t* 
     if (const int rc = token_sizes(__func__, dtype, rows, cols); rc != SP_OK) return rc;
     if (top < 0 || top > MOST_TOP) return fail(SP_ERR_ARG, "sp_token_log_probs: top must be in [0, 32], got %d", top);
     if (top > 0 && (top_logp == nullptr || top_ids == nullptr)) return fail(SP_ERR_NULL, "sp_token_log_probs: top_logp and top_ids are needed for %d alternatives", top);
-    const bool in_registers = short_rows(dtype, cols, top);
+    const bool in_registers = short_rows(dtype, rows, cols, top);
     // a launch holds fewer than 2^32 work items (chunks of a row: only where there are few rows)
-    if (rows >= ((int64_t)1 << 32) / (in_registers ? 64 : TOKEN_THREADS)) return fail(SP_ERR_SHAPE, "sp_token_log_probs: too large");
+    if (rows >= ((int64_t)1 << 32) / (in_registers ? 64 : LONG_THREADS)) return fail(SP_ERR_SHAPE, "sp_token_log_probs: too large");
     const int64_t need = sp_token_log_probs_workspace_bytes(rows, cols, top);
     if (need > 0) {
         SP_REQUIRE_PTR(workspace);
@@ -528,7 +572,8 @@ extern "C" int sp_token_log_probs_backward(int dtype, const void* logits, const 
     SP_OPTIONAL_PTR(d_lse);
     if (const int rc = token_sizes(__func__, dtype, rows, cols); rc != SP_OK) return rc;
     if (d_entropy != nullptr && entropy == nullptr) return fail(SP_ERR_NULL, "sp_token_log_probs_backward: d_entropy needs the entropy");
-    const int64_t p = dtype == SP_F32 ? 4 : 8, lanes = cols <= 16 * p ? 16 : cols <= 64 * p ? 64 : 256 * ceil_div(cols, GRAD_PIECES * 256 * p);
+    const int64_t pieces = ceil_div(cols, dtype == SP_F32 ? 4 : 8);
+    const int64_t lanes = pieces <= 256 ? by_pieces(pieces, [](auto t, auto) { return (int)decltype(t)::value; }) : 256 * ceil_div(pieces, GRAD_PIECES * 256);
     if (rows * lanes > ((int64_t)1 << 32) - 256) return fail(SP_ERR_SHAPE, "sp_token_log_probs_backward: too large");      // (work items of a launch)
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     TokenGradArgs a{};

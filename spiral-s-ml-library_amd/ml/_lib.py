@@ -108,7 +108,7 @@ SIGNATURES = {
     "sp_gemm_abt_scaled": (C.c_int, [C.c_int, C.c_int, C.c_int, _P, _P, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _F, _U32, _P]),
     "sp_gemm_abt_gated": (C.c_int, [C.c_int, C.c_int] + [_P] * 4 + [C.c_int] + [_P] * 4 + [_I64, _I64, _I64, _P]),
     "sp_gemm_abt_gated_backward": (C.c_int, [C.c_int, C.c_int] + [_P] * 4 + [C.c_int] + [_P] * 7 + [_I64, _I64, _I64, _P, _I64, _P]),
-    "sp_gemm_abt_gated_backward_workspace_bytes": (C.c_int64, [C.c_int, _I64, _I64]),
+    "sp_gemm_abt_gated_backward_workspace_bytes": (C.c_int64, [C.c_int, _I64, _I64, _I64]),
     "sp_token_log_probs": (C.c_int, [C.c_int] + [_P] * 5 + [_I32, _P, _P, _I64, _I64, _P, _I64, _P]),
     "sp_token_log_probs_backward": (C.c_int, [C.c_int] + [_P] * 8 + [_I64, _I64, _P]),
     "sp_token_log_probs_workspace_bytes": (C.c_int64, [_I64, _I64, _I32]),

@@ -272,7 +272,7 @@ def matmul_abt_gated_backward(dc, a, b_gate, b_up, kept, activation="silu", want
             return matmul_abt_gated_backward(dc, a, b_gate, b_up, kept, activation, want_input_grad, want_weight_grads)
     da = torch.empty_like(a) if want_input_grad else None
     db_gate, db_up = (torch.empty_like(b_gate) if want_weight_grads else None for _ in range(2))
-    bytes_ = lib.sp_gemm_abt_gated_backward_workspace_bytes(_lib.DTYPES[a.dtype], m, n)
+    bytes_ = lib.sp_gemm_abt_gated_backward_workspace_bytes(_lib.DTYPES[a.dtype], m, n, k)
     workspace = torch.empty((bytes_,), dtype=torch.uint8, device=a.device)                  # of this call alone: calls may overlap
     check(lib.sp_gemm_abt_gated_backward(_lib.DTYPES[a.dtype], _lib.ACTIVATIONS[activation], *addresses, _lib.SP_F8_E4M3 if f8 else _lib.DTYPES[a.dtype], *kept_at,
                                          ptr(da), ptr(db_gate), ptr(db_up), m, n, k, ptr(workspace), bytes_, stream_ptr()))

@@ -135,7 +135,9 @@ def check_backward(M, dc, x, gate, up, kept, act, **want):
 # every tile and its ends: rows, columns and K of one, below, at and above the tiles and K-tiles
 SMALL = [(1, 1, 8), (1, 33, 64), (2, 16, 16), (3, 130, 72), (17, 128, 128), (16, 2667, 1000), (33, 300, 56), (49, 129, 40), (64, 128, 64), (65, 257, 200), (128, 64, 192), (255, 129, 1000),
          (300, 700, 264), (129, 513, 520)]
-LARGE = [(2048, 1664, 64), (2047, 1663, 72), (4096, 1664, 128), (4095, 1663, 200)]     # tiles of 128 and of 256 rows, whole and not
+# every tile where there are many, whole and not
+LARGE = [(2048, 1664, 64), (2047, 1663, 72), (4096, 1664, 128), (4095, 1663, 200), (512, 2736, 1024), (511, 2735, 1000), (1024, 2736, 1024), (1021, 2731, 520), (2048, 4096, 256),
+         (2043, 4099, 264), (1, 4096, 2048), (15, 4099, 2056), (40, 4096, 512), (97, 2737, 1032)]
 
 
 @pytest.mark.parametrize("m,n,k", SMALL + LARGE)
@@ -166,7 +168,10 @@ def test_f32_in_multiples_of_four(M):
 
 # for the gradients: rows, columns and inner width each below, at and above a tile, with every other small
 BACK = [(1, 1, 8), (2, 40, 16), (64, 64, 64), (65, 63, 72), (63, 65, 56), (128, 128, 128), (129, 31, 200), (300, 700, 264), (37, 2667, 1000), (1000, 33, 24),
-        (2048, 40, 1664), (2047, 41, 1672), (4096, 64, 3336), (4095, 65, 3336), (70, 1024, 1664), (71, 1023, 1672), (70, 2048, 3336), (72, 2047, 3336)]
+        (2048, 40, 1664), (2047, 41, 1672), (4096, 64, 3336), (4095, 65, 3336), (70, 1024, 1664), (71, 1023, 1672), (70, 2048, 3336), (72, 2047, 3336),
+        # sums that several workgroups share, on every tile: of long N, of many rows, of both
+        (64, 4096, 256), (65, 5461, 264), (250, 4096, 256), (256, 5461, 2048), (509, 4099, 1032), (2048, 2736, 1024), (2043, 2731, 1032), (4096, 1024, 512), (8191, 257, 136), (8192, 1024, 128),
+        (16384, 256, 256), (4099, 4099, 264), (8192, 1024, 512), (8192, 512, 4096), (16384, 512, 4096), (2048, 5461, 2048), (2048, 512, 4096), (2043, 509, 4104)]
 
 
 @pytest.mark.parametrize("m,n,k", BACK)
