@@ -164,27 +164,38 @@ struct Loader {
     }
 };
 
-template <int TN>
-constexpr int GATED_STRIP_ROW = 16 * TN * 4 + 16;          // bytes; the pad spreads a column over the banks
-
-// COLS columns of 32 rows that stand in a strip of LDS leave as 16-byte pieces, side by side along the rows.
-template <int DT, int COLS, int STRIDE, int POLICY>
-__device__ __forceinline__ void put_strip(const unsigned char* strip, void* C, long pitch, long row0, long rows, long col0, long cols, int lane) {
-    constexpr int P = PER16<DT>, LANES = COLS / P, ROWS = 64 / LANES;
-    static_assert(32 % ROWS == 0, "a strip in whole passes");
-    const int er = lane / LANES, ec = lane % LANES * P;
-#pragma unroll
-    for (int p = 0; p < 32 / ROWS; ++p) {
-        float v[P];
-#pragma unroll
-        for (int h = 0; h < P; h += 4) {
-            const f32x4 q = *reinterpret_cast<const f32x4*>(strip + (p * ROWS + er) * STRIDE + (ec + h) * 4);
-            v[h] = q[0], v[h + 1] = q[1], v[h + 2] = q[2], v[h + 3] = q[3];
-        }
-        const long row = row0 + p * ROWS + er, left = cols - col0 - ec;
-        if (row < rows && left > 0) store16<DT, POLICY>(C, row * pitch + col0 + ec, left, v);
+// A wave's strip of LDS through which sixteen rows of COLS columns leave as 16-byte pieces, side by side along the rows; the pad spreads a column over the banks.
+template <int DT, int COLS>
+struct Strip {
+    static constexpr int E = ELEM_BYTES<DT>, P = PER16<DT>, ROW = COLS * E + 16, BYTES = 16 * ROW, LANES = COLS / P, ROWS = 64 / LANES;
+    // four columns of row fi
+    static __device__ __forceinline__ void set(unsigned char* strip, int fi, int col, const f32x4& v) {
+        if constexpr (E == 4) *reinterpret_cast<f32x4*>(strip + fi * ROW + col * 4) = v;
+        else *reinterpret_cast<u32x2*>(strip + fi * ROW + col * 2) = u32x2{pack_halves<DT>(v[0], v[1]), pack_halves<DT>(v[2], v[3])};
     }
-}
+    template <int POLICY>
+    static __device__ __forceinline__ void put(const unsigned char* strip, void* C, long pitch, long row0, long rows, long col0, long cols, int lane) {
+        const int er = lane / LANES, ec = lane % LANES * P;
+#pragma unroll
+        for (int r = 0; r < 16; r += ROWS) {
+            if (ROWS > 16 && er >= 16) break;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(strip + (r + er) * ROW + ec * E);
+            const long row = row0 + r + er, left = cols - col0 - ec;
+            unsigned char* q = (unsigned char*)C + (row * pitch + col0 + ec) * E;
+            if (row >= rows || left <= 0) continue;
+            if (left >= P) {
+                store_c<POLICY, E>(q, v);
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < P - 1; ++i)
+                if (i < left) {
+                    if constexpr (E == 4) ((unsigned*)q)[i] = v[i];
+                    else ((unsigned short*)q)[i] = (unsigned short)(v[i >> 1] >> (16 * (i & 1)));
+                }
+        }
+    }
+};
 
 // PARTS: the K-tiles are shared out over gridDim.y workgroups, whose sums go to a workspace in f32 (gated_join_kernel adds them up).
 template <int DT, int MODE, int BM, int BN, int WM, int WN, int NS, bool PARTS>
@@ -192,7 +203,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
     constexpr int ES = ELEM_BYTES<DT>, BK = ROW_BYTES / ES, NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     constexpr bool A_ACROSS = MODE == MM_WEIGHTS, B_ACROSS = MODE != MM_FORWARD;
     constexpr int A_BYTES = BM * ROW_BYTES, STAGE = (BM + BN) * ROW_BYTES;
-    static_assert(TM % 2 == 0 && TN % 2 == 0, "strips of two rows of fragments; a gate's fragment and an up's");
+    static_assert(TN % 2 == 0, "a gate's fragment and an up's");
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, fi = lane & 15, fq = lane >> 4;
@@ -311,43 +322,40 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
 
     const long row0 = m0 + wm * WTM;
     if constexpr (MODE != MM_FORWARD) {
-        constexpr int STRIDE = GATED_STRIP_ROW<TN>;
-        static_assert(NW * 32 * STRIDE <= 2 * STAGE, "strips");
-        unsigned char* strip = lds + wave * (32 * STRIDE);
+        constexpr int OT = PARTS ? SP_F32 : DT;
+        typedef Strip<OT, 16 * TN> S;
+        static_assert(NW * S::BYTES <= 2 * STAGE, "strips");
+        unsigned char* strip = lds + wave * S::BYTES;
         const long rows = MODE == MM_INPUT ? g.M : g.N, col0 = n0 + wn * WTN;
         void* const C = PARTS ? g.parts + ((MODE == MM_INPUT ? blockIdx.y : 2 * blockIdx.y + of_up) * rows) * g.K : of_up != 0 ? g.C1 : g.C0;
 #pragma unroll
-        for (int i = 0; i < TM; i += 2) {
+        for (int i = 0; i < TM; ++i) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) *reinterpret_cast<f32x4*>(strip + (16 * k + fi) * STRIDE + (16 * j + 4 * fq) * 4) = acc[i + k][j];
-            if constexpr (PARTS) put_strip<SP_F32, 16 * TN, STRIDE, ST_PLAIN>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
-            else if (g.stream) put_strip<DT, 16 * TN, STRIDE, ST_STREAM>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
-            else put_strip<DT, 16 * TN, STRIDE, ST_PLAIN>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
+            for (int j = 0; j < TN; ++j) S::set(strip, fi, 16 * j + 4 * fq, acc[i][j]);
+            if (!PARTS && g.stream) S::template put<ST_STREAM>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
+            else S::template put<ST_PLAIN>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
         }
     } else {
-        constexpr int PAIRS = TN / 2, STRIDE = GATED_STRIP_ROW<PAIRS>;
-        constexpr int STRIPS = NW * 32 * STRIDE;
+        constexpr int PAIRS = TN / 2;
+        typedef Strip<DT, 16 * PAIRS> S;
+        constexpr int STRIPS = NW * S::BYTES;
         static_assert(STRIPS + 2 * WN * BM * 4 <= 2 * STAGE, "strips, and the largest magnitudes of rows");
-        unsigned char* strip = lds + wave * (32 * STRIDE);
+        unsigned char* strip = lds + wave * S::BYTES;
         const long col0 = n0 + wn * (WTN / 2);
-        // 32 rows of what f(accumulators of a gate, of an up) gives, through the strip
+        // sixteen rows of what f(accumulators of a gate, of an up) gives, through the strip
         auto put = [&](void* C, int i, const auto& f) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int p = 0; p < PAIRS; ++p) {
+                f32x4 v;
 #pragma unroll
-                for (int p = 0; p < PAIRS; ++p) {
-                    f32x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = f(acc[i + k][2 * p][e], acc[i + k][2 * p + 1][e]);
-                    *reinterpret_cast<f32x4*>(strip + (16 * k + fi) * STRIDE + (16 * p + 4 * fq) * 4) = v;
-                }
-            if (g.stream) put_strip<DT, 16 * PAIRS, STRIDE, ST_STREAM>(strip, C, g.N, row0 + 16 * i, g.M, col0, g.N, lane);
-            else put_strip<DT, 16 * PAIRS, STRIDE, ST_PLAIN>(strip, C, g.N, row0 + 16 * i, g.M, col0, g.N, lane);
+                for (int e = 0; e < 4; ++e) v[e] = f(acc[i][2 * p][e], acc[i][2 * p + 1][e]);
+                S::set(strip, fi, 16 * p + 4 * fq, v);
+            }
+            if (g.stream) S::template put<ST_STREAM>(strip, C, g.N, row0 + 16 * i, g.M, col0, g.N, lane);
+            else S::template put<ST_PLAIN>(strip, C, g.N, row0 + 16 * i, g.M, col0, g.N, lane);
         };
 #pragma unroll
-        for (int i = 0; i < TM; i += 2) {
+        for (int i = 0; i < TM; ++i) {
             if (g.activation == SP_ACT_SILU) put(g.C0, i, [](float a, float u) { return gated_activation(a, SP_ACT_SILU) * u; });
             else if (g.activation == SP_ACT_GELU) put(g.C0, i, [](float a, float u) { return gated_activation(a, SP_ACT_GELU) * u; });
             else put(g.C0, i, [](float a, float u) { return gated_activation(a, SP_ACT_RELU) * u; });
@@ -356,8 +364,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
                 put(g.up, i, [](float, float u) { return u; });
             }
         }
-        if constexpr (BN == 256) {
-            if (g.keep != KEEP_F8) return;
+        if (BN == 256 && g.keep == KEEP_F8) {
             // blocks of one row and 128 columns, which are the tile's: the largest magnitudes of a row, as bits, from all lanes and waves that have some of it
             unsigned* const most = reinterpret_cast<unsigned*>(lds + STRIPS);            // [gate, up][wn][row]
             const long pitch = (g.N + 15) / 16 * 16, blocks = (g.N + QB - 1) / QB;
@@ -377,35 +384,31 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
                     if (fq == 0) most[(of * WN + wn) * BM + wm * WTM + 16 * i + fi] = m;
                 }
             __syncthreads();
-            constexpr int BYTES = 16 * PAIRS, LANES = BYTES / 16, ROWS = 64 / LANES, STRIDE8 = BYTES + 16;     // of a strip of bytes
-            static_assert(32 % ROWS == 0 || ROWS > 32, "a strip in whole passes");
+            constexpr int LANES = PAIRS, ROWS = 64 / LANES, STRIDE8 = 16 * PAIRS + 16;     // of a strip of bytes, 16 a lane
+            static_assert(16 * STRIDE8 <= S::BYTES, "a strip of bytes");
 #pragma unroll
-            for (int i = 0; i < TM; i += 2)
+            for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int of = 0; of < 2; ++of) {
                     unsigned char* const q = (unsigned char*)(of != 0 ? g.up : g.gate);
-                    float* const scales = of != 0 ? g.up_scale : g.gate_scale;
+                    const int in_tile = wm * WTM + 16 * i + fi;
+                    unsigned m = most[of * WN * BM + in_tile];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int row = wm * WTM + 16 * (i + k) + fi;
-                        unsigned m = most[of * WN * BM + row];
+                    for (int w = 1; w < WN; ++w) m = max_u32(m, most[(of * WN + w) * BM + in_tile]);
+                    BlockScale s;
+                    s.set<SP_F8_E4M3>(m);
+                    if (wn == 0 && fq == 0 && m0 + in_tile < g.M) (of != 0 ? g.up_scale : g.gate_scale)[(m0 + in_tile) * blocks + tn] = s.scale;
 #pragma unroll
-                        for (int w = 1; w < WN; ++w) m = max_u32(m, most[(of * WN + w) * BM + row]);
-                        BlockScale s;
-                        s.set<SP_F8_E4M3>(m);
-                        if (wn == 0 && fq == 0 && m0 + row < g.M) scales[(m0 + row) * blocks + tn] = s.scale;
-#pragma unroll
-                        for (int p = 0; p < PAIRS; ++p) {
-                            const f32x4& v = acc[i + k][2 * p + of];
-                            const unsigned bytes = first_bytes(pack_f8<SP_F8_E4M3>(s(v[0]), s(v[1]), s(v[2]), s(v[3])), left - 16 * p);
-                            *reinterpret_cast<unsigned*>(strip + (16 * k + fi) * STRIDE8 + 16 * p + 4 * fq) = bytes;
-                        }
+                    for (int p = 0; p < PAIRS; ++p) {
+                        const f32x4& v = acc[i][2 * p + of];
+                        *reinterpret_cast<unsigned*>(strip + fi * STRIDE8 + 16 * p + 4 * fq) = first_bytes(pack_f8<SP_F8_E4M3>(s(v[0]), s(v[1]), s(v[2]), s(v[3])), left - 16 * p);
                     }
                     const int er = lane / LANES, ec = lane % LANES * 16;
 #pragma unroll
-                    for (int r = er; r < 32; r += ROWS) {
-                        const u32x4 v = *reinterpret_cast<const u32x4*>(strip + r * STRIDE8 + ec);
-                        const long row = row0 + 16 * i + r;
+                    for (int r = 0; r < 16; r += ROWS) {
+                        if (ROWS > 16 && er >= 16) break;
+                        const u32x4 v = *reinterpret_cast<const u32x4*>(strip + (r + er) * STRIDE8 + ec);
+                        const long row = row0 + 16 * i + r + er;
                         if (row < g.M && col0 + ec < pitch) *reinterpret_cast<u32x4*>(q + row * pitch + col0 + ec) = v;
                     }
                 }
@@ -705,7 +708,8 @@ static int launch_split(const char* what, GatedArgs g, int parts, hipStream_t st
 
 // ---- which kernel ----
 // Estimated time of a product in us, without the launch: workgroups in rounds of as many as a unit's LDS holds at a time, each nk K-tiles (a quarter of them, where four waves share
-// them) plus an overhead; n workgroups on a unit take n times the work of a K-tile, and never less than what a lone one waits for.  Partial sums are written, read and joined.
+// them) plus an overhead; n workgroups on a unit take n times the work of a K-tile, and never less than what a lone one waits for.  Partial sums are written, read and joined, at 4 TB/s (at 8, as
+// they were fitted, 5008 x 2048 x 5461 took three of them: the gradient of A alone 281 -> 263 us, but the whole step, which the part's power limits, 657 -> 668).
 // Fitted on what every kernel took on 99 forward, 62 and 62 backward shapes, from 1 x 512 x 1365 to 16384 x 4096 x 512; the one it picks is on the mean 2 % behind the fastest forward
 // (3 with 8-bit blocks), 4 for the gradient of A and 2 for the weights'.  More tiles (64 x 128, 128 x 256 in two stages, 16 x 64 and 64 x 64 in four parts) were worth less than a hundredth.
 struct MmCost {
@@ -744,14 +748,14 @@ static MmChoice cheapest(const MmCost (&menu)[N], int mode, bool f32, long M, lo
     for (const MmCost& c : menu) {
         const double tiles = (double)gated_ceil(rows, c.bm) * (double)gated_ceil(cols, c.bn) * twice;
         if (tiles * 512 >= 4294967296.0) continue;         // (a launch holds fewer than 2^32 work items)
-        for (int parts = 1; parts <= 16; parts *= 2) {
+        for (int parts = 1; parts <= 16; ++parts) {
             if (parts > 1 && (mode == MM_FORWARD || tiles * parts > 2.0 * cus || nk < 4 * parts)) break;
             const double groups = tiles * parts, round = (double)cus * c.per_unit;
             const long mine = gated_ceil(gated_ceil(nk, parts), c.split ? 4 : 1);
             auto of = [&](double n) { return mine * (n * c.work > c.lone ? n * c.work : (double)c.lone) + c.overhead; };
             const double full = (double)(int64_t)(groups / round), rest = groups - full * round;
             double us = full * of(c.per_unit) + (rest > 0 ? of((double)(int64_t)((rest + cus - 1) / cus)) : 0);
-            if (parts > 1) us += 6 + (double)rows * cols * twice * (8.0 * parts + (f32 ? 4 : 2)) * 1e-6 / 8;
+            if (parts > 1) us += 6 + (double)rows * cols * twice * (8.0 * parts + (f32 ? 4 : 2)) * 1e-6 / 4;
             if (!any || us < best_us) {
                 any = true;
                 best_us = us;
