@@ -718,14 +718,15 @@ struct MmCost {
     bool split;
     float lone, work, overhead;
 };
-enum { SPLIT_16, SPLIT_32, TILE_64, TILE_64_BLOCKS, TILE_128, TILE_128_WIDE, TILE_256 };
+enum { SPLIT_16, SPLIT_32, TILE_32_BLOCKS, TILE_64, TILE_64_BLOCKS, TILE_128, TILE_128_WIDE, TILE_256 };
 static const MmCost kForward16[] = {{SPLIT_16, 16, 16, 3, true, 0.156f, 0.278f, 2.55f}, {SPLIT_32, 32, 16, 2, true, 0.336f, 0.387f, 2.65f}, {TILE_64, 64, 32, 2, false, 0.227f, 0.183f, 2.57f},
                                     {TILE_128, 128, 64, 1, false, 0.437f, 0.386f, 3.84f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 4.67f}, {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 5.95f}};
 static const MmCost kForward32[] = {{SPLIT_16, 16, 16, 3, true, 0.587f, 0.354f, 2.47f}, {SPLIT_32, 32, 16, 2, true, 0.587f, 0.632f, 3.2f}, {TILE_64, 64, 32, 2, false, 0.633f, 0.572f, 1.39f},
                                     {TILE_128, 128, 64, 1, false, 1.918f, 0.386f, 3.7f}};
 // tiles that hold whole blocks of 128 columns of both factors
-static const MmCost kBlocks16[] = {{TILE_64_BLOCKS, 64, 128, 1, false, 0.541f, 0.541f, 3.75f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 4.67f}, {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 5.95f}};
-static const MmCost kBlocks32[] = {{TILE_64_BLOCKS, 64, 128, 1, false, 1.972f, 1.039f, 4.06f}};
+static const MmCost kBlocks16[] = {{TILE_32_BLOCKS, 32, 128, 1, false, 0.41f, 0.41f, 4.8f}, {TILE_64_BLOCKS, 64, 128, 1, false, 0.46f, 0.46f, 5.3f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 6.7f},
+                                   {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 8.f}};
+static const MmCost kBlocks32[] = {{TILE_32_BLOCKS, 32, 128, 1, false, 1.05f, 1.05f, 5.f}, {TILE_64_BLOCKS, 64, 128, 1, false, 1.972f, 1.039f, 6.f}};
 static const MmCost kInput16[] = {{SPLIT_32, 32, 64, 1, true, 0.572f, 0.318f, 2.47f}, {TILE_64, 64, 64, 2, false, 0.225f, 0.201f, 2.96f}, {TILE_128, 128, 128, 1, false, 0.464f, 0.464f, 3.77f},
                                   {TILE_128_WIDE, 128, 256, 1, false, 0.652f, 0.652f, 4.51f}, {TILE_256, 256, 256, 1, false, 1.112f, 0.4f, 5.2f}};
 static const MmCost kWeights16[] = {{TILE_64, 64, 64, 2, false, 0.171f, 0.218f, 2.64f}, {TILE_128, 128, 128, 1, false, 0.538f, 0.424f, 4.11f}, {TILE_128_WIDE, 128, 256, 1, false, 0.766f, 0.1f, 5.53f},
@@ -781,8 +782,9 @@ static int gated_forward(const GatedArgs& g, hipStream_t stream) {
         case SPLIT_16: return launch_split<DT, MM_FORWARD, 1, 2, 2>(what, g, 1, stream);
         case SPLIT_32: return launch_split<DT, MM_FORWARD, 2, 2, 2>(what, g, 1, stream);
         case TILE_64: return launch_mm<DT, MM_FORWARD, 64, 64, 2, 2, 4>(what, g, 1, stream);
-        case TILE_64_BLOCKS: return launch_mm<DT, MM_FORWARD, 64, 256, 2, 2, 3>(what, g, 1, stream);
-        case TILE_128: return launch_mm<DT, MM_FORWARD, 128, 128, 2, 2, 4>(what, g, 1, stream);
+        case TILE_32_BLOCKS: return launch_mm<DT, MM_FORWARD, 32, 256, 1, 4, 3>(what, g, 1, stream);
+        case TILE_64_BLOCKS: return launch_mm<DT, MM_FORWARD, 64, 256, 2, 4, 3>(what, g, 1, stream);
+        case TILE_128: return launch_mm<DT, MM_FORWARD, 128, 128, 2, F32 ? 2 : 4, 4>(what, g, 1, stream);
     }
     if constexpr (!F32) {
         if (id == TILE_128_WIDE) return launch_mm<DT, MM_FORWARD, 128, 256, 4, 2, 3>(what, g, 1, stream);
@@ -803,7 +805,7 @@ static int gated_backward_product(const GatedArgs& g, hipStream_t stream) {
         return launch_mm<DT, MODE, 128, 128, 2, 2, 2>(what, g, c.parts, stream);
     } else {
         if (c.id == TILE_64) return launch_mm<DT, MODE, 64, 64, 2, 2, 4>(what, g, c.parts, stream);
-        if (c.id == TILE_128) return launch_mm<DT, MODE, 128, 128, 2, 2, 4>(what, g, c.parts, stream);
+        if (c.id == TILE_128) return launch_mm<DT, MODE, 128, 128, 2, 4, 4>(what, g, c.parts, stream);
         if (c.id == TILE_128_WIDE) return launch_mm<DT, MODE, 128, 256, 2, 4, 3>(what, g, c.parts, stream);
         return launch_mm<DT, MODE, 256, 256, 2, 4, 2>(what, g, c.parts, stream);
     }
