@@ -309,28 +309,53 @@ __global__ __launch_bounds__(256) void token_probs_join_kernel(const void* logit
     const Sums sums = join_chunks(a, row, chunks, threadIdx.x & 63);
     if ((threadIdx.x & 63) == 0) put_row<DT>(a, logits, cols, row, sums);
 }
-// The same with the alternatives, a workgroup for a row: every chunk has left its own, and the row's are among them.
+// The same with the alternatives, a workgroup for a row: every chunk has left its own, largest first, and the row's are among them.
+// With `deep` of them a chunk, the (top / deep)-th largest of the chunks' deep-th ones has `top` above it or equal, so nothing below it is taken; `deep` is such that this is one of the
+// larger half (of 34 chunks, for 32 alternatives: the 16th of their second ones, with some 60 keys left; the 32nd of their first has 100).
 template <int DT>
 __global__ __launch_bounds__(256) void token_probs_join_top_kernel(const void* logits, long cols, int chunks, const TokenArgs a) {
     constexpr int T = 256;
     const int tid = threadIdx.x;
     const long row = blockIdx.x;
     const int n = chunks * a.top;
-    auto keys = [&](int lane, int piece, const auto& f) {
-        const int i = piece * T + lane;
-        f(i < n ? key_of(a.part_top[row * n + i], a.part_ids[row * n + i]) : (Key)0);
-    };
-    const int pieces = (n + T - 1) / T;
-    Key best = 0;
-    for (int p = 0; p < pieces; ++p) keys(tid, p, [&](Key k) { best = larger(best, k); });
+    __shared__ Key keys[MOST_CHUNKS * MOST_TOP], list[MOST_CHUNKS * MOST_TOP];
+    __shared__ Key least;
+    __shared__ int count;
+    for (int i = tid; i < n; i += T) keys[i] = key_of(a.part_top[row * n + i], a.part_ids[row * n + i]);
+    if (tid == 0) {
+        least = 1;
+        count = 0;
+    }
     const Sums sums = join_chunks(a, row, chunks, tid & 63);           // (every wave for itself)
     if (tid == 0) put_row<DT>(a, logits, cols, row, sums);
     const RowResult r(sums);
-    __shared__ TopLds<T> lds;
-    largest_keys<T>(lds, best, a.top, pieces, keys, [&](int place, Key k) {
+    __syncthreads();
+    if (tid < chunks) {
+        int deep = 1;
+        while (deep < a.top && 2 * ((a.top + deep - 1) / deep) > chunks) ++deep;
+        const int place = (a.top + deep - 1) / deep - 1;
+        const Key mine = keys[tid * a.top + deep - 1];
+        int above = 0;
+        for (int c = 0; c < chunks; ++c) above += keys[c * a.top + deep - 1] > mine ? 1 : 0;
+        if (mine != 0 && above == place) least = mine;     // (keys differ, but for 0)
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += T) {
+        const Key k = keys[i];
+        if (k >= least) list[atomicAdd(&count, 1)] = k;
+    }
+    __syncthreads();
+    auto put = [&](int place, Key k) {
         a.top_logp[row * a.top + place] = k != 0 ? r.logp(logit_of(k)) : -INFINITY;
         a.top_ids[row * a.top + place] = k != 0 ? column_of(k) : -1;
-    });
+    };
+    for (int i = tid; i < count; i += T) {
+        const Key k = list[i];
+        int above = 0;
+        for (int j = 0; j < count; ++j) above += list[j] > k ? 1 : 0;
+        if (above < a.top) put(above, k);
+    }
+    for (int i = count + tid; i < a.top; i += T) put(i, (Key)0);
 }
 
 // ---- short rows: T lanes hold one in C pieces each ----
