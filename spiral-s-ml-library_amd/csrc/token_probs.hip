@@ -445,7 +445,7 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // rows in chunks where there are fewer of them than compute units, one workgroup a unit (two: 256 x 131072 with alternatives 23.7, one 18.2), of 2048 columns at least.
 constexpr int LONG_THREADS = 512, SHORT_THREADS = 256;
 constexpr int64_t LONG_COLS = 16384, LEAST_CHUNK = 2048;
-constexpr int GRAD_PIECES = 4;                // 16-byte pieces of a lane, long rows
+constexpr int GRAD_PIECES = 4, FEW_PIECES = 256;    // the gradient: 16-byte pieces of a lane of a long row, of a short row
 
 static int64_t token_chunks(int64_t rows, int64_t cols) {
     const int64_t wanted = ceil_div(device_cu_count(), rows), possible = ceil_div(cols, LEAST_CHUNK);
@@ -454,33 +454,35 @@ static int64_t token_chunks(int64_t rows, int64_t cols) {
 }
 // Whether lanes of one wave hold a row: up to 512 of its 16-byte pieces, 1024 where there are waves enough.  (us, so / a workgroup per row: bf16 16384 x 4000 28.6 / 53, 8192 x 8000 33 / 36.8,
 // 2048 x 8192 12.5 / 9.1, 16 x 4091 4.2 / 3.5 and 2.5 for the join of two chunks, 256 x 8192 6.2 / 3.5; f32 16384 x 2000 23.6 / 32.9, 8192 x 4000 24.2 / 28.4.)
+constexpr int MANY_PIECES = 1024;
 static bool short_rows(int dtype, int64_t rows, int64_t cols, int32_t top) {
     const int64_t pieces = ceil_div(cols, dtype == SP_F32 ? 4 : 8);
-    return top == 0 && (pieces <= 512 || (pieces <= 1024 && rows >= 4096));
+    return top == 0 && (pieces <= 512 || (pieces <= MANY_PIECES && rows >= 4096));
 }
 
 // Lanes to a row of so many 16-byte pieces, and pieces to a lane: few lanes, so that a wave's reductions are of many rows (us, forward and backward of 65536 x 256 f32 on 64 lanes of one
 // piece 17.3 + 27.6, on 16 of four 11.6 + 21.2; 65536 x 1024 bf16 on 64 of two 32.8 + 50.4, on 16 of eight 30.1 + 46.4).
-template <typename F>
+template <int MOST, typename F>
 static int by_pieces(long pieces, const F& f) {
-    typedef std::integral_constant<int, 1> c1;
     typedef std::integral_constant<int, 4> c4;
+    typedef std::integral_constant<int, 8> c8;
     typedef std::integral_constant<int, 16> c16;
     typedef std::integral_constant<int, 64> c64;
-    if (pieces <= 4) return f(c4{}, c1{});
+    if (pieces <= 4) return f(c4{}, std::integral_constant<int, 1>{});
     if (pieces <= 16) return f(c4{}, c4{});
     if (pieces <= 32) return f(c16{}, std::integral_constant<int, 2>{});
     if (pieces <= 64) return f(c16{}, c4{});
-    typedef std::integral_constant<int, 8> c8;
     if (pieces <= 128) return f(c16{}, c8{});
-    if (pieces <= 256) return f(c64{}, c4{});
-    if (pieces <= 512) return f(c64{}, c8{});
-    return f(c64{}, c16{});
+    if constexpr (MOST > 256) {
+        if (pieces > 512) return f(c64{}, c16{});
+        if (pieces > 256) return f(c64{}, c8{});
+    }
+    return f(c64{}, c4{});
 }
 
 template <int DT, bool ENTROPY>
 static int launch_rows(const void* logits, long cols, long rows, const TokenArgs& a, hipStream_t stream) {
-    return by_pieces(ceil_div(cols, PER16<DT>), [&](auto t, auto c) {
+    return by_pieces<MANY_PIECES>(ceil_div(cols, PER16<DT>), [&](auto t, auto c) {
         constexpr int T = decltype(t)::value, C = decltype(c)::value;
         hipLaunchKernelGGL((token_probs_rows_kernel<DT, T, C, ENTROPY>), dim3((unsigned)ceil_div(rows, 256 / T)), dim3(256), 0, stream, logits, cols, rows, a);
         return check_launch("sp_token_log_probs");
@@ -514,7 +516,7 @@ static int launch_grad(const void* logits, long cols, long rows, const TokenGrad
         return check_launch("sp_token_log_probs_backward");
     };
     const long pieces = ceil_div(cols, P);
-    if (pieces <= 256) return by_pieces(pieces, launch);
+    if (pieces <= FEW_PIECES) return by_pieces<FEW_PIECES>(pieces, launch);
     return launch(std::integral_constant<int, 256>{}, std::integral_constant<int, GRAD_PIECES>{});
 }
 
@@ -598,7 +600,7 @@ extern "C" int sp_token_log_probs_backward(int dtype, const void* logits, const 
     if (const int rc = token_sizes(__func__, dtype, rows, cols); rc != SP_OK) return rc;
     if (d_entropy != nullptr && entropy == nullptr) return fail(SP_ERR_NULL, "sp_token_log_probs_backward: d_entropy needs the entropy");
     const int64_t pieces = ceil_div(cols, dtype == SP_F32 ? 4 : 8);
-    const int64_t lanes = pieces <= 256 ? by_pieces(pieces, [](auto t, auto) { return (int)decltype(t)::value; }) : 256 * ceil_div(pieces, GRAD_PIECES * 256);
+    const int64_t lanes = pieces <= FEW_PIECES ? by_pieces<FEW_PIECES>(pieces, [](auto t, auto) { return (int)decltype(t)::value; }) : 256 * ceil_div(pieces, GRAD_PIECES * 256);
     if (rows * lanes > ((int64_t)1 << 32) - 256) return fail(SP_ERR_SHAPE, "sp_token_log_probs_backward: too large");      // (work items of a launch)
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     TokenGradArgs a{};
