@@ -30,7 +30,7 @@ struct GatedArgs {
     long half;                    // N': columns of either half of the workspace, N rounded up to a whole K-tile, zeros behind N
     int activation, keep;
     int tiles_m, tiles_n, group_m;
-    int stream;                   // C does not stay in the caches
+    int stream;                   // C does not stay in the caches; bit 1: nor do gate and up
     float* parts;                 // backward: partial sums of several workgroups, all of a result (of both weights' gradients) each
 };
 
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
         unsigned char* strip = lds + wave * S::BYTES;
         const long col0 = n0 + wn * (WTN / 2);
         // sixteen rows of what f(accumulators of a gate, of an up) gives, through the strip
-        auto put = [&](void* C, int i, const auto& f) {
+        auto put = [&](void* C, int stream, int i, const auto& f) {
 #pragma unroll
             for (int p = 0; p < PAIRS; ++p) {
                 f32x4 v;
@@ -351,17 +351,17 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
                 for (int e = 0; e < 4; ++e) v[e] = f(acc[i][2 * p][e], acc[i][2 * p + 1][e]);
                 S::set(strip, fi, 16 * p + 4 * fq, v);
             }
-            if (g.stream) S::template put<ST_STREAM>(strip, C, g.N, row0 + 16 * i, g.M, col0, g.N, lane);
+            if (stream) S::template put<ST_STREAM>(strip, C, g.N, row0 + 16 * i, g.M, col0, g.N, lane);
             else S::template put<ST_PLAIN>(strip, C, g.N, row0 + 16 * i, g.M, col0, g.N, lane);
         };
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            if (g.activation == SP_ACT_SILU) put(g.C0, i, [](float a, float u) { return gated_activation(a, SP_ACT_SILU) * u; });
-            else if (g.activation == SP_ACT_GELU) put(g.C0, i, [](float a, float u) { return gated_activation(a, SP_ACT_GELU) * u; });
-            else put(g.C0, i, [](float a, float u) { return gated_activation(a, SP_ACT_RELU) * u; });
+            if (g.activation == SP_ACT_SILU) put(g.C0, g.stream, i, [](float a, float u) { return gated_activation(a, SP_ACT_SILU) * u; });
+            else if (g.activation == SP_ACT_GELU) put(g.C0, g.stream, i, [](float a, float u) { return gated_activation(a, SP_ACT_GELU) * u; });
+            else put(g.C0, g.stream, i, [](float a, float u) { return gated_activation(a, SP_ACT_RELU) * u; });
             if (g.keep == KEEP_WHOLE) {
-                put(g.gate, i, [](float a, float) { return a; });
-                put(g.up, i, [](float, float u) { return u; });
+                put(g.gate, g.stream & 2, i, [](float a, float) { return a; });
+                put(g.up, g.stream & 2, i, [](float, float u) { return u; });
             }
         }
         if (BN == 256 && g.keep == KEEP_F8) {
@@ -721,8 +721,7 @@ struct MmCost {
 enum { SPLIT_16, SPLIT_32, TILE_32_BLOCKS, TILE_64, TILE_64_BLOCKS, TILE_128, TILE_128_WIDE, TILE_256 };
 static const MmCost kForward16[] = {{SPLIT_16, 16, 16, 3, true, 0.156f, 0.278f, 2.55f}, {SPLIT_32, 32, 16, 2, true, 0.336f, 0.387f, 2.65f}, {TILE_64, 64, 32, 2, false, 0.227f, 0.183f, 2.57f},
                                     {TILE_128, 128, 64, 1, false, 0.437f, 0.386f, 3.84f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 4.67f}, {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 5.95f}};
-static const MmCost kForward32[] = {{SPLIT_16, 16, 16, 3, true, 0.587f, 0.354f, 2.47f}, {SPLIT_32, 32, 16, 2, true, 0.587f, 0.632f, 3.2f}, {TILE_64, 64, 32, 2, false, 0.633f, 0.572f, 1.39f},
-                                    {TILE_128, 128, 64, 1, false, 1.918f, 0.386f, 3.7f}};
+static const MmCost kForward32[] = {{SPLIT_16, 16, 16, 3, true, 0.587f, 0.354f, 2.47f}, {SPLIT_32, 32, 16, 2, true, 0.587f, 0.632f, 3.2f}, {TILE_64, 64, 32, 5, false, 0.633f, 0.54f, 2.4f}};
 // tiles that hold whole blocks of 128 columns of both factors
 static const MmCost kBlocks16[] = {{TILE_32_BLOCKS, 32, 128, 1, false, 0.41f, 0.41f, 4.8f}, {TILE_64_BLOCKS, 64, 128, 1, false, 0.46f, 0.46f, 5.3f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 6.7f},
                                    {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 8.f}};
@@ -781,12 +780,12 @@ static int gated_forward(const GatedArgs& g, hipStream_t stream) {
     switch (id) {
         case SPLIT_16: return launch_split<DT, MM_FORWARD, 1, 2, 2>(what, g, 1, stream);
         case SPLIT_32: return launch_split<DT, MM_FORWARD, 2, 2, 2>(what, g, 1, stream);
-        case TILE_64: return launch_mm<DT, MM_FORWARD, 64, 64, 2, 2, 4>(what, g, 1, stream);
+        case TILE_64: return launch_mm<DT, MM_FORWARD, 64, 64, 2, 2, F32 ? 2 : 4>(what, g, 1, stream);
         case TILE_32_BLOCKS: return launch_mm<DT, MM_FORWARD, 32, 256, 1, 4, 3>(what, g, 1, stream);
         case TILE_64_BLOCKS: return launch_mm<DT, MM_FORWARD, 64, 256, 2, 4, 3>(what, g, 1, stream);
-        case TILE_128: return launch_mm<DT, MM_FORWARD, 128, 128, 2, F32 ? 2 : 4, 4>(what, g, 1, stream);
     }
     if constexpr (!F32) {
+        if (id == TILE_128) return launch_mm<DT, MM_FORWARD, 128, 128, 2, 4, 4>(what, g, 1, stream);
         if (id == TILE_128_WIDE) return launch_mm<DT, MM_FORWARD, 128, 256, 4, 2, 3>(what, g, 1, stream);
         return launch_mm<DT, MM_FORWARD, 256, 256, 4, 2, 2>(what, g, 1, stream);
     }
@@ -872,7 +871,9 @@ extern "C" int sp_gemm_abt_gated(int dtype, int activation, const void* A, const
     GatedArgs g{};
     g.A = (const unsigned char*)A; g.B0 = (const unsigned char*)B_gate; g.B1 = (const unsigned char*)B_up; g.C0 = C; g.gate = gate; g.up = up;
     g.gate_scale = gate_scale; g.up_scale = up_scale; g.M = M; g.N = N; g.K = K; g.activation = activation; g.keep = f8 ? KEEP_F8 : keeps ? KEEP_WHOLE : KEEP_NONE;
-    g.stream = M * N * (dtype == SP_F32 ? 4 : 2) > (int64_t)32 << 20;
+    // what does not stay in the caches (32 MiB of L2) is streamed past them, gate and up only where a row is of whole lines (5008 x 2048 x 5461 bf16: 205 us, 225 streamed)
+    const int64_t pitch = N * (dtype == SP_F32 ? 4 : 2);
+    g.stream = M * pitch <= (int64_t)32 << 20 ? 0 : pitch % 128 == 0 ? 3 : 1;
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == SP_F32) return gated_forward<SP_F32>(g, st);
     if (dtype == SP_F16) return gated_forward<SP_F16>(g, st);
