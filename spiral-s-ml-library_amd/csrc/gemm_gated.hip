@@ -18,6 +18,8 @@ namespace sp {
 
 enum { MM_FORWARD, MM_INPUT, MM_WEIGHTS };
 enum { KEEP_NONE, KEEP_WHOLE, KEEP_F8 };
+template <int DT>
+constexpr int STAGES_64 = DT == SP_F32 ? 2 : 4;            // of tiles of 64 x 64: of f32, whose MFMAs take longest, five workgroups to a unit
 constexpr unsigned ROTATE = 7;      // odd: it meets every one of a power of two of K-tiles
 
 struct GatedArgs {
@@ -197,9 +199,9 @@ struct Strip {
     }
 };
 
-// PARTS: the K-tiles are shared out over gridDim.y workgroups, whose sums go to a workspace in f32 (gated_join_kernel adds them up).
-template <int DT, int MODE, int BM, int BN, int WM, int WN, int NS, bool PARTS>
-__global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArgs g) {
+// One tile, or this workgroup's share of its K-tiles: with parts > 1 the sums go to a workspace in f32 (gated_join_kernel adds them up).
+template <int DT, int MODE, int BM, int BN, int WM, int WN, int NS>
+__device__ __forceinline__ void gated_mm(const GatedArgs& g, unsigned block, unsigned part, unsigned parts) {
     constexpr int ES = ELEM_BYTES<DT>, BK = ROW_BYTES / ES, NW = WM * WN, WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
     constexpr bool A_ACROSS = MODE == MM_WEIGHTS, B_ACROSS = MODE != MM_FORWARD;
     constexpr int A_BYTES = BM * ROW_BYTES, STAGE = (BM + BN) * ROW_BYTES;
@@ -208,7 +210,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, fi = lane & 15, fq = lane >> 4;
     int tm, tn;
-    gated_tile_of_block(blockIdx.x, g.tiles_m, g.tiles_n, g.group_m, tm, tn);
+    gated_tile_of_block(block, g.tiles_m, g.tiles_n, g.group_m, tm, tn);
 
     // where the tile lies, and the operands' first rows or columns of it
     const int of_up = MODE == MM_WEIGHTS && tm >= g.tiles_m / 2 ? 1 : 0;
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
 
     // the K-tiles in their order, partial ones first: where number s begins in A and in B
     const int whole = (int)(inner / BK), partial = tail != 0 ? (MODE == MM_INPUT ? 2 : 1) : 0, all = whole * (MODE == MM_INPUT ? 2 : 1) + partial;
-    const int first = PARTS ? (int)((long)all * blockIdx.y / gridDim.y) : 0, nk = PARTS ? (int)((long)all * (blockIdx.y + 1) / gridDim.y) - first : all;
+    const int first = (int)((unsigned)all * part / parts), nk = (int)((unsigned)all * (part + 1) / parts) - first;
     const unsigned char *at_a, *at_b;
     auto locate = [&](int s) {
         long t;
@@ -242,6 +244,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
         }
         at_a = uniform_ptr(at_a);
         at_b = uniform_ptr(at_b);
+    };
+    // from one whole K-tile to number s
+    const long step_a = A_ACROSS ? BK * pitch_a : (long)ROW_BYTES, step_b = B_ACROSS ? BK * pitch_b : (long)ROW_BYTES;
+    auto advance = [&](int s) {
+        at_a += step_a;
+        at_b += step_b;
+        if (MODE == MM_INPUT && s == partial + whole) locate(s);
     };
     const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds + wave * 1024);
     constexpr int NIA = la.NI, NI = la.NI + lb.NI;
@@ -286,7 +295,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
     auto tile = [&](int kt, auto more) {
         constexpr bool MORE = decltype(more)::value;
         const unsigned released = stage;
-        if constexpr (MORE) locate(first + kt + NS);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
@@ -313,8 +321,10 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
                 stage += step;
             }
         }
+        if constexpr (MORE) advance(first + kt + NS + 1);
     };
     int kt = 0;
+    if (nk > NS) locate(first + NS);                       // (whole: partial tiles are two at most)
     for (; kt + NS < nk; ++kt) tile(kt, std::true_type{});
     for (; kt < nk; ++kt) tile(kt, std::false_type{});
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -322,19 +332,21 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
 
     const long row0 = m0 + wm * WTM;
     if constexpr (MODE != MM_FORWARD) {
-        constexpr int OT = PARTS ? SP_F32 : DT;
-        typedef Strip<OT, 16 * TN> S;
-        static_assert(NW * S::BYTES <= 2 * STAGE, "strips");
-        unsigned char* strip = lds + wave * S::BYTES;
+        static_assert(NW * Strip<SP_F32, 16 * TN>::BYTES <= 2 * STAGE, "strips");
         const long rows = MODE == MM_INPUT ? g.M : g.N, col0 = n0 + wn * WTN;
-        void* const C = PARTS ? g.parts + ((MODE == MM_INPUT ? blockIdx.y : 2 * blockIdx.y + of_up) * rows) * g.K : of_up != 0 ? g.C1 : g.C0;
+        auto put = [&](void* C, auto type, auto policy) {
+            typedef Strip<decltype(type)::value, 16 * TN> S;
+            unsigned char* strip = lds + wave * S::BYTES;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
+            for (int i = 0; i < TM; ++i) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) S::set(strip, fi, 16 * j + 4 * fq, acc[i][j]);
-            if (!PARTS && g.stream) S::template put<ST_STREAM>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
-            else S::template put<ST_PLAIN>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
-        }
+                for (int j = 0; j < TN; ++j) S::set(strip, fi, 16 * j + 4 * fq, acc[i][j]);
+                S::template put<decltype(policy)::value>(strip, C, g.K, row0 + 16 * i, rows, col0, g.K, lane);
+            }
+        };
+        if (parts > 1) put(g.parts + ((MODE == MM_INPUT ? part : 2 * part + of_up) * rows) * g.K, std::integral_constant<int, SP_F32>{}, std::integral_constant<int, ST_PLAIN>{});
+        else if (g.stream) put(of_up != 0 ? g.C1 : g.C0, std::integral_constant<int, DT>{}, std::integral_constant<int, ST_STREAM>{});
+        else put(of_up != 0 ? g.C1 : g.C0, std::integral_constant<int, DT>{}, std::integral_constant<int, ST_PLAIN>{});
     } else {
         constexpr int PAIRS = TN / 2;
         typedef Strip<DT, 16 * PAIRS> S;
@@ -416,12 +428,42 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_mm_kernel(const GatedArg
     }
 }
 
+template <int DT, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(WM* WN * 64, 2) void gated_forward_kernel(const GatedArgs g) {
+    gated_mm<DT, MM_FORWARD, BM, BN, WM, WN, NS>(g, blockIdx.x, 0, 1);
+}
+
+// Both products of the backward pass in one launch, or one of them: neither waits for the other, and the tiles of one fill the units that the other's leave.
+struct GatedPair {
+    GatedArgs input, weights;
+    unsigned first_blocks;        // of those that begin first
+    int input_first;
+    unsigned input_parts, weights_parts;
+};
+template <typename Input, typename Weights>
+__device__ __forceinline__ void gated_pair(const GatedPair& p, const Input& input, const Weights& weights) {
+    const bool first = blockIdx.x < p.first_blocks;
+    const unsigned at = first ? blockIdx.x : blockIdx.x - p.first_blocks;
+    if (first == (p.input_first != 0)) {
+        const unsigned tiles = (unsigned)(p.input.tiles_m * p.input.tiles_n), part = p.input_parts > 1 ? at / tiles : 0;
+        input(p.input, at - part * tiles, part, p.input_parts);
+    } else {
+        const unsigned tiles = (unsigned)(p.weights.tiles_m * p.weights.tiles_n), part = p.weights_parts > 1 ? at / tiles : 0;
+        weights(p.weights, at - part * tiles, part, p.weights_parts);
+    }
+}
+template <int DT, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(WM* WN * 64, 2) void gated_backward_kernel(const GatedPair p) {
+    gated_pair(p, [](const GatedArgs& g, unsigned block, unsigned part, unsigned parts) { gated_mm<DT, MM_INPUT, BM, BN, WM, WN, NS>(g, block, part, parts); },
+               [](const GatedArgs& g, unsigned block, unsigned part, unsigned parts) { gated_mm<DT, MM_WEIGHTS, BM, BN, WM, WN, NS>(g, block, part, parts); });
+}
+
 // ---- few rows, or few tiles ----
 // One tile of (16 TM) x (16 TN) sums on four waves: wave w takes K-tiles w, w + 4, ... through an LDS ring of NS stages of its own, so no wave waits for another inside the loop, and the four
 // partial sums meet in LDS, in a fixed order.  Forward and the gradient of A; of the weights there are always many.
-// PARTS: the K-tiles are shared out over gridDim.y workgroups, too, whose sums go to a workspace in f32 (gated_join_kernel adds them up).
-template <int DT, int MODE, int TM, int TN, int NS, bool PARTS>
-__global__ __launch_bounds__(256) void gated_split_kernel(const GatedArgs g) {
+// Several workgroups may share the K-tiles, too, as above.
+template <int DT, int MODE, int TM, int TN, int NS>
+__device__ __forceinline__ void gated_split(const GatedArgs& g, unsigned block, unsigned share, unsigned parts) {
     constexpr int KS = 4, ES = ELEM_BYTES<DT>, BK = ROW_BYTES / ES, BM = 16 * TM, BN = 16 * TN;
     constexpr bool B_ACROSS = MODE == MM_INPUT;
     constexpr int A_BYTES = BM * ROW_BYTES, STAGE = (BM + BN) * ROW_BYTES;
@@ -429,12 +471,12 @@ __global__ __launch_bounds__(256) void gated_split_kernel(const GatedArgs g) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fi = lane & 15, fq = lane >> 4;
     int tm, tn;
-    gated_tile_of_block(blockIdx.x, g.tiles_m, g.tiles_n, g.group_m, tm, tn);
+    gated_tile_of_block(block, g.tiles_m, g.tiles_n, g.group_m, tm, tn);
     const long m0 = (long)tm * BM, n0 = (long)tn * (MODE == MM_FORWARD ? BN / 2 : BN);
     const long pitch_a = (MODE == MM_FORWARD ? g.K : 2 * g.half) * ES, pitch_b = g.K * ES;
     const long inner = MODE == MM_FORWARD ? g.K : g.N;
     const int tail = (int)(inner % BK), per_half = (int)((inner + BK - 1) / BK), all = per_half * (MODE == MM_INPUT ? 2 : 1);
-    const int first = PARTS ? (int)((long)all * blockIdx.y / gridDim.y) : 0, nk = PARTS ? (int)((long)all * (blockIdx.y + 1) / gridDim.y) - first : all;
+    const int first = (int)((unsigned)all * share / parts), nk = (int)((unsigned)all * (share + 1) / parts) - first;
     Loader<ES, false, BM, 1> la;
     Loader<ES, B_ACROSS, BN, 1> lb;
     la.template set<false>(lane, 0, pitch_a, g.M - m0, MODE == MM_INPUT ? BK : tail);
@@ -466,7 +508,7 @@ __global__ __launch_bounds__(256) void gated_split_kernel(const GatedArgs g) {
     // this wave's K-tiles: wave, wave + KS, ...; where only the weights count, from another one on in every workgroup: if all began with the first, they would ask the memory system for
     // the same columns of all rows at a time (1 x 4096 x 8192 bf16 30.3 us, so 24.8; with more rows, whose panels of A the workgroups share, 32 x 4096 x 8192 25.0 and 26.6)
     const int mine = (nk - wave + KS - 1) / KS;
-    int next = MODE == MM_FORWARD && TM == 1 && mine > 0 ? (int)(blockIdx.x * ROTATE % (unsigned)mine) : 0;
+    int next = MODE == MM_FORWARD && TM == 1 && mine > 0 ? (int)(block * ROTATE % (unsigned)mine) : 0;
     auto fetch_next = [&](unsigned stage) {
         fetch(first + wave + next * KS, stage);
         next = next + 1 == mine ? 0 : next + 1;
@@ -560,8 +602,8 @@ __global__ __launch_bounds__(256) void gated_split_kernel(const GatedArgs g) {
             for (int j = 0; j < TN; ++j)
                 if ((i * TN + j) % KS == wave) {
                     const long col = n0 + 16 * j + 4 * fq;
-                    if constexpr (PARTS) {                 // (K is a multiple of four)
-                        if (row < g.M && col < g.K) *reinterpret_cast<f32x4*>(g.parts + ((long)blockIdx.y * g.M + row) * g.K + col) = sum(i * TN + j);
+                    if (parts > 1) {                       // (K is a multiple of four)
+                        if (row < g.M && col < g.K) *reinterpret_cast<f32x4*>(g.parts + ((long)share * g.M + row) * g.K + col) = sum(i * TN + j);
                     } else {
                         put(g.C0, g.K, row, col, sum(i * TN + j));
                     }
@@ -570,16 +612,38 @@ __global__ __launch_bounds__(256) void gated_split_kernel(const GatedArgs g) {
     }
 }
 
-// The partial sums of n workgroups, in their order, to one result or two of `each` numbers; four numbers a lane.
+template <int DT, int TM, int TN, int NS>
+__global__ __launch_bounds__(256) void gated_forward_split_kernel(const GatedArgs g) {
+    gated_split<DT, MM_FORWARD, TM, TN, NS>(g, blockIdx.x, 0, 1);
+}
+// The gradient of A so, those of the weights in tiles of 64 x 64.
 template <int DT>
-__global__ __launch_bounds__(256) void gated_join_kernel(const float* parts, int n, void* C0, void* C1, long each) {
-    const long all = C1 != nullptr ? 2 * each : each;
+__global__ __launch_bounds__(256) void gated_backward_split_kernel(const GatedPair p) {
+    gated_pair(p, [](const GatedArgs& g, unsigned block, unsigned part, unsigned parts) { gated_split<DT, MM_INPUT, 2, 4, 2>(g, block, part, parts); },
+               [](const GatedArgs& g, unsigned block, unsigned part, unsigned parts) { gated_mm<DT, MM_WEIGHTS, 64, 64, 2, 2, STAGES_64<DT>>(g, block, part, parts); });
+}
+
+// The partial sums of several workgroups, in their order: dA, of `of_input` numbers, dG and dU, of half of `of_weights` each (0: nothing to add up); four numbers a lane.
+struct GatedJoin {
+    const float *input, *weights;
+    int input_parts, weights_parts;
+    long of_input, of_weights;
+    void *dA, *dG, *dU;
+};
+template <int DT>
+__global__ __launch_bounds__(256) void gated_join_kernel(const GatedJoin a) {
     long at = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (at >= all) return;
-    f32x4 v = *reinterpret_cast<const f32x4*>(parts + at);
-    for (int p = 1; p < n; ++p) v += *reinterpret_cast<const f32x4*>(parts + p * all + at);
-    void* const C = at < each ? C0 : C1;
-    at -= at < each ? 0 : each;
+    if (at >= a.of_input + a.of_weights) return;
+    const bool input = at < a.of_input;
+    at -= input ? 0 : a.of_input;
+    const float* const from = input ? a.input : a.weights;
+    const long all = input ? a.of_input : a.of_weights;
+    const int n = input ? a.input_parts : a.weights_parts;
+    f32x4 v = *reinterpret_cast<const f32x4*>(from + at);
+    for (int p = 1; p < n; ++p) v += *reinterpret_cast<const f32x4*>(from + p * all + at);
+    const bool of_up = !input && at >= all / 2;
+    void* const C = input ? a.dA : of_up ? a.dU : a.dG;
+    at -= of_up ? all / 2 : 0;
     if constexpr (DT == SP_F32) *reinterpret_cast<f32x4*>((float*)C + at) = v;
     else *reinterpret_cast<u32x2*>((unsigned short*)C + at) = u32x2{pack_halves<DT>(v[0], v[1]), pack_halves<DT>(v[2], v[3])};
 }
@@ -656,62 +720,62 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const GatedGradArgs g) 
 
 static long gated_ceil(long a, long b) { return (a + b - 1) / b; }
 
-template <int DT>
-static int launch_join(const char* what, const GatedArgs& g, long rows, int parts, hipStream_t stream) {
-    const long each = rows * g.K;
-    hipLaunchKernelGGL(gated_join_kernel<DT>, dim3((unsigned)gated_ceil(each * (g.C1 != nullptr ? 2 : 1), 1024)), dim3(256), 0, stream, g.parts, parts, g.C0, g.C1, each);
+constexpr long MOST_TILES = 1l << 22;         // (a launch holds fewer than 2^32 work items: two such products of 512)
+template <int MODE, int BM, int BN>
+static bool set_tiles(GatedArgs& g, int group_m) {
+    const long tiles_m = MODE == MM_WEIGHTS ? 2 * gated_ceil(g.N, BM) : gated_ceil(g.M, BM), tiles_n = MODE == MM_FORWARD ? gated_ceil(g.N, BN / 2) : gated_ceil(g.K, BN);
+    if (tiles_m * tiles_n >= MOST_TILES) return false;
+    g.tiles_m = (int)tiles_m;
+    g.tiles_n = (int)tiles_n;
+    g.group_m = group_m == 0 ? g.tiles_m : group_m;        // 0: the tiles of one panel of weights stand side by side
+    return true;
+}
+template <typename Kernel, typename Args>
+static int launch_lds(const char* what, Kernel kernel, unsigned blocks, unsigned threads, int lds_bytes, const Args& args, hipStream_t stream) {
+    if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), lds_bytes, stream, args);
     return check_launch(what);
 }
+constexpr int larger(int a, int b) { return a > b ? a : b; }
+constexpr int split_lds(int TM, int TN, int NS) { return larger(4 * NS * 16 * (TM + TN) * ROW_BYTES, TM * TN * 4096); }
+constexpr int mm_lds(int BM, int BN, int NS) { return NS * (BM + BN) * ROW_BYTES; }
 
-template <int DT, int MODE, int BM, int BN, int WM, int WN, int NS>
-static int launch_mm(const char* what, GatedArgs g, int parts, hipStream_t stream) {
-    constexpr int lds_bytes = NS * (BM + BN) * ROW_BYTES;
-    const long tiles_m = MODE == MM_WEIGHTS ? 2 * gated_ceil(g.N, BM) : gated_ceil(g.M, BM);
-    const long tiles_n = MODE == MM_FORWARD ? gated_ceil(g.N, BN / 2) : gated_ceil(g.K, BN);
-    if (tiles_m >= 1l << 31 || tiles_n >= 1l << 31 || tiles_m * tiles_n >= 1l << 31 || tiles_m * tiles_n * (WM * WN * 64) >= 1l << 32) return fail(SP_ERR_SHAPE, "%s: too large", what);
-    g.tiles_m = (int)tiles_m;
-    g.tiles_n = (int)tiles_n;
-    g.group_m = 4;
-    auto launch = [&](auto kernel) {
-        if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(WM * WN * 64), lds_bytes, stream, g);
-        return check_launch(what);
-    };
-    if constexpr (MODE != MM_FORWARD)
-        if (parts > 1) {
-            if (const int rc = launch(gated_mm_kernel<DT, MODE, BM, BN, WM, WN, NS, true>); rc != SP_OK) return rc;
-            return launch_join<DT>(what, g, MODE == MM_INPUT ? g.M : g.N, parts, stream);
-        }
-    return launch(gated_mm_kernel<DT, MODE, BM, BN, WM, WN, NS, false>);
+template <int DT, int BM, int BN, int WM, int WN, int NS>
+static int launch_forward(const char* what, GatedArgs g, hipStream_t stream) {
+    if (!set_tiles<MM_FORWARD, BM, BN>(g, 4)) return fail(SP_ERR_SHAPE, "%s: too large", what);
+    return launch_lds(what, gated_forward_kernel<DT, BM, BN, WM, WN, NS>, (unsigned)(g.tiles_m * g.tiles_n), WM * WN * 64, mm_lds(BM, BN, NS), g, stream);
+}
+template <int DT, int TM, int TN, int NS>
+static int launch_forward_split(const char* what, GatedArgs g, hipStream_t stream) {
+    if (!set_tiles<MM_FORWARD, 16 * TM, 16 * TN>(g, 0)) return fail(SP_ERR_SHAPE, "%s: too large", what);
+    return launch_lds(what, gated_forward_split_kernel<DT, TM, TN, NS>, (unsigned)(g.tiles_m * g.tiles_n), 256, split_lds(TM, TN, NS), g, stream);
 }
 
-template <int DT, int MODE, int TM, int TN, int NS>
-static int launch_split(const char* what, GatedArgs g, int parts, hipStream_t stream) {
-    constexpr int ring = 4 * NS * 16 * (TM + TN) * ROW_BYTES, partial = TM * TN * 4096, lds_bytes = ring > partial ? ring : partial;
-    const long tiles_m = gated_ceil(g.M, 16 * TM), tiles_n = MODE == MM_FORWARD ? gated_ceil(g.N, 8 * TN) : gated_ceil(g.K, 16 * TN);
-    if (tiles_m * tiles_n * 256 >= 1l << 32) return fail(SP_ERR_SHAPE, "%s: too large", what);
-    g.tiles_m = (int)tiles_m;
-    g.tiles_n = (int)tiles_n;
-    g.group_m = (int)tiles_m;      // the tiles of one panel of weights stand side by side
-    auto launch = [&](auto kernel) {
-        if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts), dim3(256), lds_bytes, stream, g);
-        return check_launch(what);
-    };
-    if constexpr (MODE == MM_INPUT)
-        if (parts > 1) {
-            if (const int rc = launch(gated_split_kernel<DT, MODE, TM, TN, NS, true>); rc != SP_OK) return rc;
-            return launch_join<DT>(what, g, g.M, parts, stream);
-        }
-    return launch(gated_split_kernel<DT, MODE, TM, TN, NS, false>);
+// Those of the two products that have parts; the longer ones' workgroups first.
+static unsigned set_pair(GatedPair& p, bool input_first) {
+    const unsigned input = p.input_parts * (unsigned)(p.input.tiles_m * p.input.tiles_n), weights = p.weights_parts * (unsigned)(p.weights.tiles_m * p.weights.tiles_n);
+    p.input_first = input_first;
+    p.first_blocks = input_first ? input : weights;
+    return input + weights;
+}
+template <int DT, int BM, int BN, int WM, int WN, int NS>
+static int launch_backward(const char* what, GatedPair p, bool input_first, hipStream_t stream) {
+    if (!set_tiles<MM_INPUT, BM, BN>(p.input, 4) || !set_tiles<MM_WEIGHTS, BM, BN>(p.weights, 4)) return fail(SP_ERR_SHAPE, "%s: too large", what);
+    const unsigned blocks = set_pair(p, input_first);
+    return launch_lds(what, gated_backward_kernel<DT, BM, BN, WM, WN, NS>, blocks, WM * WN * 64, mm_lds(BM, BN, NS), p, stream);
+}
+template <int DT>
+static int launch_backward_split(const char* what, GatedPair p, bool input_first, hipStream_t stream) {
+    if (!set_tiles<MM_INPUT, 32, 64>(p.input, 0) || !set_tiles<MM_WEIGHTS, 64, 64>(p.weights, 4)) return fail(SP_ERR_SHAPE, "%s: too large", what);
+    const unsigned blocks = set_pair(p, input_first);
+    return launch_lds(what, gated_backward_split_kernel<DT>, blocks, 256, larger(split_lds(2, 4, 2), mm_lds(64, 64, STAGES_64<DT>)), p, stream);
 }
 
 // ---- which kernel ----
-// Estimated time of a product in us, without the launch: workgroups in rounds of as many as a unit's LDS holds at a time, each nk K-tiles (a quarter of them, where four waves share
-// them) plus an overhead; n workgroups on a unit take n times the work of a K-tile, and never less than what a lone one waits for.  Partial sums are written, read and joined, at 4 TB/s (at 8, as
-// they were fitted, 5008 x 2048 x 5461 took three of them: the gradient of A alone 281 -> 263 us, but the whole step, which the part's power limits, 657 -> 668).
-// Fitted on what every kernel took on 99 forward, 62 and 62 backward shapes, from 1 x 512 x 1365 to 16384 x 4096 x 512; the one it picks is on the mean 2 % behind the fastest forward
-// (3 with 8-bit blocks), 4 for the gradient of A and 2 for the weights'.  More tiles (64 x 128, 128 x 256 in two stages, 16 x 64 and 64 x 64 in four parts) were worth less than a hundredth.
+// Estimated times in us, without the launch: workgroups in rounds of as many as a unit's LDS holds at a time, each nk K-tiles (a quarter of them, where four waves share
+// them) plus an overhead; n workgroups on a unit take n times the work of a K-tile, and never less than what a lone one waits for.
+// Forward: fitted on what every kernel took on 99 shapes, from 1 x 512 x 1365 to 16384 x 4096 x 512; the one it picks is on the mean 2 % behind the fastest (3 with 8-bit blocks).  More
+// tiles (64 x 128, 128 x 256 in two stages, 16 x 64 and 64 x 64 in four parts) were worth less than a hundredth.
 struct MmCost {
     int id, bm, bn;               // bn: columns of the result
     int per_unit;
@@ -726,48 +790,124 @@ static const MmCost kForward32[] = {{SPLIT_16, 16, 16, 3, true, 0.587f, 0.354f, 
 static const MmCost kBlocks16[] = {{TILE_32_BLOCKS, 32, 128, 1, false, 0.41f, 0.41f, 4.8f}, {TILE_64_BLOCKS, 64, 128, 1, false, 0.46f, 0.46f, 5.3f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 6.7f},
                                    {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 8.f}};
 static const MmCost kBlocks32[] = {{TILE_32_BLOCKS, 32, 128, 1, false, 1.05f, 1.05f, 5.f}, {TILE_64_BLOCKS, 64, 128, 1, false, 1.972f, 1.039f, 6.f}};
-static const MmCost kInput16[] = {{SPLIT_32, 32, 64, 1, true, 0.572f, 0.318f, 2.47f}, {TILE_64, 64, 64, 2, false, 0.225f, 0.201f, 2.96f}, {TILE_128, 128, 128, 1, false, 0.464f, 0.464f, 3.77f},
-                                  {TILE_128_WIDE, 128, 256, 1, false, 0.652f, 0.652f, 4.51f}, {TILE_256, 256, 256, 1, false, 1.112f, 0.4f, 5.2f}};
-static const MmCost kWeights16[] = {{TILE_64, 64, 64, 2, false, 0.171f, 0.218f, 2.64f}, {TILE_128, 128, 128, 1, false, 0.538f, 0.424f, 4.11f}, {TILE_128_WIDE, 128, 256, 1, false, 0.766f, 0.1f, 5.53f},
-                                    {TILE_256, 256, 256, 1, false, 1.282f, 0.1f, 7.04f}};
-static const MmCost kInput32[] = {{SPLIT_32, 32, 64, 1, true, 1.167f, 0.4f, 3.04f}, {TILE_64, 64, 64, 5, false, 0.594f, 0.528f, 2.36f}, {TILE_128, 128, 128, 2, false, 1.999f, 1.918f, 2.23f}};
-static const MmCost kWeights32[] = {{TILE_64, 64, 64, 5, false, 0.603f, 0.538f, 3.78f}, {TILE_128, 128, 128, 2, false, 1.896f, 2.022f, 5.08f}};
+// Backward, both products in one launch (the input's tile first in a pair, the weights' beside it): fitted on 2,700 timings of 150 shapes from 55 x 1720 x 1674 to 9344 x 2304 x 768 with
+// every tile and numbers of parts; what it picks is on the mean 4 % behind the fastest of them.  (us, each in a launch of its own with its best tile / together: 1341 x 1536 x 2992 bf16
+// 84.4 / 64.5, 1003 x 512 x 1365 29.3 / 22.8, 9344 x 896 x 1664 164 / 154, 1003 x 512 x 1365 f32 74.2 / 61.2.)  per_unit 0: as many as there is room for, which share the unit's rate.
+static const MmCost kInput16[] = {{SPLIT_32, 32, 64, 1, true, 0.585f, 0.109f, 4.213f}, {TILE_64, 64, 64, 2, false, 0.248f, 0.083f, 3.684f}, {TILE_128, 128, 128, 1, false, 0.428f, 0.424f, 2.987f},
+                                  {TILE_128_WIDE, 128, 256, 1, false, 0.695f, 0.704f, 3.237f}, {TILE_256, 256, 256, 1, false, 1.265f, 0.329f, 4.056f}};
+static const MmCost kWeights16[] = {{TILE_64, 64, 64, 1, false, 0.107f, 0.498f, 1.264f}, {TILE_64, 64, 64, 2, false, 0.262f, 0.258f, 1.686f}, {TILE_128, 128, 128, 1, false, 0.405f, 0.45f, 3.003f},
+                                    {TILE_128_WIDE, 128, 256, 1, false, 0.667f, 0.134f, 4.458f}, {TILE_256, 256, 256, 1, false, 1.45f, 0.134f, 0.053f}};
+static const MmCost kInput32[] = {{SPLIT_32, 32, 64, 1, true, 1.228f, 0.474f, 3.027f}, {TILE_64, 64, 64, 0, false, 0.778f, 0.487f, 1.19f}};
+static const MmCost kWeights32[] = {{TILE_64, 64, 64, 1, false, 0.607f, 0.609f, 2.227f}, {TILE_64, 64, 64, 0, false, 0.826f, 0.454f, 1.19f}};
 
-struct MmChoice {
-    int id, parts;
+// What a product of rows x cols asks of a tile.
+struct MmWork {
+    double tiles;
+    long nk;                      // K-tiles of one
+    double sums;                  // numbers of the result
 };
+static MmWork work_of(const MmCost& c, int mode, bool f32, long M, long N, long K) {
+    const long bk = f32 ? 32 : 64, rows = mode == MM_WEIGHTS ? N : M, cols = mode == MM_FORWARD ? N : K, twice = mode == MM_WEIGHTS ? 2 : 1;
+    return {(double)gated_ceil(rows, c.bm) * (double)gated_ceil(cols, c.bn) * twice, mode == MM_FORWARD ? gated_ceil(K, bk) : mode == MM_INPUT ? 2 * gated_ceil(N, bk) : gated_ceil(M, bk),
+            (double)rows * cols * twice};
+}
+static long tiles_of_k(const MmCost& c, long nk, int parts) { return gated_ceil(gated_ceil(nk, parts), c.split ? 4 : 1); }
+static double group_us(const MmCost& c, long k_tiles, double on_unit) { return k_tiles * (on_unit * c.work > c.lone ? on_unit * c.work : (double)c.lone) + c.overhead; }
+constexpr double JOIN_US = 5, SHARED_US = 1.9;
+static double join_us(const MmWork& w, int parts, bool f32) { return parts > 1 ? w.sums * (8.0 * parts + (f32 ? 4 : 2)) * 1e-6 / 8 : 0; }
+static bool may_split(const MmWork& w, int parts) { return parts == 1 || (w.tiles * parts <= 2.0 * device_cu_count() && w.nk >= 4l * parts); }
 
 template <size_t N>
-static MmChoice cheapest(const MmCost (&menu)[N], int mode, bool f32, long M, long N_, long K) {
-    const long cus = device_cu_count(), bk = f32 ? 32 : 64;
-    const long rows = mode == MM_WEIGHTS ? N_ : M, cols = mode == MM_FORWARD ? N_ : K, twice = mode == MM_WEIGHTS ? 2 : 1;
-    const long nk = mode == MM_FORWARD ? gated_ceil(K, bk) : mode == MM_INPUT ? 2 * gated_ceil(N_, bk) : gated_ceil(M, bk);
-    MmChoice best{menu[0].id, 1};
+static int cheapest(const MmCost (&menu)[N], bool f32, long M, long N_, long K) {
+    const long cus = device_cu_count();
+    int best = -1;
     double best_us = 0;
-    bool any = false;
     for (const MmCost& c : menu) {
-        const double tiles = (double)gated_ceil(rows, c.bm) * (double)gated_ceil(cols, c.bn) * twice;
-        if (tiles * 512 >= 4294967296.0) continue;         // (a launch holds fewer than 2^32 work items)
-        for (int parts = 1; parts <= 16; ++parts) {
-            if (parts > 1 && (mode == MM_FORWARD || tiles * parts > 2.0 * cus || nk < 4 * parts)) break;
-            const double groups = tiles * parts, round = (double)cus * c.per_unit;
-            const long mine = gated_ceil(gated_ceil(nk, parts), c.split ? 4 : 1);
-            auto of = [&](double n) { return mine * (n * c.work > c.lone ? n * c.work : (double)c.lone) + c.overhead; };
-            const double full = (double)(int64_t)(groups / round), rest = groups - full * round;
-            double us = full * of(c.per_unit) + (rest > 0 ? of((double)(int64_t)((rest + cus - 1) / cus)) : 0);
-            if (parts > 1) us += 6 + (double)rows * cols * twice * (8.0 * parts + (f32 ? 4 : 2)) * 1e-6 / 4;
-            if (!any || us < best_us) {
-                any = true;
+        const MmWork w = work_of(c, MM_FORWARD, f32, M, N_, K);
+        if (w.tiles >= MOST_TILES) continue;
+        const double round = (double)cus * c.per_unit, full = (double)(int64_t)(w.tiles / round), rest = w.tiles - full * round;
+        const long k_tiles = tiles_of_k(c, w.nk, 1);
+        const double us = full * group_us(c, k_tiles, c.per_unit) + (rest > 0 ? group_us(c, k_tiles, (double)(int64_t)((rest + cus - 1) / cus)) : 0);
+        if (best < 0 || us < best_us) {
+            best = c.id;
+            best_us = us;
+        }
+    }
+    return best;
+}
+
+// The tile and the parts of both products of the backward pass, also where one alone is wanted: a gradient does not depend on whether the other is.
+struct BackwardPlan {
+    int id, input_parts, weights_parts;
+    bool input_first;
+};
+// Estimated time of n1 workgroups of t1 us, the longer ones, and then n2 of t2, each to the slot that is free first.
+static double both_us(double slots, double n1, double t1, double n2, double t2) {
+    const double rounds = (double)(int64_t)(n1 / slots), late = n1 - rounds * slots;        // `late` slots have one round more of the first
+    if (n1 * t1 + n2 * t2 > 64 * slots * t1) return (n1 * t1 + n2 * t2) / slots + t2;
+    double count[2] = {late, slots - late}, at[2] = {(rounds + 1) * t1, rounds * t1};
+    while (n2 > 0) {
+        const int next = count[0] > 0 && at[0] < at[1] ? 0 : 1;
+        at[next] += t2;
+        n2 -= count[next];
+    }
+    return count[0] > 0 && at[0] > at[1] ? at[0] : at[1];
+}
+template <size_t N_>
+static BackwardPlan plan_of(const MmCost (&inputs)[N_], const MmCost (&weights)[N_], bool f32, long M, long N, long K) {
+    const long cus = device_cu_count();
+    BackwardPlan best{-1, 1, 1, true};
+    double best_us = 0;
+    for (size_t i = 0; i < N_; ++i) {
+        const MmCost &ci = inputs[i], &cw = weights[i];
+        const MmWork wi = work_of(ci, MM_INPUT, f32, M, N, K), ww = work_of(cw, MM_WEIGHTS, f32, M, N, K);
+        if (wi.tiles >= MOST_TILES || ww.tiles >= MOST_TILES) continue;
+        // shares of K about as long as one another's
+        const double li = wi.nk * (ci.split ? 0.25 : 1.0) * ci.work, lw = ww.nk * cw.work;
+        for (int n = 1; n <= 16; ++n) {
+            const int other = (int)(n * (li > lw ? lw / li : li / lw) + 0.5), fewer = other > 1 ? other : 1;
+            const int pi = li > lw ? n : fewer, pw = li > lw ? fewer : n;
+            if (!may_split(wi, pi) || !may_split(ww, pw)) break;
+            const double ni = wi.tiles * pi, nw = ww.tiles * pw, all = (double)(int64_t)((ni + nw + cus - 1) / cus);
+            const long ki = tiles_of_k(ci, wi.nk, pi), kw = tiles_of_k(cw, ww.nk, pw);
+            double ti, tw, us;
+            if (ci.per_unit == 0) {                        // those on a unit share its rate
+                ti = ki * ci.work + ci.overhead;
+                tw = kw * cw.work + cw.overhead;
+                us = ti > tw ? both_us(cus, ni, ti, nw, tw) : both_us(cus, nw, tw, ni, ti);
+                const double longest = ki * ci.lone > kw * cw.lone ? ki * ci.lone : kw * cw.lone;
+                us = (us > longest ? us : longest) + SHARED_US;
+            } else {
+                const double on_unit = all < ci.per_unit ? all : ci.per_unit;
+                ti = group_us(ci, ki, on_unit);
+                tw = group_us(cw, kw, on_unit);
+                us = ti > tw ? both_us(cus * on_unit, ni, ti, nw, tw) : both_us(cus * on_unit, nw, tw, ni, ti);
+            }
+            if (!f32 && ci.id != TILE_256 && us > 100) us += 0.2 * (us - 100);        // long products are limited by the part's power, of which smaller tiles take more
+            if (pi > 1 || pw > 1) us += JOIN_US + join_us(wi, pi, f32) + join_us(ww, pw, f32);
+            if (best.id < 0 || us < best_us) {
+                best = {ci.id, pi, pw, ti > tw};
                 best_us = us;
-                best = {c.id, parts};
             }
         }
     }
     return best;
 }
-static MmChoice choose_backward(int mode, bool f32, long M, long N, long K) {
-    if (mode == MM_INPUT) return f32 ? cheapest(kInput32, mode, f32, M, N, K) : cheapest(kInput16, mode, f32, M, N, K);
-    return f32 ? cheapest(kWeights32, mode, f32, M, N, K) : cheapest(kWeights16, mode, f32, M, N, K);
+// The plans of the sizes that this thread asked for last: they follow from the sizes alone, and a short call would take as long to make one as its kernels run.
+static BackwardPlan choose_backward(bool f32, long M, long N, long K) {
+    struct Known {
+        bool f32;
+        int cus;
+        long M, N, K;
+        BackwardPlan plan;
+    };
+    constexpr unsigned PLACES = 16;
+    static thread_local Known known[PLACES];
+    const int cus = device_cu_count();
+    Known& at = known[(unsigned)((unsigned long)(M * 31 + N * 17 + K) * 0x9e3779b97f4a7c15ul >> 32) % PLACES];
+    if (at.f32 != f32 || at.cus != cus || at.M != M || at.N != N || at.K != K)
+        at = {f32, cus, M, N, K, f32 ? plan_of(kInput32, kWeights32, f32, M, N, K) : plan_of(kInput16, kWeights16, f32, M, N, K)};
+    return at.plan;
 }
 
 template <int DT>
@@ -775,59 +915,60 @@ static int gated_forward(const GatedArgs& g, hipStream_t stream) {
     constexpr bool F32 = DT == SP_F32;
     const char* const what = "sp_gemm_abt_gated";
     int id;
-    if (g.keep == KEEP_F8) id = F32 ? cheapest(kBlocks32, MM_FORWARD, F32, g.M, g.N, g.K).id : cheapest(kBlocks16, MM_FORWARD, F32, g.M, g.N, g.K).id;
-    else id = F32 ? cheapest(kForward32, MM_FORWARD, F32, g.M, g.N, g.K).id : cheapest(kForward16, MM_FORWARD, F32, g.M, g.N, g.K).id;
+    if (g.keep == KEEP_F8) id = F32 ? cheapest(kBlocks32, F32, g.M, g.N, g.K) : cheapest(kBlocks16, F32, g.M, g.N, g.K);
+    else id = F32 ? cheapest(kForward32, F32, g.M, g.N, g.K) : cheapest(kForward16, F32, g.M, g.N, g.K);
     switch (id) {
-        case SPLIT_16: return launch_split<DT, MM_FORWARD, 1, 2, 2>(what, g, 1, stream);
-        case SPLIT_32: return launch_split<DT, MM_FORWARD, 2, 2, 2>(what, g, 1, stream);
-        case TILE_64: return launch_mm<DT, MM_FORWARD, 64, 64, 2, 2, F32 ? 2 : 4>(what, g, 1, stream);
-        case TILE_32_BLOCKS: return launch_mm<DT, MM_FORWARD, 32, 256, 1, 4, 3>(what, g, 1, stream);
-        case TILE_64_BLOCKS: return launch_mm<DT, MM_FORWARD, 64, 256, 2, 4, 3>(what, g, 1, stream);
+        case SPLIT_16: return launch_forward_split<DT, 1, 2, 2>(what, g, stream);
+        case SPLIT_32: return launch_forward_split<DT, 2, 2, 2>(what, g, stream);
+        case TILE_64: return launch_forward<DT, 64, 64, 2, 2, STAGES_64<DT>>(what, g, stream);
+        case TILE_32_BLOCKS: return launch_forward<DT, 32, 256, 1, 4, 3>(what, g, stream);
+        case TILE_64_BLOCKS: return launch_forward<DT, 64, 256, 2, 4, 3>(what, g, stream);
     }
     if constexpr (!F32) {
-        if (id == TILE_128) return launch_mm<DT, MM_FORWARD, 128, 128, 2, 4, 4>(what, g, 1, stream);
-        if (id == TILE_128_WIDE) return launch_mm<DT, MM_FORWARD, 128, 256, 4, 2, 3>(what, g, 1, stream);
-        return launch_mm<DT, MM_FORWARD, 256, 256, 4, 2, 2>(what, g, 1, stream);
+        if (id == TILE_128) return launch_forward<DT, 128, 128, 2, 4, 4>(what, g, stream);
+        if (id == TILE_128_WIDE) return launch_forward<DT, 128, 256, 4, 2, 3>(what, g, stream);
+        return launch_forward<DT, 256, 256, 4, 2, 2>(what, g, stream);
     }
     return fail(SP_ERR_UNSUPPORTED, "%s: no kernel", what);
 }
 
-template <int DT, int MODE>
-static int gated_backward_product(const GatedArgs& g, hipStream_t stream) {
+template <int DT>
+static int backward_products(int id, const GatedPair& p, bool input_first, hipStream_t stream) {
     constexpr bool F32 = DT == SP_F32;
     const char* const what = "sp_gemm_abt_gated_backward";
-    const MmChoice c = choose_backward(MODE, F32, g.M, g.N, g.K);
-    if constexpr (MODE == MM_INPUT)
-        if (c.id == SPLIT_32) return launch_split<DT, MODE, 2, 4, 2>(what, g, c.parts, stream);
-    if constexpr (F32) {
-        if (c.id == TILE_64) return launch_mm<DT, MODE, 64, 64, 2, 2, 2>(what, g, c.parts, stream);
-        return launch_mm<DT, MODE, 128, 128, 2, 2, 2>(what, g, c.parts, stream);
-    } else {
-        if (c.id == TILE_64) return launch_mm<DT, MODE, 64, 64, 2, 2, 4>(what, g, c.parts, stream);
-        if (c.id == TILE_128) return launch_mm<DT, MODE, 128, 128, 2, 4, 4>(what, g, c.parts, stream);
-        if (c.id == TILE_128_WIDE) return launch_mm<DT, MODE, 128, 256, 2, 4, 3>(what, g, c.parts, stream);
-        return launch_mm<DT, MODE, 256, 256, 2, 4, 2>(what, g, c.parts, stream);
+    if (id == SPLIT_32) return launch_backward_split<DT>(what, p, input_first, stream);
+    if (id == TILE_64) return launch_backward<DT, 64, 64, 2, 2, STAGES_64<DT>>(what, p, input_first, stream);
+    if constexpr (!F32) {
+        if (id == TILE_128) return launch_backward<DT, 128, 128, 2, 4, 4>(what, p, input_first, stream);
+        if (id == TILE_128_WIDE) return launch_backward<DT, 128, 256, 2, 4, 3>(what, p, input_first, stream);
+        return launch_backward<DT, 256, 256, 2, 4, 2>(what, p, input_first, stream);
     }
+    return fail(SP_ERR_SHAPE, "%s: too large", what);
 }
 
 template <int DT>
-static int gated_backward(const GatedArgs& input, const GatedArgs& weights, const GatedGradArgs& grad, bool f8, hipStream_t stream) {
+static int gated_backward(GatedArgs input, GatedArgs weights, const GatedGradArgs& grad, bool f8, hipStream_t stream) {
     const long pieces = grad.M * (grad.half / 8);
     const dim3 blocks((unsigned)gated_ceil(pieces, 256));
     if (f8) hipLaunchKernelGGL((gated_grad_kernel<DT, true>), blocks, dim3(256), 0, stream, grad);
     else hipLaunchKernelGGL((gated_grad_kernel<DT, false>), blocks, dim3(256), 0, stream, grad);
     if (const int rc = check_launch("sp_gemm_abt_gated_backward"); rc != SP_OK) return rc;
-    if (input.C0 != nullptr)
-        if (const int rc = gated_backward_product<DT, MM_INPUT>(input, stream); rc != SP_OK) return rc;
-    return weights.C0 != nullptr ? gated_backward_product<DT, MM_WEIGHTS>(weights, stream) : SP_OK;
+    const BackwardPlan plan = choose_backward(DT == SP_F32, grad.M, grad.N, input.K);
+    const unsigned input_parts = input.C0 != nullptr ? plan.input_parts : 0, weights_parts = weights.C0 != nullptr ? plan.weights_parts : 0;
+    if (plan.input_parts > 1) weights.parts = input.parts + (long)plan.input_parts * input.M * input.K;
+    if (const int rc = backward_products<DT>(plan.id, GatedPair{input, weights, 0, 0, input_parts, weights_parts}, plan.input_first, stream); rc != SP_OK) return rc;
+    if (input_parts <= 1 && weights_parts <= 1) return SP_OK;
+    GatedJoin join{input.parts, weights.parts, (int)input_parts, (int)weights_parts, input_parts > 1 ? input.M * input.K : 0, weights_parts > 1 ? 2 * weights.N * weights.K : 0,
+                   input.C0, weights.C0, weights.C1};
+    hipLaunchKernelGGL(gated_join_kernel<DT>, dim3((unsigned)gated_ceil(join.of_input + join.of_weights, 1024)), dim3(256), 0, stream, join);
+    return check_launch("sp_gemm_abt_gated_backward");
 }
 
 namespace {
 struct GatedKernelNames {
     GatedKernelNames() {
-        register_kernel("gated_forward_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_FORWARD, 256, 256, 4, 2, 2, false>, 512);
-        register_kernel("gated_input_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_INPUT, 256, 256, 2, 4, 2, false>, 512);
-        register_kernel("gated_weights_256x256", (const void*)gated_mm_kernel<SP_BF16, MM_WEIGHTS, 256, 256, 2, 4, 2, false>, 512);
+        register_kernel("gated_forward_256x256", (const void*)gated_forward_kernel<SP_BF16, 256, 256, 4, 2, 2>, 512);
+        register_kernel("gated_backward_256x256", (const void*)gated_backward_kernel<SP_BF16, 256, 256, 2, 4, 2>, 512);
     }
 } gated_kernel_names;
 }  // namespace
@@ -880,11 +1021,10 @@ extern "C" int sp_gemm_abt_gated(int dtype, int activation, const void* A, const
     return gated_forward<SP_BF16>(g, st);
 }
 
-// Partial sums of the backward products, one after the other in the same place.
+// Partial sums of the backward products, side by side.
 static int64_t gated_parts_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
-    const int64_t input = choose_backward(MM_INPUT, dtype == SP_F32, M, N, K).parts, weights = choose_backward(MM_WEIGHTS, dtype == SP_F32, M, N, K).parts;
-    const int64_t a = input > 1 ? input * M * K * 4 : 0, b = weights > 1 ? weights * 2 * N * K * 4 : 0;
-    return a > b ? a : b;
+    const BackwardPlan plan = choose_backward(dtype == SP_F32, M, N, K);
+    return (plan.input_parts > 1 ? plan.input_parts * M * K * 4 : 0) + (plan.weights_parts > 1 ? plan.weights_parts * 2 * N * K * 4 : 0);
 }
 static int64_t gated_halves_bytes(int dtype, int64_t M, int64_t N) { return M * 2 * gated_half(N) * (dtype == SP_F32 ? 4 : 2); }
 
