@@ -41,11 +41,9 @@ __device__ __forceinline__ void move_to(Sums& a, float m) {
     a.m = m;
 }
 __device__ __forceinline__ float add_f32(float a, float b) { return a + b; }
+// most: the largest of a.m and x.
 template <int N, bool ENTROPY>
-__device__ __forceinline__ void take(Sums& a, const float (&x)[N]) {
-    float most = a.m;
-#pragma unroll
-    for (int i = 0; i < N; ++i) most = fmaxf(most, x[i]);
+__device__ __forceinline__ void take(Sums& a, const float (&x)[N], float most) {
     move_to(a, most);
     const float from = finite_reference(most);
     float s = 0.f, w = 0.f;
@@ -110,13 +108,13 @@ struct TopLds {
     unsigned short who[T];
 };
 
-// The `top` largest keys of a workgroup's part of a row, in their order, to put(place, key); places behind the last one get key 0.  mine: the largest key of this lane, pieces: how
-// many pieces a lane has, keys(lane, piece, f): f of every key of that lane's piece.
+// The `top` largest keys of a workgroup's part of a row, in their order, to put(place, key); places behind the last one get key 0.  mine: at most `slack` below the largest key of this
+// lane (0: it has none), pieces: how many pieces a lane has, keys(lane, piece, f): f of every key of that lane's piece.
 // The 64 largest of lanes apart by 64 hold `top` keys (or all there are) that are no smaller than the top-th of them, so nothing below that one is taken.  The few lanes that have
 // something left are listed, their pieces shared out over all lanes, and what is left of them, some two dozen keys for 20 alternatives, goes to a list, where every key counts the larger
 // ones.  Where that list is too short (thousands of the largest logits in a few lanes) the workgroup looks for one key after the other.
 template <int T, typename Keys, typename Put>
-__device__ __forceinline__ void largest_keys(TopLds<T>& lds, Key mine, int top, int pieces, const Keys& keys, const Put& put) {
+__device__ __forceinline__ void largest_keys(TopLds<T>& lds, Key mine, Key slack, int top, int pieces, const Keys& keys, const Put& put) {
     const int tid = threadIdx.x;
     lds.lanes[tid] = mine;
     if (tid == 0) {
@@ -136,7 +134,7 @@ __device__ __forceinline__ void largest_keys(TopLds<T>& lds, Key mine, int top, 
     }
     __syncthreads();
     const Key least = lds.least;
-    if (mine >= least) lds.who[atomicAdd(&lds.found, 1)] = (unsigned short)tid;
+    if (mine != 0 && mine + slack >= least) lds.who[atomicAdd(&lds.found, 1)] = (unsigned short)tid;
     __syncthreads();
     const int all = lds.found * pieces;
     for (int i = tid; i < all; i += T)
@@ -215,8 +213,8 @@ __global__ __launch_bounds__(T) void token_probs_kernel(const void* logits, long
                 x[u * P + e] = element<DT>(raw[u], e);
                 if (!decltype(whole)::value && !inside(i0 + u * PIECES + tid * P + e)) x[u * P + e] = -INFINITY;
             }
+        float most = mine.m;
         if constexpr (TOP) {
-            float most = mine.m;
 #pragma unroll
             for (int u = 0; u < AT_ONCE; ++u) {
                 float of_piece = x[u * P];
@@ -225,8 +223,11 @@ __global__ __launch_bounds__(T) void token_probs_kernel(const void* logits, long
                 best_piece = of_piece > most ? i0 / PIECES + u : best_piece;
                 most = fmaxf(most, of_piece);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) most = fmaxf(most, x[i]);
         }
-        take<N, ENTROPY>(mine, x);
+        take<N, ENTROPY>(mine, x, most);
     };
     u32x4 ahead[AT_ONCE];
     load(0, ahead);
@@ -244,9 +245,8 @@ __global__ __launch_bounds__(T) void token_probs_kernel(const void* logits, long
 #pragma unroll
         for (int e = 0; e < P; ++e) f(inside(i + e) ? key_of(element<DT>(raw, e), (int)c0 + i + e - front) : (Key)0);
     };
-    Key best = 0;
-    if constexpr (TOP)
-        if (mine.m > -INFINITY) keys_of_piece(tid, best_piece, [&](Key k) { best = larger(best, k); });
+    // the largest logit of this lane, with the last column of its piece: which of the columns it is would be another trip to memory (256 x 131072 bf16, five alternatives: 19.0 us, so 17.8)
+    const Key best = TOP && mine.m > -INFINITY ? key_of(mine.m, (int)c0 + best_piece * PIECES + tid * P + P - 1 - front) : (Key)0;
     __shared__ Sums waves[T / 64];
     move_to(mine, group_max<64>(mine.m));
     mine.s = group_reduce<64>(mine.s, add_f32);
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(T) void token_probs_kernel(const void* logits, long
         __shared__ TopLds<T> lds;
         const long to = (long)blockIdx.x * a.top;
         const RowResult r(sums);
-        largest_keys<T>(lds, best, a.top, (here + PIECES - 1) / PIECES, keys_of_piece, [&](int place, Key k) {
+        largest_keys<T>(lds, best, P - 1, a.top, (here + PIECES - 1) / PIECES, keys_of_piece, [&](int place, Key k) {
             if (chunks == 1) {
                 a.top_logp[to + place] = k != 0 ? r.logp(logit_of(k)) : -INFINITY;
                 a.top_ids[to + place] = k != 0 ? column_of(k) : -1;
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(256) void token_probs_rows_kernel(const void* logit
     for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
     most = group_max<T>(fmaxf(most, -INFINITY));           // (a NaN alone in its lane is not handed on)
     Sums sums{most, 0.f, 0.f};
-    take<N, ENTROPY>(sums, x);
+    take<N, ENTROPY>(sums, x, most);
     sums.s = group_reduce<T>(sums.s, add_f32);
     if constexpr (ENTROPY) sums.w = group_reduce<T>(sums.w, add_f32);
     if (lane == 0) put_sums(a, row, counts, mine, sums);
