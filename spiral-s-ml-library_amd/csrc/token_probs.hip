@@ -176,6 +176,9 @@ __device__ __forceinline__ void largest_keys(TopLds<T>& lds, Key mine, Key slack
 }
 
 // ---- long rows: a workgroup for a chunk of a row ----
+// Bound by HBM with the vector ALU close behind (some 11 instructions and one exponential a logit): 256 x 131072 bf16 with entropy 13.1 us (5.1 TB/s), 4096 x 32003 bf16 50.5 us (5.2 TB/s, the ALU
+// 75 % busy).  Five alternatives cost 4.4 us more, a chain of four short steps and a trip to memory that nothing covers with one workgroup a unit; two a unit, of half a row, were slower by the join.
+// One row of 32003 f32 logits: 5.8 us in 16 chunks and 4.2 for their join, launch and latency.
 constexpr int AT_ONCE = 4;        // 16-byte pieces of a lane between two looks at m
 
 template <int DT, int T, bool ENTROPY, bool TOP>
@@ -359,6 +362,7 @@ __global__ __launch_bounds__(256) void token_probs_join_top_kernel(const void* l
 }
 
 // ---- short rows: T lanes hold one in C pieces each ----
+// Bound by HBM: 65536 x 256 f32 with entropy 11.4 us (5.9 TB/s); 5001 x 1003 f16 5.4 us, launch and latency.
 template <int DT, int T, int C, bool ENTROPY>
 __global__ __launch_bounds__(256) void token_probs_rows_kernel(const void* logits, long cols, long rows, const TokenArgs a) {
     constexpr int P = PER16<DT>, N = C * P;
@@ -397,6 +401,7 @@ struct TokenGradArgs {
     void* dx;
 };
 
+// Bound by HBM: 4096 x 32003 bf16, 524 MB, 82.5 us (6.4 TB/s); 65536 x 256 f32, 134 MB, 20.4 us (6.6).
 // T lanes to a row or a chunk of one, U pieces each.
 template <int DT, int T, int U, bool ENTROPY, int POLICY>
 __global__ __launch_bounds__(256) void token_grad_kernel(const void* logits, long cols, long rows, unsigned chunks, const TokenGradArgs a) {
