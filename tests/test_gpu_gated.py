@@ -195,6 +195,27 @@ def test_backward_from_8_bits(M, m, n, k, dtype):
     check_backward(M, dc, x, gate, up, kept, "silu")
 
 
+# both products with every tile, and what their sizes lead to: shares of K of either or both, the input's workgroups first or the weights'
+PLANS_16 = [(29, 359, 2888), (1033, 1027, 32), (3370, 197, 56), (1083, 434, 64), (2118, 296, 48), (2181, 70, 200), (7391, 43, 96), (22, 1541, 896), (4668, 859,
+     8), (186, 160, 3824), (412, 20, 3672), (4325, 252, 200), (1296, 22, 1160), (124, 1530, 160), (375, 2712, 40), (4099, 460, 16), (2646, 360, 32),
+     (267, 258, 3688), (586, 271, 3600), (9565, 1, 3224), (18, 2006, 920), (237, 1586, 1056), (1164, 528, 3392), (2790, 20, 936), (2844, 7, 1576), (4,
+     2467, 3496), (652, 2449, 1040), (10658, 1743, 160)]
+PLANS_32 = [(29, 359, 2888), (262, 48, 2408), (551, 182, 312), (7391, 43, 96), (60, 3056, 176), (237, 4767, 32), (75, 134, 3512), (412, 20, 3672), (2181, 70,
+     200), (1307, 60, 384), (179, 586, 288), (838, 4719, 8), (1083, 434, 64), (2118, 296, 48)]
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [p + ("bf16",) for p in PLANS_16] + [p + ("f16",) for p in PLANS_16[::3]] + [p + ("f32",) for p in PLANS_32])
+def test_backward_of_every_plan(M, m, n, k, dtype):
+    announce("matmul_abt_gated_backward plans %s" % ((m, n, k, dtype),))
+    x, gate, up, dc = operands(m, n, k, dtype, seed=6, with_dc=True)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    kept = tuple((torch.randn((m, n), generator=g, device="cuda") * 1.5).to(x.dtype) for _ in range(2))
+    both = check_backward(M, dc, x, gate, up, kept, "silu")
+    da, _, _ = M.matmul_abt_gated_backward(dc, x, gate, up, kept, want_weight_grads=False)
+    _, db_gate, db_up = M.matmul_abt_gated_backward(dc, x, gate, up, kept, want_input_grad=False)
+    assert torch.equal(da, both[0]) and torch.equal(db_gate, both[1]) and torch.equal(db_up, both[2])
+
+
 def test_gradients_one_by_one(M):
     announce("matmul_abt_gated_backward parts")
     x, gate, up, dc = operands(100, 130, 72, "bf16", with_dc=True)

@@ -163,6 +163,28 @@ def test_large_logits_gathered_in_few_lanes(P):
         assert torch.equal(out[2].cpu(), at[:, :32].int().repeat(260, 1))
 
 
+# rows in chunks, whose own alternatives meet: the largest logits all in one chunk, a few in each, alike, or fewer than are asked for
+@pytest.mark.parametrize("rows,cols", [(2, 69474), (1, 32003), (90, 6001), (200, 4100), (1, 131072)])
+@pytest.mark.parametrize("top", [1, 2, 7, 31, 32])
+def test_alternatives_of_chunks(P, rows, cols, top):
+    announce("token_log_probs top of chunks %s" % ((rows, cols, top),))
+    x, t = logits(rows, cols, "bf16", seed=21)
+    at = torch.arange(cols)
+    for row in range(0, rows, 2):
+        kind = row // 2 % 5 if rows > 10 else (top + row) % 5
+        if kind == 0:
+            x[row] = (at / 256).to(x.dtype)                                 # the last chunk's, many alike
+        elif kind == 1:
+            x[row] = ((at * 7919) % 251).to(x.dtype)                        # every chunk has some of the largest
+        elif kind == 2:
+            x[row] = 1.25
+        elif kind == 3:
+            x[row] = torch.where(at % (cols // 20) == 3, x[row], torch.full_like(x[row], -INF))
+        else:
+            x[row, 1000:1040] = 30 + torch.arange(40).flip(0).to(x.dtype) / 4  # one chunk's alone
+    check_forward(P, x, t, top=top)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_every_value_sorted(P, dtype):
     announce("token_log_probs sorted " + dtype)
