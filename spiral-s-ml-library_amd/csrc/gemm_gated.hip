@@ -850,7 +850,10 @@ struct BackwardPlan {
 // Estimated time of n1 workgroups of t1 us, the longer ones, and then n2 of t2, each to the slot that is free first.
 static double both_us(double slots, double n1, double t1, double n2, double t2) {
     const double rounds = (double)(int64_t)(n1 / slots), late = n1 - rounds * slots;        // `late` slots have one round more of the first
-    if (n1 * t1 + n2 * t2 > 64 * slots * t1) return (n1 * t1 + n2 * t2) / slots + t2;
+    if (n1 + n2 > 64 * slots) {                            // (many rounds: the last one is not looked at)
+        const double all = (n1 * t1 + n2 * t2) / slots + t2, first = (late > 0 ? rounds + 1 : rounds) * t1;
+        return all > first ? all : first;
+    }
     double count[2] = {late, slots - late}, at[2] = {(rounds + 1) * t1, rounds * t1};
     while (n2 > 0) {
         const int next = count[0] > 0 && at[0] < at[1] ? 0 : 1;
