@@ -726,11 +726,11 @@ __global__ __launch_bounds__(256) void gated_grad_kernel(const GatedGradArgs g) 
 
 static long gated_ceil(long a, long b) { return (a + b - 1) / b; }
 
-constexpr long MOST_TILES = 1l << 22;         // (a launch holds fewer than 2^32 work items: two such products of 512)
+constexpr double MOST_ITEMS = 4294967296.0;     // a launch holds fewer than 2^32 work items
 template <int MODE, int BM, int BN>
 static bool set_tiles(GatedArgs& g, int group_m) {
     const long tiles_m = MODE == MM_WEIGHTS ? 2 * gated_ceil(g.N, BM) : gated_ceil(g.M, BM), tiles_n = MODE == MM_FORWARD ? gated_ceil(g.N, BN / 2) : gated_ceil(g.K, BN);
-    if (tiles_m * tiles_n >= MOST_TILES) return false;
+    if (tiles_m * tiles_n >= 1l << 24) return false;
     g.tiles_m = (int)tiles_m;
     g.tiles_n = (int)tiles_n;
     g.group_m = group_m == 0 ? g.tiles_m : group_m;        // 0: the tiles of one panel of weights stand side by side
@@ -738,6 +738,7 @@ static bool set_tiles(GatedArgs& g, int group_m) {
 }
 template <typename Kernel, typename Args>
 static int launch_lds(const char* what, Kernel kernel, unsigned blocks, unsigned threads, int lds_bytes, const Args& args, hipStream_t stream) {
+    if ((double)blocks * threads >= MOST_ITEMS) return fail(SP_ERR_SHAPE, "%s: too large", what);
     if (const int rc = ensure_dynamic_lds((const void*)kernel, lds_bytes); rc != SP_OK) return rc;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), lds_bytes, stream, args);
     return check_launch(what);
@@ -789,6 +790,7 @@ struct MmCost {
     float lone, work, overhead;
 };
 enum { SPLIT_16, SPLIT_32, TILE_32_BLOCKS, TILE_64, TILE_64_BLOCKS, TILE_128, TILE_128_WIDE, TILE_256 };
+static int threads_of(int id) { return id <= TILE_64 ? 256 : 512; }
 static const MmCost kForward16[] = {{SPLIT_16, 16, 16, 3, true, 0.156f, 0.278f, 2.55f}, {SPLIT_32, 32, 16, 2, true, 0.336f, 0.387f, 2.65f}, {TILE_64, 64, 32, 2, false, 0.227f, 0.183f, 2.57f},
                                     {TILE_128, 128, 64, 1, false, 0.437f, 0.386f, 3.84f}, {TILE_128_WIDE, 128, 128, 1, false, 0.716f, 0.4f, 4.67f}, {TILE_256, 256, 128, 1, false, 1.2f, 0.1f, 5.95f}};
 static const MmCost kForward32[] = {{SPLIT_16, 16, 16, 3, true, 0.587f, 0.354f, 2.47f}, {SPLIT_32, 32, 16, 2, true, 0.587f, 0.632f, 3.2f}, {TILE_64, 64, 32, 5, false, 0.633f, 0.54f, 2.4f}};
@@ -830,7 +832,7 @@ static int cheapest(const MmCost (&menu)[N], bool f32, long M, long N_, long K) 
     double best_us = 0;
     for (const MmCost& c : menu) {
         const MmWork w = work_of(c, MM_FORWARD, f32, M, N_, K);
-        if (w.tiles >= MOST_TILES) continue;
+        if (w.tiles * threads_of(c.id) >= MOST_ITEMS) continue;
         const double round = (double)cus * c.per_unit, full = (double)(int64_t)(w.tiles / round), rest = w.tiles - full * round;
         const long k_tiles = tiles_of_k(c, w.nk, 1);
         const double us = full * group_us(c, k_tiles, c.per_unit) + (rest > 0 ? group_us(c, k_tiles, (double)(int64_t)((rest + cus - 1) / cus)) : 0);
@@ -870,7 +872,7 @@ static BackwardPlan plan_of(const MmCost (&inputs)[N_], const MmCost (&weights)[
     for (size_t i = 0; i < N_; ++i) {
         const MmCost &ci = inputs[i], &cw = weights[i];
         const MmWork wi = work_of(ci, MM_INPUT, f32, M, N, K), ww = work_of(cw, MM_WEIGHTS, f32, M, N, K);
-        if (wi.tiles >= MOST_TILES || ww.tiles >= MOST_TILES) continue;
+        if ((wi.tiles + ww.tiles) * threads_of(ci.id) >= MOST_ITEMS) continue;
         // shares of K about as long as one another's
         const double li = wi.nk * (ci.split ? 0.25 : 1.0) * ci.work, lw = ww.nk * cw.work;
         for (int n = 1; n <= 16; ++n) {
@@ -938,7 +940,7 @@ static int gated_forward(const GatedArgs& g, hipStream_t stream) {
         if (id == TILE_128_WIDE) return launch_forward<DT, 128, 256, 4, 2, 3>(what, g, stream);
         return launch_forward<DT, 256, 256, 4, 2, 2>(what, g, stream);
     }
-    return fail(SP_ERR_UNSUPPORTED, "%s: no kernel", what);
+    return fail(SP_ERR_SHAPE, "%s: too large", what);
 }
 
 template <int DT>

@@ -311,6 +311,17 @@ def test_results_behind_four_gib(M):
     assert torch.equal(dg, small[1]) and torch.equal(du, small[2])
 
 
+# more workgroups than a launch of 1024 work items each could hold
+def test_f32_results_of_many_tiles(M):
+    announce("matmul_abt_gated 4194368 tiles")
+    m, n, k = 1 << 20, 8193, 4
+    x, gate, up = operands(m, n, k, "f32", seed=10)
+    c = M.matmul_abt_gated(x, gate, up, "relu")
+    for rows in (slice(0, 40), slice(m // 2 - 3, m // 2 + 70), slice(m - 40, m)):
+        few = M.matmul_abt_gated(x[rows].contiguous(), gate, up, "relu")
+        assert torch.equal(c[rows], few)                 # one K-tile: one order of the sum in every kernel
+
+
 # ---- as they are used ----
 
 def test_repeats_bit_for_bit_and_on_two_streams(M):
