@@ -437,6 +437,17 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gated_forward_kernel(const Gat
     gated_mm<DT, MM_FORWARD, BM, BN, WM, WN, NS>(g, blockIdx.x, 0, 1);
 }
 
+// Tiles of 256 x 256 and, below them, of 128 x 256: the last round of the large ones is seldom a full one, and the small ones fill the units that it leaves.
+struct GatedRows {
+    GatedArgs large, small;
+    unsigned large_blocks;
+};
+template <int DT>
+__global__ __launch_bounds__(512, 2) void gated_forward_rows_kernel(const GatedRows p) {
+    if (blockIdx.x < p.large_blocks) gated_mm<DT, MM_FORWARD, 256, 256, 4, 2, 2>(p.large, blockIdx.x, 0, 1);
+    else gated_mm<DT, MM_FORWARD, 128, 256, 4, 2, 3>(p.small, blockIdx.x - p.large_blocks, 0, 1);
+}
+
 // Both products of the backward pass in one launch, or one of them: neither waits for the other, and the tiles of one fill the units that the other's leave.
 struct GatedPair {
     GatedArgs input, weights;
@@ -758,6 +769,31 @@ static int launch_forward_split(const char* what, GatedArgs g, hipStream_t strea
     return launch_lds(what, gated_forward_split_kernel<DT, TM, TN, NS>, (unsigned)(g.tiles_m * g.tiles_n), 256, split_lds(TM, TN, NS), g, stream);
 }
 
+// The first `rows` rows in tiles of 256 x 256, the others in tiles of 128 x 256.
+template <int DT>
+static int launch_forward_rows(const char* what, const GatedArgs& g, long rows, hipStream_t stream) {
+    constexpr long ES = ELEM_BYTES<DT>;
+    GatedRows p{g, g, 0};
+    p.large.M = rows;
+    p.small.M = g.M - rows;
+    p.small.A = g.A + rows * g.K * ES;
+    p.small.C0 = (unsigned char*)g.C0 + rows * g.N * ES;
+    if (g.keep != KEEP_NONE) {
+        const long bytes = rows * (g.keep == KEEP_F8 ? (g.N + 15) / 16 * 16 : g.N * ES);
+        p.small.gate = (unsigned char*)g.gate + bytes;
+        p.small.up = (unsigned char*)g.up + bytes;
+    }
+    if (g.keep == KEEP_F8) {
+        const long blocks = rows * ((g.N + QB - 1) / QB);
+        p.small.gate_scale = g.gate_scale + blocks;
+        p.small.up_scale = g.up_scale + blocks;
+    }
+    if (!set_tiles<MM_FORWARD, 256, 256>(p.large, 4) || !set_tiles<MM_FORWARD, 128, 256>(p.small, 4)) return fail(SP_ERR_SHAPE, "%s: too large", what);
+    p.large_blocks = (unsigned)(p.large.tiles_m * p.large.tiles_n);
+    const unsigned blocks = p.large_blocks + (unsigned)(p.small.tiles_m * p.small.tiles_n);
+    return launch_lds(what, gated_forward_rows_kernel<DT>, blocks, 512, larger(mm_lds(256, 256, 2), mm_lds(128, 256, 3)), p, stream);
+}
+
 // Those of the two products that have parts; the longer ones' workgroups first.
 static unsigned set_pair(GatedPair& p, bool input_first) {
     const unsigned input = p.input_parts * (unsigned)(p.input.tiles_m * p.input.tiles_n), weights = p.weights_parts * (unsigned)(p.weights.tiles_m * p.weights.tiles_n);
@@ -826,10 +862,9 @@ static double join_us(const MmWork& w, int parts, bool f32) { return parts > 1 ?
 static bool may_split(const MmWork& w, int parts) { return parts == 1 || (w.tiles * parts <= 2.0 * device_cu_count() && w.nk >= 4l * parts); }
 
 template <size_t N>
-static int cheapest(const MmCost (&menu)[N], bool f32, long M, long N_, long K) {
+static int cheapest(const MmCost (&menu)[N], bool f32, long M, long N_, long K, double& best_us) {
     const long cus = device_cu_count();
     int best = -1;
-    double best_us = 0;
     for (const MmCost& c : menu) {
         const MmWork w = work_of(c, MM_FORWARD, f32, M, N_, K);
         if (w.tiles * threads_of(c.id) >= MOST_ITEMS) continue;
@@ -844,11 +879,6 @@ static int cheapest(const MmCost (&menu)[N], bool f32, long M, long N_, long K) 
     return best;
 }
 
-// The tile and the parts of both products of the backward pass, also where one alone is wanted: a gradient does not depend on whether the other is.
-struct BackwardPlan {
-    int id, input_parts, weights_parts;
-    bool input_first;
-};
 // Estimated time of n1 workgroups of t1 us, the longer ones, and then n2 of t2, each to the slot that is free first.
 static double both_us(double slots, double n1, double t1, double n2, double t2) {
     const double rounds = (double)(int64_t)(n1 / slots), late = n1 - rounds * slots;        // `late` slots have one round more of the first
@@ -864,6 +894,29 @@ static double both_us(double slots, double n1, double t1, double n2, double t2) 
     }
     return count[0] > 0 && at[0] > at[1] ? at[0] : at[1];
 }
+// How many rows to take in tiles of 256 x 256 where the others take 128 x 256: all of them, unless less than `us` comes out.
+// (us, all in large ones / so: 3000 x 2048 x 5461 bf16 136 / 123, 5008 x 2048 x 5461 with 8-bit blocks 210 / 201; steps of both directions, which the part's power limits, 404 / 393 and 606 / 600.)
+template <size_t N>
+static long rows_of_large(const MmCost (&menu)[N], long M, long N_, long K, double us) {
+    const MmCost &small = menu[N - 2], &large = menu[N - 1];
+    const long cus = device_cu_count(), nk = gated_ceil(K, 64), tiles_n = gated_ceil(N_, large.bn), tiles_m = gated_ceil(M, large.bm);
+    const long tail = 2 * gated_ceil(cus, tiles_n), fewest = tiles_m - 1 < tail ? 1 : tiles_m - tail;        // what two rounds take, and a bound for the search
+    const double t1 = group_us(large, nk, 1), t2 = group_us(small, nk, 1);
+    long best = M;
+    for (long rows = tiles_m - 1; rows >= fewest && rows >= tiles_m - 64; --rows) {
+        const double one = both_us((double)cus, (double)(rows * tiles_n), t1, (double)(gated_ceil(M - rows * large.bm, small.bm) * tiles_n), t2);
+        if (one < us) {
+            us = one;
+            best = rows * large.bm;
+        }
+    }
+    return best;
+}
+// The tile and the parts of both products of the backward pass, also where one alone is wanted: a gradient does not depend on whether the other is.
+struct BackwardPlan {
+    int id, input_parts, weights_parts;
+    bool input_first;
+};
 template <size_t N_>
 static BackwardPlan plan_of(const MmCost (&inputs)[N_], const MmCost (&weights)[N_], bool f32, long M, long N, long K) {
     const long cus = device_cu_count();
@@ -925,9 +978,10 @@ template <int DT>
 static int gated_forward(const GatedArgs& g, hipStream_t stream) {
     constexpr bool F32 = DT == SP_F32;
     const char* const what = "sp_gemm_abt_gated";
+    double us = 0;
     int id;
-    if (g.keep == KEEP_F8) id = F32 ? cheapest(kBlocks32, F32, g.M, g.N, g.K) : cheapest(kBlocks16, F32, g.M, g.N, g.K);
-    else id = F32 ? cheapest(kForward32, F32, g.M, g.N, g.K) : cheapest(kForward16, F32, g.M, g.N, g.K);
+    if (g.keep == KEEP_F8) id = F32 ? cheapest(kBlocks32, F32, g.M, g.N, g.K, us) : cheapest(kBlocks16, F32, g.M, g.N, g.K, us);
+    else id = F32 ? cheapest(kForward32, F32, g.M, g.N, g.K, us) : cheapest(kForward16, F32, g.M, g.N, g.K, us);
     switch (id) {
         case SPLIT_16: return launch_forward_split<DT, 1, 2, 2>(what, g, stream);
         case SPLIT_32: return launch_forward_split<DT, 2, 2, 2>(what, g, stream);
@@ -937,6 +991,8 @@ static int gated_forward(const GatedArgs& g, hipStream_t stream) {
     }
     if constexpr (!F32) {
         if (id == TILE_128) return launch_forward<DT, 128, 128, 2, 4, 4>(what, g, stream);
+        const long rows = g.keep == KEEP_F8 ? rows_of_large(kBlocks16, g.M, g.N, g.K, us) : rows_of_large(kForward16, g.M, g.N, g.K, us);
+        if (rows < g.M) return launch_forward_rows<DT>(what, g, rows, stream);
         if (id == TILE_128_WIDE) return launch_forward<DT, 128, 256, 4, 2, 3>(what, g, stream);
         return launch_forward<DT, 256, 256, 4, 2, 2>(what, g, stream);
     }

@@ -158,6 +158,16 @@ def test_kept(M, m, n, k, dtype, keep):
     assert c.shape == (m, n)
 
 
+# large tiles and, for the rows behind them, smaller ones
+@pytest.mark.parametrize("m,n,k", [(5043, 1542, 8), (1795, 4555, 72), (2389, 3359, 128), (3440, 2411, 200), (3000, 5461, 64)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("keep", ["none", "whole", "f8"])
+def test_rows_in_two_tiles(M, m, n, k, dtype, keep):
+    announce("matmul_abt_gated two tiles %s" % ((m, n, k, dtype, keep),))
+    x, gate, up = operands(m, n, k, dtype, seed=11)
+    check_forward(M, x, gate, up, "silu", keep={"none": None, "whole": x.dtype, "f8": F8}[keep])
+
+
 def test_f32_in_multiples_of_four(M):
     for m, n, k in ((5, 7, 4), (70, 130, 12), (100, 65, 36)):
         announce("matmul_abt_gated f32 %s" % ((m, n, k),))
