@@ -912,15 +912,38 @@ static long rows_of_large(const MmCost (&menu)[N], long M, long N_, long K, doub
     }
     return best;
 }
-// The tile and the parts of both products of the backward pass, also where one alone is wanted: a gradient does not depend on whether the other is.
+// Long products are limited by the part's power, of which smaller tiles take more.
+static double of_power(double us, int id, bool f32) { return !f32 && id != TILE_256 && us > 100 ? us + 0.2 * (us - 100) : us; }
+
+// The tile and the parts of both products of the backward pass, and the tiles of one alone.  Tiles add up a K-tile after the other, all in the same order, so with the same parts a gradient has
+// the same bits whether the other is wanted or not; where four waves share K, the kernel is the same, too.  (A lone gradient, us, on the tile of both / on its own: of the input,
+// 2048 x 2048 x 5461 bf16 149 / 114, 4096 x 1024 x 4096 134 / 109; of the weights, 2048 x 1024 x 2736 45 / 37; the wrong way, 2048 x 1024 x 2736, input, 46 / 51.)
 struct BackwardPlan {
     int id, input_parts, weights_parts;
     bool input_first;
+    int input_id, weights_id;
 };
+template <size_t N_>
+static int tile_alone(const MmCost (&menu)[N_], int mode, bool f32, int parts, long M, long N, long K, int otherwise) {
+    const long cus = device_cu_count();
+    double best_us = 0;
+    int best = otherwise;
+    for (size_t i = 1; i < N_; ++i) {                      // (behind the one whose waves share K)
+        const MmCost& c = menu[i];
+        const MmWork w = work_of(c, mode, f32, M, N, K);
+        if (c.per_unit == 0 || w.tiles * parts * threads_of(c.id) >= MOST_ITEMS) continue;
+        const double alone = both_us((double)cus * c.per_unit, w.tiles * parts, group_us(c, tiles_of_k(c, w.nk, parts), c.per_unit), 0, 1), us = of_power(alone, c.id, f32);
+        if (best_us == 0 || us < best_us) {
+            best_us = us;
+            best = c.id;
+        }
+    }
+    return best;
+}
 template <size_t N_>
 static BackwardPlan plan_of(const MmCost (&inputs)[N_], const MmCost (&weights)[N_], bool f32, long M, long N, long K) {
     const long cus = device_cu_count();
-    BackwardPlan best{-1, 1, 1, true};
+    BackwardPlan best{-1, 1, 1, true, -1, -1};
     double best_us = 0;
     for (size_t i = 0; i < N_; ++i) {
         const MmCost &ci = inputs[i], &cw = weights[i];
@@ -947,13 +970,17 @@ static BackwardPlan plan_of(const MmCost (&inputs)[N_], const MmCost (&weights)[
                 tw = group_us(cw, kw, on_unit);
                 us = ti > tw ? both_us(cus * on_unit, ni, ti, nw, tw) : both_us(cus * on_unit, nw, tw, ni, ti);
             }
-            if (!f32 && ci.id != TILE_256 && us > 100) us += 0.2 * (us - 100);        // long products are limited by the part's power, of which smaller tiles take more
+            us = of_power(us, ci.id, f32);
             if (pi > 1 || pw > 1) us += JOIN_US + join_us(wi, pi, f32) + join_us(ww, pw, f32);
             if (best.id < 0 || us < best_us) {
-                best = {ci.id, pi, pw, ti > tw};
+                best = {ci.id, pi, pw, ti > tw, ci.id, ci.id};
                 best_us = us;
             }
         }
+    }
+    if (best.id > SPLIT_32) {
+        best.input_id = tile_alone(inputs, MM_INPUT, f32, best.input_parts, M, N, K, best.id);
+        best.weights_id = tile_alone(weights, MM_WEIGHTS, f32, best.weights_parts, M, N, K, best.id);
     }
     return best;
 }
@@ -1023,7 +1050,8 @@ static int gated_backward(GatedArgs input, GatedArgs weights, const GatedGradArg
     const BackwardPlan plan = choose_backward(DT == SP_F32, grad.M, grad.N, input.K);
     const unsigned input_parts = input.C0 != nullptr ? plan.input_parts : 0, weights_parts = weights.C0 != nullptr ? plan.weights_parts : 0;
     if (plan.input_parts > 1) weights.parts = input.parts + (long)plan.input_parts * input.M * input.K;
-    if (const int rc = backward_products<DT>(plan.id, GatedPair{input, weights, 0, 0, input_parts, weights_parts}, plan.input_first, stream); rc != SP_OK) return rc;
+    const int id = weights_parts == 0 ? plan.input_id : input_parts == 0 ? plan.weights_id : plan.id;
+    if (const int rc = backward_products<DT>(id, GatedPair{input, weights, 0, 0, input_parts, weights_parts}, plan.input_first, stream); rc != SP_OK) return rc;
     if (input_parts <= 1 && weights_parts <= 1) return SP_OK;
     GatedJoin join{input.parts, weights.parts, (int)input_parts, (int)weights_parts, input_parts > 1 ? input.M * input.K : 0, weights_parts > 1 ? 2 * weights.N * weights.K : 0,
                    input.C0, weights.C0, weights.C1};
