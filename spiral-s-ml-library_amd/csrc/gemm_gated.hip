@@ -37,9 +37,25 @@ struct GatedArgs {
 };
 
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504088896340736f)); }
+// Phi(g) of the normal distribution, and e^(-g^2 / 2).  Not (1 + erf(g / sqrt 2)) / 2, which loses the lower tail: half a percent of GELU at -4.5 and the whole of it at -5.6.
+// Phi(-a) e^(a^2 / 2) is t times a polynomial of t = 1 / (1 + 0.35 a), fitted by weighted least squares to a relative error of 3.2e-8 where Phi is a f32 (a to 13.3); in f32, with the
+// exponential, (1.3 g^2 + 11) roundings off at most.  It has no branch: 8192 x 2048 x 8192 bf16 forward with GELU takes 415 us, 440 with erff, 460 with erfcf.
+__device__ __forceinline__ float below_normal(float g, float& bell) {
+    constexpr float C[9] = {0.13962166f, 0.13985756f, 0.119863085f, 0.105392143f, -0.0228434224f, 0.158796564f, -0.255391002f, 0.143818408f, -0.0291150156f};
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(g), 0.35f, 1.f));
+    float v = C[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) v = __builtin_fmaf(v, t, C[i]);
+    bell = __builtin_amdgcn_exp2f(g * g * -0.72134752044448170368f);
+    const float tail = bell * (v * t);
+    return g < 0.f ? tail : 1.f - tail;
+}
 __device__ __forceinline__ float gated_activation(float g, int kind) {
     if (kind == SP_ACT_SILU) return g * sigmoid(g);
-    if (kind == SP_ACT_GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752440f));
+    if (kind == SP_ACT_GELU) {
+        float bell;
+        return g * below_normal(g, bell);
+    }
     return g < 0.f ? 0.f : g;                              // (a NaN stays)
 }
 // act(g) and act'(g).
@@ -49,9 +65,10 @@ __device__ __forceinline__ void activation_and_slope(float g, int kind, float& a
         act = g * s;
         slope = s * __builtin_fmaf(g, 1.f - s, 1.f);
     } else if (kind == SP_ACT_GELU) {
-        const float below = 0.5f * (1.f + erff(g * 0.70710678118654752440f));
+        float bell;
+        const float below = below_normal(g, bell);
         act = g * below;
-        slope = __builtin_fmaf(g * 0.39894228040143267794f, __builtin_amdgcn_exp2f(g * g * -0.72134752044448170368f), below);
+        slope = __builtin_fmaf(g * 0.39894228040143267794f, bell, below);
     } else {
         act = g < 0.f ? 0.f : g;
         slope = g > 0.f ? 1.f : 0.f;
