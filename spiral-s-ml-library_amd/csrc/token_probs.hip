@@ -422,10 +422,13 @@ __global__ __launch_bounds__(256) void token_grad_kernel(const void* logits, lon
     const bool counts = (unsigned)token < (unsigned)cols, none = lse == -INFINITY;
     const float of_token = a.d_logp != nullptr && counts && !none ? a.d_logp[row] : 0.f;
     float slope = 0.f, all = of_token;                     // dx = [j = t] of_token - p (all + slope ln p)
-    if (a.d_lse != nullptr) all -= a.d_lse[row];
+    // (a row of nothing hands an infinity back through an lse of -inf: p is 0 there, and 0 times it must stay 0)
+    if (a.d_lse != nullptr && !none) all -= a.d_lse[row];
     if constexpr (ENTROPY) {
-        slope = a.d_entropy[row];
-        all = __builtin_fmaf(slope, a.entropy[row], all);
+        if (!none) {
+            slope = a.d_entropy[row];
+            all = __builtin_fmaf(slope, a.entropy[row], all);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
