@@ -13,8 +13,10 @@ Every timed case is checked against the oracle after its timed loop, and the com
 reported next to it (`shader_clock_mhz`; the matrix-pipe peak is quoted at 2400 MHz, power-limited kernels run below).
 """
 import argparse
+import hashlib
 import json
 import os
+import re
 import sys
 import time
 
@@ -149,6 +151,21 @@ def calibrate_hbm(steps, warmup):
     print(json.dumps({"hbm_calibration": out, "unit": "GB/s", "peak": PEAK_HBM_GBS, "steps": steps, "warmup": warmup,
                       "kernels": "sp_map_f32(copy): n bytes read + n written; sp_reduce_sum(f32): n bytes read; "
                                  "torch.Tensor.fill_: n bytes written"}))
+
+
+def source_hash(src, csrc=os.path.join(ROOT, "spiral-s-ml-library_amd", "csrc")):
+    """sha256 over a kernel source and the headers of its directory that it includes, directly or through others, in name order."""
+    headers, texts = set(), [src]
+    while texts:
+        with open(os.path.join(csrc, texts.pop()), encoding="utf-8") as f:
+            found = {n for n in re.findall(r'^#include "(.+)"', f.read(), re.M) if os.path.exists(os.path.join(csrc, n))} - headers
+        headers |= found
+        texts += found
+    h = hashlib.sha256()
+    for name in [src] + sorted(headers):
+        with open(os.path.join(csrc, name), "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
 
 
 def main():
@@ -532,18 +549,8 @@ def main():
     # was measured on.  A figure is only copied into the line while that source is unchanged: after an edit it is
     # stale until the counters have been collected again, and the line says so instead.
     try:
-        import hashlib
         with open(os.path.join(ROOT, "profiles", "traffic.json")) as f:
             measured = json.load(f)
-
-        def source_hash(src):
-            """sha256 over a kernel source and the headers of its directory, in name order."""
-            csrc = os.path.join(ROOT, "spiral-s-ml-library_amd", "csrc")
-            h = hashlib.sha256()
-            for name in [src] + sorted(n for n in os.listdir(csrc) if n.endswith(".h")):
-                with open(os.path.join(csrc, name), "rb") as fh:
-                    h.update(fh.read())
-            return h.hexdigest()
 
         def source_unchanged(entry):
             src = entry.get("source")
