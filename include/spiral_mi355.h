@@ -180,7 +180,8 @@ int sp_gemm_abt_scaled(int f8_a, int f8_b, int dtype_out, const void* A, const f
 
 /*
  * A gated feed-forward block: C = act(A . B_gate^T) * (A . B_up^T), element by element.  A (M, K), B_gate, B_up (N, K), C (M, N), all of `dtype` (SP_F32, SP_F16,
- * SP_BF16), row-major; K a multiple of 16 bytes (8; 4 for f32), any M and N.  Sums, activation and product are f32, rounded once; C must not overlap the operands.
+ * SP_BF16), row-major; K a multiple of 16 bytes (8; 4 for f32), any M and N.  Sums, activation and product are f32, rounded once.  Results must not overlap
+ * the operands or one another (SP_ERR_ARG).
  *   SP_ACT_SILU g / (1 + exp(-g)),  SP_ACT_GELU g (1 + erf(g / sqrt 2)) / 2,  SP_ACT_RELU max(0, g)
  * gate, up: NULL, or what the backward pass takes, g = A . B_gate^T and u = A . B_up^T, of kept_dtype: dtype, (M, N) each; or SP_F8_E4M3, in the blocks of 1 x 128 of sp_quantize_blocks,
  * (M, N rounded up to 16) each with gate_scale, up_scale (M, ceil(N / 128)) f32.  Either way they are rounded once, from f32.
@@ -193,7 +194,8 @@ int sp_gemm_abt_gated(int dtype, int activation, const void* A, const void* B_ga
 /*
  * Its gradients from dC (M, N), at the g and u that were kept:  dg = dC u act'(g), du = dC act(g), rounded to dtype, and
  *   dA = dg . B_gate + du . B_up (M, K),   dB_gate = dg^T . A, dB_up = du^T . A (N, K)
- * in dtype, of f32 sums.  dA may be NULL, and dB_gate with dB_up.  The ReLU's slope at 0 is 0.  Every sum has one order: results repeat bit for bit, whichever
+ * in dtype, of f32 sums.  dA may be NULL, and dB_gate with dB_up.  The gradients and the workspace must not overlap A, the weights or one another, nor the workspace
+ * anything else (SP_ERR_ARG); a gradient may lie over dC, gate and up, which have been read by then.  The ReLU's slope at 0 is 0.  Every sum has one order: results repeat bit for bit, whichever
  * of the gradients are wanted.
  * `workspace`: sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K) bytes of device memory that hold dg, du and partial sums during the call (what they held before does not matter).  Calls
  * that may run at the same time need one each.

@@ -13,6 +13,7 @@
 // of a stage is in registers then, and the next one has landed.
 // K may end anywhere: what is missing of the last K-tile comes from zeros, and that tile goes first, so that the loop has whole ones only.
 #include "f8_blocks.h"
+#include "overlap.h"
 
 namespace sp {
 
@@ -1091,6 +1092,9 @@ using namespace sp;
 
 // Columns of either half of the backward pass's workspace: whole K-tiles, of 64 numbers of 16 bits (two of f32).
 static int64_t gated_half(int64_t N) { return (N + 63) / 64 * 64; }
+// Bytes of either kept factor, and of its scales.
+static int64_t gated_kept_bytes(bool f8, int es, int64_t M, int64_t N) { return M * (f8 ? (N + 15) / 16 * 16 : N * es); }
+static int64_t gated_scale_bytes(bool f8, int64_t M, int64_t N) { return f8 ? M * ((N + QB - 1) / QB) * 4 : 0; }
 
 static int gated_sizes(const char* fn, int dtype, int activation, int kept, bool keeps, int64_t M, int64_t N, int64_t K) {
     if (dtype != SP_F32 && dtype != SP_F16 && dtype != SP_BF16) return fail(SP_ERR_DTYPE, "%s: dtype must be f32, f16 or bf16, got %d", fn, dtype);
@@ -1120,12 +1124,19 @@ extern "C" int sp_gemm_abt_gated(int dtype, int activation, const void* A, const
     const bool f8 = keeps && kept_dtype == SP_F8_E4M3;
     if (keeps && (gate == nullptr || up == nullptr)) return fail(SP_ERR_NULL, "sp_gemm_abt_gated: gate and up go together");
     if (f8 && (gate_scale == nullptr || up_scale == nullptr)) return fail(SP_ERR_NULL, "sp_gemm_abt_gated: numbers and their scales go together");
+    const int es = dtype == SP_F32 ? 4 : 2;
+    const int64_t kept_bytes = gated_kept_bytes(f8, es, M, N), scale_bytes = gated_scale_bytes(f8, M, N);
+    if (const int rc = lie_apart(__func__, {{"C", C, M * N * es}, {"gate", gate, kept_bytes}, {"up", up, kept_bytes},
+                                  {"gate_scale", f8 ? gate_scale : nullptr, scale_bytes}, {"up_scale", f8 ? up_scale : nullptr, scale_bytes}},
+                                 {{"A", A, M * K * es}, {"B_gate", B_gate, N * K * es}, {"B_up", B_up, N * K * es}});
+        rc != SP_OK)
+        return rc;
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     GatedArgs g{};
     g.A = (const unsigned char*)A; g.B0 = (const unsigned char*)B_gate; g.B1 = (const unsigned char*)B_up; g.C0 = C; g.gate = gate; g.up = up;
     g.gate_scale = gate_scale; g.up_scale = up_scale; g.M = M; g.N = N; g.K = K; g.activation = activation; g.keep = f8 ? KEEP_F8 : keeps ? KEEP_WHOLE : KEEP_NONE;
     // what does not stay in the caches (32 MiB of L2) is streamed past them, gate and up only where a row is of whole lines (5008 x 2048 x 5461 bf16: 205 us, 225 streamed)
-    const int64_t pitch = N * (dtype == SP_F32 ? 4 : 2);
+    const int64_t pitch = N * es;
     g.stream = M * pitch <= (int64_t)32 << 20 ? 0 : pitch % 128 == 0 ? 3 : 1;
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == SP_F32) return gated_forward<SP_F32>(g, st);
@@ -1167,14 +1178,25 @@ extern "C" int sp_gemm_abt_gated_backward(int dtype, int activation, const void*
     if (dA == nullptr && dB_gate == nullptr) return fail(SP_ERR_NULL, "sp_gemm_abt_gated_backward: no gradient is wanted");
     const int64_t half = gated_half(N);
     if (M * (half / 8) > ((int64_t)1 << 32) - 256) return fail(SP_ERR_SHAPE, "sp_gemm_abt_gated_backward: too large");
-    if (workspace_bytes < sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K))
-        return fail(SP_ERR_ARG, "sp_gemm_abt_gated_backward: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes,
-                    (long long)sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K));
+    const int64_t need = sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K);
+    if (workspace_bytes < need)
+        return fail(SP_ERR_ARG, "sp_gemm_abt_gated_backward: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+    // (dC, gate and up are read by the first launch alone, before any gradient is written: a gradient may take their place)
+    const int es = dtype == SP_F32 ? 4 : 2;
+    const int64_t kept_bytes = gated_kept_bytes(f8, es, M, N), scale_bytes = gated_scale_bytes(f8, M, N);
+    if (const int rc = lie_apart(__func__, {{"dA", dA, M * K * es}, {"dB_gate", dB_gate, N * K * es}, {"dB_up", dB_up, N * K * es}, {"workspace", workspace, need}},
+                                 {{"A", A, M * K * es}, {"B_gate", B_gate, N * K * es}, {"B_up", B_up, N * K * es}});
+        rc != SP_OK)
+        return rc;
+    if (const int rc = lie_apart(__func__, {{"workspace", workspace, need}},
+                                 {{"dC", dC, M * N * es}, {"gate", gate, kept_bytes}, {"up", up, kept_bytes},
+                                  {"gate_scale", f8 ? gate_scale : nullptr, scale_bytes}, {"up_scale", f8 ? up_scale : nullptr, scale_bytes}});
+        rc != SP_OK)
+        return rc;
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     GatedGradArgs grad{};
     grad.dC = dC; grad.gate = gate; grad.up = up; grad.gate_scale = gate_scale; grad.up_scale = up_scale; grad.out = workspace; grad.M = M; grad.N = N; grad.half = half;
     grad.activation = activation;
-    const int es = dtype == SP_F32 ? 4 : 2;
     GatedArgs input{}, weights{};
     input.A = (const unsigned char*)workspace; input.B0 = (const unsigned char*)B_gate; input.B1 = (const unsigned char*)B_up; input.C0 = dA; input.M = M; input.N = N; input.K = K;
     input.half = half; input.parts = (float*)((unsigned char*)workspace + gated_halves_bytes(dtype, M, N)); input.stream = M * K * es > (int64_t)32 << 20;

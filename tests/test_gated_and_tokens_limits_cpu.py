@@ -1,0 +1,89 @@
+"""Memory and sizes that the gated block and the log probabilities of tokens refuse, and how near they go to that, without a GPU: what is taken ends at the missing device."""
+import ctypes as C
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses of the calls that are taken are made up")
+
+TAKEN, ARG, SHAPE = -7, -5, -2        # (TAKEN: nothing was refused, and then no device is there)
+
+
+@pytest.fixture(scope="module")
+def L():
+    from ml import _lib
+    return _lib
+
+
+class Caller:
+    """An entry point with arguments that are right, and what another value of some of them leads to."""
+
+    def __init__(self, L, name, order, good):
+        self.L, self.name, self.order, self.good = L, name, order.split(), good
+
+    def __call__(self, **other):
+        assert set(other) <= set(self.good)
+        rc = getattr(self.L.lib, self.name)(*[other.get(k, self.good[k]) for k in self.order], None)
+        said = self.L.lib.sp_last_error_string().decode()
+        return rc, said
+
+
+def places(**sizes):
+    """Addresses behind each other without a gap but for the 16-byte alignment, in an order of their own."""
+    at, out = 1 << 40, {}
+    for name, size in sizes.items():
+        out[name] = C.c_void_p(at)
+        at += -(-size // 16) * 16
+    return out
+
+
+def sweep(call, sizes, outs, may_meet):
+    """Every result moved over every other piece of memory, by its first and by its last 16 bytes: refused but for the pairs in may_meet; side by side all is taken."""
+    rc, said = call()
+    assert rc == TAKEN, said
+    address = lambda n: call.good[n].value
+    for o in outs:
+        for other in sizes:
+            if other == o:
+                continue
+            for at in (address(other), address(other) + sizes[other] - 16 & ~15, address(other) - (sizes[o] - 1 & ~15)):
+                meets = [n for n in sizes if n != o and at < address(n) + sizes[n] and address(n) < at + sizes[o]]
+                rc, said = call(**{o: C.c_void_p(at)})
+                bad = [n for n in meets if not may_meet(o, n)]
+                if bad:
+                    assert rc == ARG and "overlap" in said and o in said and any(n in said for n in bad), (o, other, meets, rc, said)
+                else:
+                    assert rc == TAKEN, (o, other, meets, said)
+
+
+@pytest.mark.parametrize("dtype,kept", [(2, 2), (0, 0), (1, 8), (0, 8)])
+def test_gated_results_over_operands(L, dtype, kept):
+    m, n, k = 37, 300, 64
+    es, f8 = (4 if dtype == 0 else 2), kept == 8
+    factor, scales = (m * 304, m * 3 * 4) if f8 else (m * n * es, 0)
+    sizes = dict(A=m * k * es, C=m * n * es, gate=factor, B_gate=n * k * es, up=factor, B_up=n * k * es)
+    if f8:
+        sizes.update(gate_scale=scales, up_scale=scales)
+    p = places(**sizes)
+    good = {**dict(dtype=dtype, act=0, kept=kept, gate_scale=None, up_scale=None, m=m, n=n, k=k), **p}
+    call = Caller(L, "sp_gemm_abt_gated", "dtype act A B_gate B_up C kept gate gate_scale up up_scale m n k", good)
+    sweep(call, sizes, [o for o in ("C", "gate", "up", "gate_scale", "up_scale") if o in sizes], lambda o, other: False)
+    assert call(B_up=p["B_gate"])[0] == TAKEN                # (operands are read alone)
+
+
+@pytest.mark.parametrize("dtype,kept", [(2, 2), (0, 0), (1, 8), (0, 8)])
+def test_gated_gradients_over_operands(L, dtype, kept):
+    m, n, k = 37, 300, 64
+    es, f8 = (4 if dtype == 0 else 2), kept == 8
+    factor, scales = (m * 304, m * 3 * 4) if f8 else (m * n * es, 0)
+    need = L.lib.sp_gemm_abt_gated_backward_workspace_bytes(dtype, m, n, k)
+    sizes = dict(dC=m * n * es, A=m * k * es, dA=m * k * es, B_gate=n * k * es, dB_up=n * k * es, B_up=n * k * es, dB_gate=n * k * es, workspace=need, gate=factor, up=factor)
+    if f8:
+        sizes.update(gate_scale=scales, up_scale=scales)
+    p = places(**sizes)
+    good = {**dict(dtype=dtype, act=0, kept=kept, gate_scale=None, up_scale=None, m=m, n=n, k=k, bytes=need + 4096), **p}      # (what is more than needed is not looked at)
+    call = Caller(L, "sp_gemm_abt_gated_backward", "dtype act dC A B_gate B_up kept gate gate_scale up up_scale dA dB_gate dB_up m n k workspace bytes", good)
+    early = {"dC", "gate", "up", "gate_scale", "up_scale"}            # read before any gradient is written
+    sweep(call, sizes, ["dA", "dB_gate", "dB_up", "workspace"], lambda o, other: o != "workspace" and other in early)
+    # what is not wanted is nowhere
+    assert call(dA=None)[0] == TAKEN and call(dB_gate=None, dB_up=None)[0] == TAKEN
