@@ -460,6 +460,12 @@ static int64_t token_chunks(int64_t rows, int64_t cols) {
     const int64_t n = wanted < possible ? wanted : possible;
     return n < MOST_CHUNKS ? n : MOST_CHUNKS;
 }
+// Columns of a chunk, whole pieces, and lanes of the workgroup that takes one.
+static int64_t chunk_columns(int dtype, int64_t cols, int64_t chunks) {
+    const int64_t piece = dtype == SP_F32 ? 4 : 8;
+    return ceil_div(ceil_div(cols, chunks), piece) * piece;
+}
+static int chunk_threads(int64_t chunk_cols) { return chunk_cols > LONG_COLS ? LONG_THREADS : SHORT_THREADS; }
 // Whether lanes of one wave hold a row: up to 512 of its 16-byte pieces, 1024 where there are waves enough.  (us, so / a workgroup per row: bf16 16384 x 4000 28.6 / 53, 8192 x 8000 33 / 36.8,
 // 2048 x 8192 12.5 / 9.1, 16 x 4091 4.2 / 3.5 and 2.5 for the join of two chunks, 256 x 8192 6.2 / 3.5; f32 16384 x 2000 23.6 / 32.9, 8192 x 4000 24.2 / 28.4.)
 constexpr int MANY_PIECES = 1024;
@@ -499,10 +505,9 @@ static int launch_rows(const void* logits, long cols, long rows, const TokenArgs
 
 template <int DT, bool ENTROPY, bool TOP>
 static int launch_long(const void* logits, long cols, long rows, const TokenArgs& a, hipStream_t stream) {
-    const long chunks = token_chunks(rows, cols), piece = PER16<DT>;
-    const long chunk_cols = ceil_div(ceil_div(cols, chunks), piece) * piece;
+    const long chunks = token_chunks(rows, cols), chunk_cols = chunk_columns(DT, cols, chunks);
     const dim3 blocks((unsigned)(rows * chunks));
-    if (chunk_cols > LONG_COLS) hipLaunchKernelGGL((token_probs_kernel<DT, LONG_THREADS, ENTROPY, TOP>), blocks, dim3(LONG_THREADS), 0, stream, logits, cols, (unsigned)chunks, chunk_cols, a);
+    if (chunk_threads(chunk_cols) == LONG_THREADS) hipLaunchKernelGGL((token_probs_kernel<DT, LONG_THREADS, ENTROPY, TOP>), blocks, dim3(LONG_THREADS), 0, stream, logits, cols, (unsigned)chunks, chunk_cols, a);
     else hipLaunchKernelGGL((token_probs_kernel<DT, SHORT_THREADS, ENTROPY, TOP>), blocks, dim3(SHORT_THREADS), 0, stream, logits, cols, (unsigned)chunks, chunk_cols, a);
     if (const int rc = check_launch("sp_token_log_probs"); rc != SP_OK || chunks == 1) return rc;
     if (TOP) hipLaunchKernelGGL(token_probs_join_top_kernel<DT>, dim3((unsigned)rows), dim3(256), 0, stream, logits, cols, (int)chunks, a);
@@ -549,6 +554,18 @@ static int token_sizes(const char* fn, int dtype, int64_t rows, int64_t cols) {
     return SP_OK;
 }
 
+// A launch holds fewer than 2^32 work items, whole workgroups of 256.
+constexpr int64_t MOST_TOKEN_ITEMS = ((int64_t)1 << 32) - 256;
+static int64_t forward_items(int dtype, int64_t rows, int64_t cols, int32_t top) {
+    if (short_rows(dtype, rows, cols, top)) return rows * by_pieces<MANY_PIECES>(ceil_div(cols, dtype == SP_F32 ? 4 : 8), [](auto t, auto) { return (int)decltype(t)::value; });
+    const int64_t chunks = token_chunks(rows, cols);
+    return rows * chunks * chunk_threads(chunk_columns(dtype, cols, chunks));
+}
+static int64_t backward_items(int dtype, int64_t rows, int64_t cols) {
+    const int64_t pieces = ceil_div(cols, dtype == SP_F32 ? 4 : 8);
+    return rows * (pieces <= FEW_PIECES ? by_pieces<FEW_PIECES>(pieces, [](auto t, auto) { return (int)decltype(t)::value; }) : 256 * ceil_div(pieces, GRAD_PIECES * 256));
+}
+
 extern "C" int64_t sp_token_log_probs_workspace_bytes(int64_t rows, int64_t cols, int32_t top) {
     if (rows <= 0 || cols <= 0 || top < 0 || top > MOST_TOP) return 0;
     const int64_t chunks = token_chunks(rows, cols);
@@ -568,8 +585,7 @@ extern "C" int sp_token_log_probs(int dtype, const void* logits, const int32_t* 
     if (top < 0 || top > MOST_TOP) return fail(SP_ERR_ARG, "sp_token_log_probs: top must be in [0, 32], got %d", top);
     if (top > 0 && (top_logp == nullptr || top_ids == nullptr)) return fail(SP_ERR_NULL, "sp_token_log_probs: top_logp and top_ids are needed for %d alternatives", top);
     const bool in_registers = short_rows(dtype, rows, cols, top);
-    // a launch holds fewer than 2^32 work items (chunks of a row: only where there are few rows)
-    if (rows >= ((int64_t)1 << 32) / (in_registers ? 64 : LONG_THREADS)) return fail(SP_ERR_SHAPE, "sp_token_log_probs: too large");
+    if (forward_items(dtype, rows, cols, top) > MOST_TOKEN_ITEMS) return fail(SP_ERR_SHAPE, "sp_token_log_probs: too large");
     const int64_t need = sp_token_log_probs_workspace_bytes(rows, cols, top);
     if (need > 0) {
         SP_REQUIRE_PTR(workspace);
@@ -607,9 +623,7 @@ extern "C" int sp_token_log_probs_backward(int dtype, const void* logits, const 
     SP_OPTIONAL_PTR(d_lse);
     if (const int rc = token_sizes(__func__, dtype, rows, cols); rc != SP_OK) return rc;
     if (d_entropy != nullptr && entropy == nullptr) return fail(SP_ERR_NULL, "sp_token_log_probs_backward: d_entropy needs the entropy");
-    const int64_t pieces = ceil_div(cols, dtype == SP_F32 ? 4 : 8);
-    const int64_t lanes = pieces <= FEW_PIECES ? by_pieces<FEW_PIECES>(pieces, [](auto t, auto) { return (int)decltype(t)::value; }) : 256 * ceil_div(pieces, GRAD_PIECES * 256);
-    if (rows * lanes > ((int64_t)1 << 32) - 256) return fail(SP_ERR_SHAPE, "sp_token_log_probs_backward: too large");      // (work items of a launch)
+    if (backward_items(dtype, rows, cols) > MOST_TOKEN_ITEMS) return fail(SP_ERR_SHAPE, "sp_token_log_probs_backward: too large");
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     TokenGradArgs a{};
     a.tokens = tokens; a.lse = lse; a.entropy = entropy; a.d_logp = d_logp; a.d_entropy = d_entropy; a.d_lse = d_lse; a.dx = d_logits;

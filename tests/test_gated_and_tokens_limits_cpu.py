@@ -87,3 +87,34 @@ def test_gated_gradients_over_operands(L, dtype, kept):
     sweep(call, sizes, ["dA", "dB_gate", "dB_up", "workspace"], lambda o, other: o != "workspace" and other in early)
     # what is not wanted is nowhere
     assert call(dA=None)[0] == TAKEN and call(dB_gate=None, dB_up=None)[0] == TAKEN
+
+
+def tokens_forward(L, **other):
+    p = {n: C.c_void_p((1 << 44) + (i << 50)) for i, n in enumerate(("logits", "tokens", "logp", "entropy", "lse", "top_logp", "top_ids", "workspace"))}      # (far apart)
+    good = {**dict(dtype=2, top=0, rows=1, cols=16, bytes=1 << 40), **p, **other}
+    return Caller(L, "sp_token_log_probs", "dtype logits tokens logp entropy lse top top_logp top_ids rows cols workspace bytes", good)
+
+
+def tokens_backward(L, **other):
+    p = {n: C.c_void_p((1 << 44) + (i << 50)) for i, n in enumerate(("logits", "tokens", "lse", "entropy", "d_logp", "d_entropy", "d_lse", "d_logits"))}
+    good = {**dict(dtype=2, rows=1, cols=16), **p, **other}
+    return Caller(L, "sp_token_log_probs_backward", "dtype logits tokens lse entropy d_logp d_entropy d_lse d_logits rows cols", good)
+
+
+# lanes to a row: 4 to 64 of a wave, a workgroup of 256 or 512
+@pytest.mark.parametrize("dtype,cols,top,lanes", [(2, 32, 0, 4), (0, 64, 0, 4), (2, 256, 0, 16), (1, 1024, 0, 16), (2, 1032, 0, 64), (2, 8192, 0, 64), (0, 4096, 0, 64), (2, 64, 1, 256), (2, 8200, 0, 256),
+                                                  (2, 16384, 0, 256), (2, 16385, 0, 512), (0, 20000, 5, 512)])
+def test_log_probabilities_take_as_many_rows_as_a_launch_holds(L, dtype, cols, top, lanes):
+    """A launch holds fewer than 2^32 work items: the last number of rows that fits is taken, one more is refused here and not by the launch."""
+    most = min((1 << 32) - 256, ((1 << 31) - 1) * lanes) // lanes
+    assert tokens_forward(L, dtype=dtype, cols=cols, top=top, rows=most)()[0] == TAKEN
+    rc, said = tokens_forward(L, dtype=dtype, cols=cols, top=top, rows=most + 1)()
+    assert rc == SHAPE and "too large" in said
+
+
+@pytest.mark.parametrize("dtype,cols,lanes", [(2, 32, 4), (0, 64, 4), (1, 1024, 16), (2, 1032, 64), (2, 2048, 64), (2, 2056, 256), (0, 4100, 512)])
+def test_their_gradient_too(L, dtype, cols, lanes):
+    most = ((1 << 32) - 256) // lanes
+    assert tokens_backward(L, dtype=dtype, cols=cols, rows=most)()[0] == TAKEN
+    rc, said = tokens_backward(L, dtype=dtype, cols=cols, rows=most + 1)()
+    assert rc == SHAPE and "too large" in said

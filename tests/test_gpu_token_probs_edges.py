@@ -35,3 +35,22 @@ def test_rows_with_nothing_in_them_have_no_gradient_whatever_comes_back(P, cols,
             got, want = grad(spoiled), grad(d)
             assert (got[1::2] == 0).all(), (bad, which)
             assert torch.equal(got[::2], want[::2]), (bad, which)
+
+
+# more rows than 2^32 work items would hold if every one took a wave, or a workgroup of 512
+@pytest.mark.parametrize("rows,cols,top", [((1 << 26) + 5, 8, 0), ((1 << 23) + 3, 40, 2)])
+def test_very_many_short_rows(P, rows, cols, top):
+    announce("token_log_probs many rows %s" % ((rows, cols, top),))
+    x, t = logits(1021, cols, "bf16", seed=32)
+    x, t = x.cuda(), t.cuda()
+    many = -(-rows // 1021)
+    out = P.token_log_probs(x.repeat(many, 1)[:rows], t.repeat(many)[:rows], top=top, want_entropy=True, want_lse=True)
+    few = P.token_log_probs(x.repeat(20, 1), t.repeat(20), top=top, want_entropy=True, want_lse=True)
+    for a, b in zip(out, few):
+        assert a.shape[0] == rows and torch.equal(a[:1021], b[:1021]) and torch.equal(a[-(rows % 1021):], b[:rows % 1021])
+        last = rows // 1021 * 1021
+        assert torch.equal(a[last - 1021 * 7:last], b[:1021 * 7])
+    if top == 0:
+        grad = P.token_log_probs_backward(out[0], x.repeat(many, 1)[:rows], t.repeat(many)[:rows], out[2])
+        want = P.token_log_probs_backward(few[0], x.repeat(20, 1), t.repeat(20), few[2])
+        assert torch.equal(grad[last - 1021:last], want[:1021]) and torch.equal(grad[last:], want[:rows - last])
