@@ -411,7 +411,7 @@ int64_t sp_logits_penalize_workspace_bytes(int64_t rows, int64_t cols);
  * the lowest column first; -inf and -1 where the row has no more above -inf (a NaN is never among them).
  * -inf has probability 0.  A row with nothing above -inf: lse and logp -inf, entropy 0.  A row with a NaN or +inf: NaN.
  * `workspace`: sp_token_log_probs_workspace_bytes(rows, cols, top) bytes of device memory (their former contents do not matter), may be NULL where that is 0; calls that
- * may run at the same time need one each.  A row's sums have one order for given sizes; in a call of another number of rows they may come out a rounding away.
+ * may run at the same time need one each.  Results and workspace must not overlap the logits, the tokens or one another (SP_ERR_ARG).  A row's sums have one order for given sizes; in a call of another number of rows they may come out a rounding away.
  * Stands beside sp_logits_penalize, sp_row_get_prob and SP_ROW_SOFTMAX (ml/primitives.spi:711-716).
  */
 int sp_token_log_probs(int dtype, const void* logits, const int32_t* tokens, float* logp, float* entropy, float* lse, int32_t top,
@@ -421,7 +421,8 @@ int64_t sp_token_log_probs_workspace_bytes(int64_t rows, int64_t cols, int32_t t
 /*
  * The gradient of the logits, from those of logp, entropy and lse (each (rows,) f32 or NULL):
  *   d_logits[j] = d_logp ([j = token] - p_j) - d_entropy p_j (ln p_j + entropy) + d_lse p_j
- * logits, tokens as in the forward call, lse (and, with d_entropy, entropy) as it wrote them.  d_logits: like the logits, whose memory it may be.  A row whose token does not count has
+ * logits, tokens as in the forward call, lse (and, with d_entropy, entropy) as it wrote them.  d_logits: like the logits, whose memory it may be; it must not overlap them otherwise, nor
+ * anything else that is read (SP_ERR_ARG).  A row whose token does not count has
  * no d_logp; one with nothing above -inf has zeros.  p is exp(x - lse) of the f32 lse: of a row of nothing but numbers as low as the type's lowest, whose lse has lost ln(count), it is 1.
  */
 int sp_token_log_probs_backward(int dtype, const void* logits, const int32_t* tokens, const float* lse, const float* entropy, const float* d_logp,

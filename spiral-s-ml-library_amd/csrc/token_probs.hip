@@ -8,6 +8,7 @@
 // What rows may hold: -inf has probability 0 (its terms are left out); a row with nothing above -inf has lse -inf, log probability -inf and entropy 0, and
 // gradients of 0; the lowest finite number is a logit like any other (x - m is taken before it is scaled, so that it does not
 // overflow to a NaN); +inf or a NaN make the sums NaN.
+#include "overlap.h"
 #include "vec_io.h"
 
 namespace sp {
@@ -591,6 +592,12 @@ extern "C" int sp_token_log_probs(int dtype, const void* logits, const int32_t* 
         SP_REQUIRE_PTR(workspace);
         if (workspace_bytes < need) return fail(SP_ERR_ARG, "sp_token_log_probs: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
     }
+    const int64_t es = dtype == SP_F32 ? 4 : 2, of_top = top > 0 ? rows * top * 4 : 0;
+    if (const int rc = lie_apart(__func__, {{"logp", logp, rows * 4}, {"entropy", entropy, rows * 4}, {"lse", lse, rows * 4}, {"top_logp", of_top > 0 ? top_logp : nullptr, of_top},
+                                            {"top_ids", of_top > 0 ? top_ids : nullptr, of_top}, {"workspace", need > 0 ? workspace : nullptr, need}},
+                                 {{"logits", logits, rows * cols * es}, {"tokens", tokens, rows * 4}});
+        rc != SP_OK)
+        return rc;
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     TokenArgs a{};
     a.tokens = tokens; a.logp = logp; a.entropy = entropy; a.lse = lse; a.top = top; a.top_logp = top_logp; a.top_ids = top_ids;
@@ -624,6 +631,13 @@ extern "C" int sp_token_log_probs_backward(int dtype, const void* logits, const 
     if (const int rc = token_sizes(__func__, dtype, rows, cols); rc != SP_OK) return rc;
     if (d_entropy != nullptr && entropy == nullptr) return fail(SP_ERR_NULL, "sp_token_log_probs_backward: d_entropy needs the entropy");
     if (backward_items(dtype, rows, cols) > MOST_TOKEN_ITEMS) return fail(SP_ERR_SHAPE, "sp_token_log_probs_backward: too large");
+    // (every number of the logits is read by the lane that writes its gradient, so they may be the same memory, but not half of it)
+    const int64_t all = rows * cols * (dtype == SP_F32 ? 4 : 2);
+    if (const int rc = lie_apart(__func__, {{"d_logits", d_logits, all}},
+                                 {{"logits", logits == d_logits ? nullptr : logits, all}, {"tokens", tokens, rows * 4}, {"lse", lse, rows * 4},
+                                  {"entropy", d_entropy != nullptr ? entropy : nullptr, rows * 4}, {"d_logp", d_logp, rows * 4}, {"d_entropy", d_entropy, rows * 4}, {"d_lse", d_lse, rows * 4}});
+        rc != SP_OK)
+        return rc;
     if (const int rc = require_gfx950(__func__); rc != SP_OK) return rc;
     TokenGradArgs a{};
     a.tokens = tokens; a.lse = lse; a.entropy = entropy; a.d_logp = d_logp; a.d_entropy = d_entropy; a.d_lse = d_lse; a.dx = d_logits;

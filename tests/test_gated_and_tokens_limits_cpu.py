@@ -89,6 +89,37 @@ def test_gated_gradients_over_operands(L, dtype, kept):
     assert call(dA=None)[0] == TAKEN and call(dB_gate=None, dB_up=None)[0] == TAKEN
 
 
+@pytest.mark.parametrize("dtype,top,cols", [(2, 5, 9001), (0, 0, 300), (1, 32, 70), (0, 0, 40000)])
+def test_log_probabilities_over_logits(L, dtype, top, cols):
+    rows = 37
+    need = L.lib.sp_token_log_probs_workspace_bytes(rows, cols, top)
+    sizes = dict(logp=rows * 4, logits=rows * cols * (4 if dtype == 0 else 2), entropy=rows * 4, tokens=rows * 4, lse=rows * 4)
+    if top:
+        sizes.update(top_logp=rows * top * 4, top_ids=rows * top * 4)
+    if need:
+        sizes.update(workspace=need)
+    call = tokens_forward(L, dtype=dtype, rows=rows, cols=cols, top=top, bytes=need, **places(**sizes))
+    sweep(call, sizes, [o for o in sizes if o not in ("logits", "tokens")], lambda o, other: False)
+
+
+@pytest.mark.parametrize("dtype,cols", [(2, 9001), (0, 300), (1, 7)])
+def test_their_gradient_over_what_it_reads(L, dtype, cols):
+    rows = 37
+    numbers = rows * cols * (4 if dtype == 0 else 2)
+    sizes = dict(logits=numbers, tokens=rows * 4, lse=rows * 4, d_logits=numbers, entropy=rows * 4, d_logp=rows * 4, d_entropy=rows * 4, d_lse=rows * 4)
+    call = tokens_backward(L, dtype=dtype, rows=rows, cols=cols, **places(**sizes))
+    assert call(d_logits=call.good["logits"])[0] == TAKEN
+    for away in (16, 32, numbers - 16 & ~15):
+        for at in (call.good["logits"].value + away, call.good["logits"].value - away):
+            rc, said = call(d_logits=C.c_void_p(at))
+            assert rc == ARG and "d_logits and logits overlap" in said
+    del sizes["logits"]                                   # (the others, at places that the logits do not reach)
+    call.good["logits"] = C.c_void_p(1 << 30)
+    sweep(call, sizes, ["d_logits"], lambda o, other: False)
+    # without d_entropy nobody looks at the entropy
+    assert call(d_entropy=None, d_logits=call.good["entropy"], entropy=call.good["entropy"], d_logp=None, d_lse=None)[0] == TAKEN
+
+
 def tokens_forward(L, **other):
     p = {n: C.c_void_p((1 << 44) + (i << 50)) for i, n in enumerate(("logits", "tokens", "logp", "entropy", "lse", "top_logp", "top_ids", "workspace"))}      # (far apart)
     good = {**dict(dtype=2, top=0, rows=1, cols=16, bytes=1 << 40), **p, **other}
