@@ -423,7 +423,9 @@ int64_t sp_token_log_probs_workspace_bytes(int64_t rows, int64_t cols, int32_t t
  *   d_logits[j] = d_logp ([j = token] - p_j) - d_entropy p_j (ln p_j + entropy) + d_lse p_j
  * logits, tokens as in the forward call, lse (and, with d_entropy, entropy) as it wrote them.  d_logits: like the logits, whose memory it may be; it must not overlap them otherwise, nor
  * anything else that is read (SP_ERR_ARG).  A row whose token does not count has
- * no d_logp; one with nothing above -inf has zeros.  p is exp(x - lse) of the f32 lse: of a row of nothing but numbers as low as the type's lowest, whose lse has lost ln(count), it is 1.
+ * no d_logp; one with nothing above -inf has zeros.  p is exp(x - lse) of the f32 lse, whose rounding is one
+ * relative error of every p of a row, |lse| 2^-24 at most (6e-4 for logits about 10^4, what moving a f32 logit of that size by half a unit in its last place does; a common
+ * offset of the logits is best left out): of a row of nothing but numbers as low as the type's lowest, whose lse has lost ln(count), p is 1.
  */
 int sp_token_log_probs_backward(int dtype, const void* logits, const int32_t* tokens, const float* lse, const float* entropy, const float* d_logp,
                                 const float* d_entropy, const float* d_lse, void* d_logits, int64_t rows, int64_t cols, void* stream);

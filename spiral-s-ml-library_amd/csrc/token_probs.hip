@@ -3,7 +3,8 @@
 // With m the largest logit, s = sum exp(x - m) and w = sum exp(x - m) (x - m): lse = m + ln s, log p_t = (x_t - m) - ln s, and the entropy
 // -sum p ln p = ln s - w / s, two numbers that are not negative, so nothing cancels.  A row is read once: a lane keeps m, s and w of what it has seen
 // and scales s and w where m grows; lanes, waves and chunks of a row then join in an order of the sizes alone.
-// Backward: dx_j = d_logp [j = t] - p_j (d_logp + d_entropy (ln p_j + H) - d_lse), one read and one write.
+// Backward: dx_j = d_logp [j = t] - p_j (d_logp + d_entropy (ln p_j + H) - d_lse), one read and one write.  p_j = exp(x_j - lse), of lse rounded to f32: that is a
+// relative error of up to |lse| 2^-24 which all p of a row share, no more than half a last place of a f32 logit of that size; m and ln s apart would be two numbers of a row to keep.
 //
 // What rows may hold: -inf has probability 0 (its terms are left out); a row with nothing above -inf has lse -inf, log probability -inf and entropy 0, and
 // gradients of 0; the lowest finite number is a logit like any other (x - m is taken before it is scaled, so that it does not

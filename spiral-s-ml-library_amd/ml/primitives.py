@@ -440,7 +440,7 @@ def token_log_probs(logits, tokens, top=0, want_entropy=False, want_lse=False):
 def token_log_probs_backward(d_log_probs, logits, tokens, lse, d_entropy=None, entropy=None, d_lse=None, out=None):
     """The gradient of the logits of `token_log_probs` (sp_token_log_probs_backward), of their type, from those of its log probabilities, entropies (with the entropies
     themselves) and lse, (...,) f32 each, any of them None; lse as the forward call returned it.  `out` may be the logits.  Rows whose token does not count have no gradient from
-    d_log_probs; the alternatives of `top` hand on none."""
+    d_log_probs; the alternatives of `top` hand on none.  Probabilities are exp(x - lse) of the f32 lse, whose rounding is a relative error, |lse| 2^-24 at most, that a row has in common."""
     if out is None:
         done = lib.whole_token_log_probs_backward(d_log_probs, logits, tokens, lse, d_entropy, entropy, d_lse)
         if done is not None:
