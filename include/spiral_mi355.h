@@ -194,7 +194,8 @@ int sp_gemm_abt_gated(int dtype, int activation, const void* A, const void* B_ga
 /*
  * Its gradients from dC (M, N), at the g and u that were kept:  dg = dC u act'(g), du = dC act(g), rounded to dtype, and
  *   dA = dg . B_gate + du . B_up (M, K),   dB_gate = dg^T . A, dB_up = du^T . A (N, K)
- * in dtype, of f32 sums.  dA may be NULL, and dB_gate with dB_up.  The gradients and the workspace must not overlap A, the weights or one another, nor the workspace
+ * in dtype, of f32 sums.  dg and du have the range of dtype, too: in f16 one above 65504 is an infinity, which spoils its row of dA and its rows of dB_gate or dB_up also where the sums
+ * would fit, and one below 2^-25 is 0; a loss is scaled for them as for the results.  dA may be NULL, and dB_gate with dB_up.  The gradients and the workspace must not overlap A, the weights or one another, nor the workspace
  * anything else (SP_ERR_ARG); a gradient may lie over dC, gate and up, which have been read by then.  The ReLU's slope at 0 is 0.  Every sum has one order: results repeat bit for bit, whichever
  * of the gradients are wanted.
  * `workspace`: sp_gemm_abt_gated_backward_workspace_bytes(dtype, M, N, K) bytes of device memory that hold dg, du and partial sums during the call (what they held before does not matter).  Calls

@@ -241,7 +241,7 @@ def matmul_abt_gated(a, b_gate, b_up, activation="silu", keep=None):
 
 def matmul_abt_gated_backward(dc, a, b_gate, b_up, kept, activation="silu", want_input_grad=True, want_weight_grads=True):
     """The gradients of `matmul_abt_gated` (sp_gemm_abt_gated_backward): (da, db_gate, db_up), of the type of a, from dc (M, N), the operands and what the forward call kept.  They
-    are those at the numbers that were kept.  da is None with want_input_grad=False, db_gate and db_up with want_weight_grads=False."""
+    are those at the numbers that were kept, with dg and du rounded to the type of a on the way: in f16 one above 65504 is an infinity, so a loss is scaled for them, too.  da is None with want_input_grad=False, db_gate and db_up with want_weight_grads=False."""
     if want_input_grad is True and want_weight_grads is True and type(kept) is tuple and len(kept) in (2, 4):
         done = lib.whole_matmul_abt_gated_backward(dc, a, b_gate, b_up, kept[0], kept[1] if len(kept) == 4 else None, kept[-2] if len(kept) == 4 else kept[1],
                                                    kept[3] if len(kept) == 4 else None, _lib.ACTIVATIONS.get(activation) if isinstance(activation, str) else None)

@@ -75,3 +75,21 @@ def test_gradients(M, act, dtype):
         worst = (off / bound).argmax()
         assert (off <= bound).all(), (what, g[worst].item(), got[worst].item(), want[worst].item())
     assert (da[:, 2:] == 0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(70, 130, 72), (300, 700, 264)])
+def test_a_loss_scaled_beyond_f16_is_seen_in_its_rows_alone(M, m, n, k):
+    """dg above 65504 is an infinity: infinite or NaN in its row of dA and of dB_gate, whichever side of the products it is on; the others have the bits that they have without it."""
+    announce("matmul_abt_gated_backward f16 range %s" % ((m, n, k),))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda a, b, s=1.0: (torch.randn((a, b), generator=g, device="cuda") * s).half()
+    x, gate, up, dc, kept = r(m, k), r(n, k, 0.1), r(n, k, 0.1), r(m, n), (r(m, n), r(m, n))
+    row, col = m - 3, n - 2
+    dc[row, col], kept[0][row, col], kept[1][row, col] = 1.0, 1.0, 2.0
+    clean = M.matmul_abt_gated_backward(dc, x, gate, up, kept)
+    dc[row, col], kept[1][row, col] = 3000.0, 30.0        # dg = 3000 * 30 * silu'(1) = 83500, du = 3000 * silu(1) = 2193
+    da, dg, du = M.matmul_abt_gated_backward(dc, x, gate, up, kept)
+    others = lambda t, i: torch.cat((t[:i], t[i + 1:]))
+    assert not da[row].isfinite().any() and torch.equal(others(da, row), others(clean[0], row))
+    assert not dg[col].isfinite().any() and torch.equal(others(dg, col), others(clean[1], col))
+    assert du.isfinite().all() and torch.equal(others(du, col), others(clean[2], col))
