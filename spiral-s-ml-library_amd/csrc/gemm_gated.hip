@@ -218,9 +218,9 @@ struct Strip {
 };
 
 // Bound by the matrix pipe and, in large products, by the part's power: 8192 x 4096 x 8192 bf16 takes 812 us, 1.35 PFLOP/s with the pipe busy 70 % of all cycles, and the gradients of
-// 8192 x 2048 x 8192 782 us, 1.41 PFLOP/s; f32, 4096 x 2048 x 4096, 980 us, 140 TFLOP/s.  Large tiles for the few bytes from LDS and L2 to an MFMA, eight waves for two on a SIMD; four waves on 256 x 256,
+// 8192 x 2048 x 8192 782 us, 1.41 PFLOP/s; f32, 4096 x 2048 x 4096, 955 us, 144 TFLOP/s.  Large tiles for the few bytes from LDS and L2 to an MFMA, eight waves for two on a SIMD; four waves on 256 x 256,
 // loads between a row's MFMAs, raised wave priorities and other groups of the walk gave nothing, a workgroup that goes on to a next tile while its results leave spilled.  So results leave bare:
-// both factors of 8192 x 2048 x 8192 kept whole cost 50 us beside 416, in 8-bit blocks (5008 x 2048 x 5461) 24 beside 182.
+// both factors of 8192 x 2048 x 8192 kept whole cost 36 us beside 375, in 8-bit blocks (5008 x 2048 x 5461) 21 beside 171.
 // One tile, or this workgroup's share of its K-tiles: with parts > 1 the sums go to a workspace in f32 (gated_join_kernel adds them up).
 template <int DT, int MODE, int BM, int BN, int WM, int WN, int NS>
 __device__ __forceinline__ void gated_mm(const GatedArgs& g, unsigned block, unsigned part, unsigned parts) {
@@ -836,8 +836,9 @@ static int launch_backward_split(const char* what, GatedPair p, bool input_first
 // ---- which kernel ----
 // Estimated times in us, without the launch: workgroups in rounds of as many as a unit's LDS holds at a time, each nk K-tiles (a quarter of them, where four waves share
 // them) plus an overhead; n workgroups on a unit take n times the work of a K-tile, and never less than what a lone one waits for.
-// Forward: fitted on what every kernel took on 99 shapes, from 1 x 512 x 1365 to 16384 x 4096 x 512; the one it picks is on the mean 2 % behind the fastest (3 with 8-bit blocks).  More
-// tiles (64 x 128, 128 x 256 in two stages, 16 x 64 and 64 x 64 in four parts) were worth less than a hundredth.
+// Forward: fitted on what every kernel took on 99 shapes, from 1 x 512 x 1365 to 16384 x 4096 x 512; the one it picks is on the mean 2 % behind the fastest (3 with 8-bit blocks).
+// Factors that are kept whole are in no menu: their results come on top, whatever the tile (8192 x 1024 x 2736 bf16 85 us with them, 76 without).
+// More tiles (64 x 128, 128 x 256 in two stages, 16 x 64 and 64 x 64 in four parts) were worth less than a hundredth.
 struct MmCost {
     int id, bm, bn;               // bn: columns of the result
     int per_unit;
@@ -1136,7 +1137,7 @@ extern "C" int sp_gemm_abt_gated(int dtype, int activation, const void* A, const
     GatedArgs g{};
     g.A = (const unsigned char*)A; g.B0 = (const unsigned char*)B_gate; g.B1 = (const unsigned char*)B_up; g.C0 = C; g.gate = gate; g.up = up;
     g.gate_scale = gate_scale; g.up_scale = up_scale; g.M = M; g.N = N; g.K = K; g.activation = activation; g.keep = f8 ? KEEP_F8 : keeps ? KEEP_WHOLE : KEEP_NONE;
-    // what does not stay in the caches (32 MiB of L2) is streamed past them, gate and up only where a row is of whole lines (5008 x 2048 x 5461 bf16: 205 us, 225 streamed)
+    // what does not stay in the caches (32 MiB of L2) is streamed past them, gate and up only where a row is of whole lines (5008 x 2048 x 5461 bf16: 188 us, 216 streamed)
     const int64_t pitch = N * es;
     g.stream = M * pitch <= (int64_t)32 << 20 ? 0 : pitch % 128 == 0 ? 3 : 1;
     const hipStream_t st = (hipStream_t)stream;

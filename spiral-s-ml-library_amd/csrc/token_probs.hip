@@ -470,6 +470,7 @@ static int64_t chunk_columns(int dtype, int64_t cols, int64_t chunks) {
 static int chunk_threads(int64_t chunk_cols) { return chunk_cols > LONG_COLS ? LONG_THREADS : SHORT_THREADS; }
 // Whether lanes of one wave hold a row: up to 512 of its 16-byte pieces, 1024 where there are waves enough.  (us, so / a workgroup per row: bf16 16384 x 4000 28.6 / 53, 8192 x 8000 33 / 36.8,
 // 2048 x 8192 12.5 / 9.1, 16 x 4091 4.2 / 3.5 and 2.5 for the join of two chunks, 256 x 8192 6.2 / 3.5; f32 16384 x 2000 23.6 / 32.9, 8192 x 4000 24.2 / 28.4.)
+// With alternatives a workgroup takes a row of any length, whose steps from barrier to barrier then are the time: 16384 x 256 f32 52 us with five of them, 4.9 without.
 constexpr int MANY_PIECES = 1024;
 static bool short_rows(int dtype, int64_t rows, int64_t cols, int32_t top) {
     const int64_t pieces = ceil_div(cols, dtype == SP_F32 ? 4 : 8);

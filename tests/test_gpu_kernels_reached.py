@@ -21,7 +21,7 @@ def kernels_of_the_library(pattern):
 
 def kernels_of(run):
     from torch.profiler import ProfilerActivity, profile
-    with profile(activities=[ProfilerActivity.CUDA]) as p:
+    with profile(activities=[ProfilerActivity.CUDA], acc_events=True) as p:
         run()
         torch.cuda.synchronize()
     names = [e.name for e in p.events()]
