@@ -184,7 +184,8 @@ int sp_gemm_abt_scaled(int f8_a, int f8_b, int dtype_out, const void* A, const f
  * the operands or one another (SP_ERR_ARG).
  *   SP_ACT_SILU g / (1 + exp(-g)),  SP_ACT_GELU g (1 + erf(g / sqrt 2)) / 2,  SP_ACT_RELU max(0, g)
  * gate, up: NULL, or what the backward pass takes, g = A . B_gate^T and u = A . B_up^T, of kept_dtype: dtype, (M, N) each; or SP_F8_E4M3, in the blocks of 1 x 128 of sp_quantize_blocks,
- * (M, N rounded up to 16) each with gate_scale, up_scale (M, ceil(N / 128)) f32.  Either way they are rounded once, from f32.
+ * (M, N rounded up to 16) each with gate_scale, up_scale (M, ceil(N / 128)) f32.  Either way they are rounded once, from f32; in f16 a sum
+ * above 65504 is kept as an infinity, and gradients at an infinite g are NaN in its row of dA and of dB_gate (the formulas' inf times 0).
  * Stands beside sp_gemm_abt with its ReLU (ml/layers.spi:194-240 multiplies and activates in two passes).
  */
 typedef enum { SP_ACT_SILU = 0, SP_ACT_GELU = 1, SP_ACT_RELU = 2 } sp_activation;

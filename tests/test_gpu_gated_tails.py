@@ -93,3 +93,25 @@ def test_a_loss_scaled_beyond_f16_is_seen_in_its_rows_alone(M, m, n, k):
     assert not da[row].isfinite().any() and torch.equal(others(da, row), others(clean[0], row))
     assert not dg[col].isfinite().any() and torch.equal(others(dg, col), others(clean[1], col))
     assert du.isfinite().all() and torch.equal(others(du, col), others(clean[2], col))
+
+
+def test_a_sum_beyond_f16_is_kept_as_an_infinity(M):
+    """C is computed of the f32 sums; the gradients at an infinite gate are NaN in its row of dA and its column's row of dB_gate, and nowhere else."""
+    announce("matmul_abt_gated f16 range of what is kept")
+    m, n, k = 70, 130, 72
+    g = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda a, b, s=1.0: (torch.randn((a, b), generator=g, device="cuda") * s).half()
+    x, gate, up, dc = r(m, k), r(n, k, 0.1), r(n, k, 0.1), r(m, n)
+    x[:, :2], gate[:, :2], up[:, :2] = 0, 0, 0
+    row, col = m - 3, n - 2
+    _, clean = M.matmul_abt_gated(x, gate, up, keep=torch.float16)
+    x[row], gate[col], up[col] = 0, 0, 0
+    x[row, 0], gate[col, 0], x[row, 1], up[col, 1] = 300, 300, 0.25, 1.0          # g = 90000, u = 0.25
+    c, kept = M.matmul_abt_gated(x, gate, up, keep=torch.float16)
+    # (f16 counts in steps of 16 from 2^14 to 2^15: 22500 = 1406.25 * 16 is rounded to 1406 * 16)
+    assert c[row, col].item() == 22496 and kept[0][row, col].item() == math.inf and kept[1][row, col].item() == 0.25
+    kept = tuple(torch.where((torch.arange(m, device="cuda") == row)[:, None] & (torch.arange(n, device="cuda") == col), a, b) for a, b in zip(kept, clean))
+    da, dg, du = M.matmul_abt_gated_backward(dc, x, gate, up, kept)
+    others = lambda t, i: torch.cat((t[:i], t[i + 1:]))
+    assert da[row].isnan().all() and not others(da, row).isnan().any()
+    assert dg[col].isnan().all() and not others(dg, col).isnan().any() and not others(du, col).isnan().any()
